@@ -25,6 +25,7 @@ pub const HX_Q8_0: i32 = 8;
 pub const HX_Q4_K: i32 = 12;
 pub const HX_Q6_K: i32 = 14;
 pub const HX_BF16: i32 = 30;
+pub const HX_MXFP4: i32 = 39;
 
 // where the pointers in hx_moe_weights live
 pub const HX_HOST: i32 = 0;

@@ -22,6 +22,7 @@
 #define HX_Q4_K 12
 #define HX_Q6_K 14
 #define HX_BF16 30
+#define HX_MXFP4 39
 
 namespace hx {
 

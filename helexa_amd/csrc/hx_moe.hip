@@ -940,7 +940,8 @@ extern "C" int hx_moe_decoder_mlp(hx_moe* m, void* x, int64_t n_tokens, const fl
 
 extern "C" int hx_quantize(int dtype, const float* src, int64_t rows, int64_t cols, void* dst, void* stream) {
   if (!src || !dst || rows < 0) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
-  if (dtype != HX_Q8_0 && dtype != HX_Q4_K && dtype != HX_Q6_K && dtype != HX_BF16 && dtype != HX_F16)
+  if (dtype != HX_Q8_0 && dtype != HX_Q4_K && dtype != HX_Q6_K && dtype != HX_MXFP4 && dtype != HX_BF16 &&
+      dtype != HX_F16)
     return fail(HX_ERR_UNSUPPORTED, "hx_quantize: dtype %d", dtype);
   if (hx_row_bytes(dtype, cols) < 0)
     return fail(HX_ERR_INVALID_ARGUMENT, "hx_quantize: %lld columns do not tile into dtype %d blocks", (long long)cols, dtype);

@@ -14,7 +14,7 @@ namespace hx {
 int64_t gguf_block_elems(int fmt) {
   switch (fmt) {
     case HX_F32: case HX_F16: case HX_BF16: return 1;
-    case HX_Q8_0: return 32;
+    case HX_Q8_0: case HX_MXFP4: return 32;
     case HX_Q4_K: case HX_Q6_K: return 256;
     default: return 0;
   }
@@ -25,6 +25,7 @@ int64_t gguf_block_bytes(int fmt) {
     case HX_F32: return 4;
     case HX_F16: case HX_BF16: return 2;
     case HX_Q8_0: return 34;
+    case HX_MXFP4: return 17;
     case HX_Q4_K: return 144;
     case HX_Q6_K: return 210;
     default: return 0;
@@ -415,6 +416,67 @@ __global__ __launch_bounds__(256) void k_quantize_q8_0(const float* src, int64_t
   qz_stage_out(out, nb * 34, dst + b0 * 34);
 }
 
+// MXFP4: 17 bytes a block of 32, the scale 2^(s - 127) as its exponent byte s, then
+// the E2M1 codes, element j in the low and j + 16 in the high half of byte j.
+// s = floor(log2 amax) - 2 + 127, in 0 .. 254, which puts the largest magnitude
+// into [4, 8); codes are x / scale rounded to nearest even, 6 at most
+// (v_cvt_scalef32_pk_fp4_f32 does both, -0 kept). A block with a NaN or an infinity
+// has no such scale: s = 255, the format's NaN, codes 0.
+// Bound by HBM; workgroup: 128 blocks, a block's 32 elements in 8 lanes.
+HX_DEV uint32_t spread_nibbles(uint32_t n) {   // 4 nibbles -> the low halves of 4 bytes
+  n = (n | (n << 8)) & 0x00ff00ffu;
+  return (n | (n << 4)) & 0x0f0f0f0fu;
+}
+__global__ __launch_bounds__(256) void k_quantize_mxfp4(const float* src, int64_t nblocks, uint8_t* dst) {
+  __shared__ __attribute__((aligned(16))) uint8_t out[128 * 17];
+  const int64_t b0 = (int64_t)blockIdx.x * 128;
+  const int nb = (int)(nblocks - b0 < 128 ? nblocks - b0 : 128);
+  const float* s = src + b0 * 32;
+  const bool al = ((uintptr_t)s & 15) == 0;
+  float4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int q = 4 * ((int)threadIdx.x + 256 * i);
+    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (q < nb * 32) {
+      if (al) v[i] = *(const float4*)(s + q);
+      else v[i] = make_float4(s[q], s[q + 1], s[q + 2], s[q + 3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    // the largest magnitude as bits: NaN above infinity above every number
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, true));
+    const int e = (int)(m >> 23);
+    const int sb = max(e - 2, 0);
+    const float sc = sb ? __uint_as_float((uint32_t)sb << 23) : __uint_as_float(0x00400000u);   // 2^(sb - 127)
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], sc, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], sc, 1);
+    c = e == 255 ? 0u : c & 0xffffu;
+    // lane + 4: the codes of the elements 16 further on
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x104, 0xf, 0xf, true);   // row_shl:4
+    const uint32_t w = spread_nibbles(c) | (spread_nibbles(hi) << 4);
+    const int p = (int)threadIdx.x + 256 * i, j = p & 7;
+    uint8_t* o = out + (p >> 3) * 17;
+    if (j == 0) o[0] = (uint8_t)(e == 255 ? 255 : sb);
+    if (j < 4) {
+      o[1 + 4 * j] = (uint8_t)w;
+      o[2 + 4 * j] = (uint8_t)(w >> 8);
+      o[3 + 4 * j] = (uint8_t)(w >> 16);
+      o[4 + 4 * j] = (uint8_t)(w >> 24);
+    }
+  }
+  __syncthreads();
+  qz_stage_out(out, nb * 17, dst + b0 * 17);
+}
+
 // f32 -> bf16 / f16, eight elements a thread where both sides are 16-byte
 // aligned, else (and for the last n % 8) one by one
 template <int FMT>
@@ -544,6 +606,49 @@ __global__ __launch_bounds__(256) void k_repack_q4_k(const uint8_t* src, int64_t
   for (int i = 0; i < 144; i++) d[i] = s[i];
 }
 
+// MXFP4 rows -> f32: bound by HBM; workgroup: 128 blocks through LDS (whole
+// 16-byte loads where src allows them), 4 elements a thread and pass, 8 lanes a
+// block. The products are exact (2^-128 is a denormal f32); s = 255 gives NaN.
+__global__ __launch_bounds__(256) void k_dequantize_mxfp4(const uint8_t* src, int64_t nblocks, float* dst) {
+  __shared__ __attribute__((aligned(16))) uint8_t in[128 * 17];
+  const int64_t b0 = (int64_t)blockIdx.x * 128;
+  const int nb = (int)(nblocks - b0 < 128 ? nblocks - b0 : 128), n = nb * 17;
+  const uint8_t* s = src + b0 * 17;
+  const int tid = threadIdx.x;
+  if (((uintptr_t)s & 15) == 0) {
+    if (16 * tid + 16 <= n) *(uint4*)(in + 16 * tid) = *(const uint4*)(s + 16 * tid);   // n <= 16 * 256
+    const int i = (n & ~15) + tid;
+    if (i < n) in[i] = s[i];
+  } else {
+    for (int i = tid; i < n; i += 256) in[i] = s[i];
+  }
+  __syncthreads();
+  float* d = dst + b0 * 32;
+  const bool al = ((uintptr_t)d & 15) == 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int p = tid + 256 * i, j = p & 7;
+    if (p >= nb * 8) break;
+    const uint8_t* b = in + (p >> 3) * 17;
+    const uint8_t* q = b + 1 + 4 * (j & 3);
+    const uint32_t w = ((uint32_t)q[0] | ((uint32_t)q[1] << 8) | ((uint32_t)q[2] << 16) | ((uint32_t)q[3] << 24)) >> (j & 4);
+    const uint32_t sb = b[0];
+    const float sc = sb ? __uint_as_float(sb == 255 ? 0x7fc00000u : sb << 23) : __uint_as_float(0x00400000u);
+    float v[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      // the code's f32: exponent and mantissa bit in place (0.5 is the denormal of the format), then the sign
+      const uint32_t c = (w >> (8 * t)) & 15u, m = c & 7u;
+      const uint32_t bits = m >= 2 ? (126u + (m >> 1)) << 23 | (m & 1u) << 22 : m ? 0x3f000000u : 0u;
+      v[t] = __uint_as_float(bits | (c & 8u) << 28) * sc;
+    }
+    if (al) *(float4*)(d + 4 * p) = make_float4(v[0], v[1], v[2], v[3]);
+    else {
+      d[4 * p] = v[0]; d[4 * p + 1] = v[1]; d[4 * p + 2] = v[2]; d[4 * p + 3] = v[3];
+    }
+  }
+}
+
 hipError_t launch_quantize(int fmt, const float* src, int64_t rows, int64_t cols, void* dst, hipStream_t s) {
   const int64_t nb = rows * (cols / gguf_block_elems(fmt));
   auto grid = [&](int per) { return dim3((unsigned)((nb + per - 1) / per)); };   // blocks a workgroup takes
@@ -552,6 +657,7 @@ hipError_t launch_quantize(int fmt, const float* src, int64_t rows, int64_t cols
     case HX_Q8_0: hipLaunchKernelGGL(k_quantize_q8_0, grid(128), dim3(256), 0, s, src, nb, d); break;
     case HX_Q4_K: hipLaunchKernelGGL(k_quantize_q4k, grid(32), dim3(256), 0, s, src, nb, d); break;
     case HX_Q6_K: hipLaunchKernelGGL(k_quantize_q6k, grid(16), dim3(256), 0, s, src, nb, d); break;
+    case HX_MXFP4: hipLaunchKernelGGL(k_quantize_mxfp4, grid(128), dim3(256), 0, s, src, nb, d); break;
     case HX_BF16: hipLaunchKernelGGL(k_round_f32<HX_BF16>, grid(2048), dim3(256), 0, s, src, nb, d); break;
     case HX_F16: hipLaunchKernelGGL(k_round_f32<HX_F16>, grid(2048), dim3(256), 0, s, src, nb, d); break;
     default: return hipErrorInvalidValue;
@@ -567,6 +673,9 @@ hipError_t launch_dequantize(int fmt, const void* src, int64_t rows, int64_t col
     case HX_Q8_0: hipLaunchKernelGGL(k_dequantize<HX_Q8_0>, grid, dim3(256), 0, s, p, nb, dst); break;
     case HX_Q4_K: hipLaunchKernelGGL(k_dequantize<HX_Q4_K>, grid, dim3(256), 0, s, p, nb, dst); break;
     case HX_Q6_K: hipLaunchKernelGGL(k_dequantize<HX_Q6_K>, grid, dim3(256), 0, s, p, nb, dst); break;
+    case HX_MXFP4:
+      hipLaunchKernelGGL(k_dequantize_mxfp4, dim3((unsigned)((nb + 127) / 128)), dim3(256), 0, s, p, nb, dst);
+      break;
     case HX_BF16: hipLaunchKernelGGL(k_dequantize<HX_BF16>, grid, dim3(256), 0, s, p, nb, dst); break;
     case HX_F16: hipLaunchKernelGGL(k_dequantize<HX_F16>, grid, dim3(256), 0, s, p, nb, dst); break;
     case HX_F32: hipLaunchKernelGGL(k_dequantize<HX_F32>, grid, dim3(256), 0, s, p, nb, dst); break;

@@ -44,13 +44,15 @@ extern "C" {
 #define HX_ERR_WORKSPACE_TOO_SMALL 4
 #define HX_ERR_OUT_OF_MEMORY 5
 
-/* storage formats: the GGML type ids */
+/* storage formats: the GGML type ids (HX_MXFP4: for the quantisers and for
+ * expert projections) */
 #define HX_F32 0
 #define HX_F16 1
 #define HX_Q8_0 8
 #define HX_Q4_K 12
 #define HX_Q6_K 14
 #define HX_BF16 30
+#define HX_MXFP4 39
 
 /* where the pointers in hx_moe_weights live */
 #define HX_HOST 0
@@ -151,14 +153,21 @@ int hx_moe_decoder_mlp(hx_moe* m, void* x, int64_t n_tokens, const float* norm_w
                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* quantize_parallel (isq.rs:39-113) on the device: f32 [rows, cols] -> GGUF
- * rows of dtype (HX_Q8_0, HX_Q4_K, HX_Q6_K, HX_BF16, HX_F16). cols must tile
- * into whole blocks. Each block follows the rule of candle's
+ * rows of dtype (HX_Q8_0, HX_Q4_K, HX_Q6_K, HX_MXFP4, HX_BF16, HX_F16). cols
+ * must tile into whole blocks. Each block follows the rule of candle's
  * GgmlType::from_float, which quantize_parallel calls (isq.rs:98): Q8_0
  * d = amax/127 with rounding half away from zero; Q4_K make_qkx1_quants
- * (5 tries) per 32 elements; Q6_K make_qx_quants (rmse_type 1) per 16. */
+ * (5 tries) per 32 elements; Q6_K make_qx_quants (rmse_type 1) per 16.
+ * HX_MXFP4 (no counterpart in the reference) is a block of 32 in 17 bytes: the
+ * exponent byte s of the scale 2^(s - 127), then 16 bytes of E2M1 codes, element j
+ * in the low and j + 16 in the high half of byte j. s - 127 =
+ * max(floor(log2 amax) - 2, -127); codes are element / scale rounded to the
+ * nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code, the sign kept).
+ * A block that holds a NaN or an infinity gets s = 255 (NaN) and codes 0. */
 int hx_quantize(int dtype, const float* src, int64_t rows, int64_t cols, void* dst, void* stream);
 
-/* GGUF rows of dtype -> f32 [rows, cols] on the device. */
+/* GGUF rows of dtype -> f32 [rows, cols] on the device. HX_MXFP4 blocks of s = 255
+ * give NaN. */
 int hx_dequantize(int dtype, const void* src, int64_t rows, int64_t cols, float* dst, void* stream);
 
 /* Bytes of one GGUF row of n elements, or -1 if n does not tile into blocks. */

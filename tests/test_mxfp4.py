@@ -1,0 +1,45 @@
+"""MXFP4 without a GPU: row sizes, the refusals of the entry points (checked
+before anything touches a device), and the numpy rules the GPU tests compare with."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import mxfp4 as M
+
+
+def test_row_bytes():
+    import helexa_amd as hx
+    assert hx.MXFP4 == 39
+    assert hx.row_bytes(hx.MXFP4, 32) == 17
+    assert hx.row_bytes(hx.MXFP4, 2048) == 1088
+    assert hx.row_bytes(hx.MXFP4, 48) == -1
+    assert hx.row_bytes(hx.MXFP4, 0) == -1
+
+
+@pytest.mark.parametrize("fn", ["hx_quantize", "hx_dequantize"])
+def test_refusals_of_the_quantiser(fn):
+    import helexa_amd as hx
+    f = getattr(hx.lib(), fn)
+    p = C.c_void_p(4096)   # never reached
+    assert f(hx.MXFP4, None, 1, 32, p, None) == 1
+    assert f(hx.MXFP4, p, 1, 32, None, None) == 1
+    assert f(hx.MXFP4, p, -1, 32, p, None) == 1
+    assert f(hx.MXFP4, p, 1, 33, p, None) == 1
+    assert f(hx.MXFP4, p, 0, 32, p, None) == 0   # nothing to do
+
+
+def test_numpy_rules():
+    """ties to the even code, saturation, both signs of zero, the scale's range"""
+    x = np.zeros((4, 32), np.float32)
+    x[0, :16] = [4, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, 7, 6.5, -0.0, -.25, -.2500001, .2500001, 7.99, -5.0001]
+    q = M.quantise(x)
+    assert q[0, 0] == 127
+    assert [int(v) & 15 for v in q[0, 1:17]] == [6, 0, 2, 2, 4, 4, 6, 6, 7, 7, 8, 8, 9, 1, 7, 15]
+    x[1] = np.float32(1e-45)
+    x[2] = np.float32(3e38)
+    x[3, 7] = np.inf
+    q = M.quantise(x)
+    assert q[1, 0] == 0 and q[2, 0] == 127 + 125 and q[3, 0] == 255 and not q[3, 1:].any()
+    assert np.isnan(M.values(q[3])).all()
+    assert M.values(q[0])[0] == 4.0 and M.values(q[0])[15] == -6.0
