@@ -83,6 +83,7 @@ extern "C" {
     pub fn hx_moe_destroy(m: *mut hx_moe) -> c_int;
     pub fn hx_moe_workspace_size(m: *const hx_moe, n_tokens: i64, bytes: *mut usize) -> c_int;
     pub fn hx_moe_forward(m: *mut hx_moe, x: *const c_void, n_tokens: i64, y: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, router_bias: *const f32, stream: *mut c_void) -> c_int;
+    pub fn hx_moe_experts(m: *mut hx_moe, x: *const c_void, n_tokens: i64, topk_idx: *const i32, topk_w: *const f32, shared_w: *const f32, y: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn hx_moe_forward_noalloc(m: *mut hx_moe, x: *const c_void, n_tokens: i64, y: *mut c_void, router_bias: *const f32, stream: *mut c_void) -> c_int;
     pub fn hx_moe_forward_host(m: *mut hx_moe, x_host: *const c_void, n_tokens: i64, y_host: *mut c_void, router_bias_host: *const f32) -> c_int;
     pub fn hx_moe_route(m: *mut hx_moe, x: *const c_void, n_tokens: i64, router_bias: *const f32, topk_idx: *mut i32, topk_w: *mut f32, perm: *mut i32, offsets: *mut i32, inv: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;

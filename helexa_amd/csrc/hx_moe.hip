@@ -25,6 +25,7 @@
 
 #include "hx_moe.h"
 #include "hx_internal.h"
+#include "hx_mx.h"
 
 using namespace hx;
 
@@ -133,7 +134,7 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct WsLayout {
   size_t logits, topk_idx, topk_w, sgw, perm, inv, offsets, slots, tiles, counts, plan, dmap, hbuf, hbf, xh, xq, xq32, xcv,
-      hrec, obuf, xn, ym, dpart, wpos, total;
+      hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, total;
   int hstride, max_slots, max_tiles;
 };
 
@@ -150,6 +151,17 @@ static ExpertArgs shape_args(const hx_moe* m) {
 }
 static bool generic_path(const hx_moe* m, int64_t T) {
   return T <= HX_DECODE_MAX_T ? !decode_fast_ok(m->shape) : !prefill_mfma_ok(m->shape);
+}
+
+// experts on MXFP4 weights (all three projections; hx_mx.hip)
+static bool is_mx(const hx_moe* m) { return m->gate.fmt == HX_MXFP4; }
+static int mx_hblocks(const hx_moe* m) {
+  return mx_blocks(std::max(m->cfg.moe_intermediate_size, m->cfg.shared_expert_intermediate_size));
+}
+// most tiles of a call, whichever rows a tile takes
+static int64_t mx_max_tiles(const hx_moe* m, int64_t T, int tile_m) {
+  const int64_t F = T * m->cfg.num_experts_per_tok;
+  return F / tile_m + std::min<int64_t>(F, m->cfg.num_experts) + T / tile_m + 2;
 }
 
 static WsLayout ws_layout(const hx_moe* m, int64_t T) {
@@ -179,6 +191,25 @@ static WsLayout ws_layout(const hx_moe* m, int64_t T) {
   L.counts = take(sizeof(int32_t) * 4);
   L.plan = take(sizeof(int32_t) * plan_ints(L.max_slots, (int)F, (int)T));
   L.dmap = decode ? 0 : take(sizeof(int32_t) * (size_t)(dispatch_chunks((int)T) + dispatch_words((int)T)) * E);
+  if (is_mx(m)) {
+    // what grows with T only: neither the rows a tile takes nor the chunks' size
+    const bool xbf = m->cfg.act_dtype == HX_BF16, mfew = mx_few((int)std::min<int64_t>(T, 1 << 24), (int)k, (int)H, xbf);
+    const size_t rec = mx_rec_bytes(xbf), act = xbf ? 2 : 4;
+    L.mx_hrec = take(rec * (size_t)(F + T) * mx_hblocks(m));
+    L.xn = take(act * T * H);
+    L.ym = take(act * T * H);
+    if (!mfew) {
+      L.mx_xrec = take(rec * (size_t)T * mx_blocks((int)H));
+      L.obuf = take(act * (size_t)(F + T) * H);
+      L.mx_perm = take(sizeof(int32_t) * F);
+      L.mx_inv = take(sizeof(int32_t) * F);
+      L.mx_hist = take(sizeof(int32_t) * (size_t)std::min<int64_t>((F + MX_CHUNK - 1) / MX_CHUNK, MX_MAX_CHUNKS) * E);
+      L.mx_tiles = take(sizeof(int32_t) * 4 * (size_t)mx_max_tiles(m, T, 32));
+      L.mx_counts = take(sizeof(int32_t) * 4);
+    }
+    L.total = o;
+    return L;
+  }
   L.hbuf = take(sizeof(float) * (F + T) * L.hstride);
   L.hbf = take(sizeof(uint16_t) * (F + T) * L.hstride);
   const size_t act = m->cfg.act_dtype == HX_BF16 ? 2 : 4;
@@ -220,13 +251,14 @@ static size_t ws_need(const hx_moe* m, int64_t T, const WsLayout& L) {
 static int chunk_elems(int fmt) {
   switch (fmt) {
     case HX_F32: case HX_BF16: return 8;
-    case HX_Q8_0: case HX_Q4_K: case HX_Q6_K: return 32;
+    case HX_Q8_0: case HX_Q4_K: case HX_Q6_K: case HX_MXFP4: return 32;
     default: return 0;
   }
 }
 
 static int check_proj(const char* name, int fmt, int64_t K) {
-  if (fmt != HX_F32 && fmt != HX_BF16 && fmt != HX_Q8_0 && fmt != HX_Q4_K && fmt != HX_Q6_K)
+  if (fmt != HX_F32 && fmt != HX_BF16 && fmt != HX_Q8_0 && fmt != HX_Q4_K && fmt != HX_Q6_K &&
+      fmt != HX_MXFP4)
     return fail(HX_ERR_UNSUPPORTED, "%s: unsupported storage dtype %d", name, fmt);
   if (hx_row_bytes(fmt, K) < 0)
     return fail(HX_ERR_INVALID_ARGUMENT, "%s: input dim %lld does not tile into dtype %d blocks", name,
@@ -246,7 +278,7 @@ static int upload_proj(WMat& w, const char* name, int fmt, const void* src, int 
   w.K = K;
   w.count = count;
   const int64_t packed = (int64_t)rows * hx_row_bytes(fmt, K);
-  w.mat_bytes = (int64_t)align256((size_t)packed);
+  w.mat_bytes = (int64_t)align256((size_t)(fmt == HX_MXFP4 ? mx_mat_bytes(rows, K) : packed));
   const size_t bytes = (size_t)w.mat_bytes * count, src_bytes = (size_t)packed * count;
   if (!src) return fail(HX_ERR_INVALID_ARGUMENT, "%s: null weight pointer", name);
   if (hipMalloc(&w.base, bytes) != hipSuccess)
@@ -263,7 +295,8 @@ static int upload_proj(WMat& w, const char* name, int fmt, const void* src, int 
     }
     dsrc = tmp;
   }
-  hipError_t e = launch_repack(fmt, dsrc, count, rows, K, w.base, w.mat_bytes, 0);
+  hipError_t e = fmt == HX_MXFP4 ? launch_mx_repack(dsrc, count, rows, K, w.base, w.mat_bytes, 0)
+                                 : launch_repack(fmt, dsrc, count, rows, K, w.base, w.mat_bytes, 0);
   if (e == hipSuccess) e = hipDeviceSynchronize();
   if (tmp) (void)hipFree(tmp);
   if (e != hipSuccess) return fail(HX_ERR_DEVICE, "%s: repack failed: %s", name, hipGetErrorString(e));
@@ -363,6 +396,8 @@ extern "C" int hx_moe_create(const hx_moe_config* cfg, const hx_moe_weights* w, 
   if ((rc = check_proj("experts.gate_proj", w->gate_dtype, H)) || (rc = check_proj("experts.up_proj", w->up_dtype, H)) ||
       (rc = check_proj("experts.down_proj", w->down_dtype, I)))
     return rc;
+  if ((w->gate_dtype == HX_MXFP4) != (w->down_dtype == HX_MXFP4))
+    return fail(HX_ERR_UNSUPPORTED, "HX_MXFP4 experts: all of gate_proj, up_proj and down_proj must be HX_MXFP4");
   if (w->gate_dtype != w->up_dtype) return fail(HX_ERR_UNSUPPORTED, "gate_proj and up_proj must share a dtype");
   if (sh) {
     if ((rc = check_proj("shared_expert.gate_proj", w->shared_gate_dtype, H)) ||
@@ -646,11 +681,83 @@ struct DecoderFuse {
   void* x;   // layer input; receives x + block(rmsnorm(x))
 };
 
+// the experts' products on MXFP4 weights and their combine (a handle of is_mx)
+static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const float* w, const float* shared_w,
+                  void* y, void* resid, uint8_t* ws, const WsLayout& L, hipStream_t s) {
+  const hx_moe_config& c = m->cfg;
+  if ((uintptr_t)ws & 15) return fail(HX_ERR_INVALID_ARGUMENT, "the workspace must start on 16 bytes");
+  MxArgs a{};
+  a.gate = m->gate; a.up = m->up; a.down = m->down;
+  a.sgate = m->sgate; a.sup = m->sup; a.sdown = m->sdown;
+  a.E = c.num_experts; a.k = c.num_experts_per_tok; a.H = c.hidden_size; a.I = c.moe_intermediate_size;
+  a.Is = shared_w ? c.shared_expert_intermediate_size : 0;
+  a.T = (int)T; a.F = (int)(T * a.k);
+  a.x = x; a.xbf = c.act_dtype == HX_BF16;
+  a.idx = idx; a.w = w; a.shared_w = shared_w;
+  a.y = y; a.resid = resid;
+  a.hrec = ws + L.mx_hrec;
+  a.hblocks = mx_hblocks(m);
+  if (mx_few(a.T, a.k, a.H, a.xbf)) {
+    tm_ext(m, SLOT_GATE_UP, s);
+    HX_HIP(launch_mx_few_gate_up(a, s));
+    tm_ext_done(m, SLOT_GATE_UP);
+    tm_ext(m, SLOT_DOWN, s);
+    HX_HIP(launch_mx_few_down(a, s));
+    tm_ext_done(m, SLOT_DOWN);
+  } else {
+    a.xrec = ws + L.mx_xrec;
+    a.obuf = ws + L.obuf;
+    a.perm = (int32_t*)(ws + L.mx_perm);
+    a.inv = (int32_t*)(ws + L.mx_inv);
+    a.hist = (int32_t*)(ws + L.mx_hist);
+    a.tiles = (int32_t*)(ws + L.mx_tiles);
+    a.counts = (int32_t*)(ws + L.mx_counts);
+    a.tile_m = mx_tile_m(a.F, a.E);
+    a.max_tiles = (int)mx_max_tiles(m, T, a.tile_m);
+    tm_ext(m, SLOT_X_F16, s);
+    HX_HIP(launch_mx_prep(a, s));
+    tm_ext_done(m, SLOT_X_F16);
+    tm_ext(m, SLOT_DISPATCH, s);
+    HX_HIP(launch_mx_dispatch(a, s));
+    tm_ext_done(m, SLOT_DISPATCH);
+    tm_ext(m, SLOT_GATE_UP, s);
+    HX_HIP(launch_mx_gate_up(a, s));
+    tm_ext_done(m, SLOT_GATE_UP);
+    tm_ext(m, SLOT_DOWN, s);
+    HX_HIP(launch_mx_down(a, s));
+    tm_ext_done(m, SLOT_DOWN);
+    tm_ext(m, SLOT_COMBINE, s);
+    HX_HIP(launch_mx_combine(a, s));
+    tm_ext_done(m, SLOT_COMBINE);
+  }
+  if (m->tm.on && m->tm.calls < m->tm.max_calls && !capturing(s)) m->tm.calls++;
+  return HX_OK;
+}
+
 static int forward_impl(hx_moe* m, const void* x, int64_t T, void* y, void* ws, size_t ws_bytes,
                         const float* bias, hipStream_t s, const DecoderFuse* fz = nullptr) {
   WsLayout L;
   int rc = get_ws(m, T, ws, ws_bytes, L);
   if (rc) return rc;
+  if (is_mx(m)) {
+    // the router and the per-token routing of every format, then hx_moe_experts' path
+    Plan p;
+    make_plan(m, x, T, y, (uint8_t*)ws, L, bias, p);
+    if (fz) {
+      void* xn = (uint8_t*)ws + L.xn;
+      HX_HIP(launch_rmsnorm(fz->x, m->cfg.act_dtype == HX_BF16, T, m->cfg.hidden_size, fz->norm_w, fz->eps, xn, s));
+      p.ra.x = x = xn;
+    }
+    if ((rc = run_router(m, p, s))) return rc;
+    tm_ext(m, SLOT_ROUTE_TOKENS, s);
+    if (T <= HX_DECODE_MAX_T) launch_route_small(p.ra, s);
+    else if (route_mfma(m, p)) launch_route_mfma(p.ra, s);
+    else launch_route_tokens(p.ra, s);
+    tm_ext_done(m, SLOT_ROUTE_TOKENS);
+    HX_HIP(hipGetLastError());
+    return run_mx(m, x, T, p.ra.d.topk_idx, p.ra.topk_w, p.ra.has_shared ? p.ra.sgw : nullptr, y, fz ? fz->x : nullptr,
+                  (uint8_t*)ws, L, s);
+  }
   Plan p;
   make_plan(m, x, T, y, (uint8_t*)ws, L, bias, p);
   const bool decode = T <= HX_DECODE_MAX_T;
@@ -832,6 +939,25 @@ extern "C" int hx_moe_forward(hx_moe* m, const void* x, int64_t n_tokens, void* 
   if (n_tokens > HX_MAX_TOKENS) return fail(HX_ERR_UNSUPPORTED, "too many tokens in one call");
   HX_HIP(hipSetDevice(m->device));
   return forward_impl(m, x, n_tokens, y, workspace, workspace_bytes, router_bias, (hipStream_t)stream);
+}
+
+extern "C" int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const int32_t* topk_idx, const float* topk_w,
+                              const float* shared_w, void* y, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!m || n_tokens < 0 || (n_tokens > 0 && (!x || !y || !topk_idx || !topk_w)))
+    return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
+  if (!is_mx(m)) return fail(HX_ERR_UNSUPPORTED, "hx_moe_experts: the block's experts are not HX_MXFP4");
+  if (shared_w && m->cfg.shared_expert_intermediate_size == 0)
+    return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_experts: shared_w for a block without a shared expert");
+  if (n_tokens == 0) return HX_OK;
+  if (n_tokens > HX_MAX_TOKENS) return fail(HX_ERR_UNSUPPORTED, "too many tokens in one call");
+  HX_HIP(hipSetDevice(m->device));
+  hipStream_t s = (hipStream_t)stream;
+  if (!workspace && capturing(s))   // the handle's own may be freed by a later call, the graph would keep it
+    return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_experts: a captured call needs the caller's workspace");
+  WsLayout L;
+  int rc = get_ws(m, n_tokens, workspace, workspace_bytes, L);
+  if (rc) return rc;
+  return run_mx(m, x, n_tokens, topk_idx, topk_w, shared_w, y, nullptr, (uint8_t*)workspace, L, s);
 }
 
 extern "C" int hx_moe_forward_noalloc(hx_moe* m, const void* x, int64_t n_tokens, void* y,

@@ -1,0 +1,870 @@
+// Experts on MXFP4 weights: y[t] = sum_j w[t,j] D_e(silu(G_e x_t) * U_e x_t) with
+// e = idx[t,j], plus shared_w[t] times the shared expert's, for a routing the caller
+// has or hx_moe_forward's router makes.
+//
+// Both products run on v_mfma_scale_f32_32x32x64_f8f6f4 with the weights as its A
+// operand, their stored codes and scales untouched, and the activations as its B
+// operand, cut into E2M3 planes (hx_mx.h). D then holds a token's outputs in a
+// column: lane l token l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4 in register i, so
+// that lanes l and l + 32 hold the 32 features of one token that make one record of
+// the next product, or 64 bytes of its row.
+//
+// Up to MX_FEW_T tokens (k_mx_few_*): two kernels, a workgroup per expert and 32
+// features. More (k_mx_*): the tokens' records and the expert counts, the dispatch,
+// grouped products over tiles of tile_m rows, and the combine.
+#include "hx_mx.h"
+
+namespace hx {
+
+typedef int mx_v8i __attribute__((ext_vector_type(8)));
+typedef uint32_t mx_v6u __attribute__((ext_vector_type(6)));
+typedef float mx_v16f __attribute__((ext_vector_type(16)));
+typedef float mx_v32f __attribute__((ext_vector_type(32)));
+
+// ---------------------------------------------------------------- stored weights
+// MXFP4 rows -> the layout of hx_mx.h: a thread per lane of a tile, padding included
+__global__ __launch_bounds__(256) void k_repack_mx(const uint8_t* src, int64_t count, int rows, int K, uint8_t* dst,
+                                                   int64_t dst_stride) {
+  const int S = mx_steps(K), S4 = (S + 3) / 4, NB = K / 32;
+  const int64_t per = (int64_t)(rows / 32) * S4 * 4 * 64;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= per * count) return;
+  const int64_t m = id / per;
+  const int64_t q = id % per;
+  const int l = (int)(q & 63), s = (int)((q >> 6) % (S4 * 4)), n = (int)((q >> 6) / (S4 * 4));
+  const int row = 32 * n + (l & 31), kb = 2 * s + (l >> 5);
+  uint4 c = make_uint4(0u, 0u, 0u, 0u);
+  uint8_t e = 127;
+  if (kb < NB) {
+    const uint8_t* b = src + ((m * rows + row) * NB + kb) * 17;   // the caller's rows: any alignment
+    e = b[0];
+    uint32_t o[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      const uint32_t v = b[1 + j];
+      o[j >> 3] |= (v & 15u) << (4 * (j & 7));
+      o[2 + (j >> 3)] |= (v >> 4) << (4 * (j & 7));
+    }
+    c = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  uint8_t* mat = dst + m * dst_stride;
+  if (s < S) *(uint4*)(mat + (((int64_t)n * S + s) * 64 + l) * 16) = c;
+  mat[mx_code_bytes(rows, K) + (((int64_t)n * S4 + s / 4) * 64 + l) * 4 + (s & 3)] = e;
+}
+
+hipError_t launch_mx_repack(const void* src, int64_t count, int64_t rows, int64_t K, void* dst, int64_t dst_stride,
+                            hipStream_t s) {
+  const int64_t n = count * (rows / 32) * ((mx_steps((int)K) + 3) / 4) * 256;
+  hipLaunchKernelGGL(k_repack_mx, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (const uint8_t*)src, count,
+                     (int)rows, (int)K, (uint8_t*)dst, dst_stride);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- records
+template <int P>
+struct MxRec {
+  static constexpr int BYTES = P == 3 ? 80 : 128, VECS = BYTES / 16, SCALE = 6 * P;   // words: codes, then scales
+};
+
+// 32 values -> the words of their record
+template <int P>
+HX_DEV void mx_record(const float (&f)[32], uint4 (&out)[MxRec<P>::VECS]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i++) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  const int e = (int)(m >> 23);
+  const bool bad = e == 255;
+  // the first scale's exponent byte; at least 20, so that all planes' scales are
+  // normal: blocks below 2^-105 lose what is under 2^-128
+  const int sb = bad ? 127 : max(e - 2, 20);
+  uint32_t w[4 * MxRec<P>::VECS];
+#pragma unroll
+  for (int i = 0; i < 4 * MxRec<P>::VECS; i++) w[i] = 0;
+  mx_v16f ev, od;   // the conversion takes the even and the odd elements
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    ev[i] = bad ? 0.f : f[2 * i];
+    od[i] = bad ? 0.f : f[2 * i + 1];
+  }
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    const int b = sb - (p == 0 ? 0 : 5 * p - 2);
+    const float sc = __uint_as_float((uint32_t)b << 23);
+    const mx_v6u c = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, sc);
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[6 * p + i] = c[i];
+    if (p + 1 < P) {
+      const mx_v32f v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(c, sc);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        ev[i] -= v[2 * i];
+        od[i] -= v[2 * i + 1];
+      }
+    }
+    w[MxRec<P>::SCALE + p / 4] |= (uint32_t)(bad ? 255 : b) << (8 * (p & 3));
+  }
+#pragma unroll
+  for (int i = 0; i < MxRec<P>::VECS; i++) out[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+// the record of 32 zeros
+template <int P>
+HX_DEV void mx_zero_record(uint4 (&out)[MxRec<P>::VECS]) {
+#pragma unroll
+  for (int i = 0; i < MxRec<P>::VECS; i++) out[i] = make_uint4(0u, 0u, 0u, 0u);
+  ((uint32_t*)out)[MxRec<P>::SCALE] = 0x7f7f7f7fu;
+  if (P > 4) ((uint32_t*)out)[MxRec<P>::SCALE + 1] = 0x7f7f7f7fu;
+}
+
+// block kb of token row x (H columns) -> its record; blocks past the row are zeros
+template <int P>
+HX_DEV void mx_token_record(const void* x, int64_t t, int H, int kb, uint4 (&out)[MxRec<P>::VECS]) {
+  if (32 * kb >= H) {
+    mx_zero_record<P>(out);
+    return;
+  }
+  float f[32];
+  if constexpr (P == 3) {
+    const uint16_t* p = (const uint16_t*)x + t * H + 32 * kb;
+    if (((uintptr_t)p & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint4 v = ((const uint4*)p)[i];
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          f[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+          f[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) f[i] = bf16_to_f32(p[i]);
+    }
+  } else {
+    const float* p = (const float*)x + t * H + 32 * kb;
+    if (((uintptr_t)p & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float4 v = ((const float4*)p)[i];
+        f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) f[i] = p[i];
+    }
+  }
+  mx_record<P>(f, out);
+}
+
+// a record's words as MFMA operands
+template <int P>
+struct MxB {
+  uint32_t w[4 * MxRec<P>::VECS];
+  HX_DEV void set(int i, const uint4& v) {
+    w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+  }
+  HX_DEV void load(const uint8_t* p) {
+#pragma unroll
+    for (int i = 0; i < MxRec<P>::VECS; i++) set(i, *(const uint4*)(p + 16 * i));
+  }
+  HX_DEV void zero() {
+#pragma unroll
+    for (int i = 0; i < 4 * MxRec<P>::VECS; i++) w[i] = i >= MxRec<P>::SCALE ? 0x7f7f7f7fu : 0u;
+  }
+};
+
+// c += weights (one step's codes, their scale in byte SA of sa) x planes of b
+template <int P, int SA>
+HX_DEV mx_v16f mx_mfma(const uint4& a, uint32_t sa, const MxB<P>& b, mx_v16f c) {
+  const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+#define MX_PLANE(p)                                                                                               \
+  if constexpr (p < P) {                                                                                          \
+    const mx_v8i bv = {(int)b.w[6 * p], (int)b.w[6 * p + 1], (int)b.w[6 * p + 2], (int)b.w[6 * p + 3],            \
+                       (int)b.w[6 * p + 4], (int)b.w[6 * p + 5], 0, 0};                                           \
+    c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 2, SA, (int)sa, (p) & 3,                    \
+                                                        (int)b.w[MxRec<P>::SCALE + (p) / 4]);                     \
+  }
+  MX_PLANE(0) MX_PLANE(1) MX_PLANE(2) MX_PLANE(3) MX_PLANE(4)
+#undef MX_PLANE
+  return c;
+}
+
+HX_DEV mx_v16f mx_zero16() {
+  mx_v16f z;
+#pragma unroll
+  for (int i = 0; i < 16; i++) z[i] = 0.f;
+  return z;
+}
+
+// silu(g) u
+HX_DEV float mx_swiglu(float g, float u) { return siluf_(g) * u; }
+
+// ---------------------------------------------------------------- few tokens
+// The experts that some token chose, ascending, as bits in LDS (32 words).
+HX_DEV void mx_few_bits(const MxArgs& a, const int* sidx, uint32_t* bits) {
+  if (threadIdx.x < 32) bits[threadIdx.x] = 0u;
+  __syncthreads();
+  for (int f = threadIdx.x; f < a.F; f += blockDim.x) {
+    const int e = sidx[f];
+    if ((unsigned)e < (unsigned)a.E) atomicOr(&bits[e >> 5], 1u << (e & 31));
+  }
+  __syncthreads();
+}
+// their number, and (in every lane) the s-th of them, -1 if there are fewer
+HX_DEV int mx_few_slot(const uint32_t* bits, int s, int& n) {
+  const int l = lane_id();
+  const uint32_t w = l < 32 ? bits[l] : 0u;
+  int c = __popc(w), x = c;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int y = __shfl_up(x, off, 64);
+    if (l >= off) x += y;
+  }
+  n = __shfl(x, 31, 64);
+  const unsigned long long hit = __ballot(l < 32 && x - c <= s && s < x);
+  if (!hit) return -1;
+  const int L = __ffsll(hit) - 1;
+  const uint32_t word = (uint32_t)__shfl((int)w, L, 64);
+  const int r = s - __shfl(x - c, L, 64);
+  const unsigned long long b =
+      __ballot(l < 32 && ((word >> l) & 1u) && __popc(word & ((1u << l) - 1u)) == r);
+  return 32 * L + __ffsll(b) - 1;
+}
+
+// steps of K a wave of W takes: few and whole words of scales
+template <int W>
+HX_DEV int mx_wave_steps(int S) {
+  const int c = (S + W - 1) / W;
+  return c <= 1 ? 1 : c == 2 ? 2 : (c + 3) / 4 * 4;
+}
+
+// gate/up of up to 8 tokens: workgroup (32 features, slot); the 8 waves split K, the
+// tokens' records are made in LDS while the first weights are on their way.
+template <int P>
+__global__ __launch_bounds__(512) void k_mx_few_gate_up(MxArgs a) {
+  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
+  extern __shared__ __align__(16) uint8_t sm[];
+  __shared__ uint32_t bits[32];
+  __shared__ int sidx[MX_FEW_T * HX_MAX_TOPK];
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, T = a.T;
+  const int slot = blockIdx.y, fb = blockIdx.x;
+  int e;
+  if (T == 1) {   // a slot per entry
+    e = slot < a.k ? a.idx[slot] : a.E;
+    if (slot < a.k && (unsigned)e >= (unsigned)a.E) return;
+  } else {
+    for (int f = tid; f < a.F; f += 512) sidx[f] = a.idx[f];
+    __syncthreads();
+    mx_few_bits(a, sidx, bits);
+    int n;
+    e = mx_few_slot(bits, slot, n);
+    if (e < 0) {
+      if (slot > n || a.Is == 0) return;
+      e = a.E;
+    }
+    e = __builtin_amdgcn_readfirstlane(e);
+  }
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I;
+  if (fb >= mx_blocks(inter)) return;
+  const int S = mx_steps(a.H), S4 = (S + 3) / 4, HB = mx_blocks(a.H);
+  const int c = mx_wave_steps<8>(S), s0 = wave * c, s1 = min(S, s0 + c);
+  const bool pad = 32 * fb >= inter;   // a record behind the last feature
+  const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
+  const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
+  const int64_t at = ((int64_t)fb * S * 64 + lane) * 16;
+  const int64_t sat = mx_code_bytes(inter, a.H) + ((int64_t)fb * S4 * 64 + lane) * 4;
+  uint4 wg[4], wu[4];
+  uint32_t sg = 0, su = 0;
+  auto fetch = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int si = min(s + i, s1 - 1);
+      wg[i] = *(const uint4*)(gm + at + (int64_t)si * 1024);
+      wu[i] = *(const uint4*)(um + at + (int64_t)si * 1024);
+    }
+    sg = *(const uint32_t*)(gm + sat + (s >> 2) * 256) >> (8 * (s & 3));
+    su = *(const uint32_t*)(um + sat + (s >> 2) * 256) >> (8 * (s & 3));
+  };
+  if (s0 < s1 && !pad) fetch(s0);
+  for (int b = tid; b < T * HB; b += 512) {
+    const int t = b / HB, kb = b % HB;
+    uint4 r[RV];
+    mx_token_record<P>(a.x, t, a.H, kb, r);
+    uint4* o = (uint4*)(sm + (size_t)(kb * T + t) * RB);
+#pragma unroll
+    for (int i = 0; i < RV; i++) o[i] = r[i];
+  }
+  __syncthreads();
+  mx_v16f ag = mx_zero16(), au = mx_zero16();
+  const int t = lane & 31, half = lane >> 5;
+  if (!pad) {
+    for (int s = s0; s < s1; s += 4) {
+      if (s > s0) fetch(s);
+#define MX_STEP(i)                                                               \
+  if (s + i < s1) {                                                              \
+    MxB<P> b;                                                                    \
+    b.zero();                                                                    \
+    if (t < T) b.load(sm + (size_t)((2 * (s + i) + half) * T + t) * RB);         \
+    ag = mx_mfma<P, i>(wg[i], sg, b, ag);                                        \
+    au = mx_mfma<P, i>(wu[i], su, b, au);                                        \
+  }
+      MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+#undef MX_STEP
+    }
+  }
+  __syncthreads();   // the records have been read: their place takes the partial sums
+  float* red = (float*)sm;   // [wave][gate, up][feature][T]
+  if (t < T) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int f = 8 * (i >> 2) + 4 * half + (i & 3);
+      red[((wave * 2 + 0) * 32 + f) * T + t] = ag[i];
+      red[((wave * 2 + 1) * 32 + f) * T + t] = au[i];
+    }
+  }
+  __syncthreads();
+  float* hv = red + 8 * 2 * 32 * T;   // [T][33]
+  for (int o = tid; o < 32 * T; o += 512) {
+    float g = 0.f, u = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) {
+      g += red[(w * 2 + 0) * 32 * T + o];
+      u += red[(w * 2 + 1) * 32 * T + o];
+    }
+    hv[(o % T) * 33 + o / T] = mx_swiglu(g, u);
+  }
+  __syncthreads();
+  if (tid < T) {
+    // the row of h: the token's first entry with this expert
+    int row = sh ? a.F + tid : -1;
+    if (!sh && T == 1) row = slot;
+    else if (!sh)
+      for (int j = a.k - 1; j >= 0; j--)
+        if (sidx[tid * a.k + j] == e) row = tid * a.k + j;
+    if (row >= 0) {
+      uint4 r[RV];
+      if (pad) {
+        mx_zero_record<P>(r);
+      } else {
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) f[i] = hv[tid * 33 + i];
+        mx_record<P>(f, r);
+      }
+      uint4* o = (uint4*)(a.hrec + ((int64_t)row * a.hblocks + fb) * RB);
+#pragma unroll
+      for (int i = 0; i < RV; i++) o[i] = r[i];
+    }
+  }
+}
+
+// bytes of LDS of k_mx_few_gate_up
+static size_t mx_few_lds(int T, int H, bool xbf) {
+  const size_t rec = (size_t)T * mx_blocks(H) * mx_rec_bytes(xbf), red = (size_t)(8 * 2 * 32 * T + 33 * T) * 4;
+  return rec > red ? rec : red;
+}
+
+bool mx_few(int T, int k, int H, bool xbf) { return T <= MX_FEW_T && mx_few_lds(T, H, xbf) <= 60 * 1024; }
+
+// down and combine of up to 8 tokens: workgroup per 32 outputs; its 16 waves take the
+// (slot, 4 steps) units in turn, weigh each unit's product per token and sum in LDS.
+template <int P>
+__global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
+  constexpr int RB = MxRec<P>::BYTES;
+  __shared__ uint32_t bits[32];
+  __shared__ int sidx[MX_FEW_T * HX_MAX_TOPK];
+  __shared__ float sw[MX_FEW_T * HX_MAX_TOPK];
+  __shared__ float red[16 * 32 * MX_FEW_T];
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, T = a.T, k = a.k;
+  const int nb = blockIdx.x;
+  for (int f = tid; f < a.F; f += 1024) {
+    sidx[f] = a.idx[f];
+    sw[f] = a.w[f];
+  }
+  int n = k;
+  __syncthreads();
+  if (T > 1) mx_few_bits(a, sidx, bits);
+  if (T > 1) mx_few_slot(bits, 0, n);
+  const int S = mx_steps(a.I), G = (S + 3) / 4, Ss = mx_steps(a.Is), Gs = a.Is ? (Ss + 3) / 4 : 0;
+  const int t = lane & 31, half = lane >> 5;
+  mx_v16f acc = mx_zero16();
+  for (int u = wave; u < n * G + Gs; u += 16) {
+    const bool sh = u >= n * G;
+    const int slot = sh ? n : u / G, g = sh ? u - n * G : u % G;
+    int e = a.E, row = -1;
+    float wt = 0.f;
+    if (sh) {
+      if (t < T) {
+        row = a.F + t;
+        wt = a.shared_w[t];
+      }
+    } else if (T == 1) {
+      e = sidx[slot];
+      if ((unsigned)e >= (unsigned)a.E) continue;
+      if (t == 0) {
+        row = slot;
+        wt = sw[slot];
+      }
+    } else {
+      int dummy;
+      e = mx_few_slot(bits, slot, dummy);
+      if (t < T) {
+        for (int j = k - 1; j >= 0; j--)
+          if (sidx[t * k + j] == e) {
+            row = t * k + j;
+            wt += sw[t * k + j];
+          }
+      }
+    }
+    e = __builtin_amdgcn_readfirstlane(e);
+    const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
+    const int inter = sh ? a.Is : a.I, St = sh ? Ss : S, S4 = (St + 3) / 4, s = 4 * g;
+    const uint8_t* wp = dm + (((int64_t)nb * St + s) * 64 + lane) * 16;
+    const uint32_t sa = *(const uint32_t*)(dm + mx_code_bytes(a.H, inter) + (((int64_t)nb * S4 + g) * 64 + lane) * 4);
+    uint4 wd[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) wd[i] = *(const uint4*)(wp + (int64_t)min(i, St - 1 - s) * 1024);
+    const uint8_t* hp = a.hrec + ((int64_t)max(row, 0) * a.hblocks + 2 * s + half) * RB;
+    mx_v16f d = mx_zero16();
+#define MX_STEP(i)                                    \
+  if (s + i < St) {                                   \
+    MxB<P> b;                                         \
+    b.zero();                                         \
+    if (row >= 0) b.load(hp + 2 * i * RB);            \
+    d = mx_mfma<P, i>(wd[i], sa, b, d);               \
+  }
+    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+#undef MX_STEP
+    // a token that is not this expert's adds nothing, whatever the weights hold
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[i] = row >= 0 ? __builtin_fmaf(wt, d[i], acc[i]) : acc[i];
+  }
+  if (t < T) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) red[wave * 32 * T + (8 * (i >> 2) + 4 * half + (i & 3)) * T + t] = acc[i];
+  }
+  __syncthreads();
+  for (int o = tid; o < 32 * T; o += 1024) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; w++) y += red[w * 32 * T + o];
+    const int64_t at = (int64_t)(o % T) * a.H + 32 * nb + o / T;
+    if constexpr (P == 3) {
+      uint16_t* p = (uint16_t*)(a.resid ? a.resid : a.y) + at;
+      const uint16_t b = f32_to_bf16(y);
+      *p = a.resid ? f32_to_bf16(bf16_to_f32(*p) + bf16_to_f32(b)) : b;
+    } else {
+      float* p = (float*)(a.resid ? a.resid : a.y) + at;
+      *p = a.resid ? *p + y : y;
+    }
+  }
+}
+
+hipError_t launch_mx_few_gate_up(const MxArgs& a, hipStream_t s) {
+  const int slots = (a.T == 1 ? a.k : min(a.F, a.E)) + (a.Is > 0 ? 1 : 0);
+  const dim3 g(a.hblocks, slots);
+  const uint32_t lds = (uint32_t)mx_few_lds(a.T, a.H, a.xbf);
+  if (a.xbf) hx_launch(k_mx_few_gate_up<3>, g, dim3(512), lds, s, a);
+  else hx_launch(k_mx_few_gate_up<5>, g, dim3(512), lds, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s) {
+  if (a.xbf) hx_launch(k_mx_few_down<3>, dim3(a.H / 32), dim3(1024), 0, s, a);
+  else hx_launch(k_mx_few_down<5>, dim3(a.H / 32), dim3(1024), 0, s, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- dispatch
+// workgroups 0 .. chunks - 1: the chunk's entries by expert; the others: the tokens' records
+template <int P>
+__global__ __launch_bounds__(256) void k_mx_prep(MxArgs a) {
+  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
+  __shared__ int cnt[HX_MAX_EXPERTS];
+  const int nch = mx_chunks(a.F), tid = threadIdx.x;
+  if ((int)blockIdx.x < nch) {
+    for (int e = tid; e < a.E; e += 256) cnt[e] = 0;
+    __syncthreads();
+    const int per = mx_chunk(a.F), f0 = blockIdx.x * per, f1 = min(a.F, f0 + per);
+    for (int f = f0 + tid; f < f1; f += 256) {
+      const int e = a.idx[f];
+      if ((unsigned)e < (unsigned)a.E) atomicAdd(&cnt[e], 1);
+    }
+    __syncthreads();
+    for (int e = tid; e < a.E; e += 256) a.hist[(int64_t)blockIdx.x * a.E + e] = cnt[e];
+    return;
+  }
+  const int HB = mx_blocks(a.H);
+  const int64_t b = (int64_t)(blockIdx.x - nch) * 256 + tid;
+  if (b >= (int64_t)a.T * HB) return;
+  uint4 r[RV];
+  mx_token_record<P>(a.x, b / HB, a.H, (int)(b % HB), r);
+  uint4* o = (uint4*)(a.xrec + b * RB);
+#pragma unroll
+  for (int i = 0; i < RV; i++) o[i] = r[i];
+}
+
+// Positions of the entries by expert and the tiles. Every workgroup sums the chunks'
+// counts itself (thread e expert e's), scans them, and places its own chunk's entries
+// by LDS counters. Their order among an expert's rows is free: a row's results do not
+// depend on its place in a tile, and the combine sums a token's entries in their order.
+__global__ __launch_bounds__(1024) void k_mx_dispatch(MxArgs a) {
+  __shared__ int s_base[HX_MAX_EXPERTS], s_off[HX_MAX_EXPERTS], s_cnt[HX_MAX_EXPERTS], s_first[HX_MAX_EXPERTS];
+  __shared__ int sh[2][17];
+  const int e = threadIdx.x, lane = lane_id(), wave = e >> 6, nch = mx_chunks(a.F), c = blockIdx.x;
+  int count = 0, pre = 0;
+  if (e < a.E) {
+    for (int c0 = 0; c0 < nch; c0 += 8) {
+      int h[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) h[i] = c0 + i < nch ? a.hist[(int64_t)(c0 + i) * a.E + e] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (c0 + i == c) pre = count;
+        count += h[i];
+      }
+    }
+  }
+  const int nt = (count + a.tile_m - 1) / a.tile_m;
+  int x0 = count, x1 = nt;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y0 = __shfl_up(x0, off, 64), y1 = __shfl_up(x1, off, 64);
+    if (lane >= off) {
+      x0 += y0;
+      x1 += y1;
+    }
+  }
+  if (lane == 63) {
+    sh[0][wave] = x0;
+    sh[1][wave] = x1;
+  }
+  __syncthreads();
+  if (e < 2) {
+    int run = 0;
+    for (int w = 0; w < 16; w++) {
+      const int v = sh[e][w];
+      sh[e][w] = run;
+      run += v;
+    }
+    sh[e][16] = run;
+  }
+  __syncthreads();
+  const int off = sh[0][wave] + x0 - count, first = sh[1][wave] + x1 - nt, total = sh[1][16];
+  if (e < a.E) {
+    s_base[e] = off + pre;
+    s_off[e] = off;
+    s_cnt[e] = count;
+    s_first[e] = first;
+  }
+  __syncthreads();
+  const int per = mx_chunk(a.F), f0 = c * per, f1 = min(a.F, f0 + per);
+  for (int f = f0 + e; f < f1; f += 1024) {
+    const int x = a.idx[f];
+    int pos = -1;
+    if ((unsigned)x < (unsigned)a.E) {
+      pos = atomicAdd(&s_base[x], 1);
+      a.perm[pos] = f;
+    }
+    a.inv[f] = pos;
+  }
+  if (c != 0) return;
+  for (int i = e; i < total; i += 1024) {
+    int lo = 0, hi = a.E - 1;   // the largest expert with s_first <= i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_first[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    const int m0 = (i - s_first[lo]) * a.tile_m;
+    ((int4*)a.tiles)[i] = make_int4(lo, s_off[lo] + m0, min(a.tile_m, s_cnt[lo] - m0), 0);
+  }
+  const int nst = a.Is > 0 ? (a.T + a.tile_m - 1) / a.tile_m : 0;
+  for (int i = e; i < nst; i += 1024) {
+    const int m0 = i * a.tile_m;
+    ((int4*)a.tiles)[total + i] = make_int4(a.E, a.F + m0, min(a.tile_m, a.T - m0), 0);
+  }
+  if (e == 0) a.counts[0] = total + nst;
+}
+
+hipError_t launch_mx_prep(const MxArgs& a, hipStream_t s) {
+  const int64_t n = ((int64_t)a.T * mx_blocks(a.H) + 255) / 256 + mx_chunks(a.F);
+  if (a.xbf) hx_launch(k_mx_prep<3>, dim3((unsigned)n), dim3(256), 0, s, a);
+  else hx_launch(k_mx_prep<5>, dim3((unsigned)n), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s) {
+  hx_launch(k_mx_dispatch, dim3(mx_chunks(a.F)), dim3(1024), 0, s, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- grouped products
+// rows of a tile: 32 when the experts have few rows each
+int mx_tile_m(int64_t F, int E) { return F <= 24 * (int64_t)E ? 32 : 64; }
+
+// LDS of a stage: [4 blocks][TM rows][record]; the stage's records come in by direct
+// loads, 16 bytes a lane, in LDS order
+template <int TM, int P>
+struct MxStage {
+  static constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
+  static constexpr int BYTES = 4 * TM * RB, LOADS = BYTES / 1024, PER = (LOADS + 3) / 4;   // loads: in all, a wave
+  const uint8_t* src[PER];
+  // rowptr(r): the records of the tile's row r
+  template <typename F>
+  HX_DEV void init(int wave, int lane, F rowptr) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int q = (wave + 4 * i) * 64 + lane;   // 16-byte piece of the stage
+      const int kb = min(q / (TM * RV), 3), r = q / RV % TM, j = q % RV;
+      src[i] = rowptr(r) + kb * RB + 16 * j;
+    }
+  }
+  HX_DEV void issue(int wave, int st, uint32_t lds) const {
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (wave + 4 * i < LOADS) dma16(src[i] + (int64_t)st * (4 * RB), lds + (wave + 4 * i) * 1024);
+  }
+};
+
+// workgroup -> (feature group, tile): the NX workgroups of a tile on one XCD
+HX_DEV void mx_tile(int NX, int& nt, int& tile) {
+  const int L = blockIdx.x;
+  nt = (L >> 3) % NX;
+  tile = L / (8 * NX) * 8 + (L & 7);
+}
+
+// the 4 waves' sums over K: NM weight matrices' 32-row tiles (one each) times the
+// tile's rows
+template <int TM, int P, int NM>
+HX_DEV void mx_products(const MxStage<TM, P>& sg, uint8_t* buf, int nst, const uint8_t* const (&codes)[NM],
+                        const uint8_t* const (&scales)[NM], bool live, mx_v16f (&acc)[NM][TM / 32]) {
+  constexpr int RB = MxRec<P>::BYTES;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
+  uint4 w[2][NM][2];
+  uint32_t sc[2][NM];
+  auto fetch = [&](int st, int b) {
+#pragma unroll
+    for (int m = 0; m < NM; m++) {
+      w[b][m][0] = *(const uint4*)(codes[m] + (int64_t)st * 2048);
+      w[b][m][1] = *(const uint4*)(codes[m] + (int64_t)st * 2048 + 1024);
+      sc[b][m] = *(const uint32_t*)(scales[m] + (st >> 1) * 256) >> (16 * (st & 1));
+    }
+  };
+  sg.issue(wave, 0, lds);
+  if (live) fetch(0, 0);
+  auto stage = [&](int st, int b) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (st + 1 < nst) {
+      sg.issue(wave, st + 1, lds + (b ^ 1) * MxStage<TM, P>::BYTES);
+      if (live) fetch(st + 1, b ^ 1);
+    }
+    if (live) {
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int n = 0; n < TM / 32; n++) {
+          MxB<P> bb;
+          bb.load(buf + b * MxStage<TM, P>::BYTES + ((2 * s + (lane >> 5)) * TM + 32 * n + (lane & 31)) * RB);
+#pragma unroll
+          for (int m = 0; m < NM; m++)
+            acc[m][n] = s == 0 ? mx_mfma<P, 0>(w[b][m][0], sc[b][m], bb, acc[m][n])
+                               : mx_mfma<P, 1>(w[b][m][1], sc[b][m], bb, acc[m][n]);
+        }
+    }
+  };
+  int st = 0;
+  for (; st + 2 <= nst; st += 2) {
+    stage(st, 0);
+    stage(st + 1, 1);
+  }
+  if (st < nst) stage(st, 0);
+}
+
+// lane l: the 32 values of column l of the tile from D's halves
+template <int TM>
+HX_DEV void mx_columns(const mx_v16f (&d)[TM / 32], float (&f)[32]) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(d[0][i]), __float_as_uint(d[TM / 32 - 1][i]), false, false);
+    const int o = 8 * (i >> 2) + (i & 3);
+    f[o] = __uint_as_float(r[0]);
+    f[o + 4] = __uint_as_float(r[1]);
+  }
+}
+
+template <int TM, int P>
+__global__ __launch_bounds__(256) void k_mx_gate_up(MxArgs a) {
+  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
+  __shared__ __align__(16) uint8_t buf[2 * MxStage<TM, P>::BYTES];
+  int nt, tile;
+  mx_tile(a.hblocks / 4, nt, tile);
+  if (tile >= a.counts[0]) return;
+  const int4 ti = ((const int4*)a.tiles)[tile];
+  const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I;
+  if (4 * nt >= mx_blocks(inter)) return;
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fb = 4 * nt + wave, HB = mx_blocks(a.H), S = mx_steps(a.H), S4 = (S + 3) / 4;
+  const bool live = 32 * fb < inter;
+  MxStage<TM, P> sg;
+  sg.init(wave, lane, [&](int r) {
+    const int p = p0 + min(r, rows - 1);
+    const int t = sh ? p - a.F : a.perm[p] / a.k;
+    return a.xrec + (int64_t)t * HB * RB;
+  });
+  const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
+  const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
+  const int64_t at = ((int64_t)fb * S * 64 + lane) * 16;
+  const int64_t sat = mx_code_bytes(inter, a.H) + ((int64_t)fb * S4 * 64 + lane) * 4;
+  const uint8_t* const codes[2] = {gm + at, um + at};
+  const uint8_t* const scales[2] = {gm + sat, um + sat};
+  mx_v16f acc[2][TM / 32];
+#pragma unroll
+  for (int n = 0; n < TM / 32; n++) acc[0][n] = acc[1][n] = mx_zero16();
+  mx_products<TM, P, 2>(sg, buf, HB / 4, codes, scales, live, acc);
+  mx_v16f h[TM / 32];
+#pragma unroll
+  for (int n = 0; n < TM / 32; n++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) h[n][i] = mx_swiglu(acc[0][n][i], acc[1][n][i]);
+  float f[32];
+  mx_columns<TM>(h, f);
+  uint4 r[RV];
+  if (live) mx_record<P>(f, r);
+  else mx_zero_record<P>(r);
+  if (lane < rows && lane < TM) {
+    uint4* o = (uint4*)(a.hrec + ((int64_t)(p0 + lane) * a.hblocks + fb) * RB);
+#pragma unroll
+    for (int i = 0; i < RV; i++) o[i] = r[i];
+  }
+}
+
+// outputs of the experts, unweighted: 64 features a wave
+template <int TM, int P>
+__global__ __launch_bounds__(256) void k_mx_down(MxArgs a) {
+  constexpr int RB = MxRec<P>::BYTES;
+  __shared__ __align__(16) uint8_t buf[2 * MxStage<TM, P>::BYTES];
+  int nt, tile;
+  mx_tile((a.H + 255) / 256, nt, tile);
+  if (tile >= a.counts[0]) return;
+  const int4 ti = ((const int4*)a.tiles)[tile];
+  const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I;
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int S = mx_steps(inter), S4 = (S + 3) / 4, nb = a.H / 32;
+  const int n0 = 8 * nt + 2 * wave;
+  const bool live = n0 < nb;
+  MxStage<TM, P> sg;
+  sg.init(wave, lane, [&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * RB; });
+  const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
+  const uint8_t *codes[2], *scales[2];
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    const int n = min(n0 + m, nb - 1);
+    codes[m] = dm + ((int64_t)n * S * 64 + lane) * 16;
+    scales[m] = dm + mx_code_bytes(a.H, inter) + ((int64_t)n * S4 * 64 + lane) * 4;
+  }
+  const uint8_t* const cc[2] = {codes[0], codes[1]};
+  const uint8_t* const ss[2] = {scales[0], scales[1]};
+  mx_v16f acc[2][TM / 32];
+#pragma unroll
+  for (int n = 0; n < TM / 32; n++) acc[0][n] = acc[1][n] = mx_zero16();
+  mx_products<TM, P, 2>(sg, buf, mx_blocks(inter) / 4, cc, ss, live, acc);
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    float f[32];
+    mx_columns<TM>(acc[m], f);
+    if (lane < TM && lane < rows && n0 + m < nb) {
+      const int64_t at = (int64_t)(p0 + lane) * a.H + 32 * (n0 + m);
+      if constexpr (P == 3) {
+        uint4* o = (uint4*)((uint16_t*)a.obuf + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t q[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            q[j] = f32_to_bf16(f[8 * i + 2 * j]) | ((uint32_t)f32_to_bf16(f[8 * i + 2 * j + 1]) << 16);
+          o[i] = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+      } else {
+        float4* o = (float4*)((float*)a.obuf + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+      }
+    }
+  }
+}
+
+#define MX_LAUNCH(KERNEL, NX)                                                              \
+  const dim3 g((unsigned)((NX) * (((int64_t)a.max_tiles + 7) / 8 * 8)));                   \
+  if (a.xbf && a.tile_m == 32) hx_launch(KERNEL<32, 3>, g, dim3(256), 0, s, a);            \
+  else if (a.xbf) hx_launch(KERNEL<64, 3>, g, dim3(256), 0, s, a);                         \
+  else if (a.tile_m == 32) hx_launch(KERNEL<32, 5>, g, dim3(256), 0, s, a);                \
+  else hx_launch(KERNEL<64, 5>, g, dim3(256), 0, s, a);                                    \
+  return hipGetLastError()
+
+hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_gate_up, a.hblocks / 4); }
+hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_down, (a.H + 255) / 256); }
+
+// y[t] = the token's entries' rows times their weights in their order, then the
+// shared expert's: 8 outputs a thread
+template <bool BF>
+__global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
+  const int t = blockIdx.x, n0 = (blockIdx.y * 256 + (int)threadIdx.x) * 8;
+  if (n0 >= a.H) return;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) acc[i] = 0.f;
+  auto add = [&](int64_t row, float w) {
+    float v[8];
+    if constexpr (BF) {
+      const uint4 q = *(const uint4*)((const uint16_t*)a.obuf + row * a.H + n0);
+      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    } else {
+      const float4* q = (const float4*)((const float*)a.obuf + row * a.H + n0);
+      const float4 x = q[0], y = q[1];
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+  };
+  for (int j = 0; j < a.k; j++) {
+    const int p = a.inv[(int64_t)t * a.k + j];
+    if (p >= 0) add(p, a.w[(int64_t)t * a.k + j]);
+  }
+  if (a.Is > 0) add((int64_t)a.F + t, a.shared_w[t]);
+  const int64_t at = (int64_t)t * a.H + n0;
+  if constexpr (BF) {
+    uint16_t* p = (uint16_t*)(a.resid ? a.resid : a.y) + at;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint16_t b = f32_to_bf16(acc[i]);
+      p[i] = a.resid ? f32_to_bf16(bf16_to_f32(p[i]) + bf16_to_f32(b)) : b;
+    }
+  } else {
+    float* p = (float*)(a.resid ? a.resid : a.y) + at;
+#pragma unroll
+    for (int i = 0; i < 8; i++) p[i] = a.resid ? p[i] + acc[i] : acc[i];
+  }
+}
+
+hipError_t launch_mx_combine(const MxArgs& a, hipStream_t s) {
+  const dim3 g(a.T, (a.H + 2047) / 2048);
+  if (a.xbf) hx_launch(k_mx_combine<true>, g, dim3(256), 0, s, a);
+  else hx_launch(k_mx_combine<false>, g, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace hx

@@ -6,6 +6,7 @@ Names follow the reference so callers and tests read like neuron's own:
     Qwen3_5MoeBlock      crates/neuron/src/harness/arch/qwen3_5/moe.rs:39-199
       .load(cfg, weights)      moe.rs:55 (validation moe.rs:56-69)
       .forward(xs)             moe.rs:164-199, input (b, l, hidden), same shape/dtype out
+      .experts(xs, idx, w)     the same with a routing of the caller's (MXFP4 experts)
       .route(xs)               route_scatter moe.rs:124-162 + the dispatch sort of
                                tp_qwen3_5.rs:1189
     quantize                   isq.rs:39-55 (on the device)
@@ -34,7 +35,7 @@ STATUS = {0: "HX_OK", 1: "HX_ERR_INVALID_ARGUMENT", 2: "HX_ERR_UNSUPPORTED", 3: 
 
 # every entry point include/hx_moe.h declares
 EXPORTS = ("hx_moe_create", "hx_moe_destroy", "hx_moe_workspace_size", "hx_moe_forward", "hx_moe_forward_noalloc",
-           "hx_moe_forward_host",
+           "hx_moe_forward_host", "hx_moe_experts",
            "hx_moe_route", "hx_moe_router_logits", "hx_moe_decoder_mlp", "hx_quantize", "hx_dequantize",
            "hx_row_bytes", "hx_quantize_activations", "hx_moe_timing_begin", "hx_moe_timing_read", "hx_moe_timing_end",
            "hx_moe_timing_name", "hx_last_error")
@@ -82,6 +83,7 @@ def lib() -> C.CDLL:
             "hx_moe_forward": (i32, [vp, vp, i64, vp, vp, C.c_size_t, vp, vp]),
             "hx_moe_forward_noalloc": (i32, [vp, vp, i64, vp, vp, vp]),
             "hx_moe_forward_host": (i32, [vp, vp, i64, vp, vp]),
+            "hx_moe_experts": (i32, [vp, vp, i64, vp, vp, vp, vp, vp, C.c_size_t, vp]),
             "hx_moe_route": (i32, [vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]),
             "hx_moe_router_logits": (i32, [vp, vp, i64, vp, vp, vp]),
             "hx_moe_decoder_mlp": (i32, [vp, vp, i64, vp, C.c_float, vp, C.c_size_t, vp]),
@@ -283,6 +285,41 @@ class Qwen3_5MoeBlock:
         T = xs.numel() // self.cfg.hidden_size
         check(lib().hx_moe_forward_noalloc(self._h, _ptr(xs), T, _ptr(out), _ptr(router_bias), _stream(stream)),
               "hx_moe_forward_noalloc")
+        return out
+
+    def experts(self, xs, topk_idx, topk_w, shared_w=None, workspace=None, stream=None, out=None):
+        """The experts' part of forward() with the caller's routing, on a block of
+        MXFP4 experts: xs (b, l, hidden) or (T, hidden), topk_idx int32 and topk_w
+        float32 with last dim k (indices outside 0 .. E - 1 are no expert), shared_w
+        float32 of one value a token, or None for a call without the shared expert
+        -> same shape as xs. `out` as in forward(). A call on another stream than the
+        current one takes contiguous tensors only."""
+        import torch
+        H, k = self.cfg.hidden_size, self.cfg.num_experts_per_tok
+        _check_acts(xs, H, self.act_dtype)
+        if not xs.is_contiguous() and stream is not None:
+            raise ValueError("xs must be contiguous on a stream of its own")
+        x = xs.contiguous()
+        T = x.numel() // H
+        if x.device.index != self.device:
+            raise ValueError(f"xs is on {x.device}, the block on cuda:{self.device}")
+        for t, dt, n, what in ((topk_idx, torch.int32, T * k, "topk_idx"), (topk_w, torch.float32, T * k, "topk_w"),
+                               (shared_w, torch.float32, T, "shared_w")):
+            if t is None and what == "shared_w":
+                continue
+            if t.dtype != dt or t.numel() != n or not t.is_contiguous() or t.device != x.device or \
+                    (what != "shared_w" and t.shape[-1] != k):
+                raise ValueError(f"{what} must be a contiguous {dt} tensor of {n} values on {x.device}"
+                                 + (f" with last dim {k}" if what != "shared_w" else ""))
+        if out is None:
+            out = torch.empty_like(x)
+            if stream is not None:
+                out.record_stream(stream)
+        elif out.shape != xs.shape or out.dtype != x.dtype or not out.is_contiguous() or out.device != x.device:
+            raise ValueError("out must be contiguous with the input's shape, dtype and device")
+        ws_ptr, ws_n = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
+        check(lib().hx_moe_experts(self._h, _ptr(x), T, _ptr(topk_idx), _ptr(topk_w), _ptr(shared_w), _ptr(out), ws_ptr,
+                                   ws_n, _stream(stream)), "hx_moe_experts")
         return out
 
     def route(self, xs, router_bias=None, stream=None):

@@ -123,7 +123,27 @@ int hx_moe_forward(hx_moe* m, const void* x, int64_t n_tokens, void* y,
 int hx_moe_forward_noalloc(hx_moe* m, const void* x, int64_t n_tokens, void* y, const float* router_bias,
                            void* stream);
 
-/* Same, for host buffers (what a candle CPU-tensor wrapper calls): copies x in,
+/* No counterpart in the reference: the experts' part of hx_moe_forward for a caller
+ * that has the routing (its own router, a routing shared by several calls, tokens
+ * sent here by another device), on a block whose expert projections are HX_MXFP4
+ * (others: HX_ERR_UNSUPPORTED):
+ *   y[t] = sum_j topk_w[t, j] * expert[topk_idx[t, j]](x[t]) + shared_w[t] * shared_expert(x[t])
+ * topk_idx int32 and topk_w f32 are device [n_tokens, k], k the block's
+ * num_experts_per_tok. An index outside 0 .. E - 1 is no expert: the entry adds
+ * nothing, its weight is not read into the sum, and a token of such entries alone
+ * gets its shared expert's part, or zeros (padding). The same index twice in a token
+ * counts twice. shared_w is device f32 [n_tokens], or NULL for a call without the
+ * shared expert. Products are of the stored weights and the activations to 13 bits
+ * below each 32-wide block's largest (act HX_F32: 23), sums in f32; h = silu(g) u is
+ * taken to the same bits; above the few tokens of a decode step each expert's
+ * output is rounded to act_dtype before the weighted sum (f32). A token that holds a
+ * NaN or an infinity (or whose h does) gets NaN in place of what it reaches. The
+ * result of a token does not depend on the others in the call. y may be x. workspace
+ * as in hx_moe_forward, 16-byte aligned; a call under stream capture must bring it. */
+int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const int32_t* topk_idx, const float* topk_w,
+                   const float* shared_w, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* hx_moe_forward for host buffers (what a candle CPU-tensor wrapper calls): copies x in,
  * runs hx_moe_forward on the default stream, copies y out, synchronises. */
 int hx_moe_forward_host(hx_moe* m, const void* x_host, int64_t n_tokens, void* y_host,
                         const float* router_bias_host);

@@ -43,3 +43,37 @@ def test_numpy_rules():
     assert q[1, 0] == 0 and q[2, 0] == 127 + 125 and q[3, 0] == 255 and not q[3, 1:].any()
     assert np.isnan(M.values(q[3])).all()
     assert M.values(q[0])[0] == 4.0 and M.values(q[0])[15] == -6.0
+
+
+def _create(**kw):
+    """hx_moe_create with pointers that no check reads"""
+    import helexa_amd.moe as hx
+    c = hx.HxConfig(64, 4, 2, 32, kw.pop("shared", 0), 1, hx.BF16)
+    w = hx.HxWeights()
+    d = dict(location=0, router_dtype=hx.BF16, gate_dtype=hx.MXFP4, up_dtype=hx.MXFP4, down_dtype=hx.MXFP4,
+             router=4096, experts_gate=4096, experts_up=4096, experts_down=4096)
+    for n in ("hidden_size", "moe_intermediate_size"):
+        if n in kw:
+            setattr(c, n, kw.pop(n))
+    for n, v in {**d, **kw}.items():
+        setattr(w, n, v)
+    out = C.c_void_p()
+    rc = hx.lib().hx_moe_create(C.byref(c), C.byref(w), 0, C.byref(out))
+    return rc, hx.last_error()
+
+
+@pytest.mark.parametrize("kw,rc,what", [
+    (dict(down_dtype=8), 2, "all of gate_proj"), (dict(gate_dtype=12, up_dtype=12, hidden_size=256), 2, "all of gate_proj"),
+    (dict(up_dtype=8), 2, "share a dtype"), (dict(hidden_size=80), 1, "does not tile"),
+    (dict(moe_intermediate_size=48), 1, "does not tile"), (dict(hidden_size=32 * 513), 2, "at most"),
+    (dict(shared=32, shared_gate_dtype=8, shared_up_dtype=39, shared_down_dtype=39), 2, "routed experts"),
+    (dict(gate_dtype=40, up_dtype=40), 2, "unsupported storage dtype")])
+def test_blocks_that_are_refused(kw, rc, what):
+    got, msg = _create(**kw)
+    assert got == rc and what in msg, (got, msg)
+
+
+def test_experts_refuses_bad_arguments():
+    import helexa_amd as hx
+    p = C.c_void_p(4096)
+    assert hx.lib().hx_moe_experts(None, p, 1, p, p, None, p, None, 0, None) == 1
