@@ -90,11 +90,16 @@ HX_DEV void mx_record(const float (&f)[32], uint4 (&out)[MxRec<P>::VECS]) {
   for (int p = 0; p < P; p++) {
     const int b = sb - (p == 0 ? 0 : 5 * p - 2);
     const float sc = __uint_as_float((uint32_t)b << 23);
-    const mx_v6u c = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, sc);
+    mx_v6u c = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, sc);
+    // these conversions write their first results before they have read all their
+    // sources, and the compiler may give both the same registers: the sources are
+    // kept alive past them
+    asm volatile("" : "+v"(c) : "v"(ev), "v"(od), "v"(sc));
 #pragma unroll
     for (int i = 0; i < 6; i++) w[6 * p + i] = c[i];
     if (p + 1 < P) {
-      const mx_v32f v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(c, sc);
+      mx_v32f v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(c, sc);
+      asm volatile("" : "+v"(v) : "v"(c), "v"(sc));
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         ev[i] -= v[2 * i];

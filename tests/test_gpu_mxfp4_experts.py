@@ -287,3 +287,36 @@ def test_python_refusals():
     other = hx.Qwen3_5MoeBlock.load(cfg, dict(router=f(E, H), gate=f(E, I, H), up=f(E, I, H), down=f(E, H, I)), act_dtype=hx.F32)
     with pytest.raises(hx.HxError, match="HX_MXFP4"):
         other.experts(a.float(), i, v)
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("T", [1, 8, 9, 70])
+def test_each_plane_of_a_record_counts(T, act):
+    """Tokens whose blocks hold one large value, at a column of zero weights, next to
+    values that only the record's second, third (.. fifth) plane can hold, exactly: the
+    block's scale is 1, the planes step by 2^-3, 2^-6, 2^-11, 2^-16, 2^-21. The outputs then are
+    within the roundings of the sums and of h and the result alone."""
+    H, E, k, I = 256, 3, 1, 64
+    rows, _ = M.block(31, H, E, I, 0)
+    for n in ("gate", "up"):
+        b = rows[n].reshape(E, I, H // 32, 17)
+        b[..., 1] &= 0xF0            # column 0 of each block
+        b[..., 0] = 127
+    vals = {n: M.values(r) for n, r in rows.items()}
+    blk = M.load(rows, H, E, k, I, 0, act)
+    rng = np.random.default_rng(T)
+    # plane p: whole multiples of twice its step, below half of the step of the plane before
+    for step, top in ([(2.0 ** -5, 2.0 ** -4), (2.0 ** -10, 2.0 ** -7)] +
+                      ([(2.0 ** -15, 2.0 ** -12), (2.0 ** -20, 2.0 ** -17)] if act == F32 else [])):
+        n = int(top / step)
+        x = (rng.integers(-n + 1, n, (T, H)) * step if n > 2 else rng.choice([-1, 0, 1], (T, H)) * step).astype(np.float32)
+        x[:, ::32] = 4.0
+        idx = rng.integers(0, E, (T, k)).astype(np.int32)
+        w = np.ones((T, k), np.float32)
+        xs = x.copy()
+        xs[:, ::32] = 0.0            # what the products see
+        y = blk.experts(cuda(x, act), cuda(idx), cuda(w)).float().cpu().numpy().astype(np.float64)
+        ref, bound = M.experts_bound(xs, idx, w, vals, None, act == BF16, few(T, H, act))
+        assert np.abs(ref).max() > 0
+        # xs has records of its own scale: the bound of its planes is far below these values
+        assert (np.abs(y - ref) <= bound).all(), (step, (np.abs(y - ref) / bound).max())
