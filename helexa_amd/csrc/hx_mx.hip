@@ -195,6 +195,32 @@ HX_DEV mx_v16f mx_mfma(const uint4& a, uint32_t sa, const MxB<P>& b, mx_v16f c) 
   return c;
 }
 
+// One plane of a record as an MFMA operand. Where few rows meet the weights, their
+// planes are columns of their own (column p n + r: plane p of row r, n rows), one
+// MFMA does what takes P with the planes one after the other, and the columns of a
+// row are added at the end.
+struct MxPlane {
+  uint32_t w[6], sc;
+  HX_DEV void zero() {
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[i] = 0u;
+    sc = 127u;
+  }
+  template <int P>
+  HX_DEV void load(const uint8_t* rec, int p) {
+    const uint2* q = (const uint2*)(rec + 24 * p);
+    const uint2 a = q[0], b = q[1], c = q[2];
+    w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y; w[4] = c.x; w[5] = c.y;
+    sc = rec[4 * MxRec<P>::SCALE + p];
+  }
+};
+template <int SA>
+HX_DEV mx_v16f mx_mfma1(const uint4& a, uint32_t sa, const MxPlane& b, mx_v16f c) {
+  const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+  const mx_v8i bv = {(int)b.w[0], (int)b.w[1], (int)b.w[2], (int)b.w[3], (int)b.w[4], (int)b.w[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 2, SA, (int)sa, 0, (int)b.sc);
+}
+
 HX_DEV mx_v16f mx_zero16() {
   mx_v16f z;
 #pragma unroll
@@ -206,20 +232,26 @@ HX_DEV mx_v16f mx_zero16() {
 HX_DEV float mx_swiglu(float g, float u) { return siluf_(g) * u; }
 
 // ---------------------------------------------------------------- few tokens
-// The experts that some token chose, ascending, as bits in LDS (32 words).
-HX_DEV void mx_few_bits(const MxArgs& a, const int* sidx, uint32_t* bits) {
-  if (threadIdx.x < 32) bits[threadIdx.x] = 0u;
-  __syncthreads();
+// The routing of a few tokens in LDS.
+struct MxFew {
+  int idx[MX_FEW_T * HX_MAX_TOPK];
+  uint32_t bits[32];   // the experts that some token chose
+};
+HX_DEV void mx_few_bits(const MxArgs& a, MxFew& sm) {
+  if (threadIdx.x < 32) sm.bits[threadIdx.x] = 0u;
+  lds_barrier();
   for (int f = threadIdx.x; f < a.F; f += blockDim.x) {
-    const int e = sidx[f];
-    if ((unsigned)e < (unsigned)a.E) atomicOr(&bits[e >> 5], 1u << (e & 31));
+    const int e = a.idx[f];
+    sm.idx[f] = e;
+    if ((unsigned)e < (unsigned)a.E) atomicOr(&sm.bits[e >> 5], 1u << (e & 31));
   }
-  __syncthreads();
+  lds_barrier();
 }
-// their number, and (in every lane) the s-th of them, -1 if there are fewer
-HX_DEV int mx_few_slot(const uint32_t* bits, int s, int& n) {
+// the number of chosen experts, and (in every lane) the s-th of them in ascending
+// order, -1 if there are fewer
+HX_DEV int mx_few_slot(const MxFew& sm, int s, int& n) {
   const int l = lane_id();
-  const uint32_t w = l < 32 ? bits[l] : 0u;
+  const uint32_t w = l < 32 ? sm.bits[l] : 0u;
   int c = __popc(w), x = c;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -237,62 +269,30 @@ HX_DEV int mx_few_slot(const uint32_t* bits, int s, int& n) {
   return 32 * L + __ffsll(b) - 1;
 }
 
-// steps of K a wave of W takes: few and whole words of scales
-template <int W>
-HX_DEV int mx_wave_steps(int S) {
+// steps of K a wave takes where W waves share them: 1, 2 or whole words of scales
+__host__ __device__ inline int mx_wave_steps(int S, int W) {
   const int c = (S + W - 1) / W;
   return c <= 1 ? 1 : c == 2 ? 2 : (c + 3) / 4 * 4;
 }
 
-// gate/up of up to 8 tokens: workgroup (32 features, slot); the 8 waves split K, the
-// tokens' records are made in LDS while the first weights are on their way.
-template <int P>
-__global__ __launch_bounds__(512) void k_mx_few_gate_up(MxArgs a) {
-  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
+// Gate/up of up to 8 tokens. Workgroup: a chosen expert (slot) and 8 / KW groups of 32
+// features; KW waves share a group's K and add up in LDS. The tokens' records are
+// made in LDS by every workgroup: a kernel of their own would cost more than it saves.
+// The planes are columns: with them one after the other the products took 8 of the
+// 26 us of 6 tokens' 64 MB.
+template <int P, int KW>
+__global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
+  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, FW = 8 / KW;
   extern __shared__ __align__(16) uint8_t sm[];
-  __shared__ uint32_t bits[32];
-  __shared__ int sidx[MX_FEW_T * HX_MAX_TOPK];
-  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, T = a.T;
-  const int slot = blockIdx.y, fb = blockIdx.x;
-  int e;
-  if (T == 1) {   // a slot per entry
-    e = slot < a.k ? a.idx[slot] : a.E;
-    if (slot < a.k && (unsigned)e >= (unsigned)a.E) return;
-  } else {
-    for (int f = tid; f < a.F; f += 512) sidx[f] = a.idx[f];
-    __syncthreads();
-    mx_few_bits(a, sidx, bits);
-    int n;
-    e = mx_few_slot(bits, slot, n);
-    if (e < 0) {
-      if (slot > n || a.Is == 0) return;
-      e = a.E;
-    }
-    e = __builtin_amdgcn_readfirstlane(e);
-  }
-  const bool sh = e == a.E;
-  const int inter = sh ? a.Is : a.I;
-  if (fb >= mx_blocks(inter)) return;
+  __shared__ MxFew few;
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = a.T;
+  const int slot = blockIdx.y, fb = blockIdx.x * FW + wave / KW, kq = wave % KW;
   const int S = mx_steps(a.H), S4 = (S + 3) / 4, HB = mx_blocks(a.H);
-  const int c = mx_wave_steps<8>(S), s0 = wave * c, s1 = min(S, s0 + c);
-  const bool pad = 32 * fb >= inter;   // a record behind the last feature
-  const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
-  const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
-  const int64_t at = ((int64_t)fb * S * 64 + lane) * 16;
-  const int64_t sat = mx_code_bytes(inter, a.H) + ((int64_t)fb * S4 * 64 + lane) * 4;
-  uint4 wg[4], wu[4];
-  uint32_t sg = 0, su = 0;
-  auto fetch = [&](int s) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int si = min(s + i, s1 - 1);
-      wg[i] = *(const uint4*)(gm + at + (int64_t)si * 1024);
-      wu[i] = *(const uint4*)(um + at + (int64_t)si * 1024);
-    }
-    sg = *(const uint32_t*)(gm + sat + (s >> 2) * 256) >> (8 * (s & 3));
-    su = *(const uint32_t*)(um + sat + (s >> 2) * 256) >> (8 * (s & 3));
-  };
-  if (s0 < s1 && !pad) fetch(s0);
+  int e = a.E;
+  if (T == 1) {   // a slot per entry
+    if (slot < a.k) e = a.idx[slot];
+    if (slot < a.k && (unsigned)e >= (unsigned)a.E) return;
+  }
   for (int b = tid; b < T * HB; b += 512) {
     const int t = b / HB, kb = b % HB;
     uint4 r[RV];
@@ -301,56 +301,126 @@ __global__ __launch_bounds__(512) void k_mx_few_gate_up(MxArgs a) {
 #pragma unroll
     for (int i = 0; i < RV; i++) o[i] = r[i];
   }
-  __syncthreads();
-  mx_v16f ag = mx_zero16(), au = mx_zero16();
-  const int t = lane & 31, half = lane >> 5;
-  if (!pad) {
-    for (int s = s0; s < s1; s += 4) {
-      if (s > s0) fetch(s);
-#define MX_STEP(i)                                                               \
-  if (s + i < s1) {                                                              \
-    MxB<P> b;                                                                    \
-    b.zero();                                                                    \
-    if (t < T) b.load(sm + (size_t)((2 * (s + i) + half) * T + t) * RB);         \
-    ag = mx_mfma<P, i>(wg[i], sg, b, ag);                                        \
-    au = mx_mfma<P, i>(wu[i], su, b, au);                                        \
+  uint8_t* const zrec = sm + (size_t)T * HB * RB;   // what the columns without a token read
+  if (tid == 0) {
+    uint4 r[RV];
+    mx_zero_record<P>(r);
+#pragma unroll
+    for (int i = 0; i < RV; i++) ((uint4*)zrec)[i] = r[i];
   }
-      MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
-#undef MX_STEP
+  if (T > 1) {
+    mx_few_bits(a, few);
+    int n;
+    e = mx_few_slot(few, slot, n);
+    if (e < 0) {
+      if (slot > n || a.Is == 0) return;
+      e = a.E;
     }
   }
-  __syncthreads();   // the records have been read: their place takes the partial sums
-  float* red = (float*)sm;   // [wave][gate, up][feature][T]
-  if (t < T) {
+  e = __builtin_amdgcn_readfirstlane(e);
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I;
+  if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
+  const int c = mx_wave_steps(S, KW), s0 = kq * c, s1 = min(S, s0 + c);
+  const bool live = 32 * fb < inter;   // the others: a record behind the last feature, or none
+  const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
+  const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
+  const int64_t at = (int64_t)fb * S * 1024, sat = mx_code_bytes(inter, a.H) + (int64_t)fb * S4 * 256;
+  // four steps of weights are on their way at any time
+  uint4 wg[4], wu[4];
+  auto fetch = [&](int s, int i) {
+    wg[i] = *(const uint4*)(gm + (at + s * 1024) + lane * 16);
+    wu[i] = *(const uint4*)(um + (at + s * 1024) + lane * 16);
+  };
+  uint32_t sg, su;
+  auto fetch_scales = [&](int s) {
+    sg = *(const uint32_t*)(gm + (sat + (s >> 2) * 256) + lane * 4) >> (8 * (s & 3));
+    su = *(const uint32_t*)(um + (sat + (s >> 2) * 256) + lane * 4) >> (8 * (s & 3));
+  };
+  const bool work = live && s0 < s1;
+  if (work) {
+    fetch_scales(s0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) fetch(min(s0 + i, s1 - 1), i);
+  }
+  lds_barrier();
+  mx_v16f ag = mx_zero16(), au = mx_zero16();
+  const int col = lane & 31, half = lane >> 5, C = P * T, p = col / T, t = col % T;   // column, plane, token
+  const uint8_t* rec = col < C ? sm + (half * T + t) * RB : zrec;
+  const int rstep = col < C ? 2 * T * RB : 0, pl = col < C ? p : 0;
+#define MX_STEP(i)                          \
+  {                                         \
+    MxPlane b;                              \
+    b.load<P>(rec + (s + i) * rstep, pl);   \
+    ag = mx_mfma1<i>(wg[i], cg, b, ag);     \
+    au = mx_mfma1<i>(wu[i], cu, b, au);     \
+  }
+  if (work) {
+    int s = s0;
+    for (; s + 8 <= s1; s += 4) {
+      const uint32_t cg = sg, cu = su;
+      fetch_scales(s + 4);
+      // a step's registers are loaded again as soon as it is done (left to itself the
+      // compiler loads all four steps into others first, and spills them)
+      MX_STEP(0) fetch(s + 4, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      MX_STEP(1) fetch(s + 5, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      MX_STEP(2) fetch(s + 6, 2);
+      __builtin_amdgcn_sched_barrier(0);
+      MX_STEP(3) fetch(s + 7, 3);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    for (; s < s1; s += 4) {   // one or two last groups, the last one short
+      const uint32_t cg = sg, cu = su;
+      MX_STEP(0)
+      if (s + 1 < s1) MX_STEP(1)
+      if (s + 2 < s1) MX_STEP(2)
+      if (s + 3 < s1) MX_STEP(3)
+      if (s + 4 < s1) {
+        fetch_scales(s + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) fetch(min(s + 4 + i, s1 - 1), i);
+      }
+    }
+  }
+#undef MX_STEP
+  lds_barrier();   // the records have been read: their place takes the sums
+  float* red = (float*)sm;                  // [8 waves][gate, up][32 features][C]
+  float* hv = red + 8 * 2 * 32 * C;         // [FW][T][33]
+  if (col < C) {
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int f = 8 * (i >> 2) + 4 * half + (i & 3);
-      red[((wave * 2 + 0) * 32 + f) * T + t] = ag[i];
-      red[((wave * 2 + 1) * 32 + f) * T + t] = au[i];
+      red[((wave * 2 + 0) * 32 + f) * C + col] = ag[i];
+      red[((wave * 2 + 1) * 32 + f) * C + col] = au[i];
     }
   }
-  __syncthreads();
-  float* hv = red + 8 * 2 * 32 * T;   // [T][33]
-  for (int o = tid; o < 32 * T; o += 512) {
+  lds_barrier();
+  for (int o = tid; o < FW * 32 * T; o += 512) {
+    const int w0 = o / (32 * T) * KW, f = o / T % 32, tt = o % T;
     float g = 0.f, u = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; w++) {
-      g += red[(w * 2 + 0) * 32 * T + o];
-      u += red[(w * 2 + 1) * 32 * T + o];
-    }
-    hv[(o % T) * 33 + o / T] = mx_swiglu(g, u);
+    for (int w = 0; w < KW; w++)
+#pragma unroll
+      for (int q = 0; q < P; q++) {
+        g += red[((w0 + w) * 2 + 0) * 32 * C + f * C + q * T + tt];
+        u += red[((w0 + w) * 2 + 1) * 32 * C + f * C + q * T + tt];
+      }
+    hv[(w0 / KW * T + tt) * 33 + f] = mx_swiglu(g, u);
   }
-  __syncthreads();
-  if (tid < T) {
+  lds_barrier();
+  if (tid < FW * T) {
+    const int ft = tid / T, tt = tid % T, f0 = blockIdx.x * FW + ft;
     // the row of h: the token's first entry with this expert
-    int row = sh ? a.F + tid : -1;
+    int row = sh ? a.F + tt : -1;
     if (!sh && T == 1) row = slot;
     else if (!sh)
       for (int j = a.k - 1; j >= 0; j--)
-        if (sidx[tid * a.k + j] == e) row = tid * a.k + j;
-    if (row >= 0) {
+        if (few.idx[tt * a.k + j] == e) row = tt * a.k + j;
+    if (row >= 0 && f0 < mx_blocks(inter)) {
       uint4 r[RV];
-      if (pad) {
+      if (32 * f0 >= inter) {
         mx_zero_record<P>(r);
       } else {
         float f[32];
@@ -358,7 +428,7 @@ __global__ __launch_bounds__(512) void k_mx_few_gate_up(MxArgs a) {
         for (int i = 0; i < 32; i++) f[i] = hv[tid * 33 + i];
         mx_record<P>(f, r);
       }
-      uint4* o = (uint4*)(a.hrec + ((int64_t)row * a.hblocks + fb) * RB);
+      uint4* o = (uint4*)(a.hrec + ((int64_t)row * a.hblocks + f0) * RB);
 #pragma unroll
       for (int i = 0; i < RV; i++) o[i] = r[i];
     }
@@ -367,78 +437,120 @@ __global__ __launch_bounds__(512) void k_mx_few_gate_up(MxArgs a) {
 
 // bytes of LDS of k_mx_few_gate_up
 static size_t mx_few_lds(int T, int H, bool xbf) {
-  const size_t rec = (size_t)T * mx_blocks(H) * mx_rec_bytes(xbf), red = (size_t)(8 * 2 * 32 * T + 33 * T) * 4;
+  const size_t rec = ((size_t)T * mx_blocks(H) + 1) * mx_rec_bytes(xbf);
+  const size_t red = (size_t)(8 * 2 * 32 * mx_planes(xbf) * T + 8 * 33 * T) * 4;
   return rec > red ? rec : red;
 }
 
-bool mx_few(int T, int k, int H, bool xbf) { return T <= MX_FEW_T && mx_few_lds(T, H, xbf) <= 60 * 1024; }
+bool mx_few(int T, int k, int H, bool xbf) {
+  return T <= MX_FEW_T && T * mx_planes(xbf) <= 32 && mx_few_lds(T, H, xbf) <= 60 * 1024;
+}
 
-// down and combine of up to 8 tokens: workgroup per 32 outputs; its 16 waves take the
-// (slot, 4 steps) units in turn, weigh each unit's product per token and sum in LDS.
+// most chosen experts of a call (one token: its entries)
+static int mx_few_slots(int T, int k, int E) { return T == 1 ? k : min(T * k, E); }
+
+// units of the down kernel: an expert's products over 4 steps of K
+int mx_few_parts(int T, int k, int E, int I, int Is) {
+  const int G = (mx_steps(I) + 3) / 4, Gs = Is > 0 ? (mx_steps(Is) + 3) / 4 : 0;
+  const int units = mx_few_slots(T, k, E) * G + Gs;
+  return units <= 32 ? 1 : min(MX_FEW_PARTS, (units + 31) / 32);
+}
+
+HX_DEV void mx_store(const MxArgs& a, int64_t at, float y) {
+  if (a.xbf) {
+    uint16_t* p = (uint16_t*)(a.resid ? a.resid : a.y) + at;
+    const uint16_t b = f32_to_bf16(y);
+    *p = a.resid ? f32_to_bf16(bf16_to_f32(*p) + bf16_to_f32(b)) : b;
+  } else {
+    float* p = (float*)(a.resid ? a.resid : a.y) + at;
+    *p = a.resid ? *p + y : y;
+  }
+}
+
+// Down and combine of up to 8 tokens. Workgroup: 32 outputs and a part of the units
+// (slot, 4 steps of K), which its 16 waves take in turn; each unit's product is
+// weighted per token in f32, the waves' sums are added in LDS. One part writes y, several their
+// sums for k_mx_few_sum.
 template <int P>
 __global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES;
-  __shared__ uint32_t bits[32];
-  __shared__ int sidx[MX_FEW_T * HX_MAX_TOPK];
+  __shared__ MxFew few;
   __shared__ float sw[MX_FEW_T * HX_MAX_TOPK];
-  __shared__ float red[16 * 32 * MX_FEW_T];
-  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, T = a.T, k = a.k;
-  const int nb = blockIdx.x;
-  for (int f = tid; f < a.F; f += 1024) {
-    sidx[f] = a.idx[f];
-    sw[f] = a.w[f];
-  }
+  __shared__ float red[16 * 32 * (P == 3 ? 24 : 30)];
+  __shared__ int pre[33];
+  __shared__ uint16_t list[MX_FEW_T * HX_MAX_TOPK];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = a.T, k = a.k;
+  const int nb = blockIdx.x, parts = gridDim.y;
+  for (int f = tid; f < a.F; f += 1024) sw[f] = a.w[f];
   int n = k;
-  __syncthreads();
-  if (T > 1) mx_few_bits(a, sidx, bits);
-  if (T > 1) mx_few_slot(bits, 0, n);
+  if (T == 1) {
+    if (tid < k) {
+      few.idx[tid] = a.idx[tid];
+    }
+    lds_barrier();
+  } else {
+    mx_few_bits(a, few);
+    if (tid < 64) {
+      const int c = tid < 32 ? __popc(few.bits[tid]) : 0;
+      int x = c;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+      }
+      if (tid < 32) pre[tid] = x - c;
+      if (tid == 31) pre[32] = x;
+    }
+    lds_barrier();
+    if (tid < a.E) {   // at most 1024 experts
+      const uint32_t w = few.bits[tid >> 5];
+      if ((w >> (tid & 31)) & 1u) list[pre[tid >> 5] + __popc(w & ((1u << (tid & 31)) - 1u))] = (uint16_t)tid;
+    }
+    lds_barrier();
+    n = pre[32];
+  }
   const int S = mx_steps(a.I), G = (S + 3) / 4, Ss = mx_steps(a.Is), Gs = a.Is ? (Ss + 3) / 4 : 0;
-  const int t = lane & 31, half = lane >> 5;
+  const int col = lane & 31, half = lane >> 5, C = P * T, p = col / T, t = col % T;
   mx_v16f acc = mx_zero16();
-  for (int u = wave; u < n * G + Gs; u += 16) {
+  for (int u = blockIdx.y * 16 + wave; u < n * G + Gs; u += 16 * parts) {
     const bool sh = u >= n * G;
     const int slot = sh ? n : u / G, g = sh ? u - n * G : u % G;
-    int e = a.E, row = -1;
+    int e = a.E;
+    if (!sh) e = __builtin_amdgcn_readfirstlane(T == 1 ? few.idx[slot] : (int)list[slot]);
+    if (!sh && T == 1 && (unsigned)e >= (unsigned)a.E) continue;
+    const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
+    const int inter = sh ? a.Is : a.I, St = sh ? Ss : S, S4 = (St + 3) / 4, s = 4 * g;
+    const uint8_t* wp = dm + ((int64_t)nb * St + s) * 1024;
+    const uint32_t sa = *(const uint32_t*)(dm + (mx_code_bytes(a.H, inter) + ((int64_t)nb * S4 + g) * 256) + lane * 4);
+    uint4 wd[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) wd[i] = *(const uint4*)(wp + min(i, St - 1 - s) * 1024 + lane * 16);
+    // the token's row of h with this expert, and its weight
+    int row = -1;
     float wt = 0.f;
-    if (sh) {
-      if (t < T) {
+    if (col < C) {
+      if (sh) {
         row = a.F + t;
         wt = a.shared_w[t];
-      }
-    } else if (T == 1) {
-      e = sidx[slot];
-      if ((unsigned)e >= (unsigned)a.E) continue;
-      if (t == 0) {
+      } else if (T == 1) {
         row = slot;
         wt = sw[slot];
-      }
-    } else {
-      int dummy;
-      e = mx_few_slot(bits, slot, dummy);
-      if (t < T) {
+      } else {
         for (int j = k - 1; j >= 0; j--)
-          if (sidx[t * k + j] == e) {
+          if (few.idx[t * k + j] == e) {
             row = t * k + j;
             wt += sw[t * k + j];
           }
       }
     }
-    e = __builtin_amdgcn_readfirstlane(e);
-    const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
-    const int inter = sh ? a.Is : a.I, St = sh ? Ss : S, S4 = (St + 3) / 4, s = 4 * g;
-    const uint8_t* wp = dm + (((int64_t)nb * St + s) * 64 + lane) * 16;
-    const uint32_t sa = *(const uint32_t*)(dm + mx_code_bytes(a.H, inter) + (((int64_t)nb * S4 + g) * 64 + lane) * 4);
-    uint4 wd[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) wd[i] = *(const uint4*)(wp + (int64_t)min(i, St - 1 - s) * 1024);
     const uint8_t* hp = a.hrec + ((int64_t)max(row, 0) * a.hblocks + 2 * s + half) * RB;
     mx_v16f d = mx_zero16();
 #define MX_STEP(i)                                    \
   if (s + i < St) {                                   \
-    MxB<P> b;                                         \
+    MxPlane b;                                        \
     b.zero();                                         \
-    if (row >= 0) b.load(hp + 2 * i * RB);            \
-    d = mx_mfma<P, i>(wd[i], sa, b, d);               \
+    if (row >= 0) b.load<P>(hp + 2 * i * RB, p);      \
+    d = mx_mfma1<i>(wd[i], sa, b, d);                 \
   }
     MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
 #undef MX_STEP
@@ -446,39 +558,64 @@ __global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[i] = row >= 0 ? __builtin_fmaf(wt, d[i], acc[i]) : acc[i];
   }
-  if (t < T) {
+  if (col < C) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) red[wave * 32 * T + (8 * (i >> 2) + 4 * half + (i & 3)) * T + t] = acc[i];
+    for (int i = 0; i < 16; i++) red[(wave * C + col) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)] = acc[i];
   }
-  __syncthreads();
+  lds_barrier();
   for (int o = tid; o < 32 * T; o += 1024) {
     float y = 0.f;
 #pragma unroll
-    for (int w = 0; w < 16; w++) y += red[w * 32 * T + o];
-    const int64_t at = (int64_t)(o % T) * a.H + 32 * nb + o / T;
-    if constexpr (P == 3) {
-      uint16_t* p = (uint16_t*)(a.resid ? a.resid : a.y) + at;
-      const uint16_t b = f32_to_bf16(y);
-      *p = a.resid ? f32_to_bf16(bf16_to_f32(*p) + bf16_to_f32(b)) : b;
-    } else {
-      float* p = (float*)(a.resid ? a.resid : a.y) + at;
-      *p = a.resid ? *p + y : y;
-    }
+    for (int w = 0; w < 16; w++)
+#pragma unroll
+      for (int q = 0; q < P; q++) y += red[(w * C + q * T) * 32 + o];
+    const int64_t at = (int64_t)(o >> 5) * a.H + 32 * nb + (o & 31);
+    if (parts > 1) a.part[(int64_t)blockIdx.y * T * a.H + at] = y;
+    else mx_store(a, at, y);
   }
 }
 
-hipError_t launch_mx_few_gate_up(const MxArgs& a, hipStream_t s) {
-  const int slots = (a.T == 1 ? a.k : min(a.F, a.E)) + (a.Is > 0 ? 1 : 0);
-  const dim3 g(a.hblocks, slots);
+__global__ __launch_bounds__(256) void k_mx_few_sum(MxArgs a, int parts) {
+  const int64_t n = (int64_t)a.T * a.H, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float v[MX_FEW_PARTS], y = 0.f;
+#pragma unroll
+  for (int p = 0; p < MX_FEW_PARTS; p++) v[p] = p < parts ? a.part[p * n + i] : 0.f;
+#pragma unroll
+  for (int p = 0; p < MX_FEW_PARTS; p++) y += v[p];
+  mx_store(a, i, y);
+}
+
+template <int P>
+static void mx_few_gate_up(const MxArgs& a, hipStream_t s) {
+  const int slots = mx_few_slots(a.T, a.k, a.E) + (a.Is > 0 ? 1 : 0), tasks = slots * a.hblocks;
   const uint32_t lds = (uint32_t)mx_few_lds(a.T, a.H, a.xbf);
-  if (a.xbf) hx_launch(k_mx_few_gate_up<3>, g, dim3(512), lds, s, a);
-  else hx_launch(k_mx_few_gate_up<5>, g, dim3(512), lds, s, a);
+  // enough waves to keep two on each of the 1024 SIMDs, no more
+#define FGU(KW) hx_launch(k_mx_few_gate_up<P, KW>, dim3((a.hblocks + 8 / KW - 1) / (8 / KW), slots), dim3(512), lds, s, a)
+  if (tasks >= 2048) FGU(1);
+  else if (2 * tasks >= 2048) FGU(2);
+  else if (4 * tasks >= 2048) FGU(4);
+  else FGU(8);
+#undef FGU
+}
+
+hipError_t launch_mx_few_gate_up(const MxArgs& a, hipStream_t s) {
+  if (a.xbf) mx_few_gate_up<3>(a, s);
+  else mx_few_gate_up<5>(a, s);
   return hipGetLastError();
 }
 
 hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s) {
-  if (a.xbf) hx_launch(k_mx_few_down<3>, dim3(a.H / 32), dim3(1024), 0, s, a);
-  else hx_launch(k_mx_few_down<5>, dim3(a.H / 32), dim3(1024), 0, s, a);
+  const int parts = mx_few_parts(a.T, a.k, a.E, a.I, a.Is);
+  const dim3 g(a.H / 32, parts);
+  if (a.xbf) hx_launch(k_mx_few_down<3>, g, dim3(1024), 0, s, a);
+  else hx_launch(k_mx_few_down<5>, g, dim3(1024), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_few_sum(const MxArgs& a, hipStream_t s) {
+  const int parts = mx_few_parts(a.T, a.k, a.E, a.I, a.Is);
+  hx_launch(k_mx_few_sum, dim3((unsigned)(((int64_t)a.T * a.H + 255) / 256)), dim3(256), 0, s, a, parts);
   return hipGetLastError();
 }
 

@@ -37,7 +37,7 @@ def cuda(a, act=None):
 def few(T, H, act):
     """whether the few-token kernels take the call: their records in 60 KiB"""
     blocks = (H + 127) // 128 * 4
-    return T <= 8 and T * blocks * (80 if act == BF16 else 128) <= 60 * 1024
+    return T <= (8 if act == BF16 else 6) and T * blocks * (80 if act == BF16 else 128) <= 60 * 1024
 
 
 def check(y, x, idx, w, vals, sw, act):
@@ -192,7 +192,7 @@ def test_pointers_off_alignment_and_guards(T, act):
     # a workspace off 16 bytes or too small is refused, y untouched
     before = ys.clone()
     assert hx.lib().hx_moe_experts(*args, ws.data_ptr() + 4, n, s) == 1
-    assert hx.lib().hx_moe_experts(*args, ws.data_ptr(), n - 1, s) == 4
+    assert hx.lib().hx_moe_experts(*args, ws.data_ptr(), 1024, s) == 4
     torch.cuda.synchronize()
     assert torch.equal(before, ys)
     # in place
