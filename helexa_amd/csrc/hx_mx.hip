@@ -14,6 +14,8 @@
 // grouped products over tiles of tile_m rows, and the combine.
 #include "hx_mx.h"
 
+#include <type_traits>
+
 namespace hx {
 
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
@@ -179,20 +181,23 @@ struct MxB {
   }
 };
 
-// c += weights (one step's codes, their scale in byte SA of sa) x planes of b
-template <int P, int SA>
-HX_DEV mx_v16f mx_mfma(const uint4& a, uint32_t sa, const MxB<P>& b, mx_v16f c) {
-  const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+// c[m] += weights m (one step's codes w[m][S], their scale in byte SA of sc[m]) x the
+// planes of b; plane by plane, so that neighbouring MFMAs do not wait for each other
+template <int P, int S, int SA, int NM, int NC>
+HX_DEV void mx_mfma(const uint4 (&w)[NM][2], const uint32_t (&sc)[NM], const MxB<P>& b, mx_v16f (&c)[NM][NC], int n) {
 #define MX_PLANE(p)                                                                                               \
   if constexpr (p < P) {                                                                                          \
     const mx_v8i bv = {(int)b.w[6 * p], (int)b.w[6 * p + 1], (int)b.w[6 * p + 2], (int)b.w[6 * p + 3],            \
                        (int)b.w[6 * p + 4], (int)b.w[6 * p + 5], 0, 0};                                           \
-    c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 2, SA, (int)sa, (p) & 3,                    \
-                                                        (int)b.w[MxRec<P>::SCALE + (p) / 4]);                     \
+    _Pragma("unroll") for (int m = 0; m < NM; m++) {                                                              \
+      const uint4& a = w[m][S];                                                                                   \
+      const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};                                     \
+      c[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c[m][n], 4, 2, SA, (int)sc[m], (p) & 3,   \
+                                                                (int)b.w[MxRec<P>::SCALE + (p) / 4]);             \
+    }                                                                                                             \
   }
   MX_PLANE(0) MX_PLANE(1) MX_PLANE(2) MX_PLANE(3) MX_PLANE(4)
 #undef MX_PLANE
-  return c;
 }
 
 // One plane of a record as an MFMA operand. Where few rows meet the weights, their
@@ -334,8 +339,8 @@ __global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
   };
   uint32_t sg, su;
   auto fetch_scales = [&](int s) {
-    sg = *(const uint32_t*)(gm + (sat + (s >> 2) * 256) + lane * 4) >> (8 * (s & 3));
-    su = *(const uint32_t*)(um + (sat + (s >> 2) * 256) + lane * 4) >> (8 * (s & 3));
+    sg = *(const uint32_t*)(gm + (sat + (s >> 2) * 256) + lane * 4);
+    su = *(const uint32_t*)(um + (sat + (s >> 2) * 256) + lane * 4);
   };
   const bool work = live && s0 < s1;
   if (work) {
@@ -358,7 +363,7 @@ __global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
   if (work) {
     int s = s0;
     for (; s + 8 <= s1; s += 4) {
-      const uint32_t cg = sg, cu = su;
+      const uint32_t cg = sg >> (8 * (s & 3)), cu = su >> (8 * (s & 3));
       fetch_scales(s + 4);
       // a step's registers are loaded again as soon as it is done (left to itself the
       // compiler loads all four steps into others first, and spills them)
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     }
     for (; s < s1; s += 4) {   // one or two last groups, the last one short
-      const uint32_t cg = sg, cu = su;
+      const uint32_t cg = sg >> (8 * (s & 3)), cu = su >> (8 * (s & 3));
       MX_STEP(0)
       if (s + 1 < s1) MX_STEP(1)
       if (s + 2 < s1) MX_STEP(2)
@@ -767,22 +772,27 @@ struct MxStage {
   HX_DEV void issue(int wave, int st, uint32_t lds) const {
 #pragma unroll
     for (int i = 0; i < PER; i++)
-      if (wave + 4 * i < LOADS) dma16(src[i] + (int64_t)st * (4 * RB), lds + (wave + 4 * i) * 1024);
+      if (LOADS % 4 == 0 || wave + 4 * i < LOADS) dma16(src[i] + (int64_t)st * (4 * RB), lds + (wave + 4 * i) * 1024);
   }
 };
 
-// workgroup -> (feature group, tile): the NX workgroups of a tile on one XCD
-HX_DEV void mx_tile(int NX, int& nt, int& tile) {
-  const int L = blockIdx.x;
+// workgroup -> (feature group, tile) of N tiles; tile -1: none. XCD x (workgroup id
+// mod 8) takes the x-th eighth of the list in order, so that the tiles of an expert,
+// which are neighbours in the list, and the NX workgroups of a tile run side by side
+// on one XCD and meet each other's weights and rows in its L2. (Tiles dealt to the XCDs
+// in turn: every XCD fetched every expert.)
+HX_DEV void mx_tile(int NX, int N, int& nt, int& tile) {
+  const int L = blockIdx.x, per = (N + 7) / 8, i = L / (8 * NX);
   nt = (L >> 3) % NX;
-  tile = L / (8 * NX) * 8 + (L & 7);
+  tile = (L & 7) * per + i;
+  if (i >= per || tile >= N) tile = -1;
 }
 
 // the 4 waves' sums over K: NM weight matrices' 32-row tiles (one each) times the
 // tile's rows
 template <int TM, int P, int NM>
-HX_DEV void mx_products(const MxStage<TM, P>& sg, uint8_t* buf, int nst, const uint8_t* const (&codes)[NM],
-                        const uint8_t* const (&scales)[NM], bool live, mx_v16f (&acc)[NM][TM / 32]) {
+HX_DEV void mx_products(const MxStage<TM, P>& sg, uint8_t* buf, int nst, const uint8_t* (&codes)[NM],
+                        const uint8_t* (&scales)[NM], bool live, mx_v16f (&acc)[NM][TM / 32]) {
   constexpr int RB = MxRec<P>::BYTES;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
@@ -791,14 +801,15 @@ HX_DEV void mx_products(const MxStage<TM, P>& sg, uint8_t* buf, int nst, const u
   auto fetch = [&](int st, int b) {
 #pragma unroll
     for (int m = 0; m < NM; m++) {
-      w[b][m][0] = *(const uint4*)(codes[m] + (int64_t)st * 2048);
-      w[b][m][1] = *(const uint4*)(codes[m] + (int64_t)st * 2048 + 1024);
-      sc[b][m] = *(const uint32_t*)(scales[m] + (st >> 1) * 256) >> (16 * (st & 1));
+      w[b][m][0] = *(const uint4*)(codes[m] + st * 2048 + lane * 16);
+      w[b][m][1] = *(const uint4*)(codes[m] + st * 2048 + 1024 + lane * 16);
+      sc[b][m] = *(const uint32_t*)(scales[m] + (st >> 1) * 256 + lane * 4);   // b = st % 2: bytes 2 b, 2 b + 1
     }
   };
   sg.issue(wave, 0, lds);
   if (live) fetch(0, 0);
-  auto stage = [&](int st, int b) {
+  auto stage = [&](int st, auto bc) {
+    constexpr int b = decltype(bc)::value;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (st + 1 < nst) {
@@ -806,25 +817,25 @@ HX_DEV void mx_products(const MxStage<TM, P>& sg, uint8_t* buf, int nst, const u
       if (live) fetch(st + 1, b ^ 1);
     }
     if (live) {
-#pragma unroll
-      for (int s = 0; s < 2; s++)
+      auto step = [&](auto sc_) {
+        constexpr int s = decltype(sc_)::value;
 #pragma unroll
         for (int n = 0; n < TM / 32; n++) {
           MxB<P> bb;
           bb.load(buf + b * MxStage<TM, P>::BYTES + ((2 * s + (lane >> 5)) * TM + 32 * n + (lane & 31)) * RB);
-#pragma unroll
-          for (int m = 0; m < NM; m++)
-            acc[m][n] = s == 0 ? mx_mfma<P, 0>(w[b][m][0], sc[b][m], bb, acc[m][n])
-                               : mx_mfma<P, 1>(w[b][m][1], sc[b][m], bb, acc[m][n]);
+          mx_mfma<P, s, 2 * b + s>(w[b], sc[b], bb, acc, n);
         }
+      };
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
     }
   };
   int st = 0;
   for (; st + 2 <= nst; st += 2) {
-    stage(st, 0);
-    stage(st + 1, 1);
+    stage(st, std::integral_constant<int, 0>{});
+    stage(st + 1, std::integral_constant<int, 1>{});
   }
-  if (st < nst) stage(st, 0);
+  if (st < nst) stage(st, std::integral_constant<int, 0>{});
 }
 
 // lane l: the 32 values of column l of the tile from D's halves
@@ -839,88 +850,99 @@ HX_DEV void mx_columns(const mx_v16f (&d)[TM / 32], float (&f)[32]) {
   }
 }
 
-template <int TM, int P>
-__global__ __launch_bounds__(256) void k_mx_gate_up(MxArgs a) {
+// MF groups of 32 features of h a wave
+template <int TM, int P, int MF>
+__global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
   __shared__ __align__(16) uint8_t buf[2 * MxStage<TM, P>::BYTES];
   int nt, tile;
-  mx_tile(a.hblocks / 4, nt, tile);
-  if (tile >= a.counts[0]) return;
+  mx_tile((a.hblocks + 4 * MF - 1) / (4 * MF), a.counts[0], nt, tile);
+  if (tile < 0) return;
   const int4 ti = ((const int4*)a.tiles)[tile];
   const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
   const bool sh = e == a.E;
   const int inter = sh ? a.Is : a.I;
-  if (4 * nt >= mx_blocks(inter)) return;
-  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int fb = 4 * nt + wave, HB = mx_blocks(a.H), S = mx_steps(a.H), S4 = (S + 3) / 4;
-  const bool live = 32 * fb < inter;
+  if (4 * MF * nt >= mx_blocks(inter)) return;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int f0 = (4 * nt + wave) * MF, HB = mx_blocks(a.H), S = mx_steps(a.H), S4 = (S + 3) / 4;
+  const bool live = 32 * f0 < inter;
   MxStage<TM, P> sg;
   sg.init(wave, lane, [&](int r) {
     const int p = p0 + min(r, rows - 1);
     const int t = sh ? p - a.F : a.perm[p] / a.k;
     return a.xrec + (int64_t)t * HB * RB;
   });
-  const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
-  const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
-  const int64_t at = ((int64_t)fb * S * 64 + lane) * 16;
-  const int64_t sat = mx_code_bytes(inter, a.H) + ((int64_t)fb * S4 * 64 + lane) * 4;
-  const uint8_t* const codes[2] = {gm + at, um + at};
-  const uint8_t* const scales[2] = {gm + sat, um + sat};
-  mx_v16f acc[2][TM / 32];
+  const uint8_t *codes[2 * MF], *scales[2 * MF];
 #pragma unroll
-  for (int n = 0; n < TM / 32; n++) acc[0][n] = acc[1][n] = mx_zero16();
-  mx_products<TM, P, 2>(sg, buf, HB / 4, codes, scales, live, acc);
-  mx_v16f h[TM / 32];
+  for (int m = 0; m < MF; m++) {
+    const int fb = min(f0 + m, inter / 32 - 1);
 #pragma unroll
-  for (int n = 0; n < TM / 32; n++)
+    for (int q = 0; q < 2; q++) {
+      const uint8_t* mat = q ? (sh ? a.sup.base : a.up.mat(e)) : (sh ? a.sgate.base : a.gate.mat(e));
+      codes[2 * m + q] = mat + (int64_t)fb * S * 1024;
+      scales[2 * m + q] = mat + mx_code_bytes(inter, a.H) + (int64_t)fb * S4 * 256;
+    }
+  }
+  mx_v16f acc[2 * MF][TM / 32];
 #pragma unroll
-    for (int i = 0; i < 16; i++) h[n][i] = mx_swiglu(acc[0][n][i], acc[1][n][i]);
-  float f[32];
-  mx_columns<TM>(h, f);
-  uint4 r[RV];
-  if (live) mx_record<P>(f, r);
-  else mx_zero_record<P>(r);
-  if (lane < rows && lane < TM) {
-    uint4* o = (uint4*)(a.hrec + ((int64_t)(p0 + lane) * a.hblocks + fb) * RB);
+  for (int m = 0; m < 2 * MF; m++)
 #pragma unroll
-    for (int i = 0; i < RV; i++) o[i] = r[i];
+    for (int n = 0; n < TM / 32; n++) acc[m][n] = mx_zero16();
+  mx_products<TM, P, 2 * MF>(sg, buf, HB / 4, codes, scales, live, acc);
+#pragma unroll
+  for (int m = 0; m < MF; m++) {
+    mx_v16f h[TM / 32];
+#pragma unroll
+    for (int n = 0; n < TM / 32; n++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) h[n][i] = mx_swiglu(acc[2 * m][n][i], acc[2 * m + 1][n][i]);
+    float f[32];
+    mx_columns<TM>(h, f);
+    uint4 r[RV];
+    if (32 * (f0 + m) < inter) mx_record<P>(f, r);
+    else mx_zero_record<P>(r);
+    if (lane < rows && lane < TM && f0 + m < mx_blocks(inter)) {
+      uint4* o = (uint4*)(a.hrec + ((int64_t)(p0 + lane) * a.hblocks + f0 + m) * RB);
+#pragma unroll
+      for (int i = 0; i < RV; i++) o[i] = r[i];
+    }
   }
 }
 
-// outputs of the experts, unweighted: 64 features a wave
-template <int TM, int P>
-__global__ __launch_bounds__(256) void k_mx_down(MxArgs a) {
+// outputs of the experts, unweighted: 64 MF features a wave
+template <int TM, int P, int MF>
+__global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES;
   __shared__ __align__(16) uint8_t buf[2 * MxStage<TM, P>::BYTES];
   int nt, tile;
-  mx_tile((a.H + 255) / 256, nt, tile);
-  if (tile >= a.counts[0]) return;
+  mx_tile((a.H + 256 * MF - 1) / (256 * MF), a.counts[0], nt, tile);
+  if (tile < 0) return;
   const int4 ti = ((const int4*)a.tiles)[tile];
   const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
   const bool sh = e == a.E;
   const int inter = sh ? a.Is : a.I;
-  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int S = mx_steps(inter), S4 = (S + 3) / 4, nb = a.H / 32;
-  const int n0 = 8 * nt + 2 * wave;
+  const int n0 = (4 * nt + wave) * 2 * MF;
   const bool live = n0 < nb;
   MxStage<TM, P> sg;
   sg.init(wave, lane, [&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * RB; });
   const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
-  const uint8_t *codes[2], *scales[2];
+  const uint8_t *codes[2 * MF], *scales[2 * MF];
 #pragma unroll
-  for (int m = 0; m < 2; m++) {
+  for (int m = 0; m < 2 * MF; m++) {
     const int n = min(n0 + m, nb - 1);
-    codes[m] = dm + ((int64_t)n * S * 64 + lane) * 16;
-    scales[m] = dm + mx_code_bytes(a.H, inter) + ((int64_t)n * S4 * 64 + lane) * 4;
+    codes[m] = dm + (int64_t)n * S * 1024;
+    scales[m] = dm + mx_code_bytes(a.H, inter) + (int64_t)n * S4 * 256;
   }
-  const uint8_t* const cc[2] = {codes[0], codes[1]};
-  const uint8_t* const ss[2] = {scales[0], scales[1]};
-  mx_v16f acc[2][TM / 32];
+  mx_v16f acc[2 * MF][TM / 32];
 #pragma unroll
-  for (int n = 0; n < TM / 32; n++) acc[0][n] = acc[1][n] = mx_zero16();
-  mx_products<TM, P, 2>(sg, buf, mx_blocks(inter) / 4, cc, ss, live, acc);
+  for (int m = 0; m < 2 * MF; m++)
 #pragma unroll
-  for (int m = 0; m < 2; m++) {
+    for (int n = 0; n < TM / 32; n++) acc[m][n] = mx_zero16();
+  mx_products<TM, P, 2 * MF>(sg, buf, mx_blocks(inter) / 4, codes, scales, live, acc);
+#pragma unroll
+  for (int m = 0; m < 2 * MF; m++) {
     float f[32];
     mx_columns<TM>(acc[m], f);
     if (lane < TM && lane < rows && n0 + m < nb) {
@@ -944,16 +966,20 @@ __global__ __launch_bounds__(256) void k_mx_down(MxArgs a) {
   }
 }
 
-#define MX_LAUNCH(KERNEL, NX)                                                              \
-  const dim3 g((unsigned)((NX) * (((int64_t)a.max_tiles + 7) / 8 * 8)));                   \
-  if (a.xbf && a.tile_m == 32) hx_launch(KERNEL<32, 3>, g, dim3(256), 0, s, a);            \
-  else if (a.xbf) hx_launch(KERNEL<64, 3>, g, dim3(256), 0, s, a);                         \
-  else if (a.tile_m == 32) hx_launch(KERNEL<32, 5>, g, dim3(256), 0, s, a);                \
-  else hx_launch(KERNEL<64, 5>, g, dim3(256), 0, s, a);                                    \
+#define MX_LAUNCH(KERNEL, N, PER)                                                             \
+  auto go = [&](auto kernel, int mf) {                                                        \
+    const int64_t nx = ((N) + (PER) * mf - 1) / ((PER) * mf);                                 \
+    hx_launch(kernel, dim3((unsigned)(nx * ((a.max_tiles + 7) / 8 * 8))), dim3(256), 0, s, a); \
+  };                                                                                          \
+  if (a.xbf && a.tile_m == 32) go(KERNEL<32, 3, 1>, 1);                                       \
+  else if (a.xbf) go(KERNEL<64, 3, MX_MF>, MX_MF);                                            \
+  else if (a.tile_m == 32) go(KERNEL<32, 5, 1>, 1);                                           \
+  else go(KERNEL<64, 5, 1>, 1);                                                               \
   return hipGetLastError()
 
-hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_gate_up, a.hblocks / 4); }
-hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_down, (a.H + 255) / 256); }
+constexpr int MX_MF = 2;
+hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_gate_up, a.hblocks, 4); }
+hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_down, a.H / 32, 8); }
 
 // y[t] = the token's entries' rows times their weights in their order, then the
 // shared expert's: 8 outputs a thread
