@@ -17,8 +17,9 @@
 // codes are exact and the MFMA sums them in f32, so a product with bf16 activations
 // costs three MFMAs at the 4 / 6-bit rate, which is four times the bf16 rate: less
 // than one bf16 MFMA, and no weight is ever expanded.
-// A record is P x 24 bytes of codes, then the P scale bytes; 16-byte multiples. A
-// block with a NaN or an infinity has scale NaN: its token's outputs are NaN.
+// A record is the first 16 of each plane's 24 bytes of codes, then the last 8 of each
+// (both are loaded straight into the registers of an MFMA operand), then the P scale
+// bytes; 80 bytes with three planes, 128 with five. A block with a NaN or an infinity has scale NaN: its token's outputs are NaN.
 #pragma once
 #include "hx_internal.h"
 

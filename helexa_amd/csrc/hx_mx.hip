@@ -19,6 +19,7 @@
 namespace hx {
 
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
+typedef uint32_t mx_v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t mx_v6u __attribute__((ext_vector_type(6)));
 typedef float mx_v16f __attribute__((ext_vector_type(16)));
 typedef float mx_v32f __attribute__((ext_vector_type(32)));
@@ -82,11 +83,11 @@ HX_DEV void mx_record(const float (&f)[32], uint4 (&out)[MxRec<P>::VECS]) {
   uint32_t w[4 * MxRec<P>::VECS];
 #pragma unroll
   for (int i = 0; i < 4 * MxRec<P>::VECS; i++) w[i] = 0;
-  mx_v16f ev, od;   // the conversion takes the even and the odd elements
+  mx_v16f ev, od;   // the conversion takes the even and the odd elements; whatever codes a bad block gets
 #pragma unroll
   for (int i = 0; i < 16; i++) {
-    ev[i] = bad ? 0.f : f[2 * i];
-    od[i] = bad ? 0.f : f[2 * i + 1];
+    ev[i] = f[2 * i];
+    od[i] = f[2 * i + 1];
   }
 #pragma unroll
   for (int p = 0; p < P; p++) {
@@ -98,7 +99,7 @@ HX_DEV void mx_record(const float (&f)[32], uint4 (&out)[MxRec<P>::VECS]) {
     // kept alive past them
     asm volatile("" : "+v"(c) : "v"(ev), "v"(od), "v"(sc));
 #pragma unroll
-    for (int i = 0; i < 6; i++) w[6 * p + i] = c[i];
+    for (int i = 0; i < 6; i++) w[i < 4 ? 4 * p + i : 4 * P + 2 * p + i - 4] = c[i];
     if (p + 1 < P) {
       mx_v32f v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(c, sc);
       asm volatile("" : "+v"(v) : "v"(c), "v"(sc));
@@ -164,36 +165,39 @@ HX_DEV void mx_token_record(const void* x, int64_t t, int H, int kb, uint4 (&out
   mx_record<P>(f, out);
 }
 
-// a record's words as MFMA operands
+// a plane of a record as the MFMA takes it: 6 words in a row
+typedef int mx_v6i __attribute__((ext_vector_type(6)));
+template <int P>
+HX_DEV mx_v6i mx_plane(const uint8_t* rec, int p) {
+  const uint4 a = *(const uint4*)(rec + 16 * p);
+  const uint2 b = *(const uint2*)(rec + 16 * P + 8 * p);
+  return mx_v6i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y};
+}
+
+// a record's planes and scales as MFMA operands
 template <int P>
 struct MxB {
-  uint32_t w[4 * MxRec<P>::VECS];
-  HX_DEV void set(int i, const uint4& v) {
-    w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-  }
-  HX_DEV void load(const uint8_t* p) {
+  mx_v6i w[P];
+  uint32_t sc[(P + 3) / 4];
+  HX_DEV void load(const uint8_t* rec) {
 #pragma unroll
-    for (int i = 0; i < MxRec<P>::VECS; i++) set(i, *(const uint4*)(p + 16 * i));
-  }
-  HX_DEV void zero() {
+    for (int p = 0; p < P; p++) w[p] = mx_plane<P>(rec, p);
 #pragma unroll
-    for (int i = 0; i < 4 * MxRec<P>::VECS; i++) w[i] = i >= MxRec<P>::SCALE ? 0x7f7f7f7fu : 0u;
+    for (int i = 0; i < (P + 3) / 4; i++) sc[i] = *(const uint32_t*)(rec + 24 * P + 4 * i);
   }
 };
 
-// c[m] += weights m (one step's codes w[m][S], their scale in byte SA of sc[m]) x the
-// planes of b; plane by plane, so that neighbouring MFMAs do not wait for each other
-template <int P, int S, int SA, int NM, int NC>
-HX_DEV void mx_mfma(const uint4 (&w)[NM][2], const uint32_t (&sc)[NM], const MxB<P>& b, mx_v16f (&c)[NM][NC], int n) {
+// c[m][n] += weights m (one step's codes, their scale in byte SA of sc[m]) x the planes
+// of b; plane by plane, so that neighbouring MFMAs do not wait for each other
+template <int P, int SA, int NM, int NC>
+HX_DEV void mx_mfma(const mx_v4u (&w)[NM], const uint32_t (&sc)[NM], const MxB<P>& b, mx_v16f (&c)[NM][NC], int n) {
 #define MX_PLANE(p)                                                                                               \
   if constexpr (p < P) {                                                                                          \
-    const mx_v8i bv = {(int)b.w[6 * p], (int)b.w[6 * p + 1], (int)b.w[6 * p + 2], (int)b.w[6 * p + 3],            \
-                       (int)b.w[6 * p + 4], (int)b.w[6 * p + 5], 0, 0};                                           \
+    const mx_v8i bv = {b.w[p][0], b.w[p][1], b.w[p][2], b.w[p][3], b.w[p][4], b.w[p][5], 0, 0};                   \
     _Pragma("unroll") for (int m = 0; m < NM; m++) {                                                              \
-      const uint4& a = w[m][S];                                                                                   \
-      const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};                                     \
+      const mx_v8i av = {(int)w[m].x, (int)w[m].y, (int)w[m].z, (int)w[m].w, 0, 0, 0, 0};                         \
       c[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c[m][n], 4, 2, SA, (int)sc[m], (p) & 3,   \
-                                                                (int)b.w[MxRec<P>::SCALE + (p) / 4]);             \
+                                                                (int)b.sc[(p) / 4]);                              \
     }                                                                                                             \
   }
   MX_PLANE(0) MX_PLANE(1) MX_PLANE(2) MX_PLANE(3) MX_PLANE(4)
@@ -205,24 +209,22 @@ HX_DEV void mx_mfma(const uint4 (&w)[NM][2], const uint32_t (&sc)[NM], const MxB
 // MFMA does what takes P with the planes one after the other, and the columns of a
 // row are added at the end.
 struct MxPlane {
-  uint32_t w[6], sc;
+  mx_v6i w;
+  uint32_t sc;
   HX_DEV void zero() {
-#pragma unroll
-    for (int i = 0; i < 6; i++) w[i] = 0u;
+    w = mx_v6i{0, 0, 0, 0, 0, 0};
     sc = 127u;
   }
   template <int P>
   HX_DEV void load(const uint8_t* rec, int p) {
-    const uint2* q = (const uint2*)(rec + 24 * p);
-    const uint2 a = q[0], b = q[1], c = q[2];
-    w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y; w[4] = c.x; w[5] = c.y;
-    sc = rec[4 * MxRec<P>::SCALE + p];
+    w = mx_plane<P>(rec, p);
+    sc = rec[24 * P + p];
   }
 };
 template <int SA>
 HX_DEV mx_v16f mx_mfma1(const uint4& a, uint32_t sa, const MxPlane& b, mx_v16f c) {
   const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-  const mx_v8i bv = {(int)b.w[0], (int)b.w[1], (int)b.w[2], (int)b.w[3], (int)b.w[4], (int)b.w[5], 0, 0};
+  const mx_v8i bv = {b.w[0], b.w[1], b.w[2], b.w[3], b.w[4], b.w[5], 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 2, SA, (int)sa, 0, (int)b.sc);
 }
 
@@ -233,8 +235,8 @@ HX_DEV mx_v16f mx_zero16() {
   return z;
 }
 
-// silu(g) u
-HX_DEV float mx_swiglu(float g, float u) { return siluf_(g) * u; }
+// silu(g) u, the division by v_rcp_f32 (1 ulp)
+HX_DEV float mx_swiglu(float g, float u) { return silu_rcp(g) * u; }
 
 // ---------------------------------------------------------------- few tokens
 // The routing of a few tokens in LDS.
@@ -752,27 +754,68 @@ hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s) {
 // rows of a tile: 32 when the experts have few rows each
 int mx_tile_m(int64_t F, int E) { return F <= 24 * (int64_t)E ? 32 : 64; }
 
-// LDS of a stage: [4 blocks][TM rows][record]; the stage's records come in by direct
-// loads, 16 bytes a lane, in LDS order
+// The tile's rows in LDS, CB blocks of K at a time: [CB blocks][TM rows][record]. The
+// records come in by direct loads, 16 bytes a lane, in LDS order; a unit of U blocks is
+// whole KiB loads.
 template <int TM, int P>
-struct MxStage {
+struct MxRows {
   static constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
-  static constexpr int BYTES = 4 * TM * RB, LOADS = BYTES / 1024, PER = (LOADS + 3) / 4;   // loads: in all, a wave
-  const uint8_t* src[PER];
+  static constexpr int CB = P == 3 ? 16 : 8, BYTES = CB * TM * RB;
+  static constexpr int U = TM * RV % 64 == 0 ? 1 : 2, LOADS = U * TM * RV / 64;
+  static_assert(U * TM * RV % 64 == 0, "whole loads");
+  const uint8_t* src[LOADS];
   // rowptr(r): the records of the tile's row r
   template <typename F>
-  HX_DEV void init(int wave, int lane, F rowptr) {
+  HX_DEV void init(F rowptr) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int q = (wave + 4 * i) * 64 + lane;   // 16-byte piece of the stage
-      const int kb = min(q / (TM * RV), 3), r = q / RV % TM, j = q % RV;
-      src[i] = rowptr(r) + kb * RB + 16 * j;
+    for (int i = 0; i < LOADS; i++) {
+      const int q = i * 64 + lane_id();   // 16-byte piece of the unit
+      src[i] = rowptr(q / RV % TM) + q / (TM * RV) * RB + q % RV * 16;
     }
   }
-  HX_DEV void issue(int wave, int st, uint32_t lds) const {
+  // blocks b0 .. min(b0 + CB, nblk) - 1 (a multiple of 4)
+  HX_DEV void load(int wave, int b0, int nblk, uint32_t lds) const {
+    const int n = min(CB, nblk - b0) / U;
+    for (int u = wave; u < n; u += 4)
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-      if (LOADS % 4 == 0 || wave + 4 * i < LOADS) dma16(src[i] + (int64_t)st * (4 * RB), lds + (wave + 4 * i) * 1024);
+      for (int i = 0; i < LOADS; i++) dma16(src[i] + (int64_t)(b0 + u * U) * RB, lds + (u * LOADS + i) * 1024);
+  }
+};
+
+// A wave's weights: NM matrices' tiles of 32 rows, R steps of K on their way at any
+// time; a step's registers are loaded again as soon as its MFMAs are issued. (Loaded a
+// stage ahead into a second set, with a barrier and a wait for everything at each
+// stage of 128 columns, the wait was never over in time: MFMAs busy 41 % at 8192 tokens.)
+template <int P, int NM>
+struct MxRing {
+  // steps, words of scales; a chunk of rows is whole turns of the ring
+  static constexpr int R = P == 3 ? (NM == 2 ? 8 : 2) : 4, U = R < 4 ? 4 : R, W = U / 4;
+  static_assert(MxRows<32, P>::CB / 2 % U == 0, "whole turns");
+  // byte offsets of the matrices' tiles from mat[m % 2]; buffer loads, so that the lanes'
+  // addresses take one register in all
+  __amdgpu_buffer_rsrc_t mat[2];
+  int codes[NM], scales[NM];
+  mx_v4u w[R][NM];
+  uint32_t sc[W][NM];
+  HX_DEV void matrix(int q, const uint8_t* base, int rows, int K) {
+    mat[q] = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)mx_mat_bytes(rows, K), 0x00027000);
+  }
+  HX_DEV void fetch(int i, int s) {
+#pragma unroll
+    for (int m = 0; m < NM; m++)
+      w[i][m] = __builtin_amdgcn_raw_buffer_load_b128(mat[m % 2], lane_id() * 16, codes[m] + s * 1024, 0);
+  }
+  HX_DEV void fetch_scales(int j, int s) {   // of steps s .. s + 3
+#pragma unroll
+    for (int m = 0; m < NM; m++)
+      sc[j][m] = __builtin_amdgcn_raw_buffer_load_b32(mat[m % 2], lane_id() * 4, scales[m] + (s >> 2) * 256, 0);
+  }
+  HX_DEV void start(int S) {
+#pragma unroll
+    for (int j = 0; j < W; j++) fetch_scales(j, min(4 * j, S - 1));
+#pragma unroll
+    for (int i = 0; i < R; i++)
+      if (i < S) fetch(i, i);
   }
 };
 
@@ -788,54 +831,52 @@ HX_DEV void mx_tile(int NX, int N, int& nt, int& tile) {
   if (i >= per || tile >= N) tile = -1;
 }
 
-// the 4 waves' sums over K: NM weight matrices' 32-row tiles (one each) times the
-// tile's rows
-template <int TM, int P, int NM>
-HX_DEV void mx_products(const MxStage<TM, P>& sg, uint8_t* buf, int nst, const uint8_t* (&codes)[NM],
-                        const uint8_t* (&scales)[NM], bool live, mx_v16f (&acc)[NM][TM / 32]) {
-  constexpr int RB = MxRec<P>::BYTES;
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
-  uint4 w[2][NM][2];
-  uint32_t sc[2][NM];
-  auto fetch = [&](int st, int b) {
+// steps s0 .. s1 - 1 (s0 a multiple of R) of S: acc += the ring's weights x the rows in buf
+template <int TM, int P, int NM, int I = 0>
+HX_DEV void mx_steps_of(MxRing<P, NM>& ring, const uint8_t* rec, int s, int s1, int S, mx_v16f (&acc)[NM][TM / 32]) {
+  constexpr int RB = MxRec<P>::BYTES, R = MxRing<P, NM>::R, U = MxRing<P, NM>::U;
+  if constexpr (I < U) {
+    if (s + I < s1) {
 #pragma unroll
-    for (int m = 0; m < NM; m++) {
-      w[b][m][0] = *(const uint4*)(codes[m] + st * 2048 + lane * 16);
-      w[b][m][1] = *(const uint4*)(codes[m] + st * 2048 + 1024 + lane * 16);
-      sc[b][m] = *(const uint32_t*)(scales[m] + (st >> 1) * 256 + lane * 4);   // b = st % 2: bytes 2 b, 2 b + 1
+      for (int n = 0; n < TM / 32; n++) {
+        MxB<P> b;
+        b.load(rec + (2 * I * TM + 32 * n) * RB);
+        mx_mfma<P, I & 3>(ring.w[I % R], ring.sc[I / 4], b, acc, n);
+      }
+      if (s + I + R < S) ring.fetch(I % R, s + I + R);
+      if (I % 4 == 3 && s + I + U - 3 < S) ring.fetch_scales(I / 4, s + I + U - 3);
+      __builtin_amdgcn_sched_barrier(0);
+      mx_steps_of<TM, P, NM, I + 1>(ring, rec, s, s1, S, acc);
     }
-  };
-  sg.issue(wave, 0, lds);
-  if (live) fetch(0, 0);
-  auto stage = [&](int st, auto bc) {
-    constexpr int b = decltype(bc)::value;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (st + 1 < nst) {
-      sg.issue(wave, st + 1, lds + (b ^ 1) * MxStage<TM, P>::BYTES);
-      if (live) fetch(st + 1, b ^ 1);
-    }
-    if (live) {
-      auto step = [&](auto sc_) {
-        constexpr int s = decltype(sc_)::value;
-#pragma unroll
-        for (int n = 0; n < TM / 32; n++) {
-          MxB<P> bb;
-          bb.load(buf + b * MxStage<TM, P>::BYTES + ((2 * s + (lane >> 5)) * TM + 32 * n + (lane & 31)) * RB);
-          mx_mfma<P, s, 2 * b + s>(w[b], sc[b], bb, acc, n);
-        }
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-    }
-  };
-  int st = 0;
-  for (; st + 2 <= nst; st += 2) {
-    stage(st, std::integral_constant<int, 0>{});
-    stage(st + 1, std::integral_constant<int, 1>{});
   }
-  if (st < nst) stage(st, std::integral_constant<int, 0>{});
+}
+// acc = the sums over nblk blocks of K of the ring's weights x the tile's rows
+template <int TM, int P, int NM>
+HX_DEV void mx_products(MxRing<P, NM>& ring, const MxRows<TM, P>& rw, int wave, uint8_t* buf, int nblk,
+                        mx_v16f (&acc)[NM][TM / 32]) {
+  constexpr int RB = MxRec<P>::BYTES, U = MxRing<P, NM>::U, CB = MxRows<TM, P>::CB;
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
+  const int lane = lane_id(), S = nblk / 2;
+  const uint8_t* rec = buf + ((lane >> 5) * TM + (lane & 31)) * RB;
+#pragma unroll
+  for (int m = 0; m < NM; m++)
+#pragma unroll
+    for (int n = 0; n < TM / 32; n++) acc[m][n] = mx_zero16();
+  ring.start(S);
+  for (int b0 = 0; b0 < nblk; b0 += CB) {
+    if (b0) lds_barrier();
+    rw.load(wave, b0, nblk, lds);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    for (int s = b0 / 2; s < min(S, (b0 + CB) / 2); s += U)
+      mx_steps_of<TM, P, NM>(ring, rec + (2 * s - b0) * TM * RB, s, min(S, (b0 + CB) / 2), S, acc);
+  }
+  // the sums leave the loop whole: seen through, their elements are carried through it
+  // one by one as well, and spilled
+#pragma unroll
+  for (int m = 0; m < NM; m++)
+#pragma unroll
+    for (int n = 0; n < TM / 32; n++) asm volatile("" : "+v"(acc[m][n]));
 }
 
 // lane l: the 32 values of column l of the tile from D's halves
@@ -854,7 +895,7 @@ HX_DEV void mx_columns(const mx_v16f (&d)[TM / 32], float (&f)[32]) {
 template <int TM, int P, int MF>
 __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
-  __shared__ __align__(16) uint8_t buf[2 * MxStage<TM, P>::BYTES];
+  __shared__ __align__(16) uint8_t buf[MxRows<TM, P>::BYTES];
   int nt, tile;
   mx_tile((a.hblocks + 4 * MF - 1) / (4 * MF), a.counts[0], nt, tile);
   if (tile < 0) return;
@@ -865,30 +906,23 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   if (4 * MF * nt >= mx_blocks(inter)) return;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int f0 = (4 * nt + wave) * MF, HB = mx_blocks(a.H), S = mx_steps(a.H), S4 = (S + 3) / 4;
-  const bool live = 32 * f0 < inter;
-  MxStage<TM, P> sg;
-  sg.init(wave, lane, [&](int r) {
+  MxRows<TM, P> rw;
+  rw.init([&](int r) {
     const int p = p0 + min(r, rows - 1);
     const int t = sh ? p - a.F : a.perm[p] / a.k;
     return a.xrec + (int64_t)t * HB * RB;
   });
-  const uint8_t *codes[2 * MF], *scales[2 * MF];
+  MxRing<P, 2 * MF> ring;
+  ring.matrix(0, sh ? a.sgate.base : a.gate.mat(e), inter, a.H);
+  ring.matrix(1, sh ? a.sup.base : a.up.mat(e), inter, a.H);
 #pragma unroll
   for (int m = 0; m < MF; m++) {
     const int fb = min(f0 + m, inter / 32 - 1);
-#pragma unroll
-    for (int q = 0; q < 2; q++) {
-      const uint8_t* mat = q ? (sh ? a.sup.base : a.up.mat(e)) : (sh ? a.sgate.base : a.gate.mat(e));
-      codes[2 * m + q] = mat + (int64_t)fb * S * 1024;
-      scales[2 * m + q] = mat + mx_code_bytes(inter, a.H) + (int64_t)fb * S4 * 256;
-    }
+    ring.codes[2 * m] = ring.codes[2 * m + 1] = fb * S * 1024;
+    ring.scales[2 * m] = ring.scales[2 * m + 1] = (int)mx_code_bytes(inter, a.H) + fb * S4 * 256;
   }
   mx_v16f acc[2 * MF][TM / 32];
-#pragma unroll
-  for (int m = 0; m < 2 * MF; m++)
-#pragma unroll
-    for (int n = 0; n < TM / 32; n++) acc[m][n] = mx_zero16();
-  mx_products<TM, P, 2 * MF>(sg, buf, HB / 4, codes, scales, live, acc);
+  mx_products<TM, P, 2 * MF>(ring, rw, wave, buf, HB, acc);
 #pragma unroll
   for (int m = 0; m < MF; m++) {
     mx_v16f h[TM / 32];
@@ -912,37 +946,34 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
 // outputs of the experts, unweighted: 64 MF features a wave
 template <int TM, int P, int MF>
 __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
-  constexpr int RB = MxRec<P>::BYTES;
-  __shared__ __align__(16) uint8_t buf[2 * MxStage<TM, P>::BYTES];
+  constexpr int RB = MxRec<P>::BYTES, NM = 2 * MF;
+  __shared__ __align__(16) uint8_t buf[MxRows<TM, P>::BYTES];
   int nt, tile;
-  mx_tile((a.H + 256 * MF - 1) / (256 * MF), a.counts[0], nt, tile);
+  const int nb = a.H / 32;
+  mx_tile((nb + 4 * NM - 1) / (4 * NM), a.counts[0], nt, tile);
   if (tile < 0) return;
   const int4 ti = ((const int4*)a.tiles)[tile];
   const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
   const bool sh = e == a.E;
   const int inter = sh ? a.Is : a.I;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int S = mx_steps(inter), S4 = (S + 3) / 4, nb = a.H / 32;
-  const int n0 = (4 * nt + wave) * 2 * MF;
-  const bool live = n0 < nb;
-  MxStage<TM, P> sg;
-  sg.init(wave, lane, [&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * RB; });
-  const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
-  const uint8_t *codes[2 * MF], *scales[2 * MF];
+  const int IB = mx_blocks(inter), S = mx_steps(inter), S4 = (S + 3) / 4, n0 = (4 * nt + wave) * NM;
+  MxRows<TM, P> rw;
+  rw.init([&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * RB; });
+  MxRing<P, NM> ring;
+  ring.matrix(0, sh ? a.sdown.base : a.down.mat(e), a.H, inter);
+  ring.mat[1] = ring.mat[0];
 #pragma unroll
-  for (int m = 0; m < 2 * MF; m++) {
-    const int n = min(n0 + m, nb - 1);
-    codes[m] = dm + (int64_t)n * S * 1024;
-    scales[m] = dm + mx_code_bytes(a.H, inter) + (int64_t)n * S4 * 256;
+  for (int m = 0; m < NM; m++) {
+    const int n = min(n0 + m, nb - 1);   // past the last: computed again, not stored
+    ring.codes[m] = n * S * 1024;
+    ring.scales[m] = (int)mx_code_bytes(a.H, inter) + n * S4 * 256;
   }
-  mx_v16f acc[2 * MF][TM / 32];
+  mx_v16f acc[NM][TM / 32];
+  mx_products<TM, P, NM>(ring, rw, wave, buf, IB, acc);
 #pragma unroll
-  for (int m = 0; m < 2 * MF; m++)
-#pragma unroll
-    for (int n = 0; n < TM / 32; n++) acc[m][n] = mx_zero16();
-  mx_products<TM, P, 2 * MF>(sg, buf, mx_blocks(inter) / 4, codes, scales, live, acc);
-#pragma unroll
-  for (int m = 0; m < 2 * MF; m++) {
+  for (int m = 0; m < NM; m++) {
+    __builtin_amdgcn_sched_barrier(0);   // one matrix's outputs after the other's: all at once do not fit the registers
     float f[32];
     mx_columns<TM>(acc[m], f);
     if (lane < TM && lane < rows && n0 + m < nb) {
@@ -966,20 +997,25 @@ __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   }
 }
 
-#define MX_LAUNCH(KERNEL, N, PER)                                                             \
-  auto go = [&](auto kernel, int mf) {                                                        \
-    const int64_t nx = ((N) + (PER) * mf - 1) / ((PER) * mf);                                 \
-    hx_launch(kernel, dim3((unsigned)(nx * ((a.max_tiles + 7) / 8 * 8))), dim3(256), 0, s, a); \
-  };                                                                                          \
-  if (a.xbf && a.tile_m == 32) go(KERNEL<32, 3, 1>, 1);                                       \
-  else if (a.xbf) go(KERNEL<64, 3, MX_MF>, MX_MF);                                            \
-  else if (a.tile_m == 32) go(KERNEL<32, 5, 1>, 1);                                           \
-  else go(KERNEL<64, 5, 1>, 1);                                                               \
-  return hipGetLastError()
-
+// groups of 32 features a wave takes at a time
 constexpr int MX_MF = 2;
-hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_gate_up, a.hblocks, 4); }
-hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) { MX_LAUNCH(k_mx_down, a.H / 32, 8); }
+#define MX_LAUNCH(KERNEL, NX)                                                                    \
+  auto go = [&](auto kernel, int mf) {                                                           \
+    hx_launch(kernel, dim3((unsigned)((int64_t)(NX) * ((a.max_tiles + 7) / 8 * 8))), dim3(256), 0, s, a); \
+  };                                                                                             \
+  if (a.xbf && a.tile_m == 32) go(KERNEL<32, 3, 1>, 1);                                          \
+  else if (a.xbf) go(KERNEL<64, 3, MX_MF>, MX_MF);                                               \
+  else if (a.tile_m == 32) go(KERNEL<32, 5, 1>, 1);                                              \
+  else go(KERNEL<64, 5, 1>, 1)
+
+hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) {
+  MX_LAUNCH(k_mx_gate_up, (a.hblocks + 4 * mf - 1) / (4 * mf));
+  return hipGetLastError();
+}
+hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) {
+  MX_LAUNCH(k_mx_down, (a.H / 32 + 8 * mf - 1) / (8 * mf));
+  return hipGetLastError();
+}
 
 // y[t] = the token's entries' rows times their weights in their order, then the
 // shared expert's: 8 outputs a thread
