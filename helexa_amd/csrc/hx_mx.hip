@@ -789,33 +789,46 @@ struct MxRows {
 template <int P, int NM>
 struct MxRing {
   // steps, words of scales; a chunk of rows is whole turns of the ring
-  static constexpr int R = P == 3 ? (NM == 2 ? 8 : 2) : 4, U = R < 4 ? 4 : R, W = U / 4;
+  static constexpr int R = 8 / NM, U = R < 4 ? 4 : R, W = U / 4;
   static_assert(MxRows<32, P>::CB / 2 % U == 0, "whole turns");
   // byte offsets of the matrices' tiles from mat[m % 2]; buffer loads, so that the lanes'
   // addresses take one register in all
   __amdgpu_buffer_rsrc_t mat[2];
   int codes[NM], scales[NM];
   mx_v4u w[R][NM];
-  uint32_t sc[W][NM];
+  uint32_t sc[W][NM], sn[W][NM];   // of this turn and of the next
   HX_DEV void matrix(int q, const uint8_t* base, int rows, int K) {
     mat[q] = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)mx_mat_bytes(rows, K), 0x00027000);
   }
-  HX_DEV void fetch(int i, int s) {
+  // Steps past the last (s >= S) are loaded from past the matrix's end, which reads
+  // nothing and gives zeros: a branch around the loads would copy the ring where it
+  // joins, and so wait for all of it.
+  HX_DEV static int lane_offset(int size, bool has) { return lane_id() * size + (has ? 0 : 0x40000000); }
+  HX_DEV void fetch(int i, int s, int S) {
+    const int o = lane_offset(16, s < S);
 #pragma unroll
     for (int m = 0; m < NM; m++)
-      w[i][m] = __builtin_amdgcn_raw_buffer_load_b128(mat[m % 2], lane_id() * 16, codes[m] + s * 1024, 0);
+      w[i][m] = __builtin_amdgcn_raw_buffer_load_b128(mat[m % 2], o, s < S ? codes[m] + s * 1024 : 0, 0);
   }
-  HX_DEV void fetch_scales(int j, int s) {   // of steps s .. s + 3
+  HX_DEV void fetch_scales(int j, int s, int S) {   // of steps s .. s + 3
+    const int o = lane_offset(4, s < S);
 #pragma unroll
     for (int m = 0; m < NM; m++)
-      sc[j][m] = __builtin_amdgcn_raw_buffer_load_b32(mat[m % 2], lane_id() * 4, scales[m] + (s >> 2) * 256, 0);
+      sn[j][m] = __builtin_amdgcn_raw_buffer_load_b32(mat[m % 2], o, s < S ? scales[m] + (s >> 2) * 256 : 0, 0);
   }
   HX_DEV void start(int S) {
 #pragma unroll
-    for (int j = 0; j < W; j++) fetch_scales(j, min(4 * j, S - 1));
+    for (int j = 0; j < W; j++) fetch_scales(j, 4 * j, S);
 #pragma unroll
-    for (int i = 0; i < R; i++)
-      if (i < S) fetch(i, i);
+    for (int i = 0; i < R; i++) fetch(i, i, S);
+  }
+  HX_DEV void turn(int s, int S) {   // the scales of steps s .. become this turn's, the next are fetched
+#pragma unroll
+    for (int j = 0; j < W; j++) {
+#pragma unroll
+      for (int m = 0; m < NM; m++) sc[j][m] = sn[j][m];
+      fetch_scales(j, s + U + 4 * j, S);
+    }
   }
 };
 
@@ -831,22 +844,22 @@ HX_DEV void mx_tile(int NX, int N, int& nt, int& tile) {
   if (i >= per || tile >= N) tile = -1;
 }
 
-// steps s0 .. s1 - 1 (s0 a multiple of R) of S: acc += the ring's weights x the rows in buf
-template <int TM, int P, int NM, int I = 0>
-HX_DEV void mx_steps_of(MxRing<P, NM>& ring, const uint8_t* rec, int s, int s1, int S, mx_v16f (&acc)[NM][TM / 32]) {
+// a turn of the ring from step s of S: acc += its weights x the rows at rec; LAST: no
+// steps of a turn after it are fetched
+template <int TM, int P, int NM, bool LAST, int I = 0>
+HX_DEV void mx_turn(MxRing<P, NM>& ring, const uint8_t* rec, int s, int S, mx_v16f (&acc)[NM][TM / 32]) {
   constexpr int RB = MxRec<P>::BYTES, R = MxRing<P, NM>::R, U = MxRing<P, NM>::U;
   if constexpr (I < U) {
-    if (s + I < s1) {
+    if (!LAST || s + I < S) {
 #pragma unroll
       for (int n = 0; n < TM / 32; n++) {
         MxB<P> b;
         b.load(rec + (2 * I * TM + 32 * n) * RB);
         mx_mfma<P, I & 3>(ring.w[I % R], ring.sc[I / 4], b, acc, n);
       }
-      if (s + I + R < S) ring.fetch(I % R, s + I + R);
-      if (I % 4 == 3 && s + I + U - 3 < S) ring.fetch_scales(I / 4, s + I + U - 3);
+      if (!LAST || I + R < U) ring.fetch(I % R, s + I + R, S);
       __builtin_amdgcn_sched_barrier(0);
-      mx_steps_of<TM, P, NM, I + 1>(ring, rec, s, s1, S, acc);
+      mx_turn<TM, P, NM, LAST, I + 1>(ring, rec, s, S, acc);
     }
   }
 }
@@ -863,14 +876,21 @@ HX_DEV void mx_products(MxRing<P, NM>& ring, const MxRows<TM, P>& rw, int wave, 
 #pragma unroll
     for (int n = 0; n < TM / 32; n++) acc[m][n] = mx_zero16();
   ring.start(S);
-  for (int b0 = 0; b0 < nblk; b0 += CB) {
-    if (b0) lds_barrier();
+  int s = 0, b0 = 0;   // a chunk is whole turns; the last turn comes after the loop
+  for (;;) {
     rw.load(wave, b0, nblk, lds);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
-    for (int s = b0 / 2; s < min(S, (b0 + CB) / 2); s += U)
-      mx_steps_of<TM, P, NM>(ring, rec + (2 * s - b0) * TM * RB, s, min(S, (b0 + CB) / 2), S, acc);
+    for (const int end = min(S - U, (b0 + CB) / 2); s < end; s += U) {
+      ring.turn(s, S);
+      mx_turn<TM, P, NM, false>(ring, rec + (2 * s - b0) * TM * RB, s, S, acc);
+    }
+    if (b0 + CB >= nblk) break;
+    b0 += CB;
+    lds_barrier();
   }
+  ring.turn(s, S);
+  mx_turn<TM, P, NM, true>(ring, rec + (2 * s - b0) * TM * RB, s, S, acc);
   // the sums leave the loop whole: seen through, their elements are carried through it
   // one by one as well, and spilled
 #pragma unroll
