@@ -287,18 +287,51 @@ __host__ __device__ inline int mx_wave_steps(int S, int W) {
 // made in LDS by every workgroup: a kernel of their own would cost more than it saves.
 // The planes are columns: with them one after the other the products took 8 of the
 // 26 us of 6 tokens' 64 MB.
-template <int P, int KW>
-__global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
+// ONE token: an expert a chosen entry, its weights on their way before anything else.
+template <int P, int KW, bool ONE>
+__global__ __launch_bounds__(512, ONE ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, FW = 8 / KW;
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ MxFew few;
-  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = a.T;
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = ONE ? 1 : a.T;
   const int slot = blockIdx.y, fb = blockIdx.x * FW + wave / KW, kq = wave % KW;
   const int S = mx_steps(a.H), S4 = (S + 3) / 4, HB = mx_blocks(a.H);
-  int e = a.E;
-  if (T == 1) {   // a slot per entry
+  const int c = mx_wave_steps(S, KW), s0 = kq * c, s1 = min(S, s0 + c);
+  int e = a.E, inter = a.Is;
+  int64_t at = 0, sat = 0;
+  const uint8_t *gm = nullptr, *um = nullptr;
+  bool work = false;
+  // four steps of weights are on their way at any time
+  uint4 wg[4], wu[4];
+  auto fetch = [&](int s, int i) {
+    wg[i] = *(const uint4*)(gm + (at + s * 1024) + lane * 16);
+    wu[i] = *(const uint4*)(um + (at + s * 1024) + lane * 16);
+  };
+  uint32_t sg, su;
+  auto fetch_scales = [&](int s) {
+    sg = *(const uint32_t*)(gm + (sat + (s >> 2) * 256) + lane * 4);
+    su = *(const uint32_t*)(um + (sat + (s >> 2) * 256) + lane * 4);
+  };
+  // the slot's expert is known: its weights
+  auto start = [&]() {
+    e = __builtin_amdgcn_readfirstlane(e);
+    const bool sh = e == a.E;
+    inter = sh ? a.Is : a.I;
+    gm = sh ? a.sgate.base : a.gate.mat(e);
+    um = sh ? a.sup.base : a.up.mat(e);
+    at = (int64_t)fb * S * 1024;
+    sat = mx_code_bytes(inter, a.H) + (int64_t)fb * S4 * 256;
+    work = 32 * fb < inter && s0 < s1;   // the others: a record behind the last feature, or none
+    if (!work) return;
+    fetch_scales(s0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) fetch(min(s0 + i, s1 - 1), i);
+  };
+  if (ONE) {
     if (slot < a.k) e = a.idx[slot];
     if (slot < a.k && (unsigned)e >= (unsigned)a.E) return;
+    start();
+    if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
   }
   for (int b = tid; b < T * HB; b += 512) {
     const int t = b / HB, kb = b % HB;
@@ -315,7 +348,7 @@ __global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
 #pragma unroll
     for (int i = 0; i < RV; i++) ((uint4*)zrec)[i] = r[i];
   }
-  if (T > 1) {
+  if (!ONE) {
     mx_few_bits(a, few);
     int n;
     e = mx_few_slot(few, slot, n);
@@ -323,32 +356,8 @@ __global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
       if (slot > n || a.Is == 0) return;
       e = a.E;
     }
-  }
-  e = __builtin_amdgcn_readfirstlane(e);
-  const bool sh = e == a.E;
-  const int inter = sh ? a.Is : a.I;
-  if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
-  const int c = mx_wave_steps(S, KW), s0 = kq * c, s1 = min(S, s0 + c);
-  const bool live = 32 * fb < inter;   // the others: a record behind the last feature, or none
-  const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
-  const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
-  const int64_t at = (int64_t)fb * S * 1024, sat = mx_code_bytes(inter, a.H) + (int64_t)fb * S4 * 256;
-  // four steps of weights are on their way at any time
-  uint4 wg[4], wu[4];
-  auto fetch = [&](int s, int i) {
-    wg[i] = *(const uint4*)(gm + (at + s * 1024) + lane * 16);
-    wu[i] = *(const uint4*)(um + (at + s * 1024) + lane * 16);
-  };
-  uint32_t sg, su;
-  auto fetch_scales = [&](int s) {
-    sg = *(const uint32_t*)(gm + (sat + (s >> 2) * 256) + lane * 4);
-    su = *(const uint32_t*)(um + (sat + (s >> 2) * 256) + lane * 4);
-  };
-  const bool work = live && s0 < s1;
-  if (work) {
-    fetch_scales(s0);
-#pragma unroll
-    for (int i = 0; i < 4; i++) fetch(min(s0 + i, s1 - 1), i);
+    start();
+    if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
   }
   lds_barrier();
   mx_v16f ag = mx_zero16(), au = mx_zero16();
@@ -420,8 +429,9 @@ __global__ __launch_bounds__(512, 4) void k_mx_few_gate_up(MxArgs a) {
   if (tid < FW * T) {
     const int ft = tid / T, tt = tid % T, f0 = blockIdx.x * FW + ft;
     // the row of h: the token's first entry with this expert
+    const bool sh = e == a.E;
     int row = sh ? a.F + tt : -1;
-    if (!sh && T == 1) row = slot;
+    if (!sh && ONE) row = slot;
     else if (!sh)
       for (int j = a.k - 1; j >= 0; j--)
         if (few.idx[tt * a.k + j] == e) row = tt * a.k + j;
@@ -456,11 +466,11 @@ bool mx_few(int T, int k, int H, bool xbf) {
 // most chosen experts of a call (one token: its entries)
 static int mx_few_slots(int T, int k, int E) { return T == 1 ? k : min(T * k, E); }
 
-// units of the down kernel: an expert's products over 4 steps of K
+// units of the down kernel: an expert's products over 8 steps of K
 int mx_few_parts(int T, int k, int E, int I, int Is) {
-  const int G = (mx_steps(I) + 3) / 4, Gs = Is > 0 ? (mx_steps(Is) + 3) / 4 : 0;
+  const int G = (mx_steps(I) + 7) / 8, Gs = Is > 0 ? (mx_steps(Is) + 7) / 8 : 0;
   const int units = mx_few_slots(T, k, E) * G + Gs;
-  return units <= 32 ? 1 : min(MX_FEW_PARTS, (units + 31) / 32);
+  return min(MX_FEW_PARTS, (units + 15) / 16);
 }
 
 HX_DEV void mx_store(const MxArgs& a, int64_t at, float y) {
@@ -475,10 +485,10 @@ HX_DEV void mx_store(const MxArgs& a, int64_t at, float y) {
 }
 
 // Down and combine of up to 8 tokens. Workgroup: 32 outputs and a part of the units
-// (slot, 4 steps of K), which its 16 waves take in turn; each unit's product is
+// (slot, 8 steps of K), which its 16 waves take in turn; each unit's product is
 // weighted per token in f32, the waves' sums are added in LDS. One part writes y, several their
 // sums for k_mx_few_sum.
-template <int P>
+template <int P, bool ONE>
 __global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES;
   __shared__ MxFew few;
@@ -486,16 +496,11 @@ __global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
   __shared__ float red[16 * 32 * (P == 3 ? 24 : 30)];
   __shared__ int pre[33];
   __shared__ uint16_t list[MX_FEW_T * HX_MAX_TOPK];
-  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = a.T, k = a.k;
-  const int nb = blockIdx.x, parts = gridDim.y;
-  for (int f = tid; f < a.F; f += 1024) sw[f] = a.w[f];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int T = ONE ? 1 : a.T, k = a.k, nb = blockIdx.x, parts = gridDim.y;
   int n = k;
-  if (T == 1) {
-    if (tid < k) {
-      few.idx[tid] = a.idx[tid];
-    }
-    lds_barrier();
-  } else {
+  if (!ONE) {
+    for (int f = tid; f < a.F; f += 1024) sw[f] = a.w[f];
     mx_few_bits(a, few);
     if (tid < 64) {
       const int c = tid < 32 ? __popc(few.bits[tid]) : 0;
@@ -516,22 +521,24 @@ __global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
     lds_barrier();
     n = pre[32];
   }
-  const int S = mx_steps(a.I), G = (S + 3) / 4, Ss = mx_steps(a.Is), Gs = a.Is ? (Ss + 3) / 4 : 0;
+  const int S = mx_steps(a.I), G = (S + 7) / 8, Ss = mx_steps(a.Is), Gs = a.Is ? (Ss + 7) / 8 : 0;
   const int col = lane & 31, half = lane >> 5, C = P * T, p = col / T, t = col % T;
   mx_v16f acc = mx_zero16();
   for (int u = blockIdx.y * 16 + wave; u < n * G + Gs; u += 16 * parts) {
     const bool sh = u >= n * G;
     const int slot = sh ? n : u / G, g = sh ? u - n * G : u % G;
     int e = a.E;
-    if (!sh) e = __builtin_amdgcn_readfirstlane(T == 1 ? few.idx[slot] : (int)list[slot]);
-    if (!sh && T == 1 && (unsigned)e >= (unsigned)a.E) continue;
+    if (!sh) e = __builtin_amdgcn_readfirstlane(ONE ? a.idx[slot] : (int)list[slot]);
+    if (!sh && ONE && (unsigned)e >= (unsigned)a.E) continue;
     const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
-    const int inter = sh ? a.Is : a.I, St = sh ? Ss : S, S4 = (St + 3) / 4, s = 4 * g;
+    const int inter = sh ? a.Is : a.I, St = sh ? Ss : S, S4 = (St + 3) / 4, s = 8 * g;
     const uint8_t* wp = dm + ((int64_t)nb * St + s) * 1024;
-    const uint32_t sa = *(const uint32_t*)(dm + (mx_code_bytes(a.H, inter) + ((int64_t)nb * S4 + g) * 256) + lane * 4);
-    uint4 wd[4];
+    const uint8_t* sp = dm + (mx_code_bytes(a.H, inter) + ((int64_t)nb * S4 + 2 * g) * 256);
+    uint4 wd[8];
+    const uint32_t sa = *(const uint32_t*)(sp + lane * 4);
+    const uint32_t sb = *(const uint32_t*)(sp + (2 * g + 1 < S4 ? 256 : 0) + lane * 4);
 #pragma unroll
-    for (int i = 0; i < 4; i++) wd[i] = *(const uint4*)(wp + min(i, St - 1 - s) * 1024 + lane * 16);
+    for (int i = 0; i < 8; i++) wd[i] = *(const uint4*)(wp + min(i, St - 1 - s) * 1024 + lane * 16);
     // the token's row of h with this expert, and its weight
     int row = -1;
     float wt = 0.f;
@@ -539,9 +546,9 @@ __global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
       if (sh) {
         row = a.F + t;
         wt = a.shared_w[t];
-      } else if (T == 1) {
+      } else if (ONE) {
         row = slot;
-        wt = sw[slot];
+        wt = a.w[slot];
       } else {
         for (int j = k - 1; j >= 0; j--)
           if (few.idx[t * k + j] == e) {
@@ -552,14 +559,14 @@ __global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
     }
     const uint8_t* hp = a.hrec + ((int64_t)max(row, 0) * a.hblocks + 2 * s + half) * RB;
     mx_v16f d = mx_zero16();
-#define MX_STEP(i)                                    \
-  if (s + i < St) {                                   \
-    MxPlane b;                                        \
-    b.zero();                                         \
-    if (row >= 0) b.load<P>(hp + 2 * i * RB, p);      \
-    d = mx_mfma1<i>(wd[i], sa, b, d);                 \
+#define MX_STEP(i)                                            \
+  if (s + i < St) {                                           \
+    MxPlane b;                                                \
+    b.zero();                                                 \
+    if (row >= 0) b.load<P>(hp + 2 * i * RB, p);              \
+    d = mx_mfma1<(i & 3)>(wd[i], i < 4 ? sa : sb, b, d);      \
   }
-    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3) MX_STEP(4) MX_STEP(5) MX_STEP(6) MX_STEP(7)
 #undef MX_STEP
     // a token that is not this expert's adds nothing, whatever the weights hold
 #pragma unroll
@@ -598,11 +605,13 @@ static void mx_few_gate_up(const MxArgs& a, hipStream_t s) {
   const int slots = mx_few_slots(a.T, a.k, a.E) + (a.Is > 0 ? 1 : 0), tasks = slots * a.hblocks;
   const uint32_t lds = (uint32_t)mx_few_lds(a.T, a.H, a.xbf);
   // enough waves to keep two on each of the 1024 SIMDs, no more
-#define FGU(KW) hx_launch(k_mx_few_gate_up<P, KW>, dim3((a.hblocks + 8 / KW - 1) / (8 / KW), slots), dim3(512), lds, s, a)
-  if (tasks >= 2048) FGU(1);
-  else if (2 * tasks >= 2048) FGU(2);
-  else if (4 * tasks >= 2048) FGU(4);
-  else FGU(8);
+#define FGU(KW, ONE) \
+  hx_launch(k_mx_few_gate_up<P, KW, ONE>, dim3((a.hblocks + 8 / KW - 1) / (8 / KW), slots), dim3(512), lds, s, a)
+  if (a.T == 1) FGU(8, true);
+  else if (tasks >= 2048) FGU(1, false);
+  else if (2 * tasks >= 2048) FGU(2, false);
+  else if (4 * tasks >= 2048) FGU(4, false);
+  else FGU(8, false);
 #undef FGU
 }
 
@@ -615,8 +624,10 @@ hipError_t launch_mx_few_gate_up(const MxArgs& a, hipStream_t s) {
 hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s) {
   const int parts = mx_few_parts(a.T, a.k, a.E, a.I, a.Is);
   const dim3 g(a.H / 32, parts);
-  if (a.xbf) hx_launch(k_mx_few_down<3>, g, dim3(1024), 0, s, a);
-  else hx_launch(k_mx_few_down<5>, g, dim3(1024), 0, s, a);
+  if (a.xbf && a.T == 1) hx_launch(k_mx_few_down<3, true>, g, dim3(1024), 0, s, a);
+  else if (a.xbf) hx_launch(k_mx_few_down<3, false>, g, dim3(1024), 0, s, a);
+  else if (a.T == 1) hx_launch(k_mx_few_down<5, true>, g, dim3(1024), 0, s, a);
+  else hx_launch(k_mx_few_down<5, false>, g, dim3(1024), 0, s, a);
   return hipGetLastError();
 }
 

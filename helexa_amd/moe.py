@@ -297,29 +297,32 @@ class Qwen3_5MoeBlock:
         import torch
         H, k = self.cfg.hidden_size, self.cfg.num_experts_per_tok
         _check_acts(xs, H, self.act_dtype)
-        if not xs.is_contiguous() and stream is not None:
-            raise ValueError("xs must be contiguous on a stream of its own")
-        x = xs.contiguous()
-        T = x.numel() // H
-        if x.device.index != self.device:
-            raise ValueError(f"xs is on {x.device}, the block on cuda:{self.device}")
-        for t, dt, n, what in ((topk_idx, torch.int32, T * k, "topk_idx"), (topk_w, torch.float32, T * k, "topk_w"),
-                               (shared_w, torch.float32, T, "shared_w")):
-            if t is None and what == "shared_w":
+        dev = xs.device
+        if dev.index != self.device:
+            raise ValueError(f"xs is on {dev}, the block on cuda:{self.device}")
+        if not xs.is_contiguous():
+            if stream is not None:
+                raise ValueError("xs must be contiguous on a stream of its own")
+            xs = xs.contiguous()
+        T = xs.numel() // H
+        for t, dt, n, last, what in ((topk_idx, torch.int32, T * k, k, "topk_idx"), (topk_w, torch.float32, T * k, k, "topk_w"),
+                                     (shared_w, torch.float32, T, None, "shared_w")):
+            if t is None and last is None:
                 continue
-            if t.dtype != dt or t.numel() != n or not t.is_contiguous() or t.device != x.device or \
-                    (what != "shared_w" and t.shape[-1] != k):
-                raise ValueError(f"{what} must be a contiguous {dt} tensor of {n} values on {x.device}"
-                                 + (f" with last dim {k}" if what != "shared_w" else ""))
+            if (t.dtype != dt or t.numel() != n or t.device != dev or not t.is_contiguous()
+                    or (last is not None and t.shape[-1] != last)):
+                raise ValueError(f"{what} must be a contiguous {dt} tensor of {n} values on {dev}"
+                                 + (f" with last dim {last}" if last else ""))
         if out is None:
-            out = torch.empty_like(x)
+            out = torch.empty_like(xs)
             if stream is not None:
                 out.record_stream(stream)
-        elif out.shape != xs.shape or out.dtype != x.dtype or not out.is_contiguous() or out.device != x.device:
+        elif out.shape != xs.shape or out.dtype != xs.dtype or not out.is_contiguous() or out.device != dev:
             raise ValueError("out must be contiguous with the input's shape, dtype and device")
-        ws_ptr, ws_n = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
-        check(lib().hx_moe_experts(self._h, _ptr(x), T, _ptr(topk_idx), _ptr(topk_w), _ptr(shared_w), _ptr(out), ws_ptr,
-                                   ws_n, _stream(stream)), "hx_moe_experts")
+        ws, ws_n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+        check(lib().hx_moe_experts(self._h, xs.data_ptr(), T, topk_idx.data_ptr(), topk_w.data_ptr(),
+                                   None if shared_w is None else shared_w.data_ptr(), out.data_ptr(), ws, ws_n,
+                                   _stream(stream)), "hx_moe_experts")
         return out
 
     def route(self, xs, router_bias=None, stream=None):
