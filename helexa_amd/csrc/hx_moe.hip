@@ -725,9 +725,11 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
     tm_ext(m, SLOT_X_F16, s);
     HX_HIP(launch_mx_prep(a, s));
     tm_ext_done(m, SLOT_X_F16);
-    tm_ext(m, SLOT_DISPATCH, s);
-    HX_HIP(launch_mx_dispatch(a, s));
-    tm_ext_done(m, SLOT_DISPATCH);
+    if (mx_chunks(a.F) > 1) {
+      tm_ext(m, SLOT_DISPATCH, s);
+      HX_HIP(launch_mx_dispatch(a, s));
+      tm_ext_done(m, SLOT_DISPATCH);
+    }
     tm_ext(m, SLOT_GATE_UP, s);
     HX_HIP(launch_mx_gate_up(a, s));
     tm_ext_done(m, SLOT_GATE_UP);

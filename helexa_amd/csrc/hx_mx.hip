@@ -638,22 +638,118 @@ hipError_t launch_mx_few_sum(const MxArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- dispatch
-// workgroups 0 .. chunks - 1: the chunk's entries by expert; the others: the tokens' records
+// Positions of a chunk's entries by expert, and (chunk 0) the tiles, from the experts'
+// counts: thread i has the counts of experts EPT i .. and how many of each come in
+// earlier chunks. The entries get their places by LDS counters; their order among an
+// expert's rows is free: a row's results do not depend on its place in a tile, and the
+// combine sums a token's entries in their order.
+struct MxPlace {
+  int base[HX_MAX_EXPERTS], off[HX_MAX_EXPERTS], cnt[HX_MAX_EXPERTS], first[HX_MAX_EXPERTS];
+  int sh[2][17];
+};
+template <int NT>
+HX_DEV void mx_place(const MxArgs& a, MxPlace& sm, int c, const int (&count)[HX_MAX_EXPERTS / NT],
+                     const int (&pre)[HX_MAX_EXPERTS / NT]) {
+  constexpr int EPT = HX_MAX_EXPERTS / NT, NW = NT / 64;
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, e0 = EPT * tid;
+  int n0 = 0, n1 = 0;   // rows, tiles
+#pragma unroll
+  for (int i = 0; i < EPT; i++) {
+    n0 += count[i];
+    n1 += (count[i] + a.tile_m - 1) / a.tile_m;
+  }
+  int x0 = n0, x1 = n1;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y0 = __shfl_up(x0, off, 64), y1 = __shfl_up(x1, off, 64);
+    if (lane >= off) {
+      x0 += y0;
+      x1 += y1;
+    }
+  }
+  if (lane == 63) {
+    sm.sh[0][wave] = x0;
+    sm.sh[1][wave] = x1;
+  }
+  __syncthreads();
+  if (tid < 2) {
+    int run = 0;
+    for (int w = 0; w < NW; w++) {
+      const int v = sm.sh[tid][w];
+      sm.sh[tid][w] = run;
+      run += v;
+    }
+    sm.sh[tid][16] = run;
+  }
+  __syncthreads();
+  int off = sm.sh[0][wave] + x0 - n0, first = sm.sh[1][wave] + x1 - n1;
+  const int total = sm.sh[1][16];
+#pragma unroll
+  for (int i = 0; i < EPT; i++) {
+    sm.base[e0 + i] = off + pre[i];
+    sm.off[e0 + i] = off;
+    sm.cnt[e0 + i] = count[i];
+    sm.first[e0 + i] = first;
+    off += count[i];
+    first += (count[i] + a.tile_m - 1) / a.tile_m;
+  }
+  __syncthreads();
+  const int per = mx_chunk(a.F), f0 = c * per, f1 = min(a.F, f0 + per);
+  for (int f = f0 + tid; f < f1; f += NT) {
+    const int x = a.idx[f];
+    int pos = -1;
+    if ((unsigned)x < (unsigned)a.E) {
+      pos = atomicAdd(&sm.base[x], 1);
+      a.perm[pos] = f;
+    }
+    a.inv[f] = pos;
+  }
+  if (c != 0) return;
+  for (int i = tid; i < total; i += NT) {
+    int lo = 0, hi = a.E - 1;   // the largest expert with first <= i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sm.first[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    const int m0 = (i - sm.first[lo]) * a.tile_m;
+    ((int4*)a.tiles)[i] = make_int4(lo, sm.off[lo] + m0, min(a.tile_m, sm.cnt[lo] - m0), 0);
+  }
+  const int nst = a.Is > 0 ? (a.T + a.tile_m - 1) / a.tile_m : 0;
+  for (int i = tid; i < nst; i += NT) {
+    const int m0 = i * a.tile_m;
+    ((int4*)a.tiles)[total + i] = make_int4(a.E, a.F + m0, min(a.tile_m, a.T - m0), 0);
+  }
+  if (tid == 0) a.counts[0] = total + nst;
+}
+
+// Workgroups 0 .. chunks - 1: the chunk's entries by expert, and where there is one
+// chunk alone (a launch less: about 4 us) their places too; the others: the tokens' records.
 template <int P>
 __global__ __launch_bounds__(256) void k_mx_prep(MxArgs a) {
-  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
-  __shared__ int cnt[HX_MAX_EXPERTS];
+  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, EPT = HX_MAX_EXPERTS / 256;
+  __shared__ MxPlace sm;
   const int nch = mx_chunks(a.F), tid = threadIdx.x;
   if ((int)blockIdx.x < nch) {
-    for (int e = tid; e < a.E; e += 256) cnt[e] = 0;
+    for (int e = tid; e < HX_MAX_EXPERTS; e += 256) sm.cnt[e] = 0;
     __syncthreads();
     const int per = mx_chunk(a.F), f0 = blockIdx.x * per, f1 = min(a.F, f0 + per);
     for (int f = f0 + tid; f < f1; f += 256) {
       const int e = a.idx[f];
-      if ((unsigned)e < (unsigned)a.E) atomicAdd(&cnt[e], 1);
+      if ((unsigned)e < (unsigned)a.E) atomicAdd(&sm.cnt[e], 1);
     }
     __syncthreads();
-    for (int e = tid; e < a.E; e += 256) a.hist[(int64_t)blockIdx.x * a.E + e] = cnt[e];
+    if (nch > 1) {
+      for (int e = tid; e < a.E; e += 256) a.hist[(int64_t)blockIdx.x * a.E + e] = sm.cnt[e];
+      return;
+    }
+    int count[EPT], pre[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+      count[i] = sm.cnt[EPT * tid + i];
+      pre[i] = 0;
+    }
+    mx_place<256>(a, sm, 0, count, pre);
     return;
   }
   const int HB = mx_blocks(a.H);
@@ -666,15 +762,11 @@ __global__ __launch_bounds__(256) void k_mx_prep(MxArgs a) {
   for (int i = 0; i < RV; i++) o[i] = r[i];
 }
 
-// Positions of the entries by expert and the tiles. Every workgroup sums the chunks'
-// counts itself (thread e expert e's), scans them, and places its own chunk's entries
-// by LDS counters. Their order among an expert's rows is free: a row's results do not
-// depend on its place in a tile, and the combine sums a token's entries in their order.
+// several chunks: every workgroup sums the chunks' counts itself and places its own entries
 __global__ __launch_bounds__(1024) void k_mx_dispatch(MxArgs a) {
-  __shared__ int s_base[HX_MAX_EXPERTS], s_off[HX_MAX_EXPERTS], s_cnt[HX_MAX_EXPERTS], s_first[HX_MAX_EXPERTS];
-  __shared__ int sh[2][17];
-  const int e = threadIdx.x, lane = lane_id(), wave = e >> 6, nch = mx_chunks(a.F), c = blockIdx.x;
-  int count = 0, pre = 0;
+  __shared__ MxPlace sm;
+  const int e = threadIdx.x, nch = mx_chunks(a.F), c = blockIdx.x;
+  int count[1] = {0}, pre[1] = {0};
   if (e < a.E) {
     for (int c0 = 0; c0 < nch; c0 += 8) {
       int h[8];
@@ -682,71 +774,12 @@ __global__ __launch_bounds__(1024) void k_mx_dispatch(MxArgs a) {
       for (int i = 0; i < 8; i++) h[i] = c0 + i < nch ? a.hist[(int64_t)(c0 + i) * a.E + e] : 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        if (c0 + i == c) pre = count;
-        count += h[i];
+        if (c0 + i == c) pre[0] = count[0];
+        count[0] += h[i];
       }
     }
   }
-  const int nt = (count + a.tile_m - 1) / a.tile_m;
-  int x0 = count, x1 = nt;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y0 = __shfl_up(x0, off, 64), y1 = __shfl_up(x1, off, 64);
-    if (lane >= off) {
-      x0 += y0;
-      x1 += y1;
-    }
-  }
-  if (lane == 63) {
-    sh[0][wave] = x0;
-    sh[1][wave] = x1;
-  }
-  __syncthreads();
-  if (e < 2) {
-    int run = 0;
-    for (int w = 0; w < 16; w++) {
-      const int v = sh[e][w];
-      sh[e][w] = run;
-      run += v;
-    }
-    sh[e][16] = run;
-  }
-  __syncthreads();
-  const int off = sh[0][wave] + x0 - count, first = sh[1][wave] + x1 - nt, total = sh[1][16];
-  if (e < a.E) {
-    s_base[e] = off + pre;
-    s_off[e] = off;
-    s_cnt[e] = count;
-    s_first[e] = first;
-  }
-  __syncthreads();
-  const int per = mx_chunk(a.F), f0 = c * per, f1 = min(a.F, f0 + per);
-  for (int f = f0 + e; f < f1; f += 1024) {
-    const int x = a.idx[f];
-    int pos = -1;
-    if ((unsigned)x < (unsigned)a.E) {
-      pos = atomicAdd(&s_base[x], 1);
-      a.perm[pos] = f;
-    }
-    a.inv[f] = pos;
-  }
-  if (c != 0) return;
-  for (int i = e; i < total; i += 1024) {
-    int lo = 0, hi = a.E - 1;   // the largest expert with s_first <= i
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_first[mid] <= i) lo = mid;
-      else hi = mid - 1;
-    }
-    const int m0 = (i - s_first[lo]) * a.tile_m;
-    ((int4*)a.tiles)[i] = make_int4(lo, s_off[lo] + m0, min(a.tile_m, s_cnt[lo] - m0), 0);
-  }
-  const int nst = a.Is > 0 ? (a.T + a.tile_m - 1) / a.tile_m : 0;
-  for (int i = e; i < nst; i += 1024) {
-    const int m0 = i * a.tile_m;
-    ((int4*)a.tiles)[total + i] = make_int4(a.E, a.F + m0, min(a.tile_m, a.T - m0), 0);
-  }
-  if (e == 0) a.counts[0] = total + nst;
+  mx_place<1024>(a, sm, c, count, pre);
 }
 
 hipError_t launch_mx_prep(const MxArgs& a, hipStream_t s) {
