@@ -1082,54 +1082,110 @@ hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) {
 }
 
 // y[t] = the token's entries' rows times their weights in their order, then the
-// shared expert's: 8 outputs a thread
+// shared expert's. A wave: 512 outputs of a token, 8 a lane, 8 rows' loads together
+// (an entry without an expert reads row 0 and counts nothing).
 template <bool BF>
 __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
-  const int t = blockIdx.x, n0 = (blockIdx.y * 256 + (int)threadIdx.x) * 8;
+  constexpr int B = 8;
+  const int lane = lane_id(), segs = (a.H + 511) / 512, k = a.k;
+  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = id / segs;
+  const int n0 = (int)(id % segs) * 512 + lane * 8;
+  if (t >= a.T) return;
+  // lane j: entry j; lane k: the shared expert's row (k <= 64: held apart)
+  const int p = lane < k ? a.inv[t * k + lane] : -1;
+  const float w = lane < k ? a.w[t * k + lane] : 0.f;
+  const int ps = a.Is > 0 ? a.F + (int)t : -1;
+  const float ws = a.Is > 0 ? a.shared_w[t] : 0.f;
   if (n0 >= a.H) return;
   float acc[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) acc[i] = 0.f;
-  auto add = [&](int64_t row, float w) {
-    float v[8];
-    if constexpr (BF) {
-      const uint4 q = *(const uint4*)((const uint16_t*)a.obuf + row * a.H + n0);
-      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+  for (int j0 = 0; j0 <= k; j0 += B) {
+    uint4 q[B], r[B];
+    int pj[B];
+    float wj[B];
+#pragma unroll
+    for (int j = 0; j < B; j++) {
+      const int jj = j0 + j;
+      pj[j] = jj < k ? __builtin_amdgcn_readlane(p, jj) : jj == k ? ps : -1;
+      wj[j] = jj < k ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), jj)) : ws;
+      const int64_t at = (int64_t)max(pj[j], 0) * a.H + n0;
+      if constexpr (BF) {
+        q[j] = *(const uint4*)((const uint16_t*)a.obuf + at);
+      } else {
+        q[j] = *(const uint4*)((const float*)a.obuf + at);
+        r[j] = *(const uint4*)((const float*)a.obuf + at + 4);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < B; j++) {
+      if (pj[j] < 0) continue;
+      const uint32_t u[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+      float v[8];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        if constexpr (BF) {
+          v[2 * i] = __uint_as_float(u[i] << 16);
+          v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        } else {
+          v[i] = __uint_as_float(u[i]);
+        }
       }
-    } else {
-      const float4* q = (const float4*)((const float*)a.obuf + row * a.H + n0);
-      const float4 x = q[0], y = q[1];
-      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+      if constexpr (!BF) {
+        v[4] = __uint_as_float(r[j].x); v[5] = __uint_as_float(r[j].y);
+        v[6] = __uint_as_float(r[j].z); v[7] = __uint_as_float(r[j].w);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wj[j], v[i], acc[i]);
     }
-#pragma unroll
-    for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
-  };
-  for (int j = 0; j < a.k; j++) {
-    const int p = a.inv[(int64_t)t * a.k + j];
-    if (p >= 0) add(p, a.w[(int64_t)t * a.k + j]);
   }
-  if (a.Is > 0) add((int64_t)a.F + t, a.shared_w[t]);
-  const int64_t at = (int64_t)t * a.H + n0;
+  const int64_t at = t * a.H + n0;
+  void* const base = a.resid ? a.resid : a.y;
   if constexpr (BF) {
-    uint16_t* p = (uint16_t*)(a.resid ? a.resid : a.y) + at;
+    uint16_t* o = (uint16_t*)base + at;
+    uint32_t h[4];
+    if (((uintptr_t)base & 15) == 0) {
+      uint32_t x[4] = {0u, 0u, 0u, 0u};
+      if (a.resid) {
+        const uint4 v = *(const uint4*)o;
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+      }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint16_t b = f32_to_bf16(acc[i]);
-      p[i] = a.resid ? f32_to_bf16(bf16_to_f32(p[i]) + bf16_to_f32(b)) : b;
+      for (int i = 0; i < 4; i++) {
+        uint16_t lo = f32_to_bf16(acc[2 * i]), hi = f32_to_bf16(acc[2 * i + 1]);
+        if (a.resid) {
+          lo = f32_to_bf16(__uint_as_float(x[i] << 16) + bf16_to_f32(lo));
+          hi = f32_to_bf16(__uint_as_float(x[i] & 0xffff0000u) + bf16_to_f32(hi));
+        }
+        h[i] = lo | ((uint32_t)hi << 16);
+      }
+      *(uint4*)o = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {
+      for (int i = 0; i < 8; i++) mx_store(a, at + i, acc[i]);
     }
   } else {
-    float* p = (float*)(a.resid ? a.resid : a.y) + at;
-#pragma unroll
-    for (int i = 0; i < 8; i++) p[i] = a.resid ? p[i] + acc[i] : acc[i];
+    float* o = (float*)base + at;
+    if (((uintptr_t)base & 15) == 0) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+      if (a.resid) {
+        x = ((const float4*)o)[0];
+        y = ((const float4*)o)[1];
+      }
+      // x + 0 only where there is a stream: -0 stays
+      ((float4*)o)[0] = a.resid ? make_float4(x.x + acc[0], x.y + acc[1], x.z + acc[2], x.w + acc[3])
+                                : make_float4(acc[0], acc[1], acc[2], acc[3]);
+      ((float4*)o)[1] = a.resid ? make_float4(y.x + acc[4], y.y + acc[5], y.z + acc[6], y.w + acc[7])
+                                : make_float4(acc[4], acc[5], acc[6], acc[7]);
+    } else {
+      for (int i = 0; i < 8; i++) mx_store(a, at + i, acc[i]);
+    }
   }
 }
 
 hipError_t launch_mx_combine(const MxArgs& a, hipStream_t s) {
-  const dim3 g(a.T, (a.H + 2047) / 2048);
+  const int64_t waves = (int64_t)a.T * ((a.H + 511) / 512);
+  const dim3 g((unsigned)((waves + 3) / 4));
   if (a.xbf) hx_launch(k_mx_combine<true>, g, dim3(256), 0, s, a);
   else hx_launch(k_mx_combine<false>, g, dim3(256), 0, s, a);
   return hipGetLastError();
