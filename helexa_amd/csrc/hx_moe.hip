@@ -720,7 +720,7 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
     a.hist = (int32_t*)(ws + L.mx_hist);
     a.tiles = (int32_t*)(ws + L.mx_tiles);
     a.counts = (int32_t*)(ws + L.mx_counts);
-    a.tile_m = mx_tile_m(a.F, a.E);
+    a.tile_m = mx_tile_m(a.F, a.E, a.xbf);
     a.max_tiles = (int)mx_max_tiles(m, T, a.tile_m);
     tm_ext(m, SLOT_X_F16, s);
     HX_HIP(launch_mx_prep(a, s));

@@ -796,7 +796,7 @@ hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s) {
 
 // ---------------------------------------------------------------- grouped products
 // rows of a tile: 32 when the experts have few rows each
-int mx_tile_m(int64_t F, int E) { return F <= 24 * (int64_t)E ? 32 : 64; }
+int mx_tile_m(int64_t F, int E, bool xbf) { return !xbf || F <= 28 * (int64_t)E ? 32 : 64; }
 
 // The tile's rows in LDS, CB blocks of K at a time: [CB blocks][TM rows][record]. The
 // records come in by direct loads, 16 bytes a lane, in LDS order; a unit of U blocks is
@@ -804,7 +804,7 @@ int mx_tile_m(int64_t F, int E) { return F <= 24 * (int64_t)E ? 32 : 64; }
 template <int TM, int P>
 struct MxRows {
   static constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
-  static constexpr int CB = P == 3 ? 16 : 8, BYTES = CB * TM * RB;
+  static constexpr int CB = 8, BYTES = CB * TM * RB;
   static constexpr int U = TM * RV % 64 == 0 ? 1 : 2, LOADS = U * TM * RV / 64;
   static_assert(U * TM * RV % 64 == 0, "whole loads");
   const uint8_t* src[LOADS];
@@ -907,11 +907,13 @@ HX_DEV void mx_turn(MxRing<P, NM>& ring, const uint8_t* rec, int s, int S, mx_v1
     }
   }
 }
-// acc = the sums over nblk blocks of K of the ring's weights x the tile's rows
+// acc = the sums over nblk blocks of K of the ring's weights x the tile's rows, which
+// come into buf's two halves in turn, a chunk ahead
 template <int TM, int P, int NM>
 HX_DEV void mx_products(MxRing<P, NM>& ring, const MxRows<TM, P>& rw, int wave, uint8_t* buf, int nblk,
                         mx_v16f (&acc)[NM][TM / 32]) {
-  constexpr int RB = MxRec<P>::BYTES, U = MxRing<P, NM>::U, CB = MxRows<TM, P>::CB;
+  constexpr int RB = MxRec<P>::BYTES, CB = MxRows<TM, P>::CB, BYTES = MxRows<TM, P>::BYTES;
+  constexpr int R = MxRing<P, NM>::R, U = MxRing<P, NM>::U, W = MxRing<P, NM>::W;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
   const int lane = lane_id(), S = nblk / 2;
   const uint8_t* rec = buf + ((lane >> 5) * TM + (lane & 31)) * RB;
@@ -919,22 +921,28 @@ HX_DEV void mx_products(MxRing<P, NM>& ring, const MxRows<TM, P>& rw, int wave, 
   for (int m = 0; m < NM; m++)
 #pragma unroll
     for (int n = 0; n < TM / 32; n++) acc[m][n] = mx_zero16();
+  rw.load(wave, 0, nblk, lds);
   ring.start(S);
-  int s = 0, b0 = 0;   // a chunk is whole turns; the last turn comes after the loop
+  // the rows are the oldest loads: what may be left are the ring's
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R + W) * NM) : "memory");
+  lds_barrier();
+  int s = 0, b0 = 0, h = 0;   // a chunk is whole turns; the last turn comes after the loop
   for (;;) {
-    rw.load(wave, b0, nblk, lds);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();
+    // the other half was read before the barrier
+    if (b0 + CB < nblk) rw.load(wave, b0 + CB, nblk, lds + (h ^ 1) * BYTES);
     for (const int end = min(S - U, (b0 + CB) / 2); s < end; s += U) {
       ring.turn(s, S);
-      mx_turn<TM, P, NM, false>(ring, rec + (2 * s - b0) * TM * RB, s, S, acc);
+      mx_turn<TM, P, NM, false>(ring, rec + h * BYTES + (2 * s - b0) * TM * RB, s, S, acc);
     }
     if (b0 + CB >= nblk) break;
-    b0 += CB;
+    // a turn's loads at least came after the next rows'
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(U * NM) : "memory");
     lds_barrier();
+    b0 += CB;
+    h ^= 1;
   }
   ring.turn(s, S);
-  mx_turn<TM, P, NM, true>(ring, rec + (2 * s - b0) * TM * RB, s, S, acc);
+  mx_turn<TM, P, NM, true>(ring, rec + h * BYTES + (2 * s - b0) * TM * RB, s, S, acc);
   // the sums leave the loop whole: seen through, their elements are carried through it
   // one by one as well, and spilled
 #pragma unroll
@@ -959,7 +967,7 @@ HX_DEV void mx_columns(const mx_v16f (&d)[TM / 32], float (&f)[32]) {
 template <int TM, int P, int MF>
 __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
-  __shared__ __align__(16) uint8_t buf[MxRows<TM, P>::BYTES];
+  __shared__ __align__(16) uint8_t buf[2 * MxRows<TM, P>::BYTES];
   int nt, tile;
   mx_tile((a.hblocks + 4 * MF - 1) / (4 * MF), a.counts[0], nt, tile);
   if (tile < 0) return;
@@ -1011,7 +1019,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
 template <int TM, int P, int MF>
 __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, NM = 2 * MF;
-  __shared__ __align__(16) uint8_t buf[MxRows<TM, P>::BYTES];
+  __shared__ __align__(16) uint8_t buf[2 * MxRows<TM, P>::BYTES];
   int nt, tile;
   const int nb = a.H / 32;
   mx_tile((nb + 4 * NM - 1) / (4 * NM), a.counts[0], nt, tile);
@@ -1069,8 +1077,7 @@ constexpr int MX_MF = 2;
   };                                                                                             \
   if (a.xbf && a.tile_m == 32) go(KERNEL<32, 3, 1>, 1);                                          \
   else if (a.xbf) go(KERNEL<64, 3, MX_MF>, MX_MF);                                               \
-  else if (a.tile_m == 32) go(KERNEL<32, 5, 1>, 1);                                              \
-  else go(KERNEL<64, 5, 1>, 1)
+  else go(KERNEL<32, 5, 1>, 1)
 
 hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) {
   MX_LAUNCH(k_mx_gate_up, (a.hblocks + 4 * mf - 1) / (4 * mf));
