@@ -319,6 +319,8 @@ class Qwen3_5MoeBlock:
                 out.record_stream(stream)
         elif out.shape != xs.shape or out.dtype != xs.dtype or not out.is_contiguous() or out.device != dev:
             raise ValueError("out must be contiguous with the input's shape, dtype and device")
+        if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
+            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
         ws, ws_n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
         check(lib().hx_moe_experts(self._h, xs.data_ptr(), T, topk_idx.data_ptr(), topk_w.data_ptr(),
                                    None if shared_w is None else shared_w.data_ptr(), out.data_ptr(), ws, ws_n,
