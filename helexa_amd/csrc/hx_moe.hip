@@ -707,7 +707,7 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
     tm_ext(m, SLOT_DOWN, s);
     HX_HIP(launch_mx_few_down(a, s));
     tm_ext_done(m, SLOT_DOWN);
-    if (mx_few_parts(a.T, a.k, a.E, a.I, a.Is) > 1) {
+    if (mx_few_parts(a.T, a.k, a.E, a.H, a.I, a.Is) > 1) {
       tm_ext(m, SLOT_COMBINE, s);
       HX_HIP(launch_mx_few_sum(a, s));
       tm_ext_done(m, SLOT_COMBINE);

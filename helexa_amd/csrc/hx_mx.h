@@ -70,7 +70,7 @@ struct MxArgs {
 
 // whether a call of T tokens takes the few-token kernels
 bool mx_few(int T, int k, int H, bool xbf);
-int mx_few_parts(int T, int k, int E, int I, int Is);   // parts the down units of such a call are cut into
+int mx_few_parts(int T, int k, int E, int H, int I, int Is);   // parts the down units of such a call are cut into
 int mx_tile_m(int64_t F, int E, bool xbf);
 hipError_t launch_mx_repack(const void* src, int64_t count, int64_t rows, int64_t K, void* dst, int64_t dst_stride,
                             hipStream_t s);

@@ -467,10 +467,14 @@ bool mx_few(int T, int k, int H, bool xbf) {
 static int mx_few_slots(int T, int k, int E) { return T == 1 ? k : min(T * k, E); }
 
 // units of the down kernel: an expert's products over 8 steps of K
-int mx_few_parts(int T, int k, int E, int I, int Is) {
+// (a wave's load at a time); their parts: a unit a wave, but one part where two units a
+// wave save the launch that adds the parts (3 tokens: 9.1 + 4.0 us against 12.9), and no
+// more workgroups than CUs, which hold one each (8 tokens: 4 parts 17.3 us, 6 parts 20.9)
+int mx_few_parts(int T, int k, int E, int H, int I, int Is) {
   const int G = (mx_steps(I) + 7) / 8, Gs = Is > 0 ? (mx_steps(Is) + 7) / 8 : 0;
   const int units = mx_few_slots(T, k, E) * G + Gs;
-  return min(MX_FEW_PARTS, (units + 15) / 16);
+  if (units <= 32) return 1;
+  return max(1, min(min(MX_FEW_PARTS, (units + 15) / 16), 256 / (H / 32)));
 }
 
 HX_DEV void mx_store(const MxArgs& a, int64_t at, float y) {
@@ -622,7 +626,7 @@ hipError_t launch_mx_few_gate_up(const MxArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s) {
-  const int parts = mx_few_parts(a.T, a.k, a.E, a.I, a.Is);
+  const int parts = mx_few_parts(a.T, a.k, a.E, a.H, a.I, a.Is);
   const dim3 g(a.H / 32, parts);
   if (a.xbf && a.T == 1) hx_launch(k_mx_few_down<3, true>, g, dim3(1024), 0, s, a);
   else if (a.xbf) hx_launch(k_mx_few_down<3, false>, g, dim3(1024), 0, s, a);
@@ -632,7 +636,7 @@ hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_mx_few_sum(const MxArgs& a, hipStream_t s) {
-  const int parts = mx_few_parts(a.T, a.k, a.E, a.I, a.Is);
+  const int parts = mx_few_parts(a.T, a.k, a.E, a.H, a.I, a.Is);
   hx_launch(k_mx_few_sum, dim3((unsigned)(((int64_t)a.T * a.H + 255) / 256)), dim3(256), 0, s, a, parts);
   return hipGetLastError();
 }
