@@ -134,7 +134,7 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct WsLayout {
   size_t logits, topk_idx, topk_w, sgw, perm, inv, offsets, slots, tiles, counts, plan, dmap, hbuf, hbf, xh, xq, xq32, xcv,
-      hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, mx_part, total;
+      hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, total;
   int hstride, max_slots, max_tiles;
 };
 
@@ -199,7 +199,7 @@ static WsLayout ws_layout(const hx_moe* m, int64_t T) {
     L.xn = take(act * T * H);
     L.ym = take(act * T * H);
     if (mfew) {
-      L.mx_part = take(sizeof(float) * (size_t)MX_FEW_PARTS * T * H);
+      L.obuf = take(sizeof(float) * (size_t)(F + T) * H);
     } else {
       L.mx_xrec = take(rec * (size_t)T * mx_blocks((int)H));
       L.obuf = take(act * (size_t)(F + T) * H);
@@ -699,7 +699,7 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
   a.y = y; a.resid = resid;
   a.hrec = ws + L.mx_hrec;
   a.hblocks = mx_hblocks(m);
-  a.part = (float*)(ws + L.mx_part);
+  a.obuf = ws + L.obuf;
   if (mx_few(a.T, a.k, a.H, a.xbf)) {
     tm_ext(m, SLOT_GATE_UP, s);
     HX_HIP(launch_mx_few_gate_up(a, s));
@@ -707,14 +707,13 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
     tm_ext(m, SLOT_DOWN, s);
     HX_HIP(launch_mx_few_down(a, s));
     tm_ext_done(m, SLOT_DOWN);
-    if (mx_few_parts(a.T, a.k, a.E, a.H, a.I, a.Is) > 1) {
+    if (a.T > 1) {   // one token's down kernel combines
       tm_ext(m, SLOT_COMBINE, s);
-      HX_HIP(launch_mx_few_sum(a, s));
+      HX_HIP(launch_mx_combine(a, s));
       tm_ext_done(m, SLOT_COMBINE);
     }
   } else {
     a.xrec = ws + L.mx_xrec;
-    a.obuf = ws + L.obuf;
     a.perm = (int32_t*)(ws + L.mx_perm);
     a.inv = (int32_t*)(ws + L.mx_inv);
     a.hist = (int32_t*)(ws + L.mx_hist);

@@ -35,8 +35,8 @@ __host__ __device__ inline int64_t mx_mat_bytes(int rows, int K) {
 __host__ __device__ inline int mx_planes(bool xbf) { return xbf ? 3 : 5; }
 __host__ __device__ inline int mx_rec_bytes(bool xbf) { return xbf ? 80 : 128; }
 
-// tokens up to which the few-token kernels are used; most parts of their down sums
-constexpr int MX_FEW_T = 8, MX_FEW_PARTS = 8;
+// tokens up to which the few-token kernels are used
+constexpr int MX_FEW_T = 8;
 // entries of the routing a dispatch workgroup takes, and the most workgroups
 constexpr int MX_CHUNK = 1024, MX_MAX_CHUNKS = 256;
 __host__ __device__ inline int mx_chunk(int64_t F) {   // entries a chunk, a multiple of MX_CHUNK
@@ -58,25 +58,22 @@ struct MxArgs {
   uint8_t* xrec;                            // [T][mx_blocks(H)] records
   uint8_t* hrec;                            // [F + T][mx_blocks(max(I, Is))] records
   int hblocks;                              // records of a row of hrec
-  void* obuf;                               // [F + T, H] expert outputs, act dtype
+  void* obuf;                               // [F + T, H] expert outputs, act dtype (few tokens: f32)
   int32_t* perm;                            // [F] entries by expert
   int32_t* inv;                             // [F] their positions, -1: no expert
   int32_t* hist;                            // [chunks][E]
   int32_t* tiles;                           // [max_tiles][4]: expert (E: shared), first row, rows
   int32_t* counts;                          // [1] tiles
   int tile_m, max_tiles;
-  float* part;                              // few tokens: [mx_few_parts][T, H] sums of the down parts
 };
 
 // whether a call of T tokens takes the few-token kernels
 bool mx_few(int T, int k, int H, bool xbf);
-int mx_few_parts(int T, int k, int E, int H, int I, int Is);   // parts the down units of such a call are cut into
 int mx_tile_m(int64_t F, int E, bool xbf);
 hipError_t launch_mx_repack(const void* src, int64_t count, int64_t rows, int64_t K, void* dst, int64_t dst_stride,
                             hipStream_t s);
 hipError_t launch_mx_few_gate_up(const MxArgs& a, hipStream_t s);
 hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s);
-hipError_t launch_mx_few_sum(const MxArgs& a, hipStream_t s);    // where mx_few_parts > 1
 hipError_t launch_mx_prep(const MxArgs& a, hipStream_t s);       // records of the tokens, expert counts
 hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s);   // positions and tiles
 hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s);

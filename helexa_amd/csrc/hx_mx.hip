@@ -466,17 +466,6 @@ bool mx_few(int T, int k, int H, bool xbf) {
 // most chosen experts of a call (one token: its entries)
 static int mx_few_slots(int T, int k, int E) { return T == 1 ? k : min(T * k, E); }
 
-// units of the down kernel: an expert's products over 8 steps of K
-// (a wave's load at a time); their parts: a unit a wave, but one part where two units a
-// wave save the launch that adds the parts (3 tokens: 9.1 + 4.0 us against 12.9), and no
-// more workgroups than CUs, which hold one each (8 tokens: 4 parts 17.3 us, 6 parts 20.9)
-int mx_few_parts(int T, int k, int E, int H, int I, int Is) {
-  const int G = (mx_steps(I) + 7) / 8, Gs = Is > 0 ? (mx_steps(Is) + 7) / 8 : 0;
-  const int units = mx_few_slots(T, k, E) * G + Gs;
-  if (units <= 32) return 1;
-  return max(1, min(min(MX_FEW_PARTS, (units + 15) / 16), 256 / (H / 32)));
-}
-
 HX_DEV void mx_store(const MxArgs& a, int64_t at, float y) {
   if (a.xbf) {
     uint16_t* p = (uint16_t*)(a.resid ? a.resid : a.y) + at;
@@ -488,120 +477,110 @@ HX_DEV void mx_store(const MxArgs& a, int64_t at, float y) {
   }
 }
 
-// Down and combine of up to 8 tokens. Workgroup: 32 outputs and a part of the units
-// (slot, 8 steps of K), which its 16 waves take in turn; each unit's product is
-// weighted per token in f32, the waves' sums are added in LDS. One part writes y, several their
-// sums for k_mx_few_sum.
-template <int P, bool ONE>
-__global__ __launch_bounds__(1024) void k_mx_few_down(MxArgs a) {
+// 8 steps of K of an expert's 32 outputs nb for up to 8 tokens: d += the weights of
+// steps s .. of mat (inter columns) x the planes of the lanes' rows (row < 0: zeros)
+template <int P>
+HX_DEV mx_v16f mx_few_unit(const MxArgs& a, const uint8_t* mat, int inter, int nb, int s, int row, int p, mx_v16f d) {
   constexpr int RB = MxRec<P>::BYTES;
-  __shared__ MxFew few;
-  __shared__ float sw[MX_FEW_T * HX_MAX_TOPK];
-  __shared__ float red[16 * 32 * (P == 3 ? 24 : 30)];
-  __shared__ int pre[33];
-  __shared__ uint16_t list[MX_FEW_T * HX_MAX_TOPK];
-  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int T = ONE ? 1 : a.T, k = a.k, nb = blockIdx.x, parts = gridDim.y;
-  int n = k;
-  if (!ONE) {
-    for (int f = tid; f < a.F; f += 1024) sw[f] = a.w[f];
-    mx_few_bits(a, few);
-    if (tid < 64) {
-      const int c = tid < 32 ? __popc(few.bits[tid]) : 0;
-      int x = c;
+  const int lane = lane_id(), half = lane >> 5, S = mx_steps(inter), S4 = (S + 3) / 4;
+  const uint8_t* wp = mat + ((int64_t)nb * S + s) * 1024;
+  const uint8_t* sp = mat + (mx_code_bytes(a.H, inter) + ((int64_t)nb * S4 + s / 4) * 256);
+  uint4 w[8];
+  const uint32_t sa = *(const uint32_t*)(sp + lane * 4);
+  const uint32_t sb = *(const uint32_t*)(sp + (s / 4 + 1 < S4 ? 256 : 0) + lane * 4);
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up(x, off, 64);
-        if (lane >= off) x += y;
-      }
-      if (tid < 32) pre[tid] = x - c;
-      if (tid == 31) pre[32] = x;
-    }
-    lds_barrier();
-    if (tid < a.E) {   // at most 1024 experts
-      const uint32_t w = few.bits[tid >> 5];
-      if ((w >> (tid & 31)) & 1u) list[pre[tid >> 5] + __popc(w & ((1u << (tid & 31)) - 1u))] = (uint16_t)tid;
-    }
-    lds_barrier();
-    n = pre[32];
-  }
-  const int S = mx_steps(a.I), G = (S + 7) / 8, Ss = mx_steps(a.Is), Gs = a.Is ? (Ss + 7) / 8 : 0;
-  const int col = lane & 31, half = lane >> 5, C = P * T, p = col / T, t = col % T;
-  mx_v16f acc = mx_zero16();
-  for (int u = blockIdx.y * 16 + wave; u < n * G + Gs; u += 16 * parts) {
-    const bool sh = u >= n * G;
-    const int slot = sh ? n : u / G, g = sh ? u - n * G : u % G;
-    int e = a.E;
-    if (!sh) e = __builtin_amdgcn_readfirstlane(ONE ? a.idx[slot] : (int)list[slot]);
-    if (!sh && ONE && (unsigned)e >= (unsigned)a.E) continue;
-    const uint8_t* dm = sh ? a.sdown.base : a.down.mat(e);
-    const int inter = sh ? a.Is : a.I, St = sh ? Ss : S, S4 = (St + 3) / 4, s = 8 * g;
-    const uint8_t* wp = dm + ((int64_t)nb * St + s) * 1024;
-    const uint8_t* sp = dm + (mx_code_bytes(a.H, inter) + ((int64_t)nb * S4 + 2 * g) * 256);
-    uint4 wd[8];
-    const uint32_t sa = *(const uint32_t*)(sp + lane * 4);
-    const uint32_t sb = *(const uint32_t*)(sp + (2 * g + 1 < S4 ? 256 : 0) + lane * 4);
-#pragma unroll
-    for (int i = 0; i < 8; i++) wd[i] = *(const uint4*)(wp + min(i, St - 1 - s) * 1024 + lane * 16);
-    // the token's row of h with this expert, and its weight
-    int row = -1;
-    float wt = 0.f;
-    if (col < C) {
-      if (sh) {
-        row = a.F + t;
-        wt = a.shared_w[t];
-      } else if (ONE) {
-        row = slot;
-        wt = a.w[slot];
-      } else {
-        for (int j = k - 1; j >= 0; j--)
-          if (few.idx[t * k + j] == e) {
-            row = t * k + j;
-            wt += sw[t * k + j];
-          }
-      }
-    }
-    const uint8_t* hp = a.hrec + ((int64_t)max(row, 0) * a.hblocks + 2 * s + half) * RB;
-    mx_v16f d = mx_zero16();
+  for (int i = 0; i < 8; i++) w[i] = *(const uint4*)(wp + min(i, S - 1 - s) * 1024 + lane * 16);
+  const uint8_t* hp = a.hrec + ((int64_t)max(row, 0) * a.hblocks + 2 * s + half) * RB;
 #define MX_STEP(i)                                            \
-  if (s + i < St) {                                           \
+  if (s + i < S) {                                            \
     MxPlane b;                                                \
     b.zero();                                                 \
     if (row >= 0) b.load<P>(hp + 2 * i * RB, p);              \
-    d = mx_mfma1<(i & 3)>(wd[i], i < 4 ? sa : sb, b, d);      \
+    d = mx_mfma1<(i & 3)>(w[i], i < 4 ? sa : sb, b, d);       \
   }
-    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3) MX_STEP(4) MX_STEP(5) MX_STEP(6) MX_STEP(7)
+  MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3) MX_STEP(4) MX_STEP(5) MX_STEP(6) MX_STEP(7)
 #undef MX_STEP
-    // a token that is not this expert's adds nothing, whatever the weights hold
+  return d;
+}
+
+// Down and combine of one token. Workgroup: 32 outputs; its 16 waves take the units
+// (entry, 8 steps of K) in turn, weigh each product in f32, and add up in LDS.
+template <int P>
+__global__ __launch_bounds__(1024) void k_mx_one_down(MxArgs a) {
+  __shared__ float red[16 * P * 32];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int k = a.k, nb = blockIdx.x, G = (mx_steps(a.I) + 7) / 8, Gs = a.Is ? (mx_steps(a.Is) + 7) / 8 : 0;
+  const int col = lane & 31, half = lane >> 5;
+  mx_v16f acc = mx_zero16();
+  for (int u = wave; u < k * G + Gs; u += 16) {
+    const bool sh = u >= k * G;
+    const int j = sh ? k : u / G, g = sh ? u - k * G : u % G;
+    int e = a.E;
+    if (!sh) e = __builtin_amdgcn_readfirstlane(a.idx[j]);
+    if (!sh && (unsigned)e >= (unsigned)a.E) continue;
+    const float wt = sh ? a.shared_w[0] : a.w[j];
+    const mx_v16f d = mx_few_unit<P>(a, sh ? a.sdown.base : a.down.mat(e), sh ? a.Is : a.I, nb, 8 * g,
+                                     col < P ? (sh ? a.F : j) : -1, col, mx_zero16());
 #pragma unroll
-    for (int i = 0; i < 16; i++) acc[i] = row >= 0 ? __builtin_fmaf(wt, d[i], acc[i]) : acc[i];
+    for (int i = 0; i < 16; i++) acc[i] = __builtin_fmaf(wt, d[i], acc[i]);
   }
-  if (col < C) {
+  if (col < P) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) red[(wave * C + col) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)] = acc[i];
+    for (int i = 0; i < 16; i++) red[(wave * P + col) * 32 + 8 * (i >> 2) + 4 * half + (i & 3)] = acc[i];
   }
   lds_barrier();
-  for (int o = tid; o < 32 * T; o += 1024) {
+  if (tid < 32) {
     float y = 0.f;
 #pragma unroll
-    for (int w = 0; w < 16; w++)
-#pragma unroll
-      for (int q = 0; q < P; q++) y += red[(w * C + q * T) * 32 + o];
-    const int64_t at = (int64_t)(o >> 5) * a.H + 32 * nb + (o & 31);
-    if (parts > 1) a.part[(int64_t)blockIdx.y * T * a.H + at] = y;
-    else mx_store(a, at, y);
+    for (int w = 0; w < 16 * P; w++) y += red[w * 32 + tid];
+    mx_store(a, 32 * nb + tid, y);
   }
 }
 
-__global__ __launch_bounds__(256) void k_mx_few_sum(MxArgs a, int parts) {
-  const int64_t n = (int64_t)a.T * a.H, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float v[MX_FEW_PARTS], y = 0.f;
+// Outputs of the experts for 2 to 8 tokens, unweighted and in f32, in the row of the
+// token's first entry with the expert. Workgroup: a chosen expert (slot) and 128
+// outputs; a wave 32 of them and all of K.
+template <int P>
+__global__ __launch_bounds__(256) void k_mx_few_down(MxArgs a) {
+  __shared__ MxFew few;
+  __shared__ float red[4][32][33];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int T = a.T, k = a.k, nb = 4 * blockIdx.x + wave, slot = blockIdx.y;
+  mx_few_bits(a, few);
+  int n;
+  int e = mx_few_slot(few, slot, n);
+  if (e < 0) {
+    if (slot > n || a.Is == 0) return;
+    e = a.E;
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
+  if (32 * nb >= a.H) return;   // no barrier behind this
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I, S = mx_steps(inter);
+  const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
+  const int col = lane & 31, half = lane >> 5, C = P * T, p = col / T, t = col % T;
+  int row = -1;
+  if (col < C) {
+    if (sh) row = a.F + t;
+    else
+      for (int j = k - 1; j >= 0; j--)
+        if (few.idx[t * k + j] == e) row = t * k + j;
+  }
+  mx_v16f d = mx_zero16();
+  for (int s = 0; s < S; s += 8) d = mx_few_unit<P>(a, mat, inter, nb, s, row, p, d);
 #pragma unroll
-  for (int p = 0; p < MX_FEW_PARTS; p++) v[p] = p < parts ? a.part[p * n + i] : 0.f;
+  for (int i = 0; i < 16; i++) red[wave][col][8 * (i >> 2) + 4 * half + (i & 3)] = d[i];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  for (int t0 = 0; t0 < T; t0 += 2) {   // a half wave a token
+    const int tt = t0 + half, r = __shfl(row, tt & 31, 64);
+    if (tt >= T || r < 0) continue;
+    float y = 0.f;
 #pragma unroll
-  for (int p = 0; p < MX_FEW_PARTS; p++) y += v[p];
-  mx_store(a, i, y);
+    for (int q = 0; q < P; q++) y += red[wave][q * T + tt][col];
+    ((float*)a.obuf)[(int64_t)r * a.H + 32 * nb + col] = y;
+  }
 }
 
 template <int P>
@@ -626,18 +605,14 @@ hipError_t launch_mx_few_gate_up(const MxArgs& a, hipStream_t s) {
 }
 
 hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s) {
-  const int parts = mx_few_parts(a.T, a.k, a.E, a.H, a.I, a.Is);
-  const dim3 g(a.H / 32, parts);
-  if (a.xbf && a.T == 1) hx_launch(k_mx_few_down<3, true>, g, dim3(1024), 0, s, a);
-  else if (a.xbf) hx_launch(k_mx_few_down<3, false>, g, dim3(1024), 0, s, a);
-  else if (a.T == 1) hx_launch(k_mx_few_down<5, true>, g, dim3(1024), 0, s, a);
-  else hx_launch(k_mx_few_down<5, false>, g, dim3(1024), 0, s, a);
-  return hipGetLastError();
-}
-
-hipError_t launch_mx_few_sum(const MxArgs& a, hipStream_t s) {
-  const int parts = mx_few_parts(a.T, a.k, a.E, a.H, a.I, a.Is);
-  hx_launch(k_mx_few_sum, dim3((unsigned)(((int64_t)a.T * a.H + 255) / 256)), dim3(256), 0, s, a, parts);
+  if (a.T == 1) {
+    if (a.xbf) hx_launch(k_mx_one_down<3>, dim3(a.H / 32), dim3(1024), 0, s, a);
+    else hx_launch(k_mx_one_down<5>, dim3(a.H / 32), dim3(1024), 0, s, a);
+  } else {
+    const dim3 g((a.H + 127) / 128, mx_few_slots(a.T, a.k, a.E) + (a.Is > 0 ? 1 : 0));
+    if (a.xbf) hx_launch(k_mx_few_down<3>, g, dim3(256), 0, s, a);
+    else hx_launch(k_mx_few_down<5>, g, dim3(256), 0, s, a);
+  }
   return hipGetLastError();
 }
 
@@ -1094,9 +1069,12 @@ hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) {
 
 // y[t] = the token's entries' rows times their weights in their order, then the
 // shared expert's. A wave: 512 outputs of a token, 8 a lane, 8 rows' loads together
-// (an entry without an expert reads row 0 and counts nothing).
-template <bool BF>
+// (an entry without an expert reads row 0 and counts nothing). FEW: rows in f32, a
+// token's entry at that of its first with the same expert; else rows in the
+// activations' type by inv.
+template <bool BF, bool FEW>
 __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
+  constexpr bool R16 = BF && !FEW;
   constexpr int B = 8;
   const int lane = lane_id(), segs = (a.H + 511) / 512, k = a.k;
   const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1104,7 +1082,15 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
   const int n0 = (int)(id % segs) * 512 + lane * 8;
   if (t >= a.T) return;
   // lane j: entry j; lane k: the shared expert's row (k <= 64: held apart)
-  const int p = lane < k ? a.inv[t * k + lane] : -1;
+  int p;
+  if constexpr (FEW) {
+    const int e = lane < k ? a.idx[t * k + lane] : -1;
+    p = (unsigned)e < (unsigned)a.E ? (int)t * k + lane : -1;
+    for (int j = k - 2; j >= 0; j--)
+      if (p >= 0 && __builtin_amdgcn_readlane(e, j) == e && j < lane) p = (int)t * k + j;
+  } else {
+    p = lane < k ? a.inv[t * k + lane] : -1;
+  }
   const float w = lane < k ? a.w[t * k + lane] : 0.f;
   const int ps = a.Is > 0 ? a.F + (int)t : -1;
   const float ws = a.Is > 0 ? a.shared_w[t] : 0.f;
@@ -1122,7 +1108,7 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
       pj[j] = jj < k ? __builtin_amdgcn_readlane(p, jj) : jj == k ? ps : -1;
       wj[j] = jj < k ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), jj)) : ws;
       const int64_t at = (int64_t)max(pj[j], 0) * a.H + n0;
-      if constexpr (BF) {
+      if constexpr (R16) {
         q[j] = *(const uint4*)((const uint16_t*)a.obuf + at);
       } else {
         q[j] = *(const uint4*)((const float*)a.obuf + at);
@@ -1136,14 +1122,14 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        if constexpr (BF) {
+        if constexpr (R16) {
           v[2 * i] = __uint_as_float(u[i] << 16);
           v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         } else {
           v[i] = __uint_as_float(u[i]);
         }
       }
-      if constexpr (!BF) {
+      if constexpr (!R16) {
         v[4] = __uint_as_float(r[j].x); v[5] = __uint_as_float(r[j].y);
         v[6] = __uint_as_float(r[j].z); v[7] = __uint_as_float(r[j].w);
       }
@@ -1197,8 +1183,11 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
 hipError_t launch_mx_combine(const MxArgs& a, hipStream_t s) {
   const int64_t waves = (int64_t)a.T * ((a.H + 511) / 512);
   const dim3 g((unsigned)((waves + 3) / 4));
-  if (a.xbf) hx_launch(k_mx_combine<true>, g, dim3(256), 0, s, a);
-  else hx_launch(k_mx_combine<false>, g, dim3(256), 0, s, a);
+  const bool few = mx_few(a.T, a.k, a.H, a.xbf);
+  if (a.xbf && few) hx_launch(k_mx_combine<true, true>, g, dim3(256), 0, s, a);
+  else if (a.xbf) hx_launch(k_mx_combine<true, false>, g, dim3(256), 0, s, a);
+  else if (few) hx_launch(k_mx_combine<false, true>, g, dim3(256), 0, s, a);
+  else hx_launch(k_mx_combine<false, false>, g, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
