@@ -289,7 +289,7 @@ __host__ __device__ inline int mx_wave_steps(int S, int W) {
 // 26 us of 6 tokens' 64 MB.
 // ONE token: an expert a chosen entry, its weights on their way before anything else.
 template <int P, int KW, bool ONE>
-__global__ __launch_bounds__(512, ONE ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
+__global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, FW = 8 / KW;
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ MxFew few;
@@ -330,9 +330,17 @@ __global__ __launch_bounds__(512, ONE ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
   if (ONE) {
     if (slot < a.k) e = a.idx[slot];
     if (slot < a.k && (unsigned)e >= (unsigned)a.E) return;
-    start();
-    if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
+  } else {
+    mx_few_bits(a, few);
+    int n;
+    e = mx_few_slot(few, slot, n);
+    if (e < 0) {
+      if (slot > n || a.Is == 0) return;
+      e = a.E;
+    }
   }
+  start();
+  if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
   for (int b = tid; b < T * HB; b += 512) {
     const int t = b / HB, kb = b % HB;
     uint4 r[RV];
@@ -347,17 +355,6 @@ __global__ __launch_bounds__(512, ONE ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
     mx_zero_record<P>(r);
 #pragma unroll
     for (int i = 0; i < RV; i++) ((uint4*)zrec)[i] = r[i];
-  }
-  if (!ONE) {
-    mx_few_bits(a, few);
-    int n;
-    e = mx_few_slot(few, slot, n);
-    if (e < 0) {
-      if (slot > n || a.Is == 0) return;
-      e = a.E;
-    }
-    start();
-    if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
   }
   lds_barrier();
   mx_v16f ag = mx_zero16(), au = mx_zero16();
