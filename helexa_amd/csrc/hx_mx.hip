@@ -939,6 +939,25 @@ HX_DEV void mx_columns(const mx_v16f (&d)[TM / 32], float (&f)[32]) {
   }
 }
 
+// A wave's results, BYTES a row in LDS (row r at tile + r PITCH), to dst(r): whole rows by
+// neighbouring lanes. (A row a lane, 16 bytes a store, touches 64 rows' lines with every
+// store: k_mx_down 260 us at 8192 tokens, 63 at 512; so 228, 58.)
+template <int BYTES>
+struct MxOut {
+  static constexpr int PITCH = BYTES + 16, PIECES = BYTES / 16;   // 16 bytes more: fewer rows on the same banks
+  HX_DEV static uint8_t* row(uint8_t* tile, int r) { return tile + r * PITCH; }
+  template <typename F>
+  HX_DEV static void store(const uint8_t* tile, int rows, int bytes, F dst) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    for (int i = lane_id(); i < rows * PIECES; i += 64) {
+      const int r = i / PIECES, b = i % PIECES * 16;
+      if (b < bytes) *(uint4*)(dst(r) + b) = *(const uint4*)(tile + r * PITCH + b);
+    }
+  }
+};
+
 // MF groups of 32 features of h a wave
 template <int TM, int P, int MF>
 __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
@@ -971,6 +990,10 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   }
   mx_v16f acc[2 * MF][TM / 32];
   mx_products<TM, P, 2 * MF>(ring, rw, wave, buf, HB, acc);
+  using Out = MxOut<MF * RB>;
+  static_assert(4 * TM * Out::PITCH <= 2 * MxRows<TM, P>::BYTES, "the rows' place holds the results");
+  lds_barrier();   // the rows have been read
+  uint8_t* const tl = buf + wave * (TM * Out::PITCH);
 #pragma unroll
   for (int m = 0; m < MF; m++) {
     mx_v16f h[TM / 32];
@@ -983,12 +1006,14 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
     uint4 r[RV];
     if (32 * (f0 + m) < inter) mx_record<P>(f, r);
     else mx_zero_record<P>(r);
-    if (lane < rows && lane < TM && f0 + m < mx_blocks(inter)) {
-      uint4* o = (uint4*)(a.hrec + ((int64_t)(p0 + lane) * a.hblocks + f0 + m) * RB);
+    if (lane < TM) {
+      uint4* o = (uint4*)(Out::row(tl, lane) + m * RB);
 #pragma unroll
       for (int i = 0; i < RV; i++) o[i] = r[i];
     }
   }
+  Out::store(tl, rows, min(MF, mx_blocks(inter) - f0) * RB,
+             [&](int r) { return a.hrec + ((int64_t)(p0 + r) * a.hblocks + f0) * RB; });
 }
 
 // outputs of the experts, unweighted: 64 MF features a wave
@@ -1019,15 +1044,19 @@ __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   }
   mx_v16f acc[NM][TM / 32];
   mx_products<TM, P, NM>(ring, rw, wave, buf, IB, acc);
+  constexpr int ES = P == 3 ? 2 : 4;   // bytes of an output
+  using Out = MxOut<32 * NM * ES>;
+  static_assert(4 * TM * Out::PITCH <= 2 * MxRows<TM, P>::BYTES, "the rows' place holds the results");
+  lds_barrier();   // the rows have been read
+  uint8_t* const tl = buf + wave * (TM * Out::PITCH);
 #pragma unroll
   for (int m = 0; m < NM; m++) {
     __builtin_amdgcn_sched_barrier(0);   // one matrix's outputs after the other's: all at once do not fit the registers
     float f[32];
     mx_columns<TM>(acc[m], f);
-    if (lane < TM && lane < rows && n0 + m < nb) {
-      const int64_t at = (int64_t)(p0 + lane) * a.H + 32 * (n0 + m);
+    if (lane < TM) {
       if constexpr (P == 3) {
-        uint4* o = (uint4*)((uint16_t*)a.obuf + at);
+        uint4* o = (uint4*)(Out::row(tl, lane) + m * 64);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           uint32_t q[4];
@@ -1037,12 +1066,14 @@ __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
           o[i] = make_uint4(q[0], q[1], q[2], q[3]);
         }
       } else {
-        float4* o = (float4*)((float*)a.obuf + at);
+        float4* o = (float4*)(Out::row(tl, lane) + m * 128);
 #pragma unroll
         for (int i = 0; i < 8; i++) o[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
       }
     }
   }
+  Out::store(tl, rows, min(NM, nb - n0) * 32 * ES,
+             [&](int r) { return (uint8_t*)a.obuf + ((int64_t)(p0 + r) * a.H + 32 * n0) * ES; });
 }
 
 // groups of 32 features a wave takes at a time
