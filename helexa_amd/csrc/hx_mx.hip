@@ -771,7 +771,9 @@ hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- grouped products
-// rows of a tile: 32 when the experts have few rows each
+// Rows of a tile: 32 while the experts have few rows each. 512 experts of 10 chosen: at
+// 20 rows an expert 197 us with tiles of 32 and 229 of 64, at 25 219 and 236, at 31 258
+// and 244, at 40 325 and 259.
 int mx_tile_m(int64_t F, int E, bool xbf) { return !xbf || F <= 28 * (int64_t)E ? 32 : 64; }
 
 // The tile's rows in LDS, CB blocks of K at a time: [CB blocks][TM rows][record]. The
@@ -806,7 +808,10 @@ struct MxRows {
 // time; a step's registers are loaded again as soon as its MFMAs are issued. (Loaded a
 // stage ahead into a second set, with a barrier and a wait for everything at each
 // stage of 128 columns, the wait was never over in time: MFMAs busy 41 % at 8192 tokens.)
-template <int P, int NM>
+// AUX 2 (non-temporal) for tiles of 32: mostly one tile reads an expert's weights, and
+// they leave the caches to the rows (512 tokens: 182 -> 172 us; 64: 123 -> 112). With
+// tiles of 64 several do, and want them in the caches (8192: 708 -> 748).
+template <int P, int NM, int AUX>
 struct MxRing {
   // steps, words of scales; a chunk of rows is whole turns of the ring
   static constexpr int R = 8 / NM, U = R < 4 ? 4 : R, W = U / 4;
@@ -828,7 +833,7 @@ struct MxRing {
     const int o = lane_offset(16, s < S);
 #pragma unroll
     for (int m = 0; m < NM; m++)
-      w[i][m] = __builtin_amdgcn_raw_buffer_load_b128(mat[m % 2], o, s < S ? codes[m] + s * 1024 : 0, 0);
+      w[i][m] = __builtin_amdgcn_raw_buffer_load_b128(mat[m % 2], o, s < S ? codes[m] + s * 1024 : 0, AUX);
   }
   HX_DEV void fetch_scales(int j, int s, int S) {   // of steps s .. s + 3
     const int o = lane_offset(4, s < S);
@@ -867,8 +872,8 @@ HX_DEV void mx_tile(int NX, int N, int& nt, int& tile) {
 // a turn of the ring from step s of S: acc += its weights x the rows at rec; LAST: no
 // steps of a turn after it are fetched
 template <int TM, int P, int NM, bool LAST, int I = 0>
-HX_DEV void mx_turn(MxRing<P, NM>& ring, const uint8_t* rec, int s, int S, mx_v16f (&acc)[NM][TM / 32]) {
-  constexpr int RB = MxRec<P>::BYTES, R = MxRing<P, NM>::R, U = MxRing<P, NM>::U;
+HX_DEV void mx_turn(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const uint8_t* rec, int s, int S, mx_v16f (&acc)[NM][TM / 32]) {
+  constexpr int RB = MxRec<P>::BYTES, R = MxRing<P, NM, 0>::R, U = MxRing<P, NM, 0>::U;
   if constexpr (I < U) {
     if (!LAST || s + I < S) {
 #pragma unroll
@@ -886,10 +891,10 @@ HX_DEV void mx_turn(MxRing<P, NM>& ring, const uint8_t* rec, int s, int S, mx_v1
 // acc = the sums over nblk blocks of K of the ring's weights x the tile's rows, which
 // come into buf's two halves in turn, a chunk ahead
 template <int TM, int P, int NM>
-HX_DEV void mx_products(MxRing<P, NM>& ring, const MxRows<TM, P>& rw, int wave, uint8_t* buf, int nblk,
+HX_DEV void mx_products(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const MxRows<TM, P>& rw, int wave, uint8_t* buf, int nblk,
                         mx_v16f (&acc)[NM][TM / 32]) {
   constexpr int RB = MxRec<P>::BYTES, CB = MxRows<TM, P>::CB, BYTES = MxRows<TM, P>::BYTES;
-  constexpr int R = MxRing<P, NM>::R, U = MxRing<P, NM>::U, W = MxRing<P, NM>::W;
+  constexpr int R = MxRing<P, NM, 0>::R, U = MxRing<P, NM, 0>::U, W = MxRing<P, NM, 0>::W;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
   const int lane = lane_id(), S = nblk / 2;
   const uint8_t* rec = buf + ((lane >> 5) * TM + (lane & 31)) * RB;
@@ -979,7 +984,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
     const int t = sh ? p - a.F : a.perm[p] / a.k;
     return a.xrec + (int64_t)t * HB * RB;
   });
-  MxRing<P, 2 * MF> ring;
+  MxRing<P, 2 * MF, TM == 32 ? 2 : 0> ring;
   ring.matrix(0, sh ? a.sgate.base : a.gate.mat(e), inter, a.H);
   ring.matrix(1, sh ? a.sup.base : a.up.mat(e), inter, a.H);
 #pragma unroll
@@ -1033,7 +1038,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   const int IB = mx_blocks(inter), S = mx_steps(inter), S4 = (S + 3) / 4, n0 = (4 * nt + wave) * NM;
   MxRows<TM, P> rw;
   rw.init([&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * RB; });
-  MxRing<P, NM> ring;
+  MxRing<P, NM, TM == 32 ? 2 : 0> ring;
   ring.matrix(0, sh ? a.sdown.base : a.down.mat(e), a.H, inter);
   ring.mat[1] = ring.mat[0];
 #pragma unroll
@@ -1095,12 +1100,25 @@ hipError_t launch_mx_down(const MxArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+constexpr int64_t MX_CACHE = 256ll << 20;   // bytes of the cache before the memory
+
+template <bool NT>
+HX_DEV uint4 mx_row16(const void* p) {
+  if constexpr (NT) {
+    const mx_v4u v = __builtin_nontemporal_load((const mx_v4u*)p);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  } else {
+    return *(const uint4*)p;
+  }
+}
+
 // y[t] = the token's entries' rows times their weights in their order, then the
 // shared expert's. A wave: 512 outputs of a token, 8 a lane, 8 rows' loads together
 // (an entry without an expert reads row 0 and counts nothing). FEW: rows in f32, a
 // token's entry at that of its first with the same expert; else rows in the
-// activations' type by inv.
-template <bool BF, bool FEW>
+// activations' type by inv; NT: more of them than MX_CACHE, read non-temporally (8192
+// tokens' 369 MB: 65 us against 78; 2048 tokens' 92 MB: 19 against 17).
+template <bool BF, bool FEW, bool NT>
 __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
   constexpr bool R16 = BF && !FEW;
   constexpr int B = 8;
@@ -1137,10 +1155,10 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
       wj[j] = jj < k ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), jj)) : ws;
       const int64_t at = (int64_t)max(pj[j], 0) * a.H + n0;
       if constexpr (R16) {
-        q[j] = *(const uint4*)((const uint16_t*)a.obuf + at);
+        q[j] = mx_row16<NT>((const uint16_t*)a.obuf + at);
       } else {
-        q[j] = *(const uint4*)((const float*)a.obuf + at);
-        r[j] = *(const uint4*)((const float*)a.obuf + at + 4);
+        q[j] = mx_row16<NT>((const float*)a.obuf + at);
+        r[j] = mx_row16<NT>((const float*)a.obuf + at + 4);
       }
     }
 #pragma unroll
@@ -1211,11 +1229,19 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
 hipError_t launch_mx_combine(const MxArgs& a, hipStream_t s) {
   const int64_t waves = (int64_t)a.T * ((a.H + 511) / 512);
   const dim3 g((unsigned)((waves + 3) / 4));
-  const bool few = mx_few(a.T, a.k, a.H, a.xbf);
-  if (a.xbf && few) hx_launch(k_mx_combine<true, true>, g, dim3(256), 0, s, a);
-  else if (a.xbf) hx_launch(k_mx_combine<true, false>, g, dim3(256), 0, s, a);
-  else if (few) hx_launch(k_mx_combine<false, true>, g, dim3(256), 0, s, a);
-  else hx_launch(k_mx_combine<false, false>, g, dim3(256), 0, s, a);
+  const int64_t rows = ((int64_t)a.F + (a.Is > 0 ? a.T : 0)) * a.H * (a.xbf ? 2 : 4);   // bytes
+  const bool few = mx_few(a.T, a.k, a.H, a.xbf), nt = rows > MX_CACHE;
+#define COMBINE(BF, FEW, NT) hx_launch(k_mx_combine<BF, FEW, NT>, g, dim3(256), 0, s, a)
+  if (a.xbf) {
+    if (few) COMBINE(true, true, false);
+    else if (nt) COMBINE(true, false, true);
+    else COMBINE(true, false, false);
+  } else {
+    if (few) COMBINE(false, true, false);
+    else if (nt) COMBINE(false, false, true);
+    else COMBINE(false, false, false);
+  }
+#undef COMBINE
   return hipGetLastError();
 }
 
