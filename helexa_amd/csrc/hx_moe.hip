@@ -15,7 +15,10 @@
 // combine. Prefill runs router (which also writes the f16 tokens), per-token
 // routing (which also writes the Q8 operand of the quantised-arm tiles),
 // dispatch, gate/up, the quantisation of h for the quantised-arm tiles, down
-// (weighted rows) and combine.
+// (weighted rows) and combine. MXFP4 experts take the router and the per-token routing
+// (hx_moe_experts: the caller's), then hx_mx.hip's kernels: gate/up, down and combine of
+// up to 8 tokens (one token's down combines), else records, dispatch, gate/up, down,
+// combine.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>

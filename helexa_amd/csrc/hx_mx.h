@@ -12,14 +12,15 @@
 // is cut into P planes of E2M3 codes (4 significant bits, largest 7.5), each with its
 // own power-of-two scale: S = 2^(floor(log2 amax) - 2) for the first, S 2^-3 for what
 // it leaves (at most S / 2), then 2^-5 of the one before for each next. Each step leaves at
-// most 2^-5 of the one before, so that three planes hold a value to S 2^-11, half a unit
-// in the 14th bit of the block's largest (bf16 has 8), and five to S 2^-21. The products of the
-// codes are exact and the MFMA sums them in f32, so a product with bf16 activations
-// costs three MFMAs at the 4 / 6-bit rate, which is four times the bf16 rate: less
-// than one bf16 MFMA, and no weight is ever expanded.
+// most 2^-5 of the one before, so that three planes hold a value to S 2^-11, at most
+// 2^-13 of the block's largest (a bf16 value's own rounding is 2^-9 of it), and five to
+// S 2^-21. The products of the codes are exact and the MFMA sums them in f32. A product
+// with bf16 activations costs three MFMAs at the 4 / 6-bit rate (9.3 PFLOP/s measured),
+// four times the bf16 rate: less than one bf16 MFMA, and no weight is ever expanded.
 // A record is the first 16 of each plane's 24 bytes of codes, then the last 8 of each
 // (both are loaded straight into the registers of an MFMA operand), then the P scale
-// bytes; 80 bytes with three planes, 128 with five. A block with a NaN or an infinity has scale NaN: its token's outputs are NaN.
+// bytes; 80 bytes with three planes, 128 with five. A block with a NaN or an infinity has
+// scale NaN: its token's outputs are NaN.
 #pragma once
 #include "hx_internal.h"
 

@@ -284,10 +284,13 @@ __host__ __device__ inline int mx_wave_steps(int S, int W) {
 
 // Gate/up of up to 8 tokens. Workgroup: a chosen expert (slot) and 8 / KW groups of 32
 // features; KW waves share a group's K and add up in LDS. The tokens' records are
-// made in LDS by every workgroup: a kernel of their own would cost more than it saves.
-// The planes are columns: with them one after the other the products took 8 of the
-// 26 us of 6 tokens' 64 MB.
+// made in LDS by every workgroup: a kernel of their own would cost a launch (about 4 us).
+// The planes are columns: with them one after the other the products alone took 8 us of
+// 6 tokens' call.
 // ONE token: an expert a chosen entry, its weights on their way before anything else.
+// Bound by latency and the weight stream: the routing, the experts' addresses, the weights
+// in flight, two sums through LDS. H 2048, I 512, 10 of 512 experts, bf16: one token's 12 MB
+// in 7 us, 6 tokens' 64 MB in 17 (3.8 TB/s), 8 tokens' 85 MB in 23.
 template <int P, int KW, bool ONE>
 __global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, FW = 8 / KW;
@@ -501,7 +504,9 @@ HX_DEV mx_v16f mx_few_unit(const MxArgs& a, const uint8_t* mat, int inter, int n
 }
 
 // Down and combine of one token. Workgroup: 32 outputs; its 16 waves take the units
-// (entry, 8 steps of K) in turn, weigh each product in f32, and add up in LDS.
+// (entry, 8 steps of K) in turn, weigh each product in f32, and add up in LDS. No
+// combine, so a launch less. 6 us for 10 experts and the shared one of 2048 x 512: a
+// launch, the routing's round trip, the weights', and the sums.
 template <int P>
 __global__ __launch_bounds__(1024) void k_mx_one_down(MxArgs a) {
   __shared__ float red[16 * P * 32];
@@ -536,7 +541,9 @@ __global__ __launch_bounds__(1024) void k_mx_one_down(MxArgs a) {
 
 // Outputs of the experts for 2 to 8 tokens, unweighted and in f32, in the row of the
 // token's first entry with the expert. Workgroup: a chosen expert (slot) and 128
-// outputs; a wave 32 of them and all of K.
+// outputs; a wave 32 of them and all of K, its 8 KB of a step group in flight together.
+// 6 tokens' 32 MB of 2048 x 512 experts: 10.5 us (3 TB/s; of them about 5 before the
+// first weights can be asked for).
 template <int P>
 __global__ __launch_bounds__(256) void k_mx_few_down(MxArgs a) {
   __shared__ MxFew few;
@@ -700,7 +707,9 @@ HX_DEV void mx_place(const MxArgs& a, MxPlace& sm, int c, const int (&count)[HX_
 }
 
 // Workgroups 0 .. chunks - 1: the chunk's entries by expert, and where there is one
-// chunk alone (a launch less: about 4 us) their places too; the others: the tokens' records.
+// chunk alone (a launch less: about 4 us) their places too; the others: the tokens' records,
+// a thread a block of 32. Bound by launch and latency up to some hundred tokens (4.5 us),
+// then by HBM: 8192 tokens of 2048, 34 MB in and 42 out, 23 us.
 template <int P>
 __global__ __launch_bounds__(256) void k_mx_prep(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, EPT = HX_MAX_EXPERTS / 256;
@@ -738,7 +747,8 @@ __global__ __launch_bounds__(256) void k_mx_prep(MxArgs a) {
   for (int i = 0; i < RV; i++) o[i] = r[i];
 }
 
-// several chunks: every workgroup sums the chunks' counts itself and places its own entries
+// several chunks: every workgroup sums the chunks' counts itself and places its own
+// entries. Bound by that sum's latency: 4 us for 5 chunks, 10 for 80 (8192 tokens).
 __global__ __launch_bounds__(1024) void k_mx_dispatch(MxArgs a) {
   __shared__ MxPlace sm;
   const int e = threadIdx.x, nch = mx_chunks(a.F), c = blockIdx.x;
@@ -963,7 +973,13 @@ struct MxOut {
   }
 };
 
-// MF groups of 32 features of h a wave
+// h = silu(G x) * (U x), as records. Workgroup: a tile of TM rows and 4 MF groups of 32
+// features, MF a wave, with gate and up of a feature in the same lane. TM 32 (few rows an
+// expert) is bound by the weight stream: 512 tokens on 512 experts of 2048 x 512, 574 MB
+// in 101 us (5.7 TB/s). TM 64 by the loads' way into the CU, at a clock of 1.93 GHz: 8192
+// tokens 338 us, the matrix cores busy 46 % of it and the load units 75 % (a wave's
+// weights meet 64 rows; MF 2 halves the rows' loads, and its sums and ring fill the
+// registers, 213 of 256, two waves a SIMD).
 template <int TM, int P, int MF>
 __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
@@ -1021,7 +1037,9 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
              [&](int r) { return a.hrec + ((int64_t)(p0 + r) * a.hblocks + f0) * RB; });
 }
 
-// outputs of the experts, unweighted: 64 MF features a wave
+// Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 MF
+// features, 64 MF a wave. K is short (I), so that a quarter of the time goes into the
+// start and the rows going out. 512 tokens: 287 MB in 56 us (5.1 TB/s); 8192 tokens 221 us.
 template <int TM, int P, int MF>
 __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, NM = 2 * MF;
@@ -1081,7 +1099,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
              [&](int r) { return (uint8_t*)a.obuf + ((int64_t)(p0 + r) * a.H + 32 * n0) * ES; });
 }
 
-// groups of 32 features a wave takes at a time
+// groups of 32 features a wave takes at a time where tiles have 64 rows
 constexpr int MX_MF = 2;
 #define MX_LAUNCH(KERNEL, NX)                                                                    \
   auto go = [&](auto kernel, int mf) {                                                           \
@@ -1114,7 +1132,8 @@ HX_DEV uint4 mx_row16(const void* p) {
 
 // y[t] = the token's entries' rows times their weights in their order, then the
 // shared expert's. A wave: 512 outputs of a token, 8 a lane, 8 rows' loads together
-// (an entry without an expert reads row 0 and counts nothing). FEW: rows in f32, a
+// (an entry without an expert reads row 0 and counts nothing). Bound by HBM, few
+// tokens by latency (4 us). FEW: rows in f32, a
 // token's entry at that of its first with the same expert; else rows in the
 // activations' type by inv; NT: more of them than MX_CACHE, read non-temporally (8192
 // tokens' 369 MB: 65 us against 78; 2048 tokens' 92 MB: 19 against 17).

@@ -137,9 +137,10 @@ int hx_moe_forward_noalloc(hx_moe* m, const void* x, int64_t n_tokens, void* y, 
  * below each 32-wide block's largest (act HX_F32: 23), sums in f32; h = silu(g) u is
  * taken to the same bits; above the few tokens of a decode step each expert's
  * output is rounded to act_dtype before the weighted sum (f32). A token that holds a
- * NaN or an infinity (or whose h does) gets NaN in place of what it reaches. The
- * result of a token does not depend on the others in the call. y may be x. workspace
- * as in hx_moe_forward, 16-byte aligned; a call under stream capture must bring it. */
+ * NaN or an infinity (or whose h does) gets NaN in place of what it reaches. What
+ * the other tokens of a call hold or choose does not change a token's result; how many
+ * they are may, in its last bits. y may be x. workspace as in hx_moe_forward, 16-byte
+ * aligned; a call under stream capture must bring it. */
 int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const int32_t* topk_idx, const float* topk_w,
                    const float* shared_w, void* y, void* workspace, size_t workspace_bytes, void* stream);
 
