@@ -1,6 +1,7 @@
 """MXFP4 without a GPU: row sizes, the refusals of the entry points (checked
 before anything touches a device), and the numpy rules the GPU tests compare with."""
 import ctypes as C
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -45,6 +46,12 @@ def test_numpy_rules():
     assert M.values(q[0])[0] == 4.0 and M.values(q[0])[15] == -6.0
 
 
+def _alone(f, **kw):
+    """f(**kw) in a thread of its own: the last error is the thread's"""
+    with ThreadPoolExecutor(1) as ex:
+        return ex.submit(f, **kw).result()
+
+
 def _create(**kw):
     """hx_moe_create with pointers that no check reads"""
     import helexa_amd.moe as hx
@@ -69,11 +76,11 @@ def _create(**kw):
     (dict(shared=32, shared_gate_dtype=8, shared_up_dtype=39, shared_down_dtype=39), 2, "routed experts"),
     (dict(gate_dtype=40, up_dtype=40), 2, "unsupported storage dtype")])
 def test_blocks_that_are_refused(kw, rc, what):
-    got, msg = _create(**kw)
+    got, msg = _alone(_create, **kw)
     assert got == rc and what in msg, (got, msg)
 
 
 def test_experts_refuses_bad_arguments():
     import helexa_amd as hx
     p = C.c_void_p(4096)
-    assert hx.lib().hx_moe_experts(None, p, 1, p, p, None, p, None, 0, None) == 1
+    assert _alone(lambda: hx.lib().hx_moe_experts(None, p, 1, p, p, None, p, None, 0, None)) == 1
