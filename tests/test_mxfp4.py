@@ -9,6 +9,12 @@ import pytest
 import mxfp4 as M
 
 
+def _alone(f, **kw):
+    """f(**kw) in a thread of its own: the last error is the thread's"""
+    with ThreadPoolExecutor(1) as ex:
+        return ex.submit(f, **kw).result()
+
+
 def test_row_bytes():
     import helexa_amd as hx
     assert hx.MXFP4 == 39
@@ -21,13 +27,17 @@ def test_row_bytes():
 @pytest.mark.parametrize("fn", ["hx_quantize", "hx_dequantize"])
 def test_refusals_of_the_quantiser(fn):
     import helexa_amd as hx
-    f = getattr(hx.lib(), fn)
     p = C.c_void_p(4096)   # never reached
-    assert f(hx.MXFP4, None, 1, 32, p, None) == 1
-    assert f(hx.MXFP4, p, 1, 32, None, None) == 1
-    assert f(hx.MXFP4, p, -1, 32, p, None) == 1
-    assert f(hx.MXFP4, p, 1, 33, p, None) == 1
-    assert f(hx.MXFP4, p, 0, 32, p, None) == 0   # nothing to do
+
+    def calls():
+        f = getattr(hx.lib(), fn)
+        assert f(hx.MXFP4, None, 1, 32, p, None) == 1
+        assert f(hx.MXFP4, p, 1, 32, None, None) == 1
+        assert f(hx.MXFP4, p, -1, 32, p, None) == 1
+        assert f(hx.MXFP4, p, 1, 33, p, None) == 1
+        assert f(hx.MXFP4, p, 0, 32, p, None) == 0   # nothing to do
+
+    _alone(calls)
 
 
 def test_numpy_rules():
@@ -44,12 +54,6 @@ def test_numpy_rules():
     assert q[1, 0] == 0 and q[2, 0] == 127 + 125 and q[3, 0] == 255 and not q[3, 1:].any()
     assert np.isnan(M.values(q[3])).all()
     assert M.values(q[0])[0] == 4.0 and M.values(q[0])[15] == -6.0
-
-
-def _alone(f, **kw):
-    """f(**kw) in a thread of its own: the last error is the thread's"""
-    with ThreadPoolExecutor(1) as ex:
-        return ex.submit(f, **kw).result()
 
 
 def _create(**kw):
