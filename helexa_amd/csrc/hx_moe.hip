@@ -953,6 +953,20 @@ extern "C" int hx_moe_forward(hx_moe* m, const void* x, int64_t n_tokens, void* 
   return forward_impl(m, x, n_tokens, y, workspace, workspace_bytes, router_bias, (hipStream_t)stream);
 }
 
+// the block's device as the current one, and the caller's again
+struct DeviceScope {
+  int was = -1;
+  hipError_t err;
+  explicit DeviceScope(int device) {
+    if ((err = hipGetDevice(&was)) != hipSuccess) return;
+    if (was == device) was = -1;
+    else err = hipSetDevice(device);
+  }
+  ~DeviceScope() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+
 extern "C" int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const int32_t* topk_idx, const float* topk_w,
                               const float* shared_w, void* y, void* workspace, size_t workspace_bytes, void* stream) {
   if (!m || n_tokens < 0 || (n_tokens > 0 && (!x || !y || !topk_idx || !topk_w)))
@@ -962,7 +976,8 @@ extern "C" int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const 
     return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_experts: shared_w for a block without a shared expert");
   if (n_tokens == 0) return HX_OK;
   if (n_tokens > HX_MAX_TOKENS) return fail(HX_ERR_UNSUPPORTED, "too many tokens in one call");
-  HX_HIP(hipSetDevice(m->device));
+  DeviceScope dev(m->device);
+  HX_HIP(dev.err);
   hipStream_t s = (hipStream_t)stream;
   if (!workspace && capturing(s))   // the handle's own may be freed by a later call, the graph would keep it
     return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_experts: a captured call needs the caller's workspace");

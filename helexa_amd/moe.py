@@ -310,7 +310,7 @@ class Qwen3_5MoeBlock:
             if t is None and last is None:
                 continue
             if (t.dtype != dt or t.numel() != n or t.device != dev or not t.is_contiguous()
-                    or (last is not None and t.shape[-1] != last)):
+                    or (last is not None and t.shape[-1:] != (last,))):
                 raise ValueError(f"{what} must be a contiguous {dt} tensor of {n} values on {dev}"
                                  + (f" with last dim {last}" if last else ""))
         if out is None:
@@ -324,7 +324,8 @@ class Qwen3_5MoeBlock:
         ws, ws_n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
         check(lib().hx_moe_experts(self._h, xs.data_ptr(), T, topk_idx.data_ptr(), topk_w.data_ptr(),
                                    None if shared_w is None else shared_w.data_ptr(), out.data_ptr(), ws, ws_n,
-                                   _stream(stream)), "hx_moe_experts")
+                                   _stream(stream if stream is not None else torch.cuda.current_stream(dev))),
+              "hx_moe_experts")
         return out
 
     def route(self, xs, router_bias=None, stream=None):

@@ -158,6 +158,34 @@ def test_many_tokens_one_call():
         assert torch.equal(blk.experts(x[a:a + 500], idx[a:a + 500], w[a:a + 500]), y[a:a + 500]), a
 
 
+@pytest.mark.parametrize("act", [BF16, F32])
+def test_more_rows_than_the_last_cache(act):
+    """experts' rows of more than 256 MB, compared with the same tokens in calls of 300"""
+    import torch
+    H, E, k, I, Is, T = 2048, 8, 8, 32, 32, 8000 if act == BF16 else 4000
+    blk, _, _ = make(7, H, E, k, I, Is, act)
+    x = tokens(3, T, H, act)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    idx = torch.randint(-1, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    w = torch.rand((T, k), generator=g, device="cuda")
+    sw = torch.rand(T, generator=g, device="cuda")
+    y = blk.experts(x, idx, w, shared_w=sw)
+    for a in (0, 100, T // 2, T - 300):
+        b = slice(a, a + 300)
+        assert torch.equal(blk.experts(x[b], idx[b], w[b], shared_w=sw[b]), y[b]), a
+    blk.close()
+
+
+def test_a_routing_without_dimensions_is_refused():
+    import torch
+    blk, _, _ = make(8, 64, 4, 1, 32, 0, BF16)
+    x, i, w = tokens(1, 1, 64, BF16), torch.tensor(1, device="cuda", dtype=torch.int32), torch.tensor(0.5, device="cuda")
+    with pytest.raises(ValueError, match="topk_idx"):
+        blk.experts(x, i, w.view(1, 1))
+    with pytest.raises(ValueError, match="topk_w"):
+        blk.experts(x, i.view(1, 1), w)
+
+
 def test_timing_slots():
     H, E, k, I, Is = 256, 16, 4, 128, 128
     blk, _, _ = make(4, H, E, k, I, Is, BF16)
