@@ -160,9 +160,9 @@ def _ptr(t) -> int:
     return 0 if t is None else int(t.data_ptr())
 
 
-def _stream(stream=None) -> int:
+def _stream(stream=None, device=None) -> int:
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
+    s = stream if stream is not None else torch.cuda.current_stream(device)
     return int(s.cuda_stream)
 
 
@@ -324,8 +324,7 @@ class Qwen3_5MoeBlock:
         ws, ws_n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
         check(lib().hx_moe_experts(self._h, xs.data_ptr(), T, topk_idx.data_ptr(), topk_w.data_ptr(),
                                    None if shared_w is None else shared_w.data_ptr(), out.data_ptr(), ws, ws_n,
-                                   _stream(stream if stream is not None else torch.cuda.current_stream(dev))),
-              "hx_moe_experts")
+                                   _stream(stream, self.device)), "hx_moe_experts")
         return out
 
     def route(self, xs, router_bias=None, stream=None):
@@ -400,22 +399,38 @@ def quantize(dtype: int, w, stream=None):
     w = w.contiguous()
     if w.dtype != torch.float32 or not w.is_cuda:
         raise TypeError("quantize needs a float32 cuda tensor")
+    dev = w.get_device()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return quantize(dtype, w, stream)
     cols = w.shape[-1]
     rb = row_bytes(dtype, cols)
     if rb < 0:
         raise ValueError(f"{cols} columns do not tile into dtype {dtype} blocks")
-    out = torch.empty(w.shape[:-1] + (rb,), dtype=torch.uint8, device=w.device)
-    check(lib().hx_quantize(dtype, _ptr(w), w.numel() // cols, cols, _ptr(out), _stream(stream)), "hx_quantize")
+    out = w.new_empty(w.shape[:-1] + (rb,), dtype=torch.uint8)
+    rows = w.numel() // cols
+    if rows:
+        check(lib().hx_quantize(dtype, w.data_ptr(), rows, cols, out.data_ptr(), _stream(stream, dev)), "hx_quantize")
     return out
 
 
 def dequantize(dtype: int, q, cols: int, stream=None):
+    """GGUF rows of dtype, cuda tensor [..., row bytes] of one-byte elements -> float32 [..., cols]."""
     import torch
     q = q.contiguous()
+    if not q.is_cuda or q.element_size() != 1:
+        raise TypeError("dequantize needs a cuda tensor of bytes")
+    dev = q.get_device()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return dequantize(dtype, q, cols, stream)
     rb = row_bytes(dtype, cols)
+    if rb < 0 or q.shape[-1:] != (rb,):
+        raise ValueError(f"rows of shape {tuple(q.shape)} are not rows of {cols} columns in dtype {dtype} ({rb} bytes)")
+    out = q.new_empty(q.shape[:-1] + (cols,), dtype=torch.float32)
     rows = q.numel() // rb
-    out = torch.empty(q.shape[:-1] + (cols,), dtype=torch.float32, device=q.device)
-    check(lib().hx_dequantize(dtype, _ptr(q), rows, cols, _ptr(out), _stream(stream)), "hx_dequantize")
+    if rows:
+        check(lib().hx_dequantize(dtype, q.data_ptr(), rows, cols, out.data_ptr(), _stream(stream, dev)), "hx_dequantize")
     return out
 
 

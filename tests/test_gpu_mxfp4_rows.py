@@ -95,3 +95,18 @@ def test_unaligned_pointers(rows):
     hx.check(hx.lib().hx_dequantize(hx.MXFP4, out.data_ptr() + 3, rows, cols, back.data_ptr() + 4, s), "hx_dequantize")
     b = back.cpu().numpy()
     assert np.array_equal(b[1:1 + rows * cols], M.values(ref).astype(np.float32)) and b[0] == 0 and not b[1 + rows * cols:].any()
+
+
+def test_rows_that_are_refused_and_no_rows():
+    """rows of another length than the columns' would be read or written past their end"""
+    import torch
+    import helexa_amd as hx
+    q = torch.zeros((4, 34), dtype=torch.uint8, device="cuda")
+    for bad, cols in ((q, 32), (q.view(-1), 64), (q, 48), (q[:, :17], 64), (q.view(2, 2, 2, 17), 64)):
+        with pytest.raises(ValueError):
+            hx.dequantize(hx.MXFP4, bad, cols)
+    with pytest.raises(TypeError):
+        hx.dequantize(hx.MXFP4, q.view(torch.int16), 64)
+    assert hx.dequantize(hx.MXFP4, q[:0], 64).shape == (0, 64)
+    assert hx.quantize(hx.MXFP4, torch.zeros((0, 64), device="cuda")).shape == (0, 34)
+    assert hx.dequantize(hx.MXFP4, q.view(2, 2, 34), 64).shape == (2, 2, 64)

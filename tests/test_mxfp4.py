@@ -40,6 +40,15 @@ def test_refusals_of_the_quantiser(fn):
     _alone(calls)
 
 
+def test_tensors_of_the_host_are_refused():
+    import torch
+    import helexa_amd as hx
+    with pytest.raises(TypeError):
+        hx.quantize(hx.MXFP4, torch.zeros(2, 32))
+    with pytest.raises(TypeError):
+        hx.dequantize(hx.MXFP4, torch.zeros((2, 17), dtype=torch.uint8), 32)
+
+
 def test_numpy_rules():
     """ties to the even code, saturation, both signs of zero, the scale's range"""
     x = np.zeros((4, 32), np.float32)
