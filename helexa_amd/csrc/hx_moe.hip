@@ -137,7 +137,7 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct WsLayout {
   size_t logits, topk_idx, topk_w, sgw, perm, inv, offsets, slots, tiles, counts, plan, dmap, hbuf, hbf, xh, xq, xq32, xcv,
-      hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, total;
+      hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_few, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, total;
   int hstride, max_slots, max_tiles;
 };
 
@@ -203,6 +203,7 @@ static WsLayout ws_layout(const hx_moe* m, int64_t T) {
     L.ym = take(act * T * H);
     if (mfew) {
       L.obuf = take(sizeof(float) * (size_t)(F + T) * H);
+      L.mx_few = take(sizeof(int32_t) * MX_FEW_TAB * (size_t)L.max_slots);
     } else {
       L.mx_xrec = take(rec * (size_t)T * mx_blocks((int)H));
       L.obuf = take(act * (size_t)(F + T) * H);
@@ -704,6 +705,7 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
   a.hblocks = mx_hblocks(m);
   a.obuf = ws + L.obuf;
   if (mx_few(a.T, a.k, a.H, a.xbf)) {
+    a.few = (int32_t*)(ws + L.mx_few);
     tm_ext(m, SLOT_GATE_UP, s);
     HX_HIP(launch_mx_few_gate_up(a, s));
     tm_ext_done(m, SLOT_GATE_UP);

@@ -38,6 +38,7 @@ __host__ __device__ inline int mx_rec_bytes(bool xbf) { return xbf ? 80 : 128; }
 
 // tokens up to which the few-token kernels are used
 constexpr int MX_FEW_T = 8;
+constexpr int MX_FEW_TAB = 64;   // ints of a slot: the row of each of 32 columns (-1: none), the expert (-1: no work)
 // entries of the routing a dispatch workgroup takes, and the most workgroups
 constexpr int MX_CHUNK = 1024, MX_MAX_CHUNKS = 256;
 __host__ __device__ inline int mx_chunk(int64_t F) {   // entries a chunk, a multiple of MX_CHUNK
@@ -60,6 +61,7 @@ struct MxArgs {
   uint8_t* hrec;                            // [F + T][mx_blocks(max(I, Is))] records
   int hblocks;                              // records of a row of hrec
   void* obuf;                               // [F + T, H] expert outputs, act dtype (few tokens: f32)
+  int32_t* few;                             // [slots][MX_FEW_TAB], 2 to 8 tokens: rows of the columns, then the expert
   int32_t* perm;                            // [F] entries by expert
   int32_t* inv;                             // [F] their positions, -1: no expert
   int32_t* hist;                            // [chunks][E]

@@ -276,6 +276,16 @@ HX_DEV int mx_few_slot(const MxFew& sm, int s, int& n) {
   return 32 * L + __ffsll(b) - 1;
 }
 
+// the row of h and of the outputs of token t with expert e (E: the shared one): at the
+// token's first entry with it, -1 if there is none
+HX_DEV int mx_few_row(const MxArgs& a, const MxFew& sm, int e, int t) {
+  int row = e == a.E ? a.F + t : -1;
+  if (e != a.E)
+    for (int j = a.k - 1; j >= 0; j--)
+      if (sm.idx[t * a.k + j] == e) row = t * a.k + j;
+  return row;
+}
+
 // steps of K a wave takes where W waves share them: 1, 2 or whole words of scales
 __host__ __device__ inline int mx_wave_steps(int S, int W) {
   const int c = (S + W - 1) / W;
@@ -338,11 +348,16 @@ __global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(M
     int n;
     e = mx_few_slot(few, slot, n);
     if (e < 0) {
-      if (slot > n || a.Is == 0) return;
+      if (slot > n || a.Is == 0) {
+        if (blockIdx.x == 0 && tid == 0) a.few[slot * MX_FEW_TAB + 32] = -1;
+        return;
+      }
       e = a.E;
     }
   }
   start();
+  if (!ONE && blockIdx.x == 0 && tid < 33)   // for the down kernel
+    a.few[slot * MX_FEW_TAB + tid] = tid == 32 ? e : tid < P * T ? mx_few_row(a, few, e, tid % T) : -1;
   if ((int)blockIdx.x * FW >= mx_blocks(inter)) return;
   for (int b = tid; b < T * HB; b += 512) {
     const int t = b / HB, kb = b % HB;
@@ -429,12 +444,7 @@ __global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(M
   if (tid < FW * T) {
     const int ft = tid / T, tt = tid % T, f0 = blockIdx.x * FW + ft;
     // the row of h: the token's first entry with this expert
-    const bool sh = e == a.E;
-    int row = sh ? a.F + tt : -1;
-    if (!sh && ONE) row = slot;
-    else if (!sh)
-      for (int j = a.k - 1; j >= 0; j--)
-        if (few.idx[tt * a.k + j] == e) row = tt * a.k + j;
+    const int row = !ONE ? mx_few_row(a, few, e, tt) : e == a.E ? a.F : slot;
     if (row >= 0 && f0 < mx_blocks(inter)) {
       uint4 r[RV];
       if (32 * f0 >= inter) {
@@ -542,34 +552,19 @@ __global__ __launch_bounds__(1024) void k_mx_one_down(MxArgs a) {
 // Outputs of the experts for 2 to 8 tokens, unweighted and in f32, in the row of the
 // token's first entry with the expert. Workgroup: a chosen expert (slot) and 128
 // outputs; a wave 32 of them and all of K, its 8 KB of a step group in flight together.
-// 6 tokens' 32 MB of 2048 x 512 experts: 10.5 us (3 TB/s; of them about 5 before the
+// 6 tokens' 32 MB of 2048 x 512 experts: 9.8 us (3.3 TB/s; of them about 4 before the
 // first weights can be asked for).
 template <int P>
 __global__ __launch_bounds__(256) void k_mx_few_down(MxArgs a) {
-  __shared__ MxFew few;
   __shared__ float red[4][32][33];
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int T = a.T, k = a.k, nb = 4 * blockIdx.x + wave, slot = blockIdx.y;
-  mx_few_bits(a, few);
-  int n;
-  int e = mx_few_slot(few, slot, n);
-  if (e < 0) {
-    if (slot > n || a.Is == 0) return;
-    e = a.E;
-  }
-  e = __builtin_amdgcn_readfirstlane(e);
-  if (32 * nb >= a.H) return;   // no barrier behind this
+  const int T = a.T, nb = 4 * blockIdx.x + wave, col = lane & 31, half = lane >> 5;
+  const int32_t* tab = a.few + blockIdx.y * MX_FEW_TAB;   // k_mx_few_gate_up's
+  const int e = tab[32], row = tab[col];
+  if (e < 0 || 32 * nb >= a.H) return;   // no barrier behind this
   const bool sh = e == a.E;
-  const int inter = sh ? a.Is : a.I, S = mx_steps(inter);
+  const int inter = sh ? a.Is : a.I, S = mx_steps(inter), p = col / T;
   const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
-  const int col = lane & 31, half = lane >> 5, C = P * T, p = col / T, t = col % T;
-  int row = -1;
-  if (col < C) {
-    if (sh) row = a.F + t;
-    else
-      for (int j = k - 1; j >= 0; j--)
-        if (few.idx[t * k + j] == e) row = t * k + j;
-  }
   mx_v16f d = mx_zero16();
   for (int s = 0; s < S; s += 8) d = mx_few_unit<P>(a, mat, inter, nb, s, row, p, d);
 #pragma unroll
