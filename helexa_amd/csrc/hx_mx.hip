@@ -300,7 +300,7 @@ __host__ __device__ inline int mx_wave_steps(int S, int W) {
 // ONE token: an expert a chosen entry, its weights on their way before anything else.
 // Bound by latency and the weight stream: the routing, the experts' addresses, the weights
 // in flight, two sums through LDS. H 2048, I 512, 10 of 512 experts, bf16: one token's 12 MB
-// in 7 us, 6 tokens' 64 MB in 17 (3.8 TB/s), 8 tokens' 85 MB in 23.
+// in 7 us, 6 tokens' 64 MB in 17 (3.8 TB/s), 8 tokens' 85 MB in 22.6.
 template <int P, int KW, bool ONE>
 __global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, FW = 8 / KW;
@@ -586,13 +586,15 @@ template <int P>
 static void mx_few_gate_up(const MxArgs& a, hipStream_t s) {
   const int slots = mx_few_slots(a.T, a.k, a.E) + (a.Is > 0 ? 1 : 0), tasks = slots * a.hblocks;
   const uint32_t lds = (uint32_t)mx_few_lds(a.T, a.H, a.xbf);
-  // enough waves to keep two on each of the 1024 SIMDs, no more
+  // A wave's start costs as much as some steps of K, so that sharing K pays only where
+  // there are too few waves. K shared by 8, 2 and 1 waves, us (512 experts of 512 x 2048
+  // and others): 72 tasks 8.3, 9.4, -; 264 11.5, 11.8, -; 336 12.4, 11.0, -; 976 22.8,
+  // 19.3, 21.2; 1296 31.4, 24.6, 22.6; 2048 -, 28.8, 28.9.
 #define FGU(KW, ONE) \
   hx_launch(k_mx_few_gate_up<P, KW, ONE>, dim3((a.hblocks + 8 / KW - 1) / (8 / KW), slots), dim3(512), lds, s, a)
   if (a.T == 1) FGU(8, true);
-  else if (tasks >= 2048) FGU(1, false);
-  else if (2 * tasks >= 2048) FGU(2, false);
-  else if (4 * tasks >= 2048) FGU(4, false);
+  else if (tasks >= 1200) FGU(1, false);
+  else if (tasks >= 300) FGU(2, false);
   else FGU(8, false);
 #undef FGU
 }

@@ -68,6 +68,19 @@ def test_experts_against_64_bits(shape, act):
 
 
 @pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("H", [32, 96, 544])
+def test_many_features_of_few_tokens(H, act):
+    """few tokens with many groups of features: K by one wave, or shared by two"""
+    E, k, I, Is = 64, 10, 1056, 1024
+    rows, vals = M.block(H, H, E, I, Is, std=0.02)
+    blk = M.load(rows, H, E, k, I, Is, act)
+    for T in (1, 2, 6, 8):
+        x, idx, w, sw = inputs(T, T, H, E, k, act)
+        check(blk.experts(cuda(x, act), cuda(idx), cuda(w), shared_w=cuda(sw)), x, idx, w, vals, sw, act)
+    blk.close()
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
 def test_many_rows_an_expert(act):
     """tiles of 64 rows, several an expert, their last rows short; experts without rows"""
     H, E, k, I, Is = 192, 6, 2, 96, 64
