@@ -796,14 +796,18 @@ hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s) {
 // and 244, at 40 325 and 259.
 int mx_tile_m(int64_t F, int E, bool xbf) { return !xbf || F <= 28 * (int64_t)E ? 32 : 64; }
 
-// The tile's rows in LDS, CB blocks of K at a time: [CB blocks][TM rows][record]. The
-// records come in by direct loads, 16 bytes a lane, in LDS order; a unit of U blocks is
-// whole KiB loads.
+// The tile's rows in LDS, CB blocks of K at a time: [CB / G groups][TM rows][G records].
+// They come in by direct loads, 16 bytes a lane, in LDS order; a unit of U blocks is whole
+// KiB loads. G 2 reads 160 bytes of a row in a piece where G 1 reads 80 (512 tokens, tiles
+// of 32: 171 -> 168 us), but the operands' 160-byte steps meet more often on a bank: with
+// tiles of 64, 653 -> 659 us at 8192 tokens. f32's records of 128 bytes would all start on
+// one bank.
 template <int TM, int P>
 struct MxRows {
   static constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
   static constexpr int CB = 8, BYTES = CB * TM * RB;
-  static constexpr int U = TM * RV % 64 == 0 ? 1 : 2, LOADS = U * TM * RV / 64;
+  static constexpr int G = P == 3 && TM == 32 ? 2 : 1;   // blocks of a row side by side
+  static constexpr int U = G == 1 && TM * RV % 64 == 0 ? 1 : 2, LOADS = U * TM * RV / 64;
   static_assert(U * TM * RV % 64 == 0, "whole loads");
   const uint8_t* src[LOADS];
   // rowptr(r): the records of the tile's row r
@@ -812,7 +816,7 @@ struct MxRows {
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
       const int q = i * 64 + lane_id();   // 16-byte piece of the unit
-      src[i] = rowptr(q / RV % TM) + q / (TM * RV) * RB + q % RV * 16;
+      src[i] = rowptr(q / (G * RV) % TM) + q / (TM * G * RV) * (G * RB) + q % (G * RV) * 16;
     }
   }
   // blocks b0 .. min(b0 + CB, nblk) - 1 (a multiple of 4)
@@ -899,7 +903,7 @@ HX_DEV void mx_turn(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const uint8_t* rec, i
 #pragma unroll
       for (int n = 0; n < TM / 32; n++) {
         MxB<P> b;
-        b.load(rec + (2 * I * TM + 32 * n) * RB);
+        b.load(rec + (2 * I * TM + 32 * MxRows<TM, P>::G * n) * RB);
         mx_mfma<P, I & 3>(ring.w[I % R], ring.sc[I / 4], b, acc, n);
       }
       if (!LAST || I + R < U) ring.fetch(I % R, s + I + R, S);
@@ -917,7 +921,7 @@ HX_DEV void mx_products(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const MxRows<TM, 
   constexpr int R = MxRing<P, NM, 0>::R, U = MxRing<P, NM, 0>::U, W = MxRing<P, NM, 0>::W;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
   const int lane = lane_id(), S = nblk / 2;
-  const uint8_t* rec = buf + ((lane >> 5) * TM + (lane & 31)) * RB;
+  const uint8_t* rec = buf + (MxRows<TM, P>::G == 2 ? lane % 32 * 2 + lane / 32 : lane / 32 * TM + lane % 32) * RB;
 #pragma unroll
   for (int m = 0; m < NM; m++)
 #pragma unroll
