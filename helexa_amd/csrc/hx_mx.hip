@@ -185,6 +185,19 @@ struct MxB {
 #pragma unroll
     for (int i = 0; i < (P + 3) / 4; i++) sc[i] = *(const uint32_t*)(rec + 24 * P + 4 * i);
   }
+  // a record of 128 bytes whose 16-byte piece j lies at j ^ x
+  HX_DEV void load_swizzled(const uint8_t* rec, int x) {
+    auto at = [&](int byte) { return rec + ((byte & ~15) ^ (16 * x)) + (byte & 15); };
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      const uint4 a = *(const uint4*)at(16 * p);
+      const uint2 b = *(const uint2*)at(16 * P + 8 * p);
+      w[p] = mx_v6i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y};
+    }
+    const uint2 q = *(const uint2*)at(24 * P);
+    sc[0] = q.x;
+    sc[(P - 1) / 4] = q.y;
+  }
 };
 
 // c[m][n] += weights m (one step's codes, their scale in byte SA of sc[m]) x the planes
@@ -796,12 +809,20 @@ hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s) {
 // and 244, at 40 325 and 259.
 int mx_tile_m(int64_t F, int E, bool xbf) { return !xbf || F <= 28 * (int64_t)E ? 32 : 64; }
 
+// Whether an expert's weights are read mostly once: non-temporally then, so that they
+// leave the caches to the rows. 64 tokens on 512 experts 123 -> 112 us, 512 tokens (10
+// rows an expert) 182 -> 172, 2048 (40) 266 -> 258, 2500 (49) 275 -> 273; 3000 (59) no
+// gain, 3500 (68, two tiles) 371 -> 384, 8192 661 -> 688: there the tiles that come
+// later want them in the caches. (f32: no difference.)
+static bool mx_once(const MxArgs& a) { return a.F <= 50 * (int64_t)a.E; }
+
 // The tile's rows in LDS, CB blocks of K at a time: [CB / G groups][TM rows][G records].
 // They come in by direct loads, 16 bytes a lane, in LDS order; a unit of U blocks is whole
 // KiB loads. G 2 reads 160 bytes of a row in a piece where G 1 reads 80 (512 tokens, tiles
 // of 32: 171 -> 168 us), but the operands' 160-byte steps meet more often on a bank: with
 // tiles of 64, 653 -> 659 us at 8192 tokens. f32's records of 128 bytes would all start on
-// one bank.
+// one bank: piece j of row r lies at j ^ r % 8 (512 tokens of 2048 on 512 experts of 512:
+// gate/up 165 -> 128 us, down 88 -> 73).
 template <int TM, int P>
 struct MxRows {
   static constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
@@ -816,7 +837,8 @@ struct MxRows {
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
       const int q = i * 64 + lane_id();   // 16-byte piece of the unit
-      src[i] = rowptr(q / (G * RV) % TM) + q / (TM * G * RV) * (G * RB) + q % (G * RV) * 16;
+      const int row = q / (G * RV) % TM, piece = q % (G * RV);
+      src[i] = rowptr(row) + q / (TM * G * RV) * (G * RB) + (P == 5 ? piece ^ (row & 7) : piece) * 16;
     }
   }
   // blocks b0 .. min(b0 + CB, nblk) - 1 (a multiple of 4)
@@ -832,9 +854,7 @@ struct MxRows {
 // time; a step's registers are loaded again as soon as its MFMAs are issued. (Loaded a
 // stage ahead into a second set, with a barrier and a wait for everything at each
 // stage of 128 columns, the wait was never over in time: MFMAs busy 41 % at 8192 tokens.)
-// AUX 2 (non-temporal) for tiles of 32: mostly one tile reads an expert's weights, and
-// they leave the caches to the rows (512 tokens: 182 -> 172 us; 64: 123 -> 112). With
-// tiles of 64 several do, and want them in the caches (8192: 708 -> 748).
+// AUX 2: non-temporal (mx_once).
 template <int P, int NM, int AUX>
 struct MxRing {
   // steps, words of scales; a chunk of rows is whole turns of the ring
@@ -895,30 +915,32 @@ HX_DEV void mx_tile(int NX, int N, int& nt, int& tile) {
 
 // a turn of the ring from step s of S: acc += its weights x the rows at rec; LAST: no
 // steps of a turn after it are fetched
-template <int TM, int P, int NM, bool LAST, int I = 0>
-HX_DEV void mx_turn(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const uint8_t* rec, int s, int S, mx_v16f (&acc)[NM][TM / 32]) {
-  constexpr int RB = MxRec<P>::BYTES, R = MxRing<P, NM, 0>::R, U = MxRing<P, NM, 0>::U;
+template <int TM, int P, int NM, bool LAST, int AUX, int I = 0>
+HX_DEV void mx_turn(MxRing<P, NM, AUX>& ring, const uint8_t* rec, int s, int S, mx_v16f (&acc)[NM][TM / 32]) {
+  constexpr int RB = MxRec<P>::BYTES, R = MxRing<P, NM, AUX>::R, U = MxRing<P, NM, AUX>::U;
   if constexpr (I < U) {
     if (!LAST || s + I < S) {
 #pragma unroll
       for (int n = 0; n < TM / 32; n++) {
         MxB<P> b;
-        b.load(rec + (2 * I * TM + 32 * MxRows<TM, P>::G * n) * RB);
+        const uint8_t* r = rec + (2 * I * TM + 32 * MxRows<TM, P>::G * n) * RB;
+        if constexpr (P == 5) b.load_swizzled(r, lane_id() & 7);
+        else b.load(r);
         mx_mfma<P, I & 3>(ring.w[I % R], ring.sc[I / 4], b, acc, n);
       }
       if (!LAST || I + R < U) ring.fetch(I % R, s + I + R, S);
       __builtin_amdgcn_sched_barrier(0);
-      mx_turn<TM, P, NM, LAST, I + 1>(ring, rec, s, S, acc);
+      mx_turn<TM, P, NM, LAST, AUX, I + 1>(ring, rec, s, S, acc);
     }
   }
 }
 // acc = the sums over nblk blocks of K of the ring's weights x the tile's rows, which
 // come into buf's two halves in turn, a chunk ahead
-template <int TM, int P, int NM>
-HX_DEV void mx_products(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const MxRows<TM, P>& rw, int wave, uint8_t* buf, int nblk,
+template <int TM, int P, int NM, int AUX>
+HX_DEV void mx_products(MxRing<P, NM, AUX>& ring, const MxRows<TM, P>& rw, int wave, uint8_t* buf, int nblk,
                         mx_v16f (&acc)[NM][TM / 32]) {
   constexpr int RB = MxRec<P>::BYTES, CB = MxRows<TM, P>::CB, BYTES = MxRows<TM, P>::BYTES;
-  constexpr int R = MxRing<P, NM, 0>::R, U = MxRing<P, NM, 0>::U, W = MxRing<P, NM, 0>::W;
+  constexpr int R = MxRing<P, NM, AUX>::R, U = MxRing<P, NM, AUX>::U, W = MxRing<P, NM, AUX>::W;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
   const int lane = lane_id(), S = nblk / 2;
   const uint8_t* rec = buf + (MxRows<TM, P>::G == 2 ? lane % 32 * 2 + lane / 32 : lane / 32 * TM + lane % 32) * RB;
@@ -937,7 +959,7 @@ HX_DEV void mx_products(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const MxRows<TM, 
     if (b0 + CB < nblk) rw.load(wave, b0 + CB, nblk, lds + (h ^ 1) * BYTES);
     for (const int end = min(S - U, (b0 + CB) / 2); s < end; s += U) {
       ring.turn(s, S);
-      mx_turn<TM, P, NM, false>(ring, rec + h * BYTES + (2 * s - b0) * TM * RB, s, S, acc);
+      mx_turn<TM, P, NM, false, AUX>(ring, rec + h * BYTES + (2 * s - b0) * TM * RB, s, S, acc);
     }
     if (b0 + CB >= nblk) break;
     // a turn's loads at least came after the next rows'
@@ -947,7 +969,7 @@ HX_DEV void mx_products(MxRing<P, NM, TM == 32 ? 2 : 0>& ring, const MxRows<TM, 
     h ^= 1;
   }
   ring.turn(s, S);
-  mx_turn<TM, P, NM, true>(ring, rec + h * BYTES + (2 * s - b0) * TM * RB, s, S, acc);
+  mx_turn<TM, P, NM, true, AUX>(ring, rec + h * BYTES + (2 * s - b0) * TM * RB, s, S, acc);
   // the sums leave the loop whole: seen through, their elements are carried through it
   // one by one as well, and spilled
 #pragma unroll
@@ -994,7 +1016,7 @@ struct MxOut {
 // tokens 338 us, the matrix cores busy 46 % of it and the load units 75 % (a wave's
 // weights meet 64 rows; MF 2 halves the rows' loads, and its sums and ring fill the
 // registers, 213 of 256, two waves a SIMD).
-template <int TM, int P, int MF>
+template <int TM, int P, int MF, bool NT>
 __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
   __shared__ __align__(16) uint8_t buf[2 * MxRows<TM, P>::BYTES];
@@ -1014,7 +1036,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
     const int t = sh ? p - a.F : a.perm[p] / a.k;
     return a.xrec + (int64_t)t * HB * RB;
   });
-  MxRing<P, 2 * MF, TM == 32 ? 2 : 0> ring;
+  MxRing<P, 2 * MF, NT ? 2 : 0> ring;
   ring.matrix(0, sh ? a.sgate.base : a.gate.mat(e), inter, a.H);
   ring.matrix(1, sh ? a.sup.base : a.up.mat(e), inter, a.H);
 #pragma unroll
@@ -1024,7 +1046,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
     ring.scales[2 * m] = ring.scales[2 * m + 1] = (int)mx_code_bytes(inter, a.H) + fb * S4 * 256;
   }
   mx_v16f acc[2 * MF][TM / 32];
-  mx_products<TM, P, 2 * MF>(ring, rw, wave, buf, HB, acc);
+  mx_products<TM, P, 2 * MF, NT ? 2 : 0>(ring, rw, wave, buf, HB, acc);
   using Out = MxOut<MF * RB>;
   static_assert(4 * TM * Out::PITCH <= 2 * MxRows<TM, P>::BYTES, "the rows' place holds the results");
   lds_barrier();   // the rows have been read
@@ -1054,7 +1076,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
 // Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 MF
 // features, 64 MF a wave. K is short (I), so that a quarter of the time goes into the
 // start and the rows going out. 512 tokens: 287 MB in 56 us (5.1 TB/s); 8192 tokens 221 us.
-template <int TM, int P, int MF>
+template <int TM, int P, int MF, bool NT>
 __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, NM = 2 * MF;
   __shared__ __align__(16) uint8_t buf[2 * MxRows<TM, P>::BYTES];
@@ -1070,7 +1092,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   const int IB = mx_blocks(inter), S = mx_steps(inter), S4 = (S + 3) / 4, n0 = (4 * nt + wave) * NM;
   MxRows<TM, P> rw;
   rw.init([&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * RB; });
-  MxRing<P, NM, TM == 32 ? 2 : 0> ring;
+  MxRing<P, NM, NT ? 2 : 0> ring;
   ring.matrix(0, sh ? a.sdown.base : a.down.mat(e), a.H, inter);
   ring.mat[1] = ring.mat[0];
 #pragma unroll
@@ -1080,7 +1102,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
     ring.scales[m] = (int)mx_code_bytes(a.H, inter) + n * S4 * 256;
   }
   mx_v16f acc[NM][TM / 32];
-  mx_products<TM, P, NM>(ring, rw, wave, buf, IB, acc);
+  mx_products<TM, P, NM, NT ? 2 : 0>(ring, rw, wave, buf, IB, acc);
   constexpr int ES = P == 3 ? 2 : 4;   // bytes of an output
   using Out = MxOut<32 * NM * ES>;
   static_assert(4 * TM * Out::PITCH <= 2 * MxRows<TM, P>::BYTES, "the rows' place holds the results");
@@ -1119,9 +1141,10 @@ constexpr int MX_MF = 2;
   auto go = [&](auto kernel, int mf) {                                                           \
     hx_launch(kernel, dim3((unsigned)((int64_t)(NX) * ((a.max_tiles + 7) / 8 * 8))), dim3(256), 0, s, a); \
   };                                                                                             \
-  if (a.xbf && a.tile_m == 32) go(KERNEL<32, 3, 1>, 1);                                          \
-  else if (a.xbf) go(KERNEL<64, 3, MX_MF>, MX_MF);                                               \
-  else go(KERNEL<32, 5, 1>, 1)
+  if (a.xbf && a.tile_m == 32) go(KERNEL<32, 3, 1, true>, 1);                                    \
+  else if (a.xbf && mx_once(a)) go(KERNEL<64, 3, MX_MF, true>, MX_MF);                           \
+  else if (a.xbf) go(KERNEL<64, 3, MX_MF, false>, MX_MF);                                        \
+  else go(KERNEL<32, 5, 1, false>, 1)
 
 hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) {
   MX_LAUNCH(k_mx_gate_up, (a.hblocks + 4 * mf - 1) / (4 * mf));
