@@ -813,8 +813,9 @@ int mx_tile_m(int64_t F, int E, bool xbf) { return !xbf || F <= 28 * (int64_t)E 
 // leave the caches to the rows. 64 tokens on 512 experts 123 -> 112 us, 512 tokens (10
 // rows an expert) 182 -> 172, 2048 (40) 266 -> 258, 2500 (49) 275 -> 273; 3000 (59) no
 // gain, 3500 (68, two tiles) 371 -> 384, 8192 661 -> 688: there the tiles that come
-// later want them in the caches. (f32: no difference.)
-static bool mx_once(const MxArgs& a) { return a.F <= 50 * (int64_t)a.E; }
+// later want them in the caches. f32, tiles of 32: 512 tokens 197 -> 191, 1000 (20) 216 ->
+// 212; 2048 366 -> 383.
+static bool mx_once(const MxArgs& a) { return a.F <= (a.tile_m == 32 ? 28 : 50) * (int64_t)a.E; }
 
 // The tile's rows in LDS, CB blocks of K at a time: [CB / G groups][TM rows][G records].
 // They come in by direct loads, 16 bytes a lane, in LDS order; a unit of U blocks is whole
@@ -1144,6 +1145,7 @@ constexpr int MX_MF = 2;
   if (a.xbf && a.tile_m == 32) go(KERNEL<32, 3, 1, true>, 1);                                    \
   else if (a.xbf && mx_once(a)) go(KERNEL<64, 3, MX_MF, true>, MX_MF);                           \
   else if (a.xbf) go(KERNEL<64, 3, MX_MF, false>, MX_MF);                                        \
+  else if (mx_once(a)) go(KERNEL<32, 5, 1, true>, 1);                                            \
   else go(KERNEL<32, 5, 1, false>, 1)
 
 hipError_t launch_mx_gate_up(const MxArgs& a, hipStream_t s) {
