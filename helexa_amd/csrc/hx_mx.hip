@@ -1013,7 +1013,7 @@ struct MxOut {
 // h = silu(G x) * (U x), as records. Workgroup: a tile of TM rows and 4 MF groups of 32
 // features, MF a wave, with gate and up of a feature in the same lane. TM 32 (few rows an
 // expert) is bound by the weight stream: 512 tokens on 512 experts of 2048 x 512, 574 MB
-// in 101 us (5.7 TB/s). TM 64 by the loads' way into the CU, at a clock of 1.93 GHz: 8192
+// in 98 us (5.8 TB/s). TM 64 by the loads' way into the CU, at a clock of 1.93 GHz: 8192
 // tokens 338 us, the matrix cores busy 46 % of it and the load units 75 % (a wave's
 // weights meet 64 rows; MF 2 halves the rows' loads, and its sums and ring fill the
 // registers, 213 of 256, two waves a SIMD).
@@ -1076,7 +1076,7 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
 
 // Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 MF
 // features, 64 MF a wave. K is short (I), so that a quarter of the time goes into the
-// start and the rows going out. 512 tokens: 287 MB in 56 us (5.1 TB/s); 8192 tokens 221 us.
+// start and the rows going out. 512 tokens: 287 MB in 55 us (5.2 TB/s); 8192 tokens 221 us.
 template <int TM, int P, int MF, bool NT>
 __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, NM = 2 * MF;
