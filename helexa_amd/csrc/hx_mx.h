@@ -14,7 +14,7 @@
 // it leaves (at most S / 2), then 2^-5 of the one before for each next. Each step leaves at
 // most 2^-5 of the one before, so that three planes hold a value to S 2^-11, at most
 // 2^-13 of the block's largest (a bf16 value's own rounding is 2^-9 of it), and five to
-// S 2^-21. The products of the codes are exact and the MFMA sums them in f32. A product
+// S 2^-21, and no plane to less than 2^-130. The products of the codes are exact and the MFMA sums them in f32. A product
 // with bf16 activations costs three MFMAs at the 4 / 6-bit rate (9.3 PFLOP/s measured),
 // four times the bf16 rate: less than one bf16 MFMA, and no weight is ever expanded.
 // A record is the first 16 of each plane's 24 bytes of codes, then the last 8 of each

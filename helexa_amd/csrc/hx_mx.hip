@@ -77,9 +77,10 @@ HX_DEV void mx_record(const float (&f)[32], uint4 (&out)[MxRec<P>::VECS]) {
   for (int i = 0; i < 32; i++) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
   const int e = (int)(m >> 23);
   const bool bad = e == 255;
-  // the first scale's exponent byte; at least 20, so that all planes' scales are
-  // normal: blocks below 2^-105 lose what is under 2^-128
-  const int sb = bad ? 127 : max(e - 2, 20);
+  // the first scale's exponent byte; at least so much that the last plane's is 1, a
+  // normal float for the conversions: 2^-126, in steps of 2^-129. Blocks of a largest
+  // magnitude below 2^-116 (three planes; five: 2^-106) lose what is under 2^-130.
+  const int sb = bad ? 127 : max(e - 2, 5 * (P - 1) - 1);
   uint32_t w[4 * MxRec<P>::VECS];
 #pragma unroll
   for (int i = 0; i < 4 * MxRec<P>::VECS; i++) w[i] = 0;

@@ -134,8 +134,8 @@ int hx_moe_forward_noalloc(hx_moe* m, const void* x, int64_t n_tokens, void* y, 
  * gets its shared expert's part, or zeros (padding). The same index twice in a token
  * counts twice. shared_w is device f32 [n_tokens], or NULL for a call without the
  * shared expert. Products are of the stored weights and the activations to 13 bits
- * below each 32-wide block's largest (act HX_F32: 23), sums in f32; h = silu(g) u is
- * taken to the same bits; above the few tokens of a decode step each expert's
+ * below each 32-wide block's largest (act HX_F32: 23) or to 2^-130 where that is more,
+ * sums in f32; h = silu(g) u is taken to the same bits; above the few tokens of a decode step each expert's
  * output is rounded to act_dtype before the weighted sum (f32). A token that holds a
  * NaN or an infinity (or whose h does) gets NaN in place of what it reaches. What
  * the other tokens of a call hold or choose does not change a token's result; how many
