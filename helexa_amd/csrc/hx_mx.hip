@@ -1186,6 +1186,9 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
   const int64_t t = id / segs;
   const int n0 = (int)(id % segs) * 512 + lane * 8;
   if (t >= a.T) return;
+  // a lane behind the row's end computes the row's first outputs and stores nothing: the
+  // others read its entry's row and weight
+  const bool mine = n0 < a.H;
   // lane j: entry j; lane k: the shared expert's row (k <= 64: held apart)
   int p;
   if constexpr (FEW) {
@@ -1199,7 +1202,6 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
   const float w = lane < k ? a.w[t * k + lane] : 0.f;
   const int ps = a.Is > 0 ? a.F + (int)t : -1;
   const float ws = a.Is > 0 ? a.shared_w[t] : 0.f;
-  if (n0 >= a.H) return;
   float acc[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) acc[i] = 0.f;
@@ -1212,7 +1214,7 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
       const int jj = j0 + j;
       pj[j] = jj < k ? __builtin_amdgcn_readlane(p, jj) : jj == k ? ps : -1;
       wj[j] = jj < k ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), jj)) : ws;
-      const int64_t at = (int64_t)max(pj[j], 0) * a.H + n0;
+      const int64_t at = (int64_t)max(pj[j], 0) * a.H + (mine ? n0 : 0);
       if constexpr (R16) {
         q[j] = mx_row16<NT>((const uint16_t*)a.obuf + at);
       } else {
@@ -1242,6 +1244,7 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
       for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wj[j], v[i], acc[i]);
     }
   }
+  if (!mine) return;
   const int64_t at = t * a.H + n0;
   void* const base = a.resid ? a.resid : a.y;
   if constexpr (BF) {
