@@ -687,11 +687,15 @@ struct DecoderFuse {
   void* x;   // layer input; receives x + block(rmsnorm(x))
 };
 
+// before a call's first launch: the records and the experts' rows move by 16 bytes
+static int check_mx_ws(const void* ws) {
+  return (uintptr_t)ws & 15 ? fail(HX_ERR_INVALID_ARGUMENT, "the workspace must start on 16 bytes") : HX_OK;
+}
+
 // the experts' products on MXFP4 weights and their combine (a handle of is_mx)
 static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const float* w, const float* shared_w,
                   void* y, void* resid, uint8_t* ws, const WsLayout& L, hipStream_t s) {
   const hx_moe_config& c = m->cfg;
-  if ((uintptr_t)ws & 15) return fail(HX_ERR_INVALID_ARGUMENT, "the workspace must start on 16 bytes");
   MxArgs a{};
   a.gate = m->gate; a.up = m->up; a.down = m->down;
   a.sgate = m->sgate; a.sup = m->sup; a.sdown = m->sdown;
@@ -755,6 +759,7 @@ static int forward_impl(hx_moe* m, const void* x, int64_t T, void* y, void* ws, 
   if (rc) return rc;
   if (is_mx(m)) {
     // the router and the per-token routing of every format, then hx_moe_experts' path
+    if ((rc = check_mx_ws(ws))) return rc;
     Plan p;
     make_plan(m, x, T, y, (uint8_t*)ws, L, bias, p);
     if (fz) {
@@ -985,7 +990,7 @@ extern "C" int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const 
     return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_experts: a captured call needs the caller's workspace");
   WsLayout L;
   int rc = get_ws(m, n_tokens, workspace, workspace_bytes, L);
-  if (rc) return rc;
+  if (rc || (rc = check_mx_ws(workspace))) return rc;
   return run_mx(m, x, n_tokens, topk_idx, topk_w, shared_w, y, nullptr, (uint8_t*)workspace, L, s);
 }
 

@@ -101,7 +101,9 @@ int hx_moe_workspace_size(const hx_moe* m, int64_t n_tokens, size_t* bytes);
 /* Module::forward (moe.rs:164-199 / tp_qwen3_5.rs:1240-1275), device resident:
  * x and y are device pointers to [n_tokens, H] in act_dtype (the reference's
  * (b, l, H) input flattened, moe.rs:166-167). workspace may be NULL, in which
- * case the handle grows its own. router_bias is an optional device [E] f32 added
+ * case the handle grows its own; on a block of HX_MXFP4 experts it must start on 16
+ * bytes (HX_ERR_INVALID_ARGUMENT before anything is launched; hx_moe_decoder_mlp
+ * alike). router_bias is an optional device [E] f32 added
  * to the router logits before the softmax (a benchmark hook with no reference
  * counterpart; NULL in production). n_tokens == 0 is a no-op. */
 int hx_moe_forward(hx_moe* m, const void* x, int64_t n_tokens, void* y,

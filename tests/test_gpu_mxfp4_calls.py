@@ -1,5 +1,5 @@
 """Calls of the MXFP4 experts whose sizes or arguments meet an edge of a kernel or of an
-entry point: rows that fill only some lanes of the combine."""
+entry point: rows that fill only some lanes of the combine, workspaces off 16 bytes."""
 import numpy as np
 import pytest
 
@@ -23,3 +23,34 @@ def test_more_entries_than_lanes_with_outputs(H, k, Is, act):
         check(blk.experts(cuda(x, act), cuda(idx), cuda(w), shared_w=cuda(sw) if Is else None), x, idx, w, vals,
               sw if Is else None, act)
     blk.close()
+
+
+@pytest.mark.parametrize("T", [1, 6, 9, 70])
+def test_a_workspace_off_16_bytes_is_refused_before_any_launch(T):
+    """hx_moe_forward, hx_moe_decoder_mlp and hx_moe_experts: the error, and workspace, y and
+    the stream of tokens as they were"""
+    import torch
+    from helexa_amd import moe as hx
+    H, E, k, I, Is = 256, 16, 4, 128, 128
+    rows, _ = M.block(3, H, E, I, Is)
+    blk = M.load(rows, H, E, k, I, Is, BF16)
+    x, idx, w, sw = inputs(T, T, H, E, k, BF16)
+    xt, it, wt, st = cuda(x, BF16), cuda(idx), cuda(w), cuda(sw)
+    nw = torch.zeros(H, device="cuda")
+    n = blk.workspace_size(T)
+    ws = torch.full((n + 16,), 7, dtype=torch.uint8, device="cuda")
+    y = torch.full_like(xt, 3.0)
+    was = xt.clone()
+    s = torch.cuda.current_stream().cuda_stream
+    for off in (4, 8):
+        p = ws.data_ptr() + off
+        assert hx.lib().hx_moe_forward(blk.handle, xt.data_ptr(), T, y.data_ptr(), p, n, None, s) == 1
+        assert "16 bytes" in hx.last_error()
+        assert hx.lib().hx_moe_decoder_mlp(blk.handle, xt.data_ptr(), T, nw.data_ptr(), 1e-6, p, n, s) == 1
+        assert hx.lib().hx_moe_experts(blk.handle, xt.data_ptr(), T, it.data_ptr(), wt.data_ptr(), st.data_ptr(),
+                                       y.data_ptr(), p, n, s) == 1
+    torch.cuda.synchronize()
+    assert (ws == 7).all() and (y == 3).all() and torch.equal(xt, was)
+    # 16 bytes are enough
+    want = blk.forward(xt)
+    assert torch.equal(blk.forward(xt, workspace=ws[16:]), want)
