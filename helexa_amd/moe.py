@@ -293,7 +293,9 @@ class Qwen3_5MoeBlock:
         float32 with last dim k (indices outside 0 .. E - 1 are no expert), shared_w
         float32 of one value a token, or None for a call without the shared expert
         -> same shape as xs. `out` as in forward(). A call on another stream than the
-        current one takes contiguous tensors only."""
+        current one takes contiguous tensors only; their memory is kept until that
+        stream is done with it, also where the caller drops them at once. What is in
+        flight on the current stream is the caller's to wait for."""
         import torch
         H, k = self.cfg.hidden_size, self.cfg.num_experts_per_tok
         _check_acts(xs, H, self.act_dtype)
@@ -315,12 +317,14 @@ class Qwen3_5MoeBlock:
                                  + (f" with last dim {last}" if last else ""))
         if out is None:
             out = torch.empty_like(xs)
-            if stream is not None:
-                out.record_stream(stream)
         elif out.shape != xs.shape or out.dtype != xs.dtype or not out.is_contiguous() or out.device != dev:
             raise ValueError("out must be contiguous with the input's shape, dtype and device")
         if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
             raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+        if stream is not None:
+            for t in (xs, topk_idx, topk_w, shared_w, workspace, out):
+                if t is not None:
+                    t.record_stream(stream)
         ws, ws_n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
         check(lib().hx_moe_experts(self._h, xs.data_ptr(), T, topk_idx.data_ptr(), topk_w.data_ptr(),
                                    None if shared_w is None else shared_w.data_ptr(), out.data_ptr(), ws, ws_n,

@@ -1,5 +1,6 @@
 """Calls of the MXFP4 experts whose sizes or arguments meet an edge of a kernel or of an
-entry point: rows that fill only some lanes of the combine, workspaces off 16 bytes."""
+entry point: rows that fill only some lanes of the combine, workspaces off 16 bytes,
+tensors dropped while another stream uses them."""
 import numpy as np
 import pytest
 
@@ -54,3 +55,32 @@ def test_a_workspace_off_16_bytes_is_refused_before_any_launch(T):
     # 16 bytes are enough
     want = blk.forward(xt)
     assert torch.equal(blk.forward(xt, workspace=ws[16:]), want)
+
+
+@pytest.mark.parametrize("T", [1, 6, 30])
+def test_tensors_dropped_while_another_stream_uses_them(T):
+    """a call on a busy stream whose tensors the caller drops at once: their memory goes to
+    nobody else before that stream has read and written it"""
+    import torch
+    H, E, k, I, Is = 256, 16, 4, 128, 128
+    rows, _ = M.block(3, H, E, I, Is)
+    blk = M.load(rows, H, E, k, I, Is, BF16)
+    x, idx, w, sw = inputs(T, T, H, E, k, BF16)
+    ref = blk.experts(cuda(x, BF16), cuda(idx), cuda(w), shared_w=cuda(sw))
+    n = blk.workspace_size(T)
+    # sizes of their own, so that the memory of each comes back for a tensor of its size
+    torch.cuda.empty_cache()
+    s = torch.cuda.Stream()
+    ts = [cuda(x, BF16), cuda(idx), cuda(w), cuda(sw), torch.empty(n, dtype=torch.uint8, device="cuda")]
+    torch.cuda.synchronize()
+    shapes = [(t.shape, t.dtype) for t in ts]
+    places = {t.data_ptr() for t in ts}
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(200_000_000)
+    y = blk.experts(*ts[:3], shared_w=ts[3], workspace=ts[4], stream=s)
+    del ts
+    again = [torch.zeros(sh, dtype=dt, device="cuda") for sh, dt in shapes for _ in range(2)]
+    assert not s.query(), "the stream was done too early to show anything"
+    assert not places & {t.data_ptr() for t in again}
+    s.synchronize()
+    assert torch.equal(y, ref)
