@@ -121,8 +121,11 @@ template <int P>
 HX_DEV void mx_zero_record(uint4 (&out)[MxRec<P>::VECS]) {
 #pragma unroll
   for (int i = 0; i < MxRec<P>::VECS; i++) out[i] = make_uint4(0u, 0u, 0u, 0u);
-  ((uint32_t*)out)[MxRec<P>::SCALE] = 0x7f7f7f7fu;
-  if (P > 4) ((uint32_t*)out)[MxRec<P>::SCALE + 1] = 0x7f7f7f7fu;
+  // by components: a store through a pointer to words puts the record into scratch memory
+  constexpr int V = MxRec<P>::SCALE / 4;
+  static_assert(MxRec<P>::SCALE % 4 == 2, "the scales' words are .z and .w");
+  out[V].z = 0x7f7f7f7fu;
+  if (P > 4) out[V].w = 0x7f7f7f7fu;
 }
 
 // block kb of token row x (H columns) -> its record; blocks past the row are zeros
