@@ -36,7 +36,7 @@ __host__ __device__ inline int64_t mx_mat_bytes(int rows, int K) {
 __host__ __device__ inline int mx_planes(bool xbf) { return xbf ? 3 : 5; }
 __host__ __device__ inline int mx_rec_bytes(bool xbf) { return xbf ? 80 : 128; }
 
-// tokens up to which the few-token kernels are used
+// tokens up to which the few-token kernels may be used (mx_few)
 constexpr int MX_FEW_T = 8;
 constexpr int MX_FEW_TAB = 64;   // ints of a slot: the row of each of 32 columns (-1: none), the expert (-1: no work)
 // entries of the routing a dispatch workgroup takes, and the most workgroups

@@ -479,16 +479,18 @@ __global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(M
   }
 }
 
-// bytes of LDS of k_mx_few_gate_up
+// bytes of LDS of k_mx_few_gate_up: the tokens' records and the one of zeros, then the sums
 static size_t mx_few_lds(int T, int H, bool xbf) {
   const size_t rec = ((size_t)T * mx_blocks(H) + 1) * mx_rec_bytes(xbf);
   const size_t red = (size_t)(8 * 2 * 32 * mx_planes(xbf) * T + 8 * 33 * T) * 4;
   return rec > red ? rec : red;
 }
 
-bool mx_few(int T, int k, int H, bool xbf) {
-  return T <= MX_FEW_T && T * mx_planes(xbf) <= 32 && mx_few_lds(T, H, xbf) <= 60 * 1024;
-}
+// LDS decides. By the sums bf16 has 8 tokens at most (56 KB), f32 5 (55 KB; 6 would be 66);
+// by the records that many up to 2944 columns, fewer of more.
+constexpr size_t MX_FEW_LDS = 60 * 1024;
+static_assert(8 * 2 * 32 * 33 * 4 > MX_FEW_LDS, "the sums of more planes than an MFMA's 32 columns do not fit");
+bool mx_few(int T, int k, int H, bool xbf) { return T <= MX_FEW_T && mx_few_lds(T, H, xbf) <= MX_FEW_LDS; }
 
 // most chosen experts of a call (one token: its entries)
 static int mx_few_slots(int T, int k, int E) { return T == 1 ? k : min(T * k, E); }

@@ -1,13 +1,30 @@
 """Calls of the MXFP4 experts whose sizes or arguments meet an edge of a kernel or of an
 entry point: rows that fill only some lanes of the combine, workspaces off 16 bytes,
-tensors dropped while another stream uses them."""
+tensors dropped while another stream uses them, the border between the few-token kernels
+and the others."""
 import numpy as np
 import pytest
 
 import mxfp4 as M
-from test_gpu_mxfp4_experts import BF16, F32, check, cuda, inputs
+from test_gpu_mxfp4_experts import BF16, F32, cuda, inputs
 
 pytestmark = pytest.mark.gpu
+
+
+def few(T, H, act):
+    """whether the few-token kernels take the call: at most 8 tokens, whose records with one of
+    zeros, and whose sums (8 waves, gate and up, 32 features, a column a plane and token; then
+    h), fit 60 KiB"""
+    planes, rec = (3, 80) if act == BF16 else (5, 128)
+    records, sums = (T * ((H + 127) // 128 * 4) + 1) * rec, (8 * 2 * 32 * planes * T + 8 * 33 * T) * 4
+    return T <= 8 and max(records, sums) <= 60 * 1024
+
+
+def check(y, x, idx, w, vals, sw, act):
+    ref, bound = M.experts_bound(x, idx, w, vals, sw, act == BF16, few(*x.shape, act))
+    off = np.abs(y.float().cpu().numpy().astype(np.float64) - ref) / bound
+    print(f"[err] worst {off.max():.3f} of the bound", flush=True)
+    assert off.max() <= 1.0, np.unravel_index(off.argmax(), off.shape)
 
 
 @pytest.mark.parametrize("act", [BF16, F32])
@@ -84,3 +101,22 @@ def test_tensors_dropped_while_another_stream_uses_them(T):
     assert not places & {t.data_ptr() for t in again}
     s.synchronize()
     assert torch.equal(y, ref)
+
+
+@pytest.mark.parametrize("act,H,most", [(BF16, 64, 8), (F32, 64, 5), (BF16, 2944, 8), (BF16, 2976, 7), (F32, 2944, 5),
+                                        (F32, 2976, 4), (BF16, 4864, 5), (BF16, 4896, 4)])
+def test_which_calls_take_the_few_token_kernels(act, H, most):
+    """up to `most` tokens no records are made ahead of gate/up (the x_f16 slot), from there on they are"""
+    assert few(most, H, act) and not few(most + 1, H, act)
+    E, k, I = 4, 2, 32
+    rows, vals = M.block(1, H, E, I, 0)
+    blk = M.load(rows, H, E, k, I, 0, act)
+    for T in (most, most + 1):
+        x, idx, w, _ = inputs(T, T, H, E, k, act)
+        blk.experts(cuda(x, act), cuda(idx), cuda(w))
+        blk.timing_begin(1)
+        y = blk.experts(cuda(x, act), cuda(idx), cuda(w))
+        slots = {n for n, (ms, c) in blk.timing_end().items() if c}
+        assert ("x_f16" in slots) == (T > most), (T, slots)
+        check(y, x, idx, w, vals, None, act)
+    blk.close()
