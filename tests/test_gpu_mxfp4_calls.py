@@ -1,7 +1,7 @@
 """Calls of the MXFP4 experts whose sizes or arguments meet an edge of a kernel or of an
 entry point: rows that fill only some lanes of the combine, workspaces off 16 bytes,
 tensors dropped while another stream uses them, the border between the few-token kernels
-and the others."""
+and the others, and their instance for many features in f32."""
 import numpy as np
 import pytest
 
@@ -119,4 +119,20 @@ def test_which_calls_take_the_few_token_kernels(act, H, most):
         slots = {n for n, (ms, c) in blk.timing_end().items() if c}
         assert ("x_f16" in slots) == (T > most), (T, slots)
         check(y, x, idx, w, vals, None, act)
+    blk.close()
+
+
+@pytest.mark.parametrize("T,H,I,Is", [(5, 256, 736, 768), (5, 96, 800, 0), (4, 1024, 928, 928), (5, 2048, 736, 64)])
+def test_many_features_of_few_f32_tokens(T, H, I, Is):
+    """at least 1200 groups of 32 features in all: K by one wave, with five planes"""
+    E, k = 64, 10
+    groups = (T * k + (Is > 0)) * ((max(I, Is) + 127) // 128 * 4)
+    assert groups >= 1200
+    rows, vals = M.block(H, H, E, I, Is, std=0.02)
+    blk = M.load(rows, H, E, k, I, Is, F32)
+    x, idx, w, sw = inputs(T, T, H, E, k, F32)
+    # every token its own experts, so that no two entries share a slot
+    idx[:] = np.random.default_rng(H).permutation(E)[:T * k].reshape(T, k)
+    check(blk.experts(cuda(x), cuda(idx), cuda(w), shared_w=cuda(sw) if Is else None), x, idx, w, vals,
+          sw if Is else None, F32)
     blk.close()
