@@ -1,5 +1,6 @@
 """hx_moe_experts on MXFP4 blocks over the range of its types: activations and h whose
-blocks lie near the smallest normal float, against 64-bit products of the stored weights within the bound that the formats and the
+blocks lie near the smallest normal float, weights at both ends of the scale byte,
+against 64-bit products of the stored weights within the bound that the formats and the
 sums allow."""
 import numpy as np
 import pytest
@@ -112,3 +113,59 @@ def test_blocks_of_small_h(T, act):
         idx, w = routing(T - top, T)
         check(blk, to_act(x, act), idx, w, vals, act, f"h about 2^{top}, {T} tokens")
         blk.close()
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("T", [1, 4, 24, 300])
+@pytest.mark.parametrize("size,gate,up,down", [
+    (60, [62, 64], [0, 1, 2, 40], [252, 253, 254]),        # up at the lower end, down at the upper
+    (-60, [182, 184], [253, 254, 200], [0, 1, 2, 60]),     # up at the upper end, down at the lower
+    (117, [0, 1, 2], [5, 10], [122, 127]),                 # gate at the lower end
+    (-121, [253, 254, 240], [243, 244], [120])])           # gate at the upper end
+def test_weights_at_both_ends_of_the_scale(size, gate, up, down, T, act):
+    rows, vals = weights(abs(size), gate, up, down)
+    blk = M.load(rows, H, E, K, I, 0, act)
+    x = np.random.default_rng(T).standard_normal((T, H)) * 2.0 ** size
+    idx, w = routing(T, T)
+    check(blk, to_act(x, act), idx, w, vals, act, f"scales {gate} {up} {down}, {T} tokens")
+    blk.close()
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("T", [1, 4, 12, 300])
+def test_blocks_of_zeros_tiny_and_large_values(T, act):
+    """each element of tokens of zeros, of about 1e-30, and with one block a million times
+    the others"""
+    rows, vals = M.block(4, H, E, I, 0)
+    blk = M.load(rows, H, E, K, I, 0, act)
+    x = np.random.default_rng(T).standard_normal((T, H))
+    idx, w = routing(T, T)
+    for first in range(3):   # one token: each of the three in turn
+        z = x.copy()
+        kind = (np.arange(T) + first) % 3
+        z[kind == 0] = 0.0
+        z[kind == 1] *= 1e-30
+        z[kind == 2, 32:64] *= 1e6
+        check(blk, to_act(z, act), idx, w, vals, act, f"kind {first}, {T} tokens")
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("T", [1, 4, 12, 300])
+def test_a_token_whose_h_overflows(T, act):
+    """a token of 2^100 has an h past the largest float with every expert: NaN for that token,
+    the others' bits as they were"""
+    import torch
+    rows, vals = M.block(4, H, E, I, 0)
+    blk = M.load(rows, H, E, K, I, 0, act)
+    x = to_act(np.random.default_rng(T).standard_normal((T, H)), act)
+    idx, w = routing(T, T)
+    y = blk.experts(cuda(x, act), cuda(idx), cuda(w))
+    big = x.copy()
+    big[T // 2] = 2.0 ** 100
+    for e in idx[T // 2]:
+        g, u = vals["gate"][e] @ big[T // 2].astype(np.float64), vals["up"][e] @ big[T // 2].astype(np.float64)
+        assert (np.maximum(g, 0) * np.abs(u)).max() > 1e39 and np.abs(g).max() < 3e38 and np.abs(u).max() < 3e38
+    yb = blk.experts(cuda(big, act), cuda(idx), cuda(w))
+    others = [t for t in range(T) if t != T // 2]
+    assert yb[T // 2].isnan().all()
+    assert torch.equal(yb[others], y[others])
