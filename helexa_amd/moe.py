@@ -166,6 +166,25 @@ def _stream(stream=None, device=None) -> int:
     return int(s.cuda_stream)
 
 
+def _used_on(stream, *tensors) -> None:
+    """tensors that a call on another stream than the current one reads or writes: their
+    memory goes to nobody else before that stream is done with it"""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
+def _contiguous(t, stream):
+    """t.contiguous(), the copy made on the stream that reads it"""
+    import torch
+    if stream is None or t.is_contiguous():
+        return t.contiguous()
+    t.record_stream(stream)
+    with torch.cuda.stream(stream):
+        return t.contiguous()
+
+
 def _check_bias(bias, E: int, device) -> None:
     """router_bias: None or a contiguous float32 [E] tensor on the block's device"""
     import torch
@@ -321,10 +340,7 @@ class Qwen3_5MoeBlock:
             raise ValueError("out must be contiguous with the input's shape, dtype and device")
         if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
             raise ValueError(f"workspace must be a contiguous tensor on {dev}")
-        if stream is not None:
-            for t in (xs, topk_idx, topk_w, shared_w, workspace, out):
-                if t is not None:
-                    t.record_stream(stream)
+        _used_on(stream, xs, topk_idx, topk_w, shared_w, workspace, out)
         ws, ws_n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
         check(lib().hx_moe_experts(self._h, xs.data_ptr(), T, topk_idx.data_ptr(), topk_w.data_ptr(),
                                    None if shared_w is None else shared_w.data_ptr(), out.data_ptr(), ws, ws_n,
@@ -400,9 +416,9 @@ class Qwen3_5MoeBlock:
 def quantize(dtype: int, w, stream=None):
     """quantize_parallel on the device: float32 cuda tensor [..., cols] -> uint8 GGUF rows."""
     import torch
-    w = w.contiguous()
     if w.dtype != torch.float32 or not w.is_cuda:
         raise TypeError("quantize needs a float32 cuda tensor")
+    w = _contiguous(w, stream)
     dev = w.get_device()
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
@@ -412,6 +428,7 @@ def quantize(dtype: int, w, stream=None):
     if rb < 0:
         raise ValueError(f"{cols} columns do not tile into dtype {dtype} blocks")
     out = w.new_empty(w.shape[:-1] + (rb,), dtype=torch.uint8)
+    _used_on(stream, w, out)
     rows = w.numel() // cols
     if rows:
         check(lib().hx_quantize(dtype, w.data_ptr(), rows, cols, out.data_ptr(), _stream(stream, dev)), "hx_quantize")
@@ -421,9 +438,9 @@ def quantize(dtype: int, w, stream=None):
 def dequantize(dtype: int, q, cols: int, stream=None):
     """GGUF rows of dtype, cuda tensor [..., row bytes] of one-byte elements -> float32 [..., cols]."""
     import torch
-    q = q.contiguous()
     if not q.is_cuda or q.element_size() != 1:
         raise TypeError("dequantize needs a cuda tensor of bytes")
+    q = _contiguous(q, stream)
     dev = q.get_device()
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
@@ -432,6 +449,7 @@ def dequantize(dtype: int, q, cols: int, stream=None):
     if rb < 0 or q.shape[-1:] != (rb,):
         raise ValueError(f"rows of shape {tuple(q.shape)} are not rows of {cols} columns in dtype {dtype} ({rb} bytes)")
     out = q.new_empty(q.shape[:-1] + (cols,), dtype=torch.float32)
+    _used_on(stream, q, out)
     rows = q.numel() // rb
     if rows:
         check(lib().hx_dequantize(dtype, q.data_ptr(), rows, cols, out.data_ptr(), _stream(stream, dev)), "hx_dequantize")

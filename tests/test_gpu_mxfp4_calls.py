@@ -1,7 +1,7 @@
 """Calls of the MXFP4 experts whose sizes or arguments meet an edge of a kernel or of an
 entry point: rows that fill only some lanes of the combine, workspaces off 16 bytes,
 tensors dropped while another stream uses them, the border between the few-token kernels
-and the others, and their instance for many features in f32."""
+and the others, and their instance for many features in f32, rows on another stream."""
 import numpy as np
 import pytest
 
@@ -136,3 +136,45 @@ def test_many_features_of_few_f32_tokens(T, H, I, Is):
     check(blk.experts(cuda(x), cuda(idx), cuda(w), shared_w=cuda(sw) if Is else None), x, idx, w, vals,
           sw if Is else None, F32)
     blk.close()
+
+
+@pytest.mark.parametrize("fn", ["quantize", "dequantize"])
+def test_rows_on_another_stream(fn):
+    """a call on another stream: rows that are no contiguous tensor are copied on that stream, not
+    on the busy current one, and memory that the caller drops while the stream is busy
+    goes to nobody else"""
+    import torch
+    import helexa_amd as hx
+    rows, cols = 300, 96
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randn((rows, cols), generator=g, device="cuda")
+    q = hx.quantize(hx.MXFP4, w)
+    if fn == "quantize":
+        call, src, want = lambda t, **kw: hx.quantize(hx.MXFP4, t, **kw), w, q
+    else:
+        call, src, want = lambda t, **kw: hx.dequantize(hx.MXFP4, t, cols, **kw), q, hx.dequantize(hx.MXFP4, q, cols)
+    s = torch.cuda.Stream()
+    turned = src.t().contiguous()   # its .t() is src again, not contiguous
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    got = call(turned.t(), stream=s)
+    s.synchronize()
+    there = torch.empty_like(want)
+    with torch.cuda.stream(s):
+        there.copy_(got)
+    s.synchronize()
+    assert not torch.cuda.current_stream().query(), "the current stream was done too early to show anything"
+    torch.cuda.synchronize()
+    assert torch.equal(there, want)
+    x = src.clone()
+    torch.cuda.synchronize()
+    place, like = x.data_ptr(), (x.shape, x.dtype)
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(200_000_000)
+    got = call(x, stream=s)
+    del x
+    again = [torch.zeros(like[0], dtype=like[1], device="cuda") for _ in range(2)]
+    assert not s.query(), "the stream was done too early to show anything"
+    assert place not in [t.data_ptr() for t in again]
+    s.synchronize()
+    assert torch.equal(got, want)
