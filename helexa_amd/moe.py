@@ -175,6 +175,18 @@ def _used_on(stream, *tensors) -> None:
                 t.record_stream(stream)
 
 
+def _empty(like, stream, shape, dtype):
+    """a result that a call on `stream` writes: of that stream's memory, since what the
+    current stream has still to do may be with memory that is free there already"""
+    import torch
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        out = like.new_empty(shape, dtype=dtype)
+    out.record_stream(torch.cuda.current_stream(out.device))
+    return out
+
+
 def _contiguous(t, stream):
     """t.contiguous(), the copy made on the stream that reads it"""
     import torch
@@ -313,8 +325,8 @@ class Qwen3_5MoeBlock:
         float32 of one value a token, or None for a call without the shared expert
         -> same shape as xs. `out` as in forward(). A call on another stream than the
         current one takes contiguous tensors only; their memory is kept until that
-        stream is done with it, also where the caller drops them at once. What is in
-        flight on the current stream is the caller's to wait for."""
+        stream is done with it, also where the caller drops them at once. That stream's wait for
+        what makes them, and the current one's for the result, are the caller's."""
         import torch
         H, k = self.cfg.hidden_size, self.cfg.num_experts_per_tok
         _check_acts(xs, H, self.act_dtype)
@@ -335,7 +347,7 @@ class Qwen3_5MoeBlock:
                 raise ValueError(f"{what} must be a contiguous {dt} tensor of {n} values on {dev}"
                                  + (f" with last dim {last}" if last else ""))
         if out is None:
-            out = torch.empty_like(xs)
+            out = _empty(xs, stream, xs.shape, xs.dtype)
         elif out.shape != xs.shape or out.dtype != xs.dtype or not out.is_contiguous() or out.device != dev:
             raise ValueError("out must be contiguous with the input's shape, dtype and device")
         if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
@@ -427,8 +439,8 @@ def quantize(dtype: int, w, stream=None):
     rb = row_bytes(dtype, cols)
     if rb < 0:
         raise ValueError(f"{cols} columns do not tile into dtype {dtype} blocks")
-    out = w.new_empty(w.shape[:-1] + (rb,), dtype=torch.uint8)
-    _used_on(stream, w, out)
+    out = _empty(w, stream, w.shape[:-1] + (rb,), torch.uint8)
+    _used_on(stream, w)
     rows = w.numel() // cols
     if rows:
         check(lib().hx_quantize(dtype, w.data_ptr(), rows, cols, out.data_ptr(), _stream(stream, dev)), "hx_quantize")
@@ -448,8 +460,8 @@ def dequantize(dtype: int, q, cols: int, stream=None):
     rb = row_bytes(dtype, cols)
     if rb < 0 or q.shape[-1:] != (rb,):
         raise ValueError(f"rows of shape {tuple(q.shape)} are not rows of {cols} columns in dtype {dtype} ({rb} bytes)")
-    out = q.new_empty(q.shape[:-1] + (cols,), dtype=torch.float32)
-    _used_on(stream, q, out)
+    out = _empty(q, stream, q.shape[:-1] + (cols,), torch.float32)
+    _used_on(stream, q)
     rows = q.numel() // rb
     if rows:
         check(lib().hx_dequantize(dtype, q.data_ptr(), rows, cols, out.data_ptr(), _stream(stream, dev)), "hx_dequantize")

@@ -1,7 +1,8 @@
 """Calls of the MXFP4 experts whose sizes or arguments meet an edge of a kernel or of an
 entry point: rows that fill only some lanes of the combine, workspaces off 16 bytes,
 tensors dropped while another stream uses them, the border between the few-token kernels
-and the others, and their instance for many features in f32, rows on another stream."""
+and the others, and their instance for many features in f32, rows and results on another
+stream."""
 import numpy as np
 import pytest
 
@@ -177,4 +178,36 @@ def test_rows_on_another_stream(fn):
     assert not s.query(), "the stream was done too early to show anything"
     assert place not in [t.data_ptr() for t in again]
     s.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("fn", ["quantize", "dequantize", "experts"])
+def test_a_result_on_another_stream_keeps_off_what_the_current_one_has_to_do(fn):
+    """memory of the result's size that the current stream frees but has still to write: the call
+    on another stream does not take it"""
+    import torch
+    import helexa_amd as hx
+    rows, cols = 300, 96
+    w = torch.randn((rows, cols), device="cuda")
+    q = hx.quantize(hx.MXFP4, w)
+    if fn == "quantize":
+        call = lambda **kw: hx.quantize(hx.MXFP4, w, **kw)
+    elif fn == "dequantize":
+        call = lambda **kw: hx.dequantize(hx.MXFP4, q, cols, **kw)
+    else:
+        H, E, k, I, Is = 256, 16, 4, 128, 0
+        blk = M.load(M.block(3, H, E, I, Is)[0], H, E, k, I, Is, BF16)
+        x, idx, wt, _ = (cuda(a, BF16 if i == 0 else None) for i, a in enumerate(inputs(1, 90, H, E, k, BF16)))
+        ws = torch.empty(blk.workspace_size(90), dtype=torch.uint8, device="cuda")
+        call = lambda **kw: blk.experts(x, idx, wt, workspace=ws, **kw)
+    want = call()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    late = [torch.full_like(want, 5) for _ in range(4)]
+    del late
+    got = call(stream=s)
+    s.synchronize()
+    assert not torch.cuda.current_stream().query(), "the current stream was done too early to show anything"
+    torch.cuda.synchronize()
     assert torch.equal(got, want)
