@@ -287,16 +287,16 @@ class Qwen3_5MoeBlock:
     def forward(self, xs, router_bias=None, workspace=None, stream=None, out=None):
         """Module::forward: xs (b, l, hidden) or (T, hidden) on this GPU -> same shape.
         `out`, if given, is a contiguous tensor of xs's shape and dtype to write."""
-        import torch
         _check_acts(xs, self.cfg.hidden_size, self.act_dtype)
-        x = xs.contiguous()
+        x = _contiguous(xs, stream)
         _check_bias(router_bias, self.cfg.num_experts, x.device)
         if out is None:
-            y = torch.empty_like(x)
+            y = _empty(x, stream, x.shape, x.dtype)
         else:
             if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
                 raise ValueError("out must be contiguous with the input's shape and dtype")
             y = out
+        _used_on(stream, x, router_bias, workspace, out)
         T = x.numel() // self.cfg.hidden_size
         ws_ptr, ws_n = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
         check(lib().hx_moe_forward(self._h, _ptr(x), T, _ptr(y), ws_ptr, ws_n, _ptr(router_bias), _stream(stream)),
@@ -313,6 +313,7 @@ class Qwen3_5MoeBlock:
             raise ValueError("xs must be contiguous (no copy is made here)")
         if out.shape != xs.shape or out.dtype != xs.dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous with the input's shape and dtype")
+        _used_on(stream, xs, router_bias, out)
         T = xs.numel() // self.cfg.hidden_size
         check(lib().hx_moe_forward_noalloc(self._h, _ptr(xs), T, _ptr(out), _ptr(router_bias), _stream(stream)),
               "hx_moe_forward_noalloc")
@@ -363,16 +364,14 @@ class Qwen3_5MoeBlock:
         """-> dict(topk_idx [T,k] i32, topk_w [T,k] f32, perm [T*k], offsets [E+1], inv [T*k])"""
         import torch
         _check_acts(xs, self.cfg.hidden_size, self.act_dtype)
-        x = xs.contiguous()
+        x = _contiguous(xs, stream)
         _check_bias(router_bias, self.cfg.num_experts, x.device)
+        _used_on(stream, x, router_bias)
         T = x.numel() // self.cfg.hidden_size
         k, E = self.cfg.num_experts_per_tok, self.cfg.num_experts
-        dev = x.device
-        out = dict(topk_idx=torch.empty((T, k), dtype=torch.int32, device=dev),
-                   topk_w=torch.empty((T, k), dtype=torch.float32, device=dev),
-                   perm=torch.empty(T * k, dtype=torch.int32, device=dev),
-                   offsets=torch.empty(E + 1, dtype=torch.int32, device=dev),
-                   inv=torch.empty(T * k, dtype=torch.int32, device=dev))
+        out = dict(topk_idx=_empty(x, stream, (T, k), torch.int32), topk_w=_empty(x, stream, (T, k), torch.float32),
+                   perm=_empty(x, stream, T * k, torch.int32), offsets=_empty(x, stream, E + 1, torch.int32),
+                   inv=_empty(x, stream, T * k, torch.int32))
         check(lib().hx_moe_route(self._h, _ptr(x), T, _ptr(router_bias), _ptr(out["topk_idx"]), _ptr(out["topk_w"]),
                                  _ptr(out["perm"]), _ptr(out["offsets"]), _ptr(out["inv"]), None, 0,
                                  _stream(stream)), "hx_moe_route")
@@ -381,10 +380,11 @@ class Qwen3_5MoeBlock:
     def router_logits(self, xs, router_bias=None, stream=None):
         import torch
         _check_acts(xs, self.cfg.hidden_size, self.act_dtype)
-        x = xs.contiguous()
+        x = _contiguous(xs, stream)
         _check_bias(router_bias, self.cfg.num_experts, x.device)
+        _used_on(stream, x, router_bias)
         T = x.numel() // self.cfg.hidden_size
-        out = torch.empty((T, self.cfg.num_experts), dtype=torch.float32, device=x.device)
+        out = _empty(x, stream, (T, self.cfg.num_experts), torch.float32)
         check(lib().hx_moe_router_logits(self._h, _ptr(x), T, _ptr(router_bias), _ptr(out), _stream(stream)),
               "hx_moe_router_logits")
         return out
@@ -401,6 +401,7 @@ class Qwen3_5MoeBlock:
         if (norm_w.dtype != torch.float32 or tuple(norm_w.shape) != (H,) or not norm_w.is_contiguous()
                 or norm_w.device != x.device):
             raise ValueError(f"norm_w must be a contiguous float32 [{H}] tensor on {x.device}")
+        _used_on(stream, x, norm_w, workspace)
         T = x.numel() // H
         ws_ptr, ws_n = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
         check(lib().hx_moe_decoder_mlp(self._h, _ptr(x), T, _ptr(norm_w), float(eps), ws_ptr, ws_n, _stream(stream)),
@@ -475,14 +476,15 @@ def quantize_activations(weight_dtype: int, x, stream=None):
     float32 or bfloat16 cuda tensor [rows, cols] -> (int8 codes [rows, cols],
     float32 d [rows, cols / block])."""
     import torch
-    x = x.contiguous()
     if not x.is_cuda or x.dim() != 2:
         raise TypeError("quantize_activations needs a 2-d cuda tensor")
+    x = _contiguous(x, stream)
+    _used_on(stream, x)
     act = _act_dtype(x.dtype)
     rows, cols = x.shape
     blk = 32 if weight_dtype == Q8_0 else 256
-    codes = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
-    d = torch.empty((rows, max(cols // blk, 1)), dtype=torch.float32, device=x.device)
+    codes = _empty(x, stream, (rows, cols), torch.int8)
+    d = _empty(x, stream, (rows, max(cols // blk, 1)), torch.float32)
     check(lib().hx_quantize_activations(weight_dtype, _ptr(x), act, rows, cols, _ptr(codes), _ptr(d), _stream(stream)),
           "hx_quantize_activations")
     return codes, d
