@@ -13,10 +13,13 @@
 // own power-of-two scale: S = 2^(floor(log2 amax) - 2) for the first, S 2^-3 for what
 // it leaves (at most S / 2), then 2^-5 of the one before for each next. Each step leaves at
 // most 2^-5 of the one before, so that three planes hold a value to S 2^-11, at most
-// 2^-13 of the block's largest (a bf16 value's own rounding is 2^-9 of it), and five to
-// S 2^-21, and no plane to less than 2^-130. The products of the codes are exact and the MFMA sums them in f32. A product
-// with bf16 activations costs three MFMAs at the 4 / 6-bit rate (9.3 PFLOP/s measured),
-// four times the bf16 rate: less than one bf16 MFMA, and no weight is ever expanded.
+// 2^-13 of the block's largest, and five to S 2^-21; no plane is held to less than 2^-130.
+// A bf16 value below about 2^-6 of its block's largest so loses some of its bits. That is
+// far below the rounding of a product with the large value; it shows only where that one's
+// weight is zero, and a fourth plane would cost a third more MFMAs. The products of the
+// codes are exact and the MFMA sums them in f32. A product with bf16 activations costs
+// three MFMAs at the 4 / 6-bit rate (9.3 PFLOP/s measured), four times the bf16 rate: less
+// than one bf16 MFMA, and no weight is ever expanded.
 // A record is the first 16 of each plane's 24 bytes of codes, then the last 8 of each
 // (both are loaded straight into the registers of an MFMA operand), then the P scale
 // bytes; 80 bytes with three planes, 128 with five. A block with a NaN or an infinity has

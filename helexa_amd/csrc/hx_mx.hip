@@ -9,9 +9,10 @@
 // that lanes l and l + 32 hold the 32 features of one token that make one record of
 // the next product, or 64 bytes of its row.
 //
-// Up to MX_FEW_T tokens (k_mx_few_*): two kernels, a workgroup per expert and 32
-// features. More (k_mx_*): the tokens' records and the expert counts, the dispatch,
-// grouped products over tiles of tile_m rows, and the combine.
+// A few tokens (mx_few): gate/up with a workgroup per expert and 8 / KW groups of 32
+// features, then one token's down, which combines, or down with a workgroup per expert and
+// 128 outputs, and the combine. More: the tokens' records and the expert counts, the
+// dispatch, grouped products over tiles of tile_m rows, and the combine.
 #include "hx_mx.h"
 
 #include <type_traits>
@@ -317,7 +318,8 @@ __host__ __device__ inline int mx_wave_steps(int S, int W) {
 // ONE token: an expert a chosen entry, its weights on their way before anything else.
 // Bound by latency and the weight stream: the routing, the experts' addresses, the weights
 // in flight, two sums through LDS. H 2048, I 512, 10 of 512 experts, bf16: one token's 12 MB
-// in 7 us, 6 tokens' 64 MB in 17 (3.8 TB/s), 8 tokens' 85 MB in 22.6.
+// in 6.7 us, 6 tokens' 64 MB in 17.5 (3.7 TB/s), 8 tokens' 85 MB in 21.8 (3.9); five planes
+// 7.7 for one token, 17.1 for 5.
 template <int P, int KW, bool ONE>
 __global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, FW = 8 / KW;
@@ -534,8 +536,10 @@ HX_DEV mx_v16f mx_few_unit(const MxArgs& a, const uint8_t* mat, int inter, int n
 
 // Down and combine of one token. Workgroup: 32 outputs; its 16 waves take the units
 // (entry, 8 steps of K) in turn, weigh each product in f32, and add up in LDS. No
-// combine, so a launch less. 6 us for 10 experts and the shared one of 2048 x 512: a
-// launch, the routing's round trip, the weights', and the sums.
+// combine, so a launch less. 6.4 us for 10 experts and the shared one of 2048 x 512, 6 MB:
+// bound by latency (routing, weights and records, the last sum of 16 P values by one lane
+// an output) on 64 workgroups, a quarter of the CUs. Twice the bytes of Q8_0 take 5.4 in
+// their own kernel, which spreads them over more.
 template <int P>
 __global__ __launch_bounds__(1024) void k_mx_one_down(MxArgs a) {
   __shared__ float red[16 * P * 32];
@@ -571,7 +575,7 @@ __global__ __launch_bounds__(1024) void k_mx_one_down(MxArgs a) {
 // Outputs of the experts for 2 to 8 tokens, unweighted and in f32, in the row of the
 // token's first entry with the expert. Workgroup: a chosen expert (slot) and 128
 // outputs; a wave 32 of them and all of K, its 8 KB of a step group in flight together.
-// 6 tokens' 32 MB of 2048 x 512 experts: 9.8 us (3.3 TB/s; of them about 4 before the
+// 6 tokens' 32 MB of 2048 x 512 experts: 10.8 us (3.0 TB/s; of them about 4 before the
 // first weights can be asked for).
 template <int P>
 __global__ __launch_bounds__(256) void k_mx_few_down(MxArgs a) {
@@ -777,7 +781,7 @@ __global__ __launch_bounds__(256) void k_mx_prep(MxArgs a) {
 }
 
 // several chunks: every workgroup sums the chunks' counts itself and places its own
-// entries. Bound by that sum's latency: 4 us for 5 chunks, 10 for 80 (8192 tokens).
+// entries. Bound by that sum's latency: 4.9 us for 5 chunks, 10 to 12 for 80 (8192 tokens).
 __global__ __launch_bounds__(1024) void k_mx_dispatch(MxArgs a) {
   __shared__ MxPlace sm;
   const int e = threadIdx.x, nch = mx_chunks(a.F), c = blockIdx.x;
@@ -810,7 +814,8 @@ hipError_t launch_mx_dispatch(const MxArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- grouped products
-// Rows of a tile: 32 while the experts have few rows each. 512 experts of 10 chosen: at
+// Rows of a tile: 32 while the experts have few rows each: F entries over all E experts, so
+// that padding and experts without rows count too (the routing is on the device). 512 experts of 10 chosen: at
 // 20 rows an expert 197 us with tiles of 32 and 229 of 64, at 25 219 and 236, at 31 258
 // and 244, at 40 325 and 259.
 int mx_tile_m(int64_t F, int E, bool xbf) { return !xbf || F <= 28 * (int64_t)E ? 32 : 64; }
@@ -1019,10 +1024,11 @@ struct MxOut {
 // h = silu(G x) * (U x), as records. Workgroup: a tile of TM rows and 4 MF groups of 32
 // features, MF a wave, with gate and up of a feature in the same lane. TM 32 (few rows an
 // expert) is bound by the weight stream: 512 tokens on 512 experts of 2048 x 512, 574 MB
-// in 98 us (5.8 TB/s). TM 64 by the loads' way into the CU, at a clock of 1.93 GHz: 8192
-// tokens 338 us, the matrix cores busy 46 % of it and the load units 75 % (a wave's
-// weights meet 64 rows; MF 2 halves the rows' loads, and its sums and ring fill the
-// registers, 213 of 256, two waves a SIMD).
+// in 99 us (5.8 TB/s; the load units busy 96 %). TM 64 by the loads' way into the CU: 8192
+// tokens 310 to 360 us, the load units busy 86 % of it and the matrix cores 60 %, at a
+// clock of about 1.7 GHz; 2048 tokens 150, 96 and 39 % (a wave's weights meet 64 rows; MF 2
+// halves the rows' loads, and its sums and ring fill the registers, 213 of 256, two waves a
+// SIMD).
 template <int TM, int P, int MF, bool NT>
 __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
@@ -1082,7 +1088,12 @@ __global__ __launch_bounds__(256, 2) void k_mx_gate_up(MxArgs a) {
 
 // Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 MF
 // features, 64 MF a wave. K is short (I), so that a quarter of the time goes into the
-// start and the rows going out. 512 tokens: 287 MB in 55 us (5.2 TB/s); 8192 tokens 221 us.
+// start and the rows going out. 512 tokens: 287 MB in 55 us (5.2 TB/s); 8192 tokens 212 to
+// 239 us, the load units busy 88 %.
+// A row leaves in the activations' type: bf16 rows are half of what this kernel writes and
+// the combine reads (8192 tokens: 369 MB each way, the combine at the HBM's rate), for a
+// rounding of each expert's part by at most 2^-8 of it, as the result's own: 0.0024 of the
+// output's norm from 64 bits in place of 0.0017. The weighted sum is in f32.
 template <int TM, int P, int MF, bool NT>
 __global__ __launch_bounds__(256, 2) void k_mx_down(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, NM = 2 * MF;
@@ -1181,7 +1192,8 @@ HX_DEV uint4 mx_row16(const void* p) {
 // tokens by latency (4 us). FEW: rows in f32, a
 // token's entry at that of its first with the same expert; else rows in the
 // activations' type by inv; NT: more of them than MX_CACHE, read non-temporally (8192
-// tokens' 369 MB: 65 us against 78; 2048 tokens' 92 MB: 19 against 17).
+// tokens' 369 MB: 65 us against 78; 2048 tokens' 92 MB: 19 against 17). f32 rows of 2048 tokens:
+// 34 us.
 template <bool BF, bool FEW, bool NT>
 __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
   constexpr bool R16 = BF && !FEW;
