@@ -88,6 +88,9 @@ extern "C" {
     pub fn hx_moe_forward_host(m: *mut hx_moe, x_host: *const c_void, n_tokens: i64, y_host: *mut c_void, router_bias_host: *const f32) -> c_int;
     pub fn hx_moe_route(m: *mut hx_moe, x: *const c_void, n_tokens: i64, router_bias: *const f32, topk_idx: *mut i32, topk_w: *mut f32, perm: *mut i32, offsets: *mut i32, inv: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn hx_moe_router_logits(m: *mut hx_moe, x: *const c_void, n_tokens: i64, router_bias: *const f32, logits: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn hx_moe_balance_workspace_size(n_tokens: i64, num_experts: c_int, bytes: *mut usize) -> c_int;
+    pub fn hx_moe_expert_counts(topk_idx: *const i32, n_tokens: i64, k: c_int, num_experts: c_int, counts: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn hx_moe_balance_loss(logits: *const c_void, logits_dtype: c_int, n_tokens: i64, num_experts: c_int, topk_idx: *const i32, k: c_int, given_counts: *const i32, coef: f32, loss: *mut f32, counts: *mut i32, probs: *mut f32, dlogits: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn hx_moe_decoder_mlp(m: *mut hx_moe, x: *mut c_void, n_tokens: i64, norm_w: *const f32, eps: f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn hx_quantize(dtype: c_int, src: *const f32, rows: i64, cols: i64, dst: *mut c_void, stream: *mut c_void) -> c_int;
     pub fn hx_dequantize(dtype: c_int, src: *const c_void, rows: i64, cols: i64, dst: *mut f32, stream: *mut c_void) -> c_int;

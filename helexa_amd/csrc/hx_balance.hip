@@ -1,0 +1,396 @@
+// Per-expert counts of a routing and the router's balance loss with its gradient:
+//   L = coef E sum_e f_e P_e,  f_e = k c_e / sum c,  P_e = (1 / n) sum_t p_te,  p_t = softmax(l_t)
+// over the n live tokens t, those with an index in 0 .. E - 1; c_e the entries of expert e,
+// taken as given. With s_t = sum_j f_j p_tj,
+//   L = coef E / n sum_t s_t,   dL / dl_te = coef E / n p_te (f_e - s_t),
+// so that one pass over the logits gives the loss, the means and the gradient: the counts
+// come first, from the routing alone. Sums over tokens stay in a lane's registers, one a
+// column, then go through LDS and a table of one row a workgroup, which a last kernel adds
+// up in 64 bits: no float atomics, the same bits every time.
+#include <algorithm>
+
+#include "hx_abi.h"
+#include "hx_device.h"
+#include "hx_internal.h"
+
+namespace hx {
+
+struct BalArgs {
+  const void* logits;        // [T, E]
+  int64_t T;
+  int E, k;
+  const int32_t* idx;        // [T, k]
+  const int32_t* given;      // [E] counts that f goes by, or null: the routing's own
+  float coef;
+  int32_t* counts;           // [E] or null
+  float* probs;              // [E]
+  float* loss;               // [1]
+  void* dlogits;             // [T, E] or null
+  int32_t* hist;             // [G1][E + 1] entries by expert, live tokens
+  float* part;               // [G2][E + 1] sums of p, sum of s
+  int G1, G2;
+  int lpr;                   // lanes of a row, a power of two
+};
+
+// tokens a workgroup of the counts takes, and their most
+constexpr int BAL_CHUNK = 1024, BAL_MAX_G1 = 64, BAL_MAX_G2 = 1024;
+static int bal_g1(int64_t T) { return (int)std::min<int64_t>((T + BAL_CHUNK - 1) / BAL_CHUNK, BAL_MAX_G1); }
+// the most of the row pass: a wave has two turns at least
+static int bal_g2(int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t>((T + 7) / 8, BAL_MAX_G2)); }
+
+// hist[0 .. E - 1] += the entries by expert of tokens t0 .. t1 - 1, hist[E] += the live ones
+HX_DEV void bal_count(const BalArgs& a, int64_t t0, int64_t t1, int* hist) {
+  for (int64_t t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
+    bool live = false;
+    for (int j = 0; j < a.k; j++) {
+      const int e = a.idx[t * a.k + j];
+      if ((unsigned)e >= (unsigned)a.E) continue;
+      live = true;
+      atomicAdd(&hist[e], 1);
+    }
+    if (live) atomicAdd(&hist[a.E], 1);
+  }
+}
+
+__global__ __launch_bounds__(256) void k_bal_counts(BalArgs a) {
+  __shared__ int hist[HX_MAX_EXPERTS + 1];
+  for (int e = threadIdx.x; e <= a.E; e += 256) hist[e] = 0;
+  __syncthreads();
+  const int64_t per = (a.T + a.G1 - 1) / a.G1, t0 = blockIdx.x * per;
+  bal_count(a, t0, min(a.T, t0 + per), hist);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= a.E; e += 256) a.hist[(int64_t)blockIdx.x * (a.E + 1) + e] = hist[e];
+}
+
+// the chunks' counts of column e, eight loads on their way together
+HX_DEV int bal_sum(const BalArgs& a, int e) {
+  int n = 0;
+  for (int g0 = 0; g0 < a.G1; g0 += 8) {
+    int h[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) h[i] = g0 + i < a.G1 ? a.hist[(int64_t)(g0 + i) * (a.E + 1) + e] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) n += h[i];
+  }
+  return n;
+}
+
+__global__ __launch_bounds__(256) void k_bal_counts_sum(BalArgs a) {
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (e < a.E) a.counts[e] = bal_sum(a, e);
+}
+
+// sum / maximum over the lpr lanes of a row, in all of them
+HX_DEV float bal_row_sum(float v, int lpr) {
+  if (lpr == 64) return wave_sum<64>(v);
+  for (int off = lpr / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+HX_DEV float bal_row_max(float v, int lpr) {
+  if (lpr == 64) return wave_max_dpp(v);
+  for (int off = lpr / 2; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
+}
+
+// exp(x), x <= 0 or NaN: the product with log2 e in two parts, so that its rounding (3e-6 of
+// the result at -60) is not in the exponent
+HX_DEV float bal_exp(float x) {
+  x = x < -150.f ? -150.f : x;   // not a maximum: a NaN stays
+  const float hi = x * 1.44269502e+00f;
+  const float lo = __builtin_fmaf(x, 1.44269502e+00f, -hi) + x * 1.92596303e-08f;
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return __builtin_fmaf(e, lo * 6.93147182e-01f, e);
+}
+
+// V elements at p
+template <bool BF, int V>
+HX_DEV void bal_load(const void* base, int64_t at, float (&f)[V]) {
+  if constexpr (BF && V == 8) {
+    const uint4 v = *(const uint4*)((const uint16_t*)base + at);
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      f[2 * i] = __uint_as_float(u[i] << 16);
+      f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  } else if constexpr (!BF && V == 4) {
+    const float4 v = *(const float4*)((const float*)base + at);
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  } else {
+    static_assert(V == 1, "16 bytes or one element");
+    f[0] = ld_act(base, at, BF);
+  }
+}
+template <bool BF, int V>
+HX_DEV void bal_store(void* base, int64_t at, const float (&f)[V]) {
+  if constexpr (BF && V == 8) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) u[i] = f32_to_bf16(f[2 * i]) | ((uint32_t)f32_to_bf16(f[2 * i + 1]) << 16);
+    *(uint4*)((uint16_t*)base + at) = make_uint4(u[0], u[1], u[2], u[3]);
+  } else if constexpr (!BF && V == 4) {
+    *(float4*)((float*)base + at) = make_float4(f[0], f[1], f[2], f[3]);
+  } else if constexpr (BF) {
+    ((uint16_t*)base)[at] = f32_to_bf16(f[0]);
+  } else {
+    ((float*)base)[at] = f[0];
+  }
+}
+
+// The row pass: lpr lanes a row (64 / lpr rows a wave at a time), lane j of a row its
+// columns (i lpr + j) V .. + V - 1 for i < NJ. ONE: one workgroup does it all, counts and
+// last sums included.
+template <bool BF, int V, int NJ, bool ONE>
+__global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
+  constexpr int NW = ONE ? 16 : 4, NT = 64 * NW;
+  extern __shared__ __align__(16) float sm[];
+  float* const f_of = sm;                         // [E] f
+  float* const sums = sm + a.E;                   // [NW][E + 1] the waves' sums
+  int* const hist = (int*)(sums + NW * (a.E + 1));   // [E + 1]
+  __shared__ double total_of[NW];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), E = a.E, k = a.k;
+  for (int e = tid; e <= E; e += NT) hist[e] = ONE ? 0 : bal_sum(a, e);
+  __syncthreads();
+  if (ONE) {
+    bal_count(a, 0, a.T, hist);
+    __syncthreads();
+  }
+  const int live_n = hist[E];
+  double total = 0.0;   // whole numbers: exact in any order; the counts of many devices may pass 32 bits
+  for (int e = tid; e < E; e += NT) {
+    total += a.given ? a.given[e] : hist[e];
+    if (blockIdx.x == 0 && a.counts) a.counts[e] = hist[e];
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+  if (lane == 0) total_of[wave] = total;
+  __syncthreads();
+  total = 0.0;
+#pragma unroll
+  for (int w = 0; w < NW; w++) total += total_of[w];
+  for (int e = tid; e < E; e += NT) {
+    const int c = a.given ? a.given[e] : hist[e];
+    f_of[e] = total > 0.0 ? (float)((double)k * c / total) : 0.f;
+  }
+  __syncthreads();
+  const int lpr = a.lpr, rpw = 64 / lpr, sub = lane & (lpr - 1), grp = lane / lpr;
+  float f[NJ][V], sum[NJ][V];
+#pragma unroll
+  for (int i = 0; i < NJ; i++)
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const int c = (i * lpr + sub) * V + v;
+      f[i][v] = c < E ? f_of[c] : 0.f;
+      sum[i][v] = 0.f;
+    }
+  const float scale = live_n > 0 ? a.coef * E / live_n : 0.f;
+  float s_sum = 0.f;
+  const int64_t step = (int64_t)gridDim.x * NW * rpw;
+  for (int64_t t0 = ((int64_t)blockIdx.x * NW + wave) * rpw; t0 < a.T; t0 += step) {
+    const int64_t t = t0 + grp;
+    const bool row = t < a.T;
+    float x[NJ][V];
+#pragma unroll
+    for (int i = 0; i < NJ; i++) {
+      const int c = (i * lpr + sub) * V;
+      if (row && c < E) bal_load<BF, V>(a.logits, t * E + c, x[i]);
+      else
+#pragma unroll
+        for (int v = 0; v < V; v++) x[i][v] = -__builtin_inff();
+    }
+    bool mine = false;
+    for (int j = sub; row && j < k; j += lpr) mine |= (unsigned)a.idx[t * k + j] < (unsigned)E;
+    const unsigned long long any = __ballot(mine);
+    const bool live = lpr == 64 ? any != 0 : ((any >> (grp * lpr)) & ((1ull << lpr) - 1)) != 0;
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < NJ; i++)
+#pragma unroll
+      for (int v = 0; v < V; v++) m = fmaxf(m, x[i][v]);
+    m = bal_row_max(m, lpr);
+    float z = 0.f, s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NJ; i++)
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        const bool in = (i * lpr + sub) * V < E;
+        x[i][v] = in ? bal_exp(x[i][v] - m) : 0.f;
+        z += x[i][v];
+        s = __builtin_fmaf(f[i][v], x[i][v], s);
+      }
+    z = bal_row_sum(z, lpr);
+    s = bal_row_sum(s, lpr);
+    const float r = 1.f / z;
+    s *= r;
+    // a row that is not live, whatever it holds, adds nothing
+    if (live) s_sum += s;
+#pragma unroll
+    for (int i = 0; i < NJ; i++) {
+      const int c = (i * lpr + sub) * V;
+      float g[V];
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        const float p = live ? x[i][v] * r : 0.f;
+        sum[i][v] += p;
+        g[v] = live ? scale * p * (f[i][v] - s) : 0.f;
+      }
+      if (row && a.dlogits && c < E) bal_store<BF, V>(a.dlogits, t * E + c, g);
+    }
+  }
+  // the rows' groups, then the waves
+#pragma unroll
+  for (int i = 0; i < NJ; i++)
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      for (int off = 32; off >= lpr; off >>= 1) sum[i][v] += __shfl_xor(sum[i][v], off, 64);
+      const int c = (i * lpr + sub) * V + v;
+      if (grp == 0 && c < E) sums[wave * (E + 1) + c] = sum[i][v];
+    }
+  for (int off = 32; off >= lpr; off >>= 1) s_sum += __shfl_xor(s_sum, off, 64);
+  if (lane == 0) sums[wave * (E + 1) + E] = s_sum;
+  __syncthreads();
+  for (int e = tid; e <= E; e += NT) {
+    if (ONE) {
+      double v = 0.0;
+      for (int w = 0; w < NW; w++) v += sums[w * (E + 1) + e];
+      if (e < E) a.probs[e] = live_n > 0 ? (float)(v / live_n) : 0.f;
+      else a.loss[0] = live_n > 0 ? (float)(v * a.coef * E / live_n) : 0.f;
+    } else {
+      float v = 0.f;
+      for (int w = 0; w < NW; w++) v += sums[w * (E + 1) + e];
+      a.part[(int64_t)blockIdx.x * (E + 1) + e] = v;
+    }
+  }
+}
+
+// the workgroups' sums: a workgroup 64 columns (of the E + 1), 16 threads a column
+__global__ __launch_bounds__(1024) void k_bal_last(BalArgs a) {
+  __shared__ double red[16][64];
+  __shared__ int live_sm;
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6, e = blockIdx.x * 64 + c;
+  if (threadIdx.x == 0) live_sm = 0;
+  __syncthreads();
+  if (threadIdx.x < a.G1) atomicAdd(&live_sm, a.hist[(int64_t)threadIdx.x * (a.E + 1) + a.E]);
+  double v = 0.0;
+  if (e <= a.E)
+    for (int g = q; g < a.G2; g += 16) v += a.part[(int64_t)g * (a.E + 1) + e];
+  red[q][c] = v;
+  __syncthreads();
+  if (q == 0 && e <= a.E) {
+    const int n = live_sm;
+    v = 0.0;
+    for (int w = 0; w < 16; w++) v += red[w][c];
+    if (e < a.E) a.probs[e] = n > 0 ? (float)(v / n) : 0.f;
+    else a.loss[0] = n > 0 ? (float)(v * a.coef * a.E / n) : 0.f;
+  }
+}
+
+static uint32_t bal_lds(int E, int waves) { return (uint32_t)((E + (waves + 1) * (E + 1)) * 4); }
+
+template <bool BF, int V, int NJ>
+static void launch_rows(const BalArgs& a, bool one, hipStream_t s) {
+  if (one) hx_launch(k_bal_rows<BF, V, NJ, true>, dim3(1), dim3(1024), bal_lds(a.E, 16), s, a);
+  else hx_launch(k_bal_rows<BF, V, NJ, false>, dim3(a.G2), dim3(256), bal_lds(a.E, 4), s, a);
+}
+
+// Where one workgroup does it all: what two more launches cost (about 4 us each) is less
+// than what one CU takes longer.
+static bool bal_one(int64_t T, int E) { return T * E <= 32768 && T <= 1024 && bal_lds(E, 16) <= 60 * 1024; }
+
+static hipError_t launch_balance(BalArgs a, bool bf, hipStream_t s) {
+  const bool one = bal_one(a.T, a.E);
+  const int per = bf ? 8 : 4;
+  const bool vec = a.E % per == 0 && (((uintptr_t)a.logits | (uintptr_t)a.dlogits) & 15) == 0;
+  const int chunks = vec ? a.E / per : a.E;
+  a.lpr = 64;
+  while (a.lpr > 1 && a.lpr / 2 >= chunks) a.lpr /= 2;
+  if (!one) hx_launch(k_bal_counts, dim3(a.G1), dim3(256), 0, s, a);
+  const int nj = (chunks + 63) / 64;
+  if (bf && vec) {
+    if (nj <= 1) launch_rows<true, 8, 1>(a, one, s);
+    else launch_rows<true, 8, 2>(a, one, s);
+  } else if (vec) {
+    if (nj <= 1) launch_rows<false, 4, 1>(a, one, s);
+    else if (nj <= 2) launch_rows<false, 4, 2>(a, one, s);
+    else launch_rows<false, 4, 4>(a, one, s);
+  } else if (bf) {
+    if (nj <= 4) launch_rows<true, 1, 4>(a, one, s);
+    else launch_rows<true, 1, 16>(a, one, s);
+  } else {
+    if (nj <= 4) launch_rows<false, 1, 4>(a, one, s);
+    else launch_rows<false, 1, 16>(a, one, s);
+  }
+  if (!one) hx_launch(k_bal_last, dim3((a.E + 1 + 63) / 64), dim3(1024), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace hx
+
+using namespace hx;
+
+static size_t bal_up(size_t v) { return (v + 255) & ~(size_t)255; }
+static size_t bal_hist_bytes(int64_t T, int E) { return bal_up(sizeof(int32_t) * (size_t)bal_g1(T) * (E + 1)); }
+
+static int check_balance(int64_t n_tokens, int num_experts, int k) {
+  if (n_tokens < 0 || num_experts < 1 || k < 1) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
+  if (num_experts > HX_MAX_EXPERTS || k > HX_MAX_TOPK)
+    return fail(HX_ERR_UNSUPPORTED, "at most %d experts and top-%d are supported", HX_MAX_EXPERTS, HX_MAX_TOPK);
+  if (n_tokens > HX_MAX_TOKENS) return fail(HX_ERR_UNSUPPORTED, "too many tokens in one call");
+  return HX_OK;
+}
+
+extern "C" int hx_moe_balance_workspace_size(int64_t n_tokens, int num_experts, size_t* bytes) {
+  if (!bytes) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
+  int rc = check_balance(n_tokens, num_experts, 1);
+  if (rc) return rc;
+  *bytes = bal_hist_bytes(n_tokens, num_experts) + bal_up(sizeof(float) * (size_t)bal_g2(n_tokens) * (num_experts + 1));
+  return HX_OK;
+}
+
+// the workspace of a call, checked
+static int bal_args(BalArgs& a, const int32_t* topk_idx, int64_t T, int k, int E, void* ws, size_t ws_bytes) {
+  size_t need;
+  int rc = hx_moe_balance_workspace_size(T, E, &need);
+  if (rc) return rc;
+  if (!ws) return fail(HX_ERR_INVALID_ARGUMENT, "null workspace");
+  if (ws_bytes < need)
+    return fail(HX_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed for %lld tokens", ws_bytes, need, (long long)T);
+  if ((uintptr_t)ws & 15) return fail(HX_ERR_INVALID_ARGUMENT, "the workspace must start on 16 bytes");
+  a.T = T; a.E = E; a.k = k; a.idx = topk_idx;
+  a.G1 = bal_g1(T); a.G2 = bal_g2(T);
+  a.hist = (int32_t*)ws;
+  a.part = (float*)((uint8_t*)ws + bal_hist_bytes(T, E));
+  return HX_OK;
+}
+
+extern "C" int hx_moe_expert_counts(const int32_t* topk_idx, int64_t n_tokens, int k, int num_experts, int32_t* counts,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_balance(n_tokens, num_experts, k);
+  if (rc) return rc;
+  if (!counts || (n_tokens > 0 && !topk_idx)) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
+  BalArgs a{};
+  if ((rc = bal_args(a, topk_idx, n_tokens, k, num_experts, workspace, workspace_bytes))) return rc;
+  a.counts = counts;
+  hipStream_t s = (hipStream_t)stream;
+  if (n_tokens > 0) hx_launch(k_bal_counts, dim3(a.G1), dim3(256), 0, s, a);
+  hx_launch(k_bal_counts_sum, dim3((num_experts + 255) / 256), dim3(256), 0, s, a);
+  HX_HIP(hipGetLastError());
+  return HX_OK;
+}
+
+extern "C" int hx_moe_balance_loss(const void* logits, int logits_dtype, int64_t n_tokens, int num_experts,
+                                   const int32_t* topk_idx, int k, const int32_t* given_counts, float coef,
+                                   float* loss, int32_t* counts, float* probs, void* dlogits, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  int rc = check_balance(n_tokens, num_experts, k);
+  if (rc) return rc;
+  if (!loss || !probs || (n_tokens > 0 && (!logits || !topk_idx))) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
+  if (logits_dtype != HX_F32 && logits_dtype != HX_BF16)
+    return fail(HX_ERR_UNSUPPORTED, "hx_moe_balance_loss: logits dtype %d", logits_dtype);
+  BalArgs a{};
+  if ((rc = bal_args(a, topk_idx, n_tokens, k, num_experts, workspace, workspace_bytes))) return rc;
+  a.logits = logits; a.given = given_counts; a.coef = coef;
+  a.loss = loss; a.counts = counts; a.probs = probs; a.dlogits = dlogits;
+  HX_HIP(launch_balance(a, logits_dtype == HX_BF16, (hipStream_t)stream));
+  return HX_OK;
+}

@@ -27,6 +27,7 @@
 #include <mutex>
 
 #include "hx_moe.h"
+#include "hx_abi.h"
 #include "hx_internal.h"
 #include "hx_mx.h"
 
@@ -34,7 +35,7 @@ using namespace hx;
 
 static thread_local char g_err[512];
 
-static int fail(int code, const char* fmt, ...) {
+int hx::fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof g_err, fmt, ap);
@@ -74,13 +75,6 @@ static void* scratch_ptr(int device) {
   std::lock_guard<std::mutex> lock(g_scratch_mu);
   return g_scratch_ptr[device];
 }
-
-#define HX_HIP(call)                                                                               \
-  do {                                                                                             \
-    hipError_t e_ = (call);                                                                        \
-    if (e_ != hipSuccess) return fail(HX_ERR_DEVICE, "%s failed: %s (%s:%d)", #call, hipGetErrorString(e_), \
-                                      __FILE__, __LINE__);                                         \
-  } while (0)
 
 extern "C" const char* hx_last_error(void) { return g_err; }
 
@@ -130,10 +124,6 @@ struct hx_moe {
 };
 
 static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
-
-// token counts above this are refused by every entry point: the kernels index
-// the T * k assignments with 32-bit integers (k <= HX_MAX_TOPK)
-#define HX_MAX_TOKENS ((int64_t)1 << 24)
 
 struct WsLayout {
   size_t logits, topk_idx, topk_w, sgw, perm, inv, offsets, slots, tiles, counts, plan, dmap, hbuf, hbf, xh, xq, xq32, xcv,
@@ -586,12 +576,6 @@ thread_local ExtTiming g_ext_timing;
 // event helpers for the optional per-kernel timing
 // forwards recorded under stream capture are not timed: no event is recorded
 // into the graph, no slot is marked and the call is not counted
-static bool capturing(hipStream_t s) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  (void)hipStreamIsCapturing(s, &st);
-  return st != hipStreamCaptureStatusNone;
-}
-
 static void tm_mark(hx_moe* m, int slot, int which, hipStream_t s) {
   Timing& t = m->tm;
   if (!t.on || t.calls >= t.max_calls || capturing(s)) return;
@@ -959,20 +943,6 @@ extern "C" int hx_moe_forward(hx_moe* m, const void* x, int64_t n_tokens, void* 
   HX_HIP(hipSetDevice(m->device));
   return forward_impl(m, x, n_tokens, y, workspace, workspace_bytes, router_bias, (hipStream_t)stream);
 }
-
-// the block's device as the current one, and the caller's again
-struct DeviceScope {
-  int was = -1;
-  hipError_t err;
-  explicit DeviceScope(int device) {
-    if ((err = hipGetDevice(&was)) != hipSuccess) return;
-    if (was == device) was = -1;
-    else err = hipSetDevice(device);
-  }
-  ~DeviceScope() {
-    if (was >= 0) (void)hipSetDevice(was);
-  }
-};
 
 extern "C" int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const int32_t* topk_idx, const float* topk_w,
                               const float* shared_w, void* y, void* workspace, size_t workspace_bytes, void* stream) {

@@ -36,6 +36,7 @@ STATUS = {0: "HX_OK", 1: "HX_ERR_INVALID_ARGUMENT", 2: "HX_ERR_UNSUPPORTED", 3: 
 # every entry point include/hx_moe.h declares
 EXPORTS = ("hx_moe_create", "hx_moe_destroy", "hx_moe_workspace_size", "hx_moe_forward", "hx_moe_forward_noalloc",
            "hx_moe_forward_host", "hx_moe_experts",
+           "hx_moe_balance_workspace_size", "hx_moe_expert_counts", "hx_moe_balance_loss",
            "hx_moe_route", "hx_moe_router_logits", "hx_moe_decoder_mlp", "hx_quantize", "hx_dequantize",
            "hx_row_bytes", "hx_quantize_activations", "hx_moe_timing_begin", "hx_moe_timing_read", "hx_moe_timing_end",
            "hx_moe_timing_name", "hx_last_error")
@@ -86,6 +87,9 @@ def lib() -> C.CDLL:
             "hx_moe_experts": (i32, [vp, vp, i64, vp, vp, vp, vp, vp, C.c_size_t, vp]),
             "hx_moe_route": (i32, [vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]),
             "hx_moe_router_logits": (i32, [vp, vp, i64, vp, vp, vp]),
+            "hx_moe_balance_workspace_size": (i32, [i64, i32, C.POINTER(C.c_size_t)]),
+            "hx_moe_expert_counts": (i32, [vp, i64, i32, i32, vp, vp, C.c_size_t, vp]),
+            "hx_moe_balance_loss": (i32, [vp, i32, i64, i32, vp, i32, vp, C.c_float, vp, vp, vp, vp, vp, C.c_size_t, vp]),
             "hx_moe_decoder_mlp": (i32, [vp, vp, i64, vp, C.c_float, vp, C.c_size_t, vp]),
             "hx_quantize": (i32, [i32, vp, i64, i64, vp, vp]),
             "hx_dequantize": (i32, [i32, vp, i64, i64, vp, vp]),
@@ -488,3 +492,70 @@ def quantize_activations(weight_dtype: int, x, stream=None):
     check(lib().hx_quantize_activations(weight_dtype, _ptr(x), act, rows, cols, _ptr(codes), _ptr(d), _stream(stream)),
           "hx_quantize_activations")
     return codes, d
+
+
+# ---------------------------------------------------------------------------- balance
+def balance_workspace_size(n_tokens: int, num_experts: int) -> int:
+    """bytes of workspace of expert_counts() and balance_loss() for n_tokens tokens"""
+    n = C.c_size_t()
+    check(lib().hx_moe_balance_workspace_size(n_tokens, num_experts, C.byref(n)), "hx_moe_balance_workspace_size")
+    return n.value
+
+
+def _balance_call(topk_idx, E: int, counts, workspace, stream, logits=None):
+    """what the two calls share: the checked routing, its tokens and k, a workspace"""
+    import torch
+    if topk_idx.dtype != torch.int32 or not topk_idx.is_cuda or topk_idx.dim() == 0 or topk_idx.shape[-1] == 0:
+        raise ValueError("topk_idx must be an int32 cuda tensor [..., k]")
+    dev, k = topk_idx.device, topk_idx.shape[-1]
+    idx = _contiguous(topk_idx, stream)
+    T = idx.numel() // k
+    if logits is not None and (logits.device != dev or logits.shape[:-1].numel() != T):
+        raise ValueError(f"logits must be [..., experts] of {T} tokens on {dev}")
+    if counts is not None and (counts.dtype != torch.int32 or tuple(counts.shape) != (E,) or counts.device != dev
+                               or not counts.is_contiguous()):
+        raise ValueError(f"counts must be a contiguous int32 [{E}] tensor on {dev}")
+    if workspace is None:
+        workspace = _empty(idx, stream, balance_workspace_size(T, E), torch.uint8)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+    _used_on(stream, idx, counts, workspace)
+    return idx, T, k, workspace
+
+
+def expert_counts(topk_idx, num_experts: int, workspace=None, stream=None):
+    """The entries of each expert in a routing: topk_idx int32 [..., k] as route() gives
+    it (indices outside 0 .. E - 1 are no expert) -> int32 [E]."""
+    import torch
+    idx, T, k, ws = _balance_call(topk_idx, num_experts, None, workspace, stream)
+    out = _empty(idx, stream, num_experts, torch.int32)
+    with torch.cuda.device(idx.device):
+        check(lib().hx_moe_expert_counts(_ptr(idx), T, k, num_experts, _ptr(out), _ptr(ws), ws.nbytes,
+                                         _stream(stream, idx.device)), "hx_moe_expert_counts")
+    return out
+
+
+def balance_loss(logits, topk_idx, coef: float = 1.0, counts=None, grad: bool = True, workspace=None, stream=None):
+    """The balance loss of a router, coef E sum_e f_e P_e, with its gradient: logits
+    [..., E] float32 or bfloat16 (router_logits()), topk_idx int32 [..., k] of the same
+    tokens (route()); f_e = k c_e / sum c of the experts' entries c, P_e the mean softmax
+    probability over the live tokens, those with an index in 0 .. E - 1. c is the
+    routing's own counts, or `counts`, an int32 [E] tensor, where several calls or
+    devices are balanced together (expert_counts(), added up).
+    -> dict(loss, a float32 scalar; counts int32 [E], the routing's own; probs float32
+    [E]; dlogits like logits, the loss's gradient, zero for tokens that are not live, or
+    None with grad=False)."""
+    import torch
+    if not logits.is_cuda or logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError("logits must be a cuda tensor [..., experts]")
+    dt, E = _act_dtype(logits.dtype), logits.shape[-1]
+    idx, T, k, ws = _balance_call(topk_idx, E, counts, workspace, stream, logits)
+    x = _contiguous(logits, stream)
+    _used_on(stream, x)
+    out = dict(loss=_empty(x, stream, (), torch.float32), counts=_empty(x, stream, E, torch.int32),
+               probs=_empty(x, stream, E, torch.float32), dlogits=_empty(x, stream, x.shape, x.dtype) if grad else None)
+    with torch.cuda.device(x.device):
+        check(lib().hx_moe_balance_loss(_ptr(x), dt, T, E, _ptr(idx), k, _ptr(counts), float(coef), _ptr(out["loss"]),
+                                        _ptr(out["counts"]), _ptr(out["probs"]), _ptr(out["dlogits"]), _ptr(ws), ws.nbytes,
+                                        _stream(stream, x.device)), "hx_moe_balance_loss")
+    return out

@@ -168,6 +168,34 @@ int hx_moe_route(hx_moe* m, const void* x, int64_t n_tokens, const float* router
 int hx_moe_router_logits(hx_moe* m, const void* x, int64_t n_tokens, const float* router_bias,
                          float* logits, void* stream);
 
+/* No counterpart in the reference: what a routing does to the experts' load, for
+ * training the router and for placing experts. topk_idx is device int32
+ * [n_tokens, k] as hx_moe_route gives it; an index outside 0 .. E - 1 is no expert,
+ * and a token of such entries alone is not live (padding): nothing of its logits'
+ * row is used, whatever it holds.
+ * hx_moe_expert_counts: counts [E] int32, the entries of each expert.
+ * hx_moe_balance_loss: with n live tokens, c the counts, p_t the softmax of row t of
+ * logits [n_tokens, E] (HX_F32 or HX_BF16, as hx_moe_router_logits gives them),
+ *   f_e = k c_e / sum c, P_e = (1 / n) sum over live t of p_te, loss = coef E sum_e f_e P_e,
+ *   dlogits_te = coef E / n p_te (f_e - sum_j f_j p_tj) for live t, else 0
+ * (the counts are no function of the logits). c is the routing's own counts, or
+ * given_counts (device int32 [E]; null: own) where the load of several calls or
+ * devices is balanced together. Outputs: loss f32 [1], probs f32 [E] (P), counts
+ * int32 [E] (the routing's own; may be null), dlogits (logits' type; may be null, may
+ * be logits). No live token, or no entry in c: loss 0, gradient 0. A live row that
+ * holds a NaN, +inf or nothing but -inf makes loss, probs and its own gradient NaN.
+ * Sums run in a fixed order: the same bits for the same inputs. Both calls run on the
+ * current device, allocate nothing and need workspace of
+ * hx_moe_balance_workspace_size bytes, 16-byte aligned, which no other call in flight
+ * may use. E and k as in hx_moe_create (at most 1024 and 64). */
+int hx_moe_balance_workspace_size(int64_t n_tokens, int num_experts, size_t* bytes);
+int hx_moe_expert_counts(const int32_t* topk_idx, int64_t n_tokens, int k, int num_experts, int32_t* counts,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int hx_moe_balance_loss(const void* logits, int logits_dtype, int64_t n_tokens, int num_experts,
+                        const int32_t* topk_idx, int k, const int32_t* given_counts, float coef, float* loss,
+                        int32_t* counts, float* probs, void* dlogits, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 /* Decoder-layer MLP half on a residual stream (decoder.rs:129-132 with the
  * attention half skipped): x <- x + moe(rmsnorm(x)), where rmsnorm is
  * Qwen3_5RmsNorm, x * rsqrt(mean(x^2) + eps) * (1 + norm_w) in f32
