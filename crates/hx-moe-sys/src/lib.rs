@@ -26,6 +26,7 @@ pub const HX_Q4_K: i32 = 12;
 pub const HX_Q6_K: i32 = 14;
 pub const HX_BF16: i32 = 30;
 pub const HX_MXFP4: i32 = 39;
+pub const HX_F8_E4M3: i32 = 256;
 
 // where the pointers in hx_moe_weights live
 pub const HX_HOST: i32 = 0;
@@ -71,15 +72,34 @@ pub struct hx_moe_weights {
     pub shared_expert_gate: *const c_void,
 }
 
+/// Scales of a block of HX_F8_E4M3 projections.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct hx_moe_f8_scales {
+    pub experts_gate: *const f32,
+    pub experts_up: *const f32,
+    pub experts_down: *const f32,
+    pub shared_gate: *const f32,
+    pub shared_up: *const f32,
+    pub shared_down: *const f32,
+}
+
 /// Opaque handle.
 #[repr(C)]
 pub struct hx_moe {
     _private: [u8; 0],
 }
 
+/// Opaque handle of a linear layer.
+#[repr(C)]
+pub struct hx_linear {
+    _private: [u8; 0],
+}
+
 #[link(name = "hxmoe")]
 extern "C" {
     pub fn hx_moe_create(cfg: *const hx_moe_config, w: *const hx_moe_weights, device: c_int, out: *mut *mut hx_moe) -> c_int;
+    pub fn hx_moe_create_f8(cfg: *const hx_moe_config, w: *const hx_moe_weights, scales: *const hx_moe_f8_scales, device: c_int, out: *mut *mut hx_moe) -> c_int;
     pub fn hx_moe_destroy(m: *mut hx_moe) -> c_int;
     pub fn hx_moe_workspace_size(m: *const hx_moe, n_tokens: i64, bytes: *mut usize) -> c_int;
     pub fn hx_moe_forward(m: *mut hx_moe, x: *const c_void, n_tokens: i64, y: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, router_bias: *const f32, stream: *mut c_void) -> c_int;
@@ -96,6 +116,11 @@ extern "C" {
     pub fn hx_dequantize(dtype: c_int, src: *const c_void, rows: i64, cols: i64, dst: *mut f32, stream: *mut c_void) -> c_int;
     pub fn hx_row_bytes(dtype: c_int, n: i64) -> i64;
     pub fn hx_quantize_activations(weight_dtype: c_int, x: *const c_void, x_dtype: c_int, rows: i64, cols: i64, codes: *mut i8, d: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn hx_quantize_f8(x: *const c_void, x_dtype: c_int, rows: i64, cols: i64, block_rows: c_int, codes: *mut c_void, scales: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn hx_linear_create(out_features: i64, in_features: i64, codes: *const c_void, scales: *const f32, location: c_int, device: c_int, out: *mut *mut hx_linear) -> c_int;
+    pub fn hx_linear_destroy(l: *mut hx_linear) -> c_int;
+    pub fn hx_linear_workspace_size(l: *const hx_linear, n_rows: i64, bytes: *mut usize) -> c_int;
+    pub fn hx_linear_forward(l: *mut hx_linear, x: *const c_void, x_dtype: c_int, n_rows: i64, y: *mut c_void, y_dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn hx_moe_timing_begin(m: *mut hx_moe, max_calls: c_int) -> c_int;
     pub fn hx_moe_timing_read(m: *mut hx_moe, ms: *mut f64, launches: *mut i64, n_slots: *mut c_int) -> c_int;
     pub fn hx_moe_timing_end(m: *mut hx_moe, ms: *mut f64, launches: *mut i64, n_slots: *mut c_int) -> c_int;

@@ -1,0 +1,898 @@
+// E4M3 weights and activations with float32 scales by blocks of 128: quantisation, the
+// linear layer y = q(x) W^T, and experts y[t] = sum_j w[t,j] D_e(q(silu(G_e q(x_t)) * U_e q(x_t))).
+//
+// Quantisation of a block: s = max(max|x| / 448, 2^-126), codes the E4M3 values nearest to
+// x / s (the exact quotient, ties to even); a block with a NaN or an infinity has scale NaN.
+//
+// Products run on v_mfma_f32_16x16x128_f8f6f4 with the weights as its A operand and the
+// activations as its B operand: one instruction is one block of K. Its D (lane l: row
+// l % 16 of the activations, features 4 (l / 16) + i in register i) starts from zero and
+// is added to the sums times sx sw, a lane's one scale of its row and block times the
+// scale of the weights' block, which a wave's features share: four multiply-adds a lane
+// for the instruction's 32 cycles.
+//
+// The instruction adds the products that a lane holds in fixed point, 13 bits below the
+// exponent of the largest (measured: 2^14 + 2^1 is kept, of 2^14 + 2^0 the second is lost; what
+// the four lanes of a row hold is added in float32). A sum is off by about 1e-5 of its norm so,
+// far below a bf16 result's own rounding. Float32 results (WIDE) take the codes as bf16,
+// which is exact, and v_mfma_f32_16x16x32_bf16, four for a block at half the rate: 3e-7.
+#include <algorithm>
+
+#include "hx_f8.h"
+#include "hx_mx_routing.h"
+
+namespace hx {
+
+typedef int f8_v8i __attribute__((ext_vector_type(8)));
+typedef float f8_v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 f8_v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 f8_v8bf __attribute__((ext_vector_type(8)));
+
+// ---------------------------------------------------------------- quantisation
+// a block's scale from the bits of its largest magnitude (NaN and infinity above all
+// others), and whether it is a number
+HX_DEV bool f8_scale(uint32_t m, float& s) {
+  const bool fine = m < 0x7f800000u;
+  s = fine ? fmaxf(__uint_as_float(m) / 448.f, 0x1p-126f) : __builtin_nanf("");
+  return fine;
+}
+
+// x / s for the conversion to E4M3: within half a step of float32 of the quotient, and
+// where the quotient is no float32 with the last bit set. The borders between codes have
+// few bits, so that the value lies on the same side of each as the quotient, and on one
+// only if the quotient does. s is scaled up where the remainders would be subnormal.
+struct F8Div {
+  float s, r, up;
+  HX_DEV explicit F8Div(float scale) {
+    up = scale < 0x1p-60f ? 0x1p64f : 1.f;
+    s = scale * up;
+    r = 1.f / s;
+  }
+  HX_DEV float operator()(float x) const {
+    x *= up;
+    const float q0 = x * r;
+    // what the quotients are too much: of this sign, -0 stays -0
+    const float q = __builtin_fmaf(-__builtin_fmaf(q0, s, -x), r, q0);
+    const float rem = __builtin_fmaf(q, s, -x);
+    const int b = __float_as_int(q), step = (__float_as_int(rem) ^ b) < 0 ? 1 : -1;
+    return __int_as_float(rem != 0.f && (b & 1) == 0 ? b + step : b);
+  }
+};
+
+// four codes in a word
+HX_DEV uint32_t f8_pack(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+template <int N>
+HX_DEV uint32_t f8_amax(const float (&f)[N]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  return m;
+}
+
+// N values with a scale -> N / 4 words of codes; a block that is no number: zeros
+template <int N>
+HX_DEV void f8_codes(const float (&f)[N], float s, bool fine, uint32_t (&w)[N / 4]) {
+  const F8Div div(fine ? s : 1.f);
+#pragma unroll
+  for (int i = 0; i < N / 4; i++)
+    w[i] = fine ? f8_pack(div(f[4 * i]), div(f[4 * i + 1]), div(f[4 * i + 2]), div(f[4 * i + 3])) : 0u;
+}
+
+// N elements from p, 16 bytes at a time (VEC: aligned) or n of them singly, zeros behind
+template <bool BF, bool VEC, int N>
+HX_DEV void f8_load(const void* base, int64_t at, int n, float (&f)[N]) {
+  if constexpr (VEC) {
+    if (n <= 0) {
+#pragma unroll
+      for (int i = 0; i < N; i++) f[i] = 0.f;
+      return;
+    }
+    if constexpr (BF) {
+#pragma unroll
+      for (int i = 0; i < N / 8; i++) {
+        const uint4 v = ((const uint4*)((const uint16_t*)base + at))[i];
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          f[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+          f[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 4; i++) {
+        const float4 v = ((const float4*)((const float*)base + at))[i];
+        f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = i < n ? ld_act(base, at + i, BF) : 0.f;
+  }
+}
+
+// One block of a row by 8 lanes, 16 values a lane. The lanes' codes of columns c0 ..
+template <bool BF, bool VEC>
+HX_DEV void f8_row_block(const void* x, int64_t rows, int64_t cols, int64_t r, int b, uint4& codes, float& s) {
+  const int c0 = 128 * b + 16 * (lane_id() & 7);
+  float f[16];
+  f8_load<BF, VEC>(x, r * cols + c0, (int)min<int64_t>(cols - c0, 16), f);
+  uint32_t m = f8_amax(f);
+  m = max(m, (uint32_t)dpp_mov<0xB1>((int)m));    // quad_perm 1,0,3,2
+  m = max(m, (uint32_t)dpp_mov<0x4E>((int)m));    // quad_perm 2,3,0,1
+  m = max(m, (uint32_t)dpp_mov<0x141>((int)m));   // row_half_mirror
+  const bool fine = f8_scale(m, s);
+  uint32_t w[4];
+  f8_codes(f, s, fine, w);
+  codes = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// codes to a row's place, 16 bytes or n of them singly
+HX_DEV void f8_put(uint8_t* p, const uint4& c, bool vec, int n) {
+  if (vec) {
+    if (n > 0) *(uint4*)p = c;
+    return;
+  }
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  for (int i = 0; i < n && i < 16; i++) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+}
+
+struct F8Rows {
+  const void* x;
+  int64_t rows, cols;
+  uint8_t* codes;
+  int64_t ldc;       // bytes of a row of codes, cols or more
+  float* scales;
+  int lds;           // floats of a row of scales
+  bool vec_out;
+};
+
+// rows of x, a thread 16 of its values (x and the codes 16-byte aligned: VEC)
+template <bool BF, bool VEC>
+HX_DEV void f8_quant_rows(const F8Rows& q, int64_t id) {
+  const int nb = f8_blocks(q.cols);
+  const int64_t blk = id >> 3, r = blk / nb;
+  const int b = (int)(blk % nb), c0 = 128 * b + 16 * (int)(id & 7);
+  const bool has = r < q.rows;   // the lanes of a block agree
+  uint4 c;
+  float s;
+  f8_row_block<BF, VEC>(q.x, q.rows, q.cols, has ? r : 0, b, c, s);
+  if (!has) return;
+  f8_put(q.codes + r * q.ldc + c0, c, q.vec_out, (int)min<int64_t>(q.ldc - c0, 16));
+  if ((id & 7) == 0) q.scales[r * q.lds + b] = s;
+}
+template <bool BF, bool VEC>
+__global__ __launch_bounds__(256) void k_f8_rows(F8Rows q) {
+  f8_quant_rows<BF, VEC>(q, (int64_t)blockIdx.x * 256 + threadIdx.x);
+}
+
+hipError_t launch_f8_rows(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, bool padded,
+                          hipStream_t s) {
+  F8Rows q{x, rows, cols, (uint8_t*)codes, padded ? f8_row(cols) : cols, scales, padded ? f8_scale_row(cols) : f8_blocks(cols), false};
+  q.vec_out = (q.ldc & 15) == 0 && ((uintptr_t)codes & 15) == 0;
+  const bool vec = cols % 16 == 0 && ((uintptr_t)x & 15) == 0;
+  const dim3 g((unsigned)((rows * f8_blocks(cols) * 8 + 255) / 256));
+  if (xbf && vec) hx_launch(k_f8_rows<true, true>, g, dim3(256), 0, s, q);
+  else if (xbf) hx_launch(k_f8_rows<true, false>, g, dim3(256), 0, s, q);
+  else if (vec) hx_launch(k_f8_rows<false, true>, g, dim3(256), 0, s, q);
+  else hx_launch(k_f8_rows<false, false>, g, dim3(256), 0, s, q);
+  return hipGetLastError();
+}
+
+// blocks of 128 x 128: a workgroup a block, 64 values a thread in registers, 4 columns of
+// 16 rows, 8 rows apart
+template <bool BF, bool VEC>
+__global__ __launch_bounds__(256) void k_f8_blocks(F8Rows q) {
+  __shared__ uint32_t part[4];
+  const int nb = f8_blocks(q.cols), tid = threadIdx.x;
+  const int64_t rb = blockIdx.x / nb;
+  const int b = (int)(blockIdx.x % nb), c0 = 128 * b + 4 * (tid & 31);
+  const int64_t r0 = 128 * rb + (tid >> 5);
+  const int n = (int)min<int64_t>(q.cols - c0, 4);
+  float f[16][4];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const int64_t r = r0 + 8 * i;
+    const int has = r < q.rows ? n : 0;
+    if constexpr (VEC && BF) {
+      uint2 v = make_uint2(0u, 0u);
+      if (has > 0) v = *(const uint2*)((const uint16_t*)q.x + r * q.cols + c0);
+      f[i][0] = __uint_as_float(v.x << 16); f[i][1] = __uint_as_float(v.x & 0xffff0000u);
+      f[i][2] = __uint_as_float(v.y << 16); f[i][3] = __uint_as_float(v.y & 0xffff0000u);
+    } else {
+      f8_load<BF, VEC>(q.x, r * q.cols + c0, has, f[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i++) m = max(m, f8_amax(f[i]));
+  m = wave_max_u32(m);
+  if (lane_id() == 0) part[tid >> 6] = m;
+  __syncthreads();
+  m = max(max(part[0], part[1]), max(part[2], part[3]));
+  float s;
+  const bool fine = f8_scale(m, s);
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const int64_t r = r0 + 8 * i;
+    uint32_t w[1];
+    f8_codes(f[i], s, fine, w);
+    if (r >= q.rows) continue;
+    uint8_t* p = q.codes + r * q.cols + c0;
+    if (VEC && q.vec_out) {
+      if (n > 0) *(uint32_t*)p = w[0];
+    } else {
+      for (int j = 0; j < n; j++) p[j] = (uint8_t)(w[0] >> (8 * j));
+    }
+  }
+  if (tid == 0) q.scales[rb * nb + b] = s;
+}
+
+hipError_t launch_f8_blocks(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, hipStream_t s) {
+  F8Rows q{x, rows, cols, (uint8_t*)codes, cols, scales, f8_blocks(cols), ((uintptr_t)codes & 3) == 0};
+  const bool vec = cols % 4 == 0 && ((uintptr_t)x & (xbf ? 7 : 15)) == 0;
+  const dim3 g((unsigned)((int64_t)f8_blocks(rows) * f8_blocks(cols)));
+  if (xbf && vec) hx_launch(k_f8_blocks<true, true>, g, dim3(256), 0, s, q);
+  else if (xbf) hx_launch(k_f8_blocks<true, false>, g, dim3(256), 0, s, q);
+  else if (vec) hx_launch(k_f8_blocks<false, true>, g, dim3(256), 0, s, q);
+  else hx_launch(k_f8_blocks<false, false>, g, dim3(256), 0, s, q);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- stored weights
+// a thread per 16 bytes of a tile, padding included, then the scales
+__global__ __launch_bounds__(256) void k_repack_f8(const uint8_t* codes, const float* scales, int64_t count, int64_t rows,
+                                                   int64_t K, uint8_t* dst, int64_t dst_stride) {
+  const int KB = f8_blocks(K), SR = f8_scale_row(K), RB = f8_blocks(rows);
+  const int64_t pieces = (int64_t)f8_tiles(rows) * KB * 128, per = pieces + (int64_t)RB * SR;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= per * count) return;
+  const int64_t m = id / per, q = id % per;
+  uint8_t* mat = dst + m * dst_stride;
+  if (q >= pieces) {
+    const int64_t at = q - pieces;
+    const int rb = (int)(at / SR), b = (int)(at % SR);
+    ((float*)(mat + f8_code_bytes(rows, K)))[at] = b < KB ? scales[(m * RB + rb) * KB + b] : 0.f;
+    return;
+  }
+  const int l = (int)(q & 63), h = (int)((q >> 6) & 1);
+  const int64_t tile = q >> 7, row = 16 * (tile / KB) + (l & 15), c0 = 128 * (tile % KB) + 64 * h + 16 * (l >> 4);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  const uint8_t* src = codes + (m * rows + row) * K + c0;   // the caller's rows: any alignment
+  if (row < rows) {
+    if (c0 + 16 <= K && ((uintptr_t)src & 15) == 0) {
+      const uint4 v = *(const uint4*)src;
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (c0 + i < K) w[i >> 2] |= (uint32_t)src[i] << (8 * (i & 3));
+    }
+  }
+  *(uint4*)(mat + q * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+hipError_t launch_f8_repack(const void* codes, const float* scales, int64_t count, int64_t rows, int64_t K, void* dst,
+                            int64_t dst_stride, hipStream_t s) {
+  const int64_t per = (int64_t)f8_tiles(rows) * f8_blocks(K) * 128 + (int64_t)f8_blocks(rows) * f8_scale_row(K);
+  hipLaunchKernelGGL(k_repack_f8, dim3((unsigned)((per * count + 255) / 256)), dim3(256), 0, s, (const uint8_t*)codes, scales,
+                     count, rows, K, (uint8_t*)dst, dst_stride);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- operands
+HX_DEV f8_v4f f8_zero4() { return f8_v4f{0.f, 0.f, 0.f, 0.f}; }
+
+// a lane's two halves as an operand
+HX_DEV f8_v8i f8_op(const uint4& a, const uint4& b) {
+  return f8_v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+}
+// an operand as the products take it
+template <bool WIDE>
+struct F8Arg;
+template <>
+struct F8Arg<false> {
+  f8_v8i v;
+  HX_DEV F8Arg() {}
+  HX_DEV explicit F8Arg(const f8_v8i& c) : v(c) {}
+};
+template <>
+struct F8Arg<true> {
+  f8_v8bf v[4];
+  HX_DEV F8Arg() {}
+  HX_DEV explicit F8Arg(const f8_v8i& c) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const f8_v2bf lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)c[2 * i + j], 1.f, false);
+        const f8_v2bf hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)c[2 * i + j], 1.f, true);
+        v[i][4 * j] = lo[0]; v[i][4 * j + 1] = lo[1]; v[i][4 * j + 2] = hi[0]; v[i][4 * j + 3] = hi[1];
+      }
+  }
+};
+// a block of K: scales of 0 select the instruction's form without any
+HX_DEV f8_v4f f8_mfma(const F8Arg<false>& w, const F8Arg<false>& x) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f8_zero4(), 0, 0, 0, 0, 0, 0);
+}
+HX_DEV f8_v4f f8_mfma(const F8Arg<true>& w, const F8Arg<true>& x) {
+  f8_v4f d = f8_zero4();
+#pragma unroll
+  for (int i = 0; i < 4; i++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], d, 0, 0, 0);
+  return d;
+}
+HX_DEV void f8_add(f8_v4f& acc, const f8_v4f& d, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
+}
+
+// the largest of the four lanes that hold a row's block, in all of them
+HX_DEV uint32_t f8_max_of_4(uint32_t m) {
+  const auto a = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = max((uint32_t)a[0], (uint32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+
+// A lane's values of a block of its row (columns 64 h + 16 (l / 16) .. of it) and their
+// quantised form: the rows of a call of few are quantised by every wave that reads them
+struct F8Operand {
+  f8_v8i v;
+  float s;
+  template <bool BF, bool VEC>
+  HX_DEV void load(const void* x, int64_t row_at, int64_t K, int b) {
+    float f[32];
+    const int c = 128 * b + 16 * (lane_id() >> 4);
+    float lo[16], hi[16];
+    f8_load<BF, VEC>(x, row_at + c, (int)min<int64_t>(K - c, 16), lo);
+    f8_load<BF, VEC>(x, row_at + c + 64, (int)min<int64_t>(K - c - 64, 16), hi);
+    const uint32_t m = f8_max_of_4(max(f8_amax(lo), f8_amax(hi)));
+    const bool fine = f8_scale(m, s);
+    uint32_t a[4], z[4];
+    f8_codes(lo, s, fine, a);
+    f8_codes(hi, s, fine, z);
+    v = f8_v8i{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)z[0], (int)z[1], (int)z[2], (int)z[3]};
+  }
+  // quantised rows
+  HX_DEV void load(const uint8_t* codes, const float* scales, int b) {
+    const uint8_t* p = codes + 128 * b + 16 * (lane_id() >> 4);
+    v = f8_op(*(const uint4*)p, *(const uint4*)(p + 64));
+    s = scales[b];
+  }
+};
+
+HX_DEV void f8_store(void* y, int64_t at, float v, bool bf) {
+  if (bf) ((uint16_t*)y)[at] = f32_to_bf16(v);
+  else ((float*)y)[at] = v;
+}
+
+// ---------------------------------------------------------------- linear layer, few rows
+// Workgroup: 16 features; its 8 waves share K block by block and add up in LDS. CT columns
+// of 16 rows; QUANT: rows as the caller has them, quantised by each wave for its blocks.
+template <bool BF, bool VEC, int CT, bool QUANT, bool WIDE>
+__global__ __launch_bounds__(512) void k_f8_few_rows(F8LinearArgs a) {
+  constexpr int PITCH = 16 * CT + 1;
+  __shared__ float red[8 * 16 * PITCH];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = blockIdx.x, KB = f8_blocks(a.K), M = (int)a.M, col = lane & 15;
+  const uint8_t* w = a.w + (int64_t)n * KB * 2048 + lane * 16;
+  const float* ws = (const float*)(a.w + f8_code_bytes(a.N, a.K)) + (int64_t)(n >> 3) * f8_scale_row(a.K);
+  f8_v4f acc[CT];
+#pragma unroll
+  for (int c = 0; c < CT; c++) acc[c] = f8_zero4();
+  for (int b = wave; b < KB; b += 8) {
+    const F8Arg<WIDE> wv(f8_op(*(const uint4*)(w + (int64_t)b * 2048), *(const uint4*)(w + (int64_t)b * 2048 + 1024)));
+    const float sw = ws[b];
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+      const int r = min(16 * c + col, M - 1);
+      F8Operand x;
+      if constexpr (QUANT) x.load<BF, VEC>(a.x, (int64_t)r * a.K, a.K, b);
+      else x.load(a.xq + r * f8_row(a.K), a.xs + (int64_t)r * f8_scale_row(a.K), b);
+      f8_add(acc[c], f8_mfma(wv, F8Arg<WIDE>(x.v)), x.s * sw);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CT; c++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) red[(wave * 16 + 4 * (lane >> 4) + i) * PITCH + 16 * c + col] = acc[c][i];
+  __syncthreads();
+  for (int o = tid; o < 16 * min(M, 16 * CT); o += 512) {
+    const int f = o & 15, r = o >> 4;
+    float y = 0.f;
+#pragma unroll
+    for (int v = 0; v < 8; v++) y += red[(v * 16 + f) * PITCH + r];
+    if (16 * n + f < a.N) f8_store(a.y, (int64_t)r * a.N + 16 * n + f, y, !WIDE);
+  }
+}
+
+// ---------------------------------------------------------------- products over tiles of rows
+// A tile's rows in LDS, 4 blocks of K at a time: [4][TM][128 bytes], 16-byte piece j of row r
+// at j ^ r % 8 (the rows' pieces would all start on one bank). They come in by direct
+// loads, a chunk ahead.
+template <int TM>
+struct F8Tile {
+  static constexpr int CB = 4, BYTES = CB * TM * 128, LOADS = BYTES / 4096;   // KiB a wave and chunk
+  const uint8_t* src[LOADS];
+  // rowptr(r): the quantised row r of the tile
+  template <typename F>
+  HX_DEV void init(int wave, F rowptr) {
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+      const int q = (i * 4 + wave) * 64 + lane_id(), row = q / 8 % TM;
+      src[i] = rowptr(row) + q / (8 * TM) * 128 + ((q % 8) ^ (row & 7)) * 16;
+    }
+  }
+  // blocks b0 .. min(b0 + 4, nblk) - 1
+  HX_DEV void load(int wave, int b0, int nblk, uint32_t lds) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; i++)
+      if (b0 + (i * 4 + wave) * 8 / TM < nblk) dma16(src[i] + (int64_t)b0 * 128, lds + (i * 4 + wave) * 1024);
+  }
+};
+
+// acc[m][t] = the sums over KB blocks of K of a wave's NM tiles of 16 features (their codes
+// from w[m], a lane's place in it included; tiles m with m % 2 == q, or all, by the scales ws[q])
+// times the tile's rows; xs[t]: a lane's row's scales. Two blocks of weights are on their way.
+template <bool WIDE, int TM, int NM, int NQ>
+HX_DEV void f8_products(const uint8_t* const (&w)[NM], const float* const (&ws)[NQ], const F8Tile<TM>& rows,
+                        const float* const (&xs)[TM / 16], int wave, uint8_t* buf, int KB, f8_v4f (&acc)[NM][TM / 16]) {
+  constexpr int TT = TM / 16, CB = F8Tile<TM>::CB, BYTES = F8Tile<TM>::BYTES, R = 2;
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
+  const int lane = lane_id();
+#pragma unroll
+  for (int m = 0; m < NM; m++)
+#pragma unroll
+    for (int t = 0; t < TT; t++) acc[m][t] = f8_zero4();
+  uint4 ring[R][NM][2];
+  auto fetch = [&](int i, int b) {   // past the last: the last again
+    const int64_t at = (int64_t)min(b, KB - 1) * 2048;
+#pragma unroll
+    for (int m = 0; m < NM; m++) {
+      ring[i][m][0] = *(const uint4*)(w[m] + at);
+      ring[i][m][1] = *(const uint4*)(w[m] + at + 1024);
+    }
+  };
+  rows.load(wave, 0, KB, lds);
+#pragma unroll
+  for (int i = 0; i < R; i++) fetch(i, i);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R * NM * 2) : "memory");   // the rows are the oldest
+  lds_barrier();
+  const uint8_t* const mine = buf + (lane & 15) * 128;
+  const int p0 = ((lane >> 4) ^ (lane & 7)) * 16, p1 = ((4 + (lane >> 4)) ^ (lane & 7)) * 16;
+  int h = 0;
+  for (int b0 = 0; b0 < KB; b0 += CB, h ^= 1) {
+    float4 sx[TT], sw[NQ];
+#pragma unroll
+    for (int t = 0; t < TT; t++) sx[t] = *(const float4*)(xs[t] + b0);
+#pragma unroll
+    for (int q = 0; q < NQ; q++) sw[q] = *(const float4*)(ws[q] + b0);
+    if (b0 + CB < KB) rows.load(wave, b0 + CB, KB, lds + (h ^ 1) * BYTES);   // that half was read before the barrier
+#pragma unroll
+    for (int i = 0; i < CB; i++) {
+      if (b0 + i >= KB) break;
+      F8Arg<WIDE> wv[NM];
+#pragma unroll
+      for (int m = 0; m < NM; m++) wv[m] = F8Arg<WIDE>(f8_op(ring[i % R][m][0], ring[i % R][m][1]));
+      const uint8_t* const at = mine + h * BYTES + i * TM * 128;
+#pragma unroll
+      for (int t = 0; t < TT; t++) {
+        const F8Arg<WIDE> xv(f8_op(*(const uint4*)(at + t * 2048 + p0), *(const uint4*)(at + t * 2048 + p1)));
+        const float x = i == 0 ? sx[t].x : i == 1 ? sx[t].y : i == 2 ? sx[t].z : sx[t].w;
+        f8_v4f d[NM];
+#pragma unroll
+        for (int m = 0; m < NM; m++) d[m] = f8_mfma(wv[m], xv);
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+          const float4& q = sw[m % NQ];
+          f8_add(acc[m][t], d[m], x * (i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w));
+        }
+      }
+      fetch(i % R, b0 + i + R);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (b0 + CB >= KB) break;
+    // a chunk's blocks of weights came after the next rows
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R * NM * 2) : "memory");
+    lds_barrier();
+  }
+}
+
+// Linear layer over tiles of TM rows: workgroup: a tile and 256 features, 64 a wave
+template <int TM, bool WIDE>
+__global__ __launch_bounds__(256, 2) void k_f8_linear(F8LinearArgs a) {
+  constexpr int TT = TM / 16, NM = 4;
+  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM>::BYTES];
+  int nt, tile;
+  const int NT = f8_tiles(a.N);
+  mx_tile((NT + 15) / 16, (int)((a.M + TM - 1) / TM), nt, tile);
+  if (tile < 0) return;
+  const int64_t r0 = (int64_t)tile * TM;
+  const int rows = (int)min<int64_t>(TM, a.M - r0), KB = f8_blocks(a.K);
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = (4 * nt + wave) * NM;
+  F8Tile<TM> rw;
+  rw.init(wave, [&](int r) { return a.xq + (r0 + min(r, rows - 1)) * f8_row(a.K); });
+  const float* xs[TT];
+#pragma unroll
+  for (int t = 0; t < TT; t++) xs[t] = a.xs + (r0 + min(16 * t + (lane & 15), rows - 1)) * f8_scale_row(a.K);
+  const uint8_t* w[NM];
+#pragma unroll
+  for (int m = 0; m < NM; m++) w[m] = a.w + (int64_t)min(n0 + m, NT - 1) * KB * 2048 + lane * 16;
+  const float* const ws[1] = {(const float*)(a.w + f8_code_bytes(a.N, a.K)) + (int64_t)(min(n0, NT - 1) >> 3) * f8_scale_row(a.K)};
+  f8_v4f acc[NM][TT];
+  f8_products<WIDE, TM, NM, 1>(w, ws, rw, xs, wave, buf, KB, acc);
+  const bool vec = a.N % 4 == 0 && ((uintptr_t)a.y & 15) == 0;
+#pragma unroll
+  for (int t = 0; t < TT; t++) {
+    const int r = 16 * t + (lane & 15);
+    if (r >= rows) continue;
+#pragma unroll
+    for (int m = 0; m < NM; m++) {
+      const int f = 16 * (n0 + m) + 4 * (lane >> 4);
+      const int64_t at = (r0 + r) * a.N + f;
+      const f8_v4f& v = acc[m][t];
+      if (vec && f < a.N) {
+        if (!WIDE) *(uint2*)((uint16_t*)a.y + at) = make_uint2(f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
+                                                               f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
+        else *(float4*)((float*)a.y + at) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (f + i < a.N) f8_store(a.y, at + i, v[i], !WIDE);
+      }
+    }
+  }
+}
+
+template <bool WIDE>
+static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
+  const dim3 few((unsigned)f8_tiles(a.N));
+  if (a.M <= F8_QUANT_ROWS) {
+    const bool vec = a.K % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
+    if (a.xbf && vec) hx_launch(k_f8_few_rows<true, true, 1, true, WIDE>, few, dim3(512), 0, s, a);
+    else if (a.xbf) hx_launch(k_f8_few_rows<true, false, 1, true, WIDE>, few, dim3(512), 0, s, a);
+    else if (vec) hx_launch(k_f8_few_rows<false, true, 1, true, WIDE>, few, dim3(512), 0, s, a);
+    else hx_launch(k_f8_few_rows<false, false, 1, true, WIDE>, few, dim3(512), 0, s, a);
+    return hipGetLastError();
+  }
+  hipError_t e = launch_f8_rows(a.x, a.xbf, a.M, a.K, a.xq, a.xs, true, s);
+  if (e != hipSuccess) return e;
+  if (a.M <= 32) hx_launch(k_f8_few_rows<true, true, 2, false, WIDE>, few, dim3(512), 0, s, a);
+  else if (a.M <= F8_FEW_ROWS) hx_launch(k_f8_few_rows<true, true, 4, false, WIDE>, few, dim3(512), 0, s, a);
+  else {
+    const int64_t tiles = (a.M + 63) / 64, nx = (f8_tiles(a.N) + 15) / 16;
+    hx_launch(k_f8_linear<64, WIDE>, dim3((unsigned)(nx * ((tiles + 7) / 8 * 8))), dim3(256), 0, s, a);
+  }
+  return hipGetLastError();
+}
+hipError_t launch_f8_linear(const F8LinearArgs& a, hipStream_t s) { return a.ybf ? f8_linear<false>(a, s) : f8_linear<true>(a, s); }
+
+// ---------------------------------------------------------------- experts, few tokens
+// Gate/up of up to 16 tokens. Workgroup: a chosen expert (slot) and 8 / KW groups of 16
+// features; KW waves share a group's K and add up in LDS. h leaves in f32: its blocks of 128
+// are of several workgroups, the down kernels quantise it.
+template <bool BF, bool VEC, int KW, bool ONE>
+__global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
+  constexpr int FW = 8 / KW;
+  __shared__ MxFewT<ONE ? 1 : F8_FEW_T> few;
+  __shared__ float red[8][2][16][17];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = ONE ? 1 : a.T;
+  const int slot = blockIdx.y, fb = blockIdx.x * FW + wave / KW, kq = wave % KW, KB = f8_blocks(a.H), col = lane & 15;
+  int e = a.E;
+  if (ONE) {
+    if (slot < a.k) e = a.idx[slot];
+    if (slot < a.k && (unsigned)e >= (unsigned)a.E) return;
+  } else {
+    mx_few_bits(a, few);
+    int n;
+    e = mx_few_slot(few, slot, n);
+    if (e < 0) {
+      if (slot > n || a.Is == 0) {
+        if (blockIdx.x == 0 && tid == 0) a.few[slot * MX_FEW_TAB + 32] = -1;
+        return;
+      }
+      e = a.E;
+    }
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I;
+  if (!ONE && blockIdx.x == 0 && tid < 33)   // for the down kernel
+    a.few[slot * MX_FEW_TAB + tid] = tid == 32 ? e : tid < T ? mx_few_row(a, few, e, tid) : -1;
+  if (16 * (int)blockIdx.x * FW >= inter) return;
+  f8_v4f ag = f8_zero4(), au = f8_zero4();
+  if (16 * fb < inter) {
+    const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
+    const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
+    const int64_t at = (int64_t)fb * KB * 2048 + lane * 16, sat = f8_code_bytes(inter, a.H) + (int64_t)(fb >> 3) * f8_scale_row(a.H) * 4;
+    const int64_t row = (int64_t)min(col, T - 1) * a.H;
+    for (int b = kq; b < KB; b += KW) {
+      const uint8_t *g = gm + at + (int64_t)b * 2048, *u = um + at + (int64_t)b * 2048;
+      const F8Arg<!BF> wg(f8_op(*(const uint4*)g, *(const uint4*)(g + 1024))), wu(f8_op(*(const uint4*)u, *(const uint4*)(u + 1024)));
+      const float sg = ((const float*)(gm + sat))[b], su = ((const float*)(um + sat))[b];
+      F8Operand x;
+      x.load<BF, VEC>(a.x, row, a.H, b);
+      const F8Arg<!BF> xv(x.v);
+      f8_add(ag, f8_mfma(wg, xv), x.s * sg);
+      f8_add(au, f8_mfma(wu, xv), x.s * su);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    red[wave][0][4 * (lane >> 4) + i][col] = ag[i];
+    red[wave][1][4 * (lane >> 4) + i][col] = au[i];
+  }
+  lds_barrier();
+  for (int o = tid; o < FW * 16 * T; o += 512) {
+    const int f = o & 15, t = (o >> 4) % T, w0 = (o >> 4) / T * KW, fo = 16 * (blockIdx.x * FW + w0 / KW) + f;
+    const int r = ONE ? (sh ? a.F : slot) : mx_few_row(a, few, e, t);
+    if (r < 0 || fo >= inter) continue;
+    float g = 0.f, u = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; w++) {
+      g += red[w0 + w][0][f][t];
+      u += red[w0 + w][1][f][t];
+    }
+    a.hf[(int64_t)r * a.hcols + fo] = silu_rcp(g) * u;
+  }
+}
+
+// most chosen experts of a call (one token: its entries), and the shared one
+static int f8_few_slots(const F8Args& a) { return (a.T == 1 ? a.k : std::min(a.T * a.k, a.E)) + (a.Is > 0 ? 1 : 0); }
+
+// Down and combine of one token. Workgroup: 16 outputs; its 16 waves take the units (entry,
+// block of K) in turn, weigh each product in f32, and add up in LDS.
+template <bool WIDE>
+__global__ __launch_bounds__(1024) void k_f8_one_down(F8Args a) {
+  __shared__ float red[16][16];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), nb = blockIdx.x;
+  const int k = a.k, KB = f8_blocks(a.I), KS = a.Is ? f8_blocks(a.Is) : 0;
+  f8_v4f acc = f8_zero4();
+  for (int u = wave; u < k * KB + KS; u += 16) {
+    const bool sh = u >= k * KB;
+    const int j = sh ? k : u / KB, b = sh ? u - k * KB : u % KB;
+    int e = a.E;
+    if (!sh) e = __builtin_amdgcn_readfirstlane(a.idx[j]);
+    if (!sh && (unsigned)e >= (unsigned)a.E) continue;
+    const float wt = sh ? a.shared_w[0] : a.w[j];
+    const int inter = sh ? a.Is : a.I, kb = sh ? KS : KB;
+    const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
+    const uint8_t* w = mat + ((int64_t)nb * kb + b) * 2048 + lane * 16;
+    const F8Arg<WIDE> wv(f8_op(*(const uint4*)w, *(const uint4*)(w + 1024)));
+    const float sw = ((const float*)(mat + f8_code_bytes(a.H, inter)))[(int64_t)(nb >> 3) * f8_scale_row(inter) + b];
+    F8Operand h;
+    h.load<false, true>(a.hf, (int64_t)(sh ? a.F : j) * a.hcols, inter, b);
+    f8_v4f d = f8_zero4();
+    f8_add(d, f8_mfma(wv, F8Arg<WIDE>(h.v)), h.s * sw);
+    f8_add(acc, d, wt);
+  }
+  if ((lane & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) red[wave][4 * (lane >> 4) + i] = acc[i];
+  }
+  lds_barrier();
+  if (tid < 16) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; w++) y += red[w][tid];
+    mx_store(a, 16 * nb + tid, y);
+  }
+}
+
+// Outputs of the experts for 2 to 16 tokens, unweighted and in f32, in the row of the token's
+// first entry with the expert. Workgroup: a chosen expert (slot) and 128 outputs, 32 a wave.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void k_f8_few_down(F8Args a) {
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = 8 * blockIdx.x + 2 * wave;
+  const int32_t* tab = a.few + blockIdx.y * MX_FEW_TAB;   // k_f8_few_gate_up's
+  const int e = tab[32], row = tab[lane & 15];
+  if (e < 0 || 16 * n0 >= a.H) return;
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter);
+  const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
+  const uint8_t* w = mat + (int64_t)n0 * KB * 2048 + lane * 16;
+  const float* ws = (const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)(n0 >> 3) * f8_scale_row(inter);
+  f8_v4f acc[2] = {f8_zero4(), f8_zero4()};
+  for (int b = 0; b < KB; b++) {
+    F8Arg<WIDE> wv[2];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      const uint8_t* p = w + ((int64_t)m * KB + b) * 2048;
+      wv[m] = F8Arg<WIDE>(f8_op(*(const uint4*)p, *(const uint4*)(p + 1024)));
+    }
+    F8Operand h;   // columns without a row read row 0 and are not stored
+    h.load<false, true>(a.hf, (int64_t)max(row, 0) * a.hcols, inter, b);
+    const F8Arg<WIDE> hv(h.v);
+#pragma unroll
+    for (int m = 0; m < 2; m++) f8_add(acc[m], f8_mfma(wv[m], hv), h.s * ws[b]);
+  }
+  if (row < 0) return;
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+    *(float4*)((float*)a.obuf + (int64_t)row * a.H + 16 * (n0 + m) + 4 * (lane >> 4)) =
+        make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+}
+
+bool f8_few(int T) { return T <= F8_FEW_T; }
+
+template <bool BF, bool VEC>
+static void f8_few_gate_up(const F8Args& a, hipStream_t s) {
+  const int slots = f8_few_slots(a), groups = (std::max(a.I, a.Is) + 15) / 16;
+  if (a.T == 1) hx_launch(k_f8_few_gate_up<BF, VEC, 8, true>, dim3(groups, slots), dim3(512), 0, s, a);
+  else if (slots * groups >= 1200) hx_launch(k_f8_few_gate_up<BF, VEC, 2, false>, dim3((groups + 3) / 4, slots), dim3(512), 0, s, a);
+  else hx_launch(k_f8_few_gate_up<BF, VEC, 8, false>, dim3(groups, slots), dim3(512), 0, s, a);
+}
+
+hipError_t launch_f8_few_gate_up(const F8Args& a, hipStream_t s) {
+  const bool vec = a.H % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
+  if (a.xbf && vec) f8_few_gate_up<true, true>(a, s);
+  else if (a.xbf) f8_few_gate_up<true, false>(a, s);
+  else if (vec) f8_few_gate_up<false, true>(a, s);
+  else f8_few_gate_up<false, false>(a, s);
+  return hipGetLastError();
+}
+
+template <bool WIDE>
+static void f8_few_down(const F8Args& a, hipStream_t s) {
+  if (a.T == 1) hx_launch(k_f8_one_down<WIDE>, dim3(a.H / 16), dim3(1024), 0, s, a);
+  else hx_launch(k_f8_few_down<WIDE>, dim3((a.H + 127) / 128, f8_few_slots(a)), dim3(256), 0, s, a);
+}
+hipError_t launch_f8_few_down(const F8Args& a, hipStream_t s) {
+  if (a.xbf) f8_few_down<false>(a, s);
+  else f8_few_down<true>(a, s);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- experts, grouped
+// Workgroups 0 .. chunks - 1: the chunk's entries by expert (mx_chunk_entries); the others: the
+// tokens' rows, a thread 16 values.
+template <bool BF, bool VEC>
+__global__ __launch_bounds__(256) void k_f8_prep(F8Args a) {
+  __shared__ MxPlace sm;
+  const int nch = mx_chunks(a.F);
+  if ((int)blockIdx.x < nch) {
+    mx_chunk_entries(a, sm, nch);
+    return;
+  }
+  const F8Rows q{a.x, a.T, a.H, a.xrec, f8_row(a.H), a.xs, f8_scale_row(a.H), true};
+  f8_quant_rows<BF, VEC>(q, (int64_t)(blockIdx.x - nch) * 256 + threadIdx.x);
+}
+
+hipError_t launch_f8_prep(const F8Args& a, hipStream_t s) {
+  const bool vec = a.H % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
+  const dim3 g((unsigned)(((int64_t)a.T * f8_blocks(a.H) * 8 + 255) / 256 + mx_chunks(a.F)));
+  if (a.xbf && vec) hx_launch(k_f8_prep<true, true>, g, dim3(256), 0, s, a);
+  else if (a.xbf) hx_launch(k_f8_prep<true, false>, g, dim3(256), 0, s, a);
+  else if (vec) hx_launch(k_f8_prep<false, true>, g, dim3(256), 0, s, a);
+  else hx_launch(k_f8_prep<false, false>, g, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+int f8_tile_m(int64_t F, int E, bool xbf) { return F <= 12 * (int64_t)E ? 16 : !xbf || F <= 28 * (int64_t)E ? 32 : 64; }
+
+// h = q(silu(G x) * (U x)). Workgroup: a tile of TM rows and 128 features, a block of h's
+// columns: 32 a wave, gate and up of a feature in the same lane.
+template <int TM, bool WIDE>
+__global__ __launch_bounds__(256, 2) void k_f8_gate_up(F8Args a) {
+  constexpr int TT = TM / 16, NM = 4;
+  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM>::BYTES];
+  __shared__ uint32_t amax[4][TM];
+  int nt, tile;
+  mx_tile(a.hblocks, a.counts[0], nt, tile);
+  if (tile < 0) return;
+  const int4 ti = ((const int4*)a.tiles)[tile];
+  const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I;
+  if (128 * nt >= inter) return;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), KB = f8_blocks(a.H);
+  auto token = [&](int r) {
+    const int p = p0 + min(r, rows - 1);
+    return (int64_t)(sh ? p - a.F : a.perm[p] / a.k);
+  };
+  F8Tile<TM> rw;
+  rw.init(wave, [&](int r) { return a.xrec + token(r) * f8_row(a.H); });
+  const float* xs[TT];
+#pragma unroll
+  for (int t = 0; t < TT; t++) xs[t] = a.xs + token(16 * t + (lane & 15)) * f8_scale_row(a.H);
+  const uint8_t* const mat[2] = {sh ? a.sgate.base : a.gate.mat(e), sh ? a.sup.base : a.up.mat(e)};
+  const uint8_t* w[NM];   // gate, up, gate, up
+#pragma unroll
+  for (int m = 0; m < NM; m++)
+    w[m] = mat[m & 1] + (int64_t)min(8 * nt + 2 * wave + (m >> 1), inter / 16 - 1) * KB * 2048 + lane * 16;
+  const int64_t sat = f8_code_bytes(inter, a.H) + (int64_t)nt * f8_scale_row(a.H) * 4;
+  const float* const ws[2] = {(const float*)(mat[0] + sat), (const float*)(mat[1] + sat)};
+  f8_v4f acc[NM][TT];
+  f8_products<WIDE, TM, NM, 2>(w, ws, rw, xs, wave, buf, KB, acc);
+  const bool in = 128 * nt + 32 * wave < inter;   // features behind the last are zeros
+  float h[TT][8];
+#pragma unroll
+  for (int t = 0; t < TT; t++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int m = 2 * (i >> 2);
+      h[t][i] = in ? silu_rcp(acc[m][t][i & 3]) * acc[m + 1][t][i & 3] : 0.f;
+    }
+    const uint32_t m = f8_max_of_4(f8_amax(h[t]));
+    if (lane < 16) amax[wave][16 * t + lane] = m;
+  }
+  lds_barrier();
+#pragma unroll
+  for (int t = 0; t < TT; t++) {
+    const int r = 16 * t + (lane & 15);
+    float s;
+    const bool fine = f8_scale(max(max(amax[0][r], amax[1][r]), max(amax[2][r], amax[3][r])), s);
+    uint32_t c[2];
+    f8_codes(h[t], s, fine, c);
+    if (r >= rows) continue;
+    uint32_t* o = (uint32_t*)(a.hrec + ((int64_t)(p0 + r) * a.hblocks + nt) * 128 + 32 * wave + 4 * (lane >> 4));
+    o[0] = c[0];
+    o[4] = c[1];
+    if (wave == 0 && lane < 16) a.hs[(int64_t)(p0 + r) * a.hscale + nt] = s;
+  }
+}
+
+// Outputs of the experts, unweighted: D h, in the activations' type. Workgroup: a tile of TM
+// rows and 256 outputs, 64 a wave.
+template <int TM, bool WIDE>
+__global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
+  constexpr int TT = TM / 16, NM = 4;
+  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM>::BYTES];
+  int nt, tile;
+  mx_tile((a.H + 255) / 256, a.counts[0], nt, tile);
+  if (tile < 0) return;
+  const int4 ti = ((const int4*)a.tiles)[tile];
+  const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter), NT = a.H / 16;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = (4 * nt + wave) * NM;
+  F8Tile<TM> rw;
+  rw.init(wave, [&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * 128; });
+  const float* xs[TT];
+#pragma unroll
+  for (int t = 0; t < TT; t++) xs[t] = a.hs + (int64_t)(p0 + min(16 * t + (lane & 15), rows - 1)) * a.hscale;
+  const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
+  const uint8_t* w[NM];
+#pragma unroll
+  for (int m = 0; m < NM; m++) w[m] = mat + (int64_t)min(n0 + m, NT - 1) * KB * 2048 + lane * 16;   // past the last: not stored
+  const float* const ws[1] = {(const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)(min(n0, NT - 1) >> 3) * f8_scale_row(inter)};
+  f8_v4f acc[NM][TT];
+  f8_products<WIDE, TM, NM, 1>(w, ws, rw, xs, wave, buf, KB, acc);
+#pragma unroll
+  for (int t = 0; t < TT; t++) {
+    const int r = 16 * t + (lane & 15);
+    if (r >= rows) continue;
+#pragma unroll
+    for (int m = 0; m < NM; m++) {
+      if (n0 + m >= NT) continue;
+      const int64_t at = (int64_t)(p0 + r) * a.H + 16 * (n0 + m) + 4 * (lane >> 4);
+      const f8_v4f& v = acc[m][t];
+      if (!WIDE) *(uint2*)((uint16_t*)a.obuf + at) = make_uint2(f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
+                                                                f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
+      else *(float4*)((float*)a.obuf + at) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+#define F8_LAUNCH(KERNEL, NX)                                                                  \
+  const dim3 g((unsigned)((int64_t)(NX) * ((a.max_tiles + 7) / 8 * 8)));                       \
+  if (a.xbf && a.tile_m == 16) hx_launch(KERNEL<16, false>, g, dim3(256), 0, s, a);            \
+  else if (a.xbf && a.tile_m == 32) hx_launch(KERNEL<32, false>, g, dim3(256), 0, s, a);       \
+  else if (a.xbf) hx_launch(KERNEL<64, false>, g, dim3(256), 0, s, a);                         \
+  else if (a.tile_m == 16) hx_launch(KERNEL<16, true>, g, dim3(256), 0, s, a);                 \
+  else hx_launch(KERNEL<32, true>, g, dim3(256), 0, s, a)
+
+hipError_t launch_f8_gate_up(const F8Args& a, hipStream_t s) {
+  F8_LAUNCH(k_f8_gate_up, a.hblocks);
+  return hipGetLastError();
+}
+hipError_t launch_f8_down(const F8Args& a, hipStream_t s) {
+  F8_LAUNCH(k_f8_down, (a.H + 255) / 256);
+  return hipGetLastError();
+}
+
+}  // namespace hx

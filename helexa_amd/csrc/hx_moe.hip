@@ -30,6 +30,7 @@
 #include "hx_abi.h"
 #include "hx_internal.h"
 #include "hx_mx.h"
+#include "hx_f8.h"
 
 using namespace hx;
 
@@ -113,7 +114,7 @@ struct hx_moe {
   WMat gate, up, down, sgate, sup, sdown;
   ExpertArgs shape;   // widths and formats only: what picks a call's kernels
   // [T]: the most workspace a call of up to T tokens takes
-  size_t small_ws[HX_DECODE_MAX_T + 1] = {};
+  size_t small_ws[F8_FEW_T + 1] = {};
   void* own_ws = nullptr;
   size_t own_ws_bytes = 0;
   Timing tm;
@@ -127,7 +128,8 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct WsLayout {
   size_t logits, topk_idx, topk_w, sgw, perm, inv, offsets, slots, tiles, counts, plan, dmap, hbuf, hbf, xh, xq, xq32, xcv,
-      hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_few, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, total;
+      hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_few, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, f8_xs,
+      f8_hs, f8_hf, total;
   int hstride, max_slots, max_tiles;
 };
 
@@ -155,6 +157,12 @@ static int mx_hblocks(const hx_moe* m) {
 static int64_t mx_max_tiles(const hx_moe* m, int64_t T, int tile_m) {
   const int64_t F = T * m->cfg.num_experts_per_tok;
   return F / tile_m + std::min<int64_t>(F, m->cfg.num_experts) + T / tile_m + 2;
+}
+
+// experts on E4M3 weights (all three projections; hx_f8.hip)
+static bool is_f8(const hx_moe* m) { return m->gate.fmt == HX_F8_E4M3; }
+static int f8_inter(const hx_moe* m) {
+  return std::max(m->cfg.moe_intermediate_size, m->cfg.shared_expert_intermediate_size);
 }
 
 static WsLayout ws_layout(const hx_moe* m, int64_t T) {
@@ -206,6 +214,30 @@ static WsLayout ws_layout(const hx_moe* m, int64_t T) {
     L.total = o;
     return L;
   }
+  if (is_f8(m)) {   // what grows with T only, too
+    const size_t act = m->cfg.act_dtype == HX_BF16 ? 2 : 4;
+    const int inter = f8_inter(m);
+    L.xn = take(act * T * H);
+    L.ym = take(act * T * H);
+    if (T <= F8_FEW_T) {
+      L.f8_hf = take(sizeof(float) * (size_t)(F + T) * inter);
+      L.obuf = take(sizeof(float) * (size_t)(F + T) * H);
+      L.mx_few = take(sizeof(int32_t) * MX_FEW_TAB * (size_t)L.max_slots);
+    } else {
+      L.mx_xrec = take((size_t)T * f8_row(H));
+      L.f8_xs = take(sizeof(float) * (size_t)T * f8_scale_row(H));
+      L.mx_hrec = take((size_t)(F + T) * f8_row(inter));
+      L.f8_hs = take(sizeof(float) * (size_t)(F + T) * f8_scale_row(inter));
+      L.obuf = take(act * (size_t)(F + T) * H);
+      L.mx_perm = take(sizeof(int32_t) * F);
+      L.mx_inv = take(sizeof(int32_t) * F);
+      L.mx_hist = take(sizeof(int32_t) * (size_t)std::min<int64_t>((F + MX_CHUNK - 1) / MX_CHUNK, MX_MAX_CHUNKS) * E);
+      L.mx_tiles = take(sizeof(int32_t) * 4 * (size_t)mx_max_tiles(m, T, 16));
+      L.mx_counts = take(sizeof(int32_t) * 4);
+    }
+    L.total = o;
+    return L;
+  }
   L.hbuf = take(sizeof(float) * (F + T) * L.hstride);
   L.hbf = take(sizeof(uint16_t) * (F + T) * L.hstride);
   const size_t act = m->cfg.act_dtype == HX_BF16 ? 2 : 4;
@@ -234,11 +266,11 @@ static WsLayout ws_layout(const hx_moe* m, int64_t T) {
 
 // what a buffer for calls of T tokens holds: never less than a call of fewer
 // takes, so that a buffer sized once serves every smaller batch. Past
-// HX_DECODE_MAX_T tokens the layout grows with T; up to there it changes with the
-// kernels (records on GGUF experts, f32 weighted rows on bf16 ones) and may need
-// more than the smallest prefill layouts.
+// F8_FEW_T tokens the layout grows with T; up to there it changes with the
+// kernels (records on GGUF experts, f32 weighted rows on bf16 and E4M3 ones) and
+// may need more than the smallest prefill layouts.
 static size_t ws_need(const hx_moe* m, int64_t T, const WsLayout& L) {
-  return std::max(L.total, m->small_ws[T < HX_DECODE_MAX_T ? T : HX_DECODE_MAX_T]);
+  return std::max(L.total, m->small_ws[T < F8_FEW_T ? T : F8_FEW_T]);
 }
 
 // ----------------------------------------------------------------------------
@@ -247,16 +279,16 @@ static size_t ws_need(const hx_moe* m, int64_t T, const WsLayout& L) {
 static int chunk_elems(int fmt) {
   switch (fmt) {
     case HX_F32: case HX_BF16: return 8;
-    case HX_Q8_0: case HX_Q4_K: case HX_Q6_K: case HX_MXFP4: return 32;
+    case HX_Q8_0: case HX_Q4_K: case HX_Q6_K: case HX_MXFP4: case HX_F8_E4M3: return 32;
     default: return 0;
   }
 }
 
 static int check_proj(const char* name, int fmt, int64_t K) {
   if (fmt != HX_F32 && fmt != HX_BF16 && fmt != HX_Q8_0 && fmt != HX_Q4_K && fmt != HX_Q6_K &&
-      fmt != HX_MXFP4)
+      fmt != HX_MXFP4 && fmt != HX_F8_E4M3)
     return fail(HX_ERR_UNSUPPORTED, "%s: unsupported storage dtype %d", name, fmt);
-  if (hx_row_bytes(fmt, K) < 0)
+  if (fmt != HX_F8_E4M3 && hx_row_bytes(fmt, K) < 0)
     return fail(HX_ERR_INVALID_ARGUMENT, "%s: input dim %lld does not tile into dtype %d blocks", name,
                 (long long)K, fmt);
   int ch = chunk_elems(fmt);
@@ -267,16 +299,21 @@ static int check_proj(const char* name, int fmt, int64_t K) {
 }
 
 // upload one projection stack ([count][rows][K] GGUF rows) into the internal
-// layout; every expert matrix starts on a 256-byte boundary
-static int upload_proj(WMat& w, const char* name, int fmt, const void* src, int loc, int count, int rows, int K) {
+// layout; every expert matrix starts on a 256-byte boundary. HX_F8_E4M3: [count][rows][K]
+// codes and their scales [count][ceil(rows / 128)][ceil(K / 128)].
+static int upload_proj(WMat& w, const char* name, int fmt, const void* src, const float* scales, int loc, int count, int rows,
+                       int K) {
   w.fmt = fmt;
   w.rows = rows;
   w.K = K;
   w.count = count;
-  const int64_t packed = (int64_t)rows * hx_row_bytes(fmt, K);
-  w.mat_bytes = (int64_t)align256((size_t)(fmt == HX_MXFP4 ? mx_mat_bytes(rows, K) : packed));
-  const size_t bytes = (size_t)w.mat_bytes * count, src_bytes = (size_t)packed * count;
-  if (!src) return fail(HX_ERR_INVALID_ARGUMENT, "%s: null weight pointer", name);
+  const bool f8 = fmt == HX_F8_E4M3;
+  const int64_t packed = f8 ? (int64_t)rows * K : (int64_t)rows * hx_row_bytes(fmt, K);
+  w.mat_bytes = (int64_t)align256((size_t)(fmt == HX_MXFP4 ? mx_mat_bytes(rows, K) : f8 ? f8_mat_bytes(rows, K) : packed));
+  const size_t codes = (size_t)packed * count, scale_at = align256(codes);
+  const size_t scale_bytes = f8 ? sizeof(float) * (size_t)count * f8_blocks(rows) * f8_blocks(K) : 0;
+  const size_t bytes = (size_t)w.mat_bytes * count, src_bytes = f8 ? scale_at + scale_bytes : codes;
+  if (!src || (f8 && !scales)) return fail(HX_ERR_INVALID_ARGUMENT, "%s: null weight pointer", name);
   if (hipMalloc(&w.base, bytes) != hipSuccess)
     return fail(HX_ERR_OUT_OF_MEMORY, "%s: cannot allocate %zu bytes", name, bytes);
   const void* dsrc = src;
@@ -284,15 +321,18 @@ static int upload_proj(WMat& w, const char* name, int fmt, const void* src, int 
   if (loc == HX_HOST) {
     if (hipMalloc(&tmp, src_bytes) != hipSuccess)
       return fail(HX_ERR_OUT_OF_MEMORY, "%s: cannot allocate %zu staging bytes", name, src_bytes);
-    hipError_t e = hipMemcpy(tmp, src, src_bytes, hipMemcpyHostToDevice);
+    hipError_t e = hipMemcpy(tmp, src, codes, hipMemcpyHostToDevice);
+    if (f8 && e == hipSuccess) e = hipMemcpy((uint8_t*)tmp + scale_at, scales, scale_bytes, hipMemcpyHostToDevice);
     if (e != hipSuccess) {
       (void)hipFree(tmp);
       return fail(HX_ERR_DEVICE, "%s: upload failed: %s", name, hipGetErrorString(e));
     }
     dsrc = tmp;
+    scales = (const float*)((uint8_t*)tmp + scale_at);
   }
-  hipError_t e = fmt == HX_MXFP4 ? launch_mx_repack(dsrc, count, rows, K, w.base, w.mat_bytes, 0)
-                                 : launch_repack(fmt, dsrc, count, rows, K, w.base, w.mat_bytes, 0);
+  hipError_t e = f8 ? launch_f8_repack(dsrc, scales, count, rows, K, w.base, w.mat_bytes, 0)
+                 : fmt == HX_MXFP4 ? launch_mx_repack(dsrc, count, rows, K, w.base, w.mat_bytes, 0)
+                                   : launch_repack(fmt, dsrc, count, rows, K, w.base, w.mat_bytes, 0);
   if (e == hipSuccess) e = hipDeviceSynchronize();
   if (tmp) (void)hipFree(tmp);
   if (e != hipSuccess) return fail(HX_ERR_DEVICE, "%s: repack failed: %s", name, hipGetErrorString(e));
@@ -364,7 +404,8 @@ static int build_router(hx_moe* m, const hx_moe_weights* w) {
   return HX_OK;
 }
 
-extern "C" int hx_moe_create(const hx_moe_config* cfg, const hx_moe_weights* w, int device, hx_moe** out) {
+static int create_block(const hx_moe_config* cfg, const hx_moe_weights* w, const hx_moe_f8_scales& f8, bool with_scales,
+                        int device, hx_moe** out) {
   if (!cfg || !w || !out) return fail(HX_ERR_INVALID_ARGUMENT, "null argument");
   *out = nullptr;
   const hx_moe_config c = *cfg;
@@ -394,6 +435,10 @@ extern "C" int hx_moe_create(const hx_moe_config* cfg, const hx_moe_weights* w, 
     return rc;
   if ((w->gate_dtype == HX_MXFP4) != (w->down_dtype == HX_MXFP4))
     return fail(HX_ERR_UNSUPPORTED, "HX_MXFP4 experts: all of gate_proj, up_proj and down_proj must be HX_MXFP4");
+  if ((w->gate_dtype == HX_F8_E4M3) != (w->down_dtype == HX_F8_E4M3))
+    return fail(HX_ERR_UNSUPPORTED, "HX_F8_E4M3 experts: all of gate_proj, up_proj and down_proj must be HX_F8_E4M3");
+  if ((w->gate_dtype == HX_F8_E4M3) != with_scales)
+    return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_create_f8 is for HX_F8_E4M3 projections, and they for it alone");
   if (w->gate_dtype != w->up_dtype) return fail(HX_ERR_UNSUPPORTED, "gate_proj and up_proj must share a dtype");
   if (sh) {
     if ((rc = check_proj("shared_expert.gate_proj", w->shared_gate_dtype, H)) ||
@@ -431,23 +476,33 @@ extern "C" int hx_moe_create(const hx_moe_config* cfg, const hx_moe_weights* w, 
     return fail(HX_ERR_DEVICE, "cannot create the handle's side stream / events");
   }
   const int E = c.num_experts;
-  if ((rc = build_router(m, w)) || (rc = upload_proj(m->gate, "experts.gate_proj", w->gate_dtype, w->experts_gate, w->location, E, I, H)) ||
-      (rc = upload_proj(m->up, "experts.up_proj", w->up_dtype, w->experts_up, w->location, E, I, H)) ||
-      (rc = upload_proj(m->down, "experts.down_proj", w->down_dtype, w->experts_down, w->location, E, H, I))) {
+  if ((rc = build_router(m, w)) || (rc = upload_proj(m->gate, "experts.gate_proj", w->gate_dtype, w->experts_gate, f8.experts_gate, w->location, E, I, H)) ||
+      (rc = upload_proj(m->up, "experts.up_proj", w->up_dtype, w->experts_up, f8.experts_up, w->location, E, I, H)) ||
+      (rc = upload_proj(m->down, "experts.down_proj", w->down_dtype, w->experts_down, f8.experts_down, w->location, E, H, I))) {
     hx_moe_destroy(m);
     return rc;
   }
-  if (sh && ((rc = upload_proj(m->sgate, "shared_expert.gate_proj", w->shared_gate_dtype, w->shared_gate, w->location, 1, Is, H)) ||
-             (rc = upload_proj(m->sup, "shared_expert.up_proj", w->shared_up_dtype, w->shared_up, w->location, 1, Is, H)) ||
-             (rc = upload_proj(m->sdown, "shared_expert.down_proj", w->shared_down_dtype, w->shared_down, w->location, 1, H, Is)))) {
+  if (sh && ((rc = upload_proj(m->sgate, "shared_expert.gate_proj", w->shared_gate_dtype, w->shared_gate, f8.shared_gate, w->location, 1, Is, H)) ||
+             (rc = upload_proj(m->sup, "shared_expert.up_proj", w->shared_up_dtype, w->shared_up, f8.shared_up, w->location, 1, Is, H)) ||
+             (rc = upload_proj(m->sdown, "shared_expert.down_proj", w->shared_down_dtype, w->shared_down, f8.shared_down, w->location, 1, H, Is)))) {
     hx_moe_destroy(m);
     return rc;
   }
   m->shape = shape_args(m);
-  for (int T = 0; T <= HX_DECODE_MAX_T; T++)
+  for (int T = 0; T <= F8_FEW_T; T++)
     m->small_ws[T] = std::max(ws_layout(m, T).total, T ? m->small_ws[T - 1] : 0);
   *out = m;
   return HX_OK;
+}
+
+extern "C" int hx_moe_create(const hx_moe_config* cfg, const hx_moe_weights* w, int device, hx_moe** out) {
+  return create_block(cfg, w, hx_moe_f8_scales{}, false, device, out);
+}
+
+extern "C" int hx_moe_create_f8(const hx_moe_config* cfg, const hx_moe_weights* w, const hx_moe_f8_scales* scales, int device,
+                                hx_moe** out) {
+  if (!scales) return fail(HX_ERR_INVALID_ARGUMENT, "null argument");
+  return create_block(cfg, w, *scales, true, device, out);
 }
 
 extern "C" int hx_moe_workspace_size(const hx_moe* m, int64_t n_tokens, size_t* bytes) {
@@ -692,7 +747,8 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
   a.hrec = ws + L.mx_hrec;
   a.hblocks = mx_hblocks(m);
   a.obuf = ws + L.obuf;
-  if (mx_few(a.T, a.k, a.H, a.xbf)) {
+  a.few_rows = mx_few(a.T, a.k, a.H, a.xbf);
+  if (a.few_rows) {
     a.few = (int32_t*)(ws + L.mx_few);
     tm_ext(m, SLOT_GATE_UP, s);
     HX_HIP(launch_mx_few_gate_up(a, s));
@@ -736,12 +792,69 @@ static int run_mx(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
   return HX_OK;
 }
 
+// the experts' products on E4M3 weights and their combine (a handle of is_f8)
+static int run_f8(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const float* w, const float* shared_w,
+                  void* y, void* resid, uint8_t* ws, const WsLayout& L, hipStream_t s) {
+  const hx_moe_config& c = m->cfg;
+  F8Args a{};
+  a.gate = m->gate; a.up = m->up; a.down = m->down;
+  a.sgate = m->sgate; a.sup = m->sup; a.sdown = m->sdown;
+  a.E = c.num_experts; a.k = c.num_experts_per_tok; a.H = c.hidden_size; a.I = c.moe_intermediate_size;
+  a.Is = shared_w ? c.shared_expert_intermediate_size : 0;
+  a.T = (int)T; a.F = (int)(T * a.k);
+  a.x = x; a.xbf = c.act_dtype == HX_BF16;
+  a.idx = idx; a.w = w; a.shared_w = shared_w;
+  a.y = y; a.resid = resid;
+  a.hblocks = f8_blocks(f8_inter(m));
+  a.hscale = f8_scale_row(f8_inter(m));
+  a.hcols = f8_inter(m);
+  a.obuf = ws + L.obuf;
+  a.few_rows = f8_few(a.T);
+  if (a.few_rows) {
+    a.few = (int32_t*)(ws + L.mx_few);
+    a.hf = (float*)(ws + L.f8_hf);
+  } else {
+    a.xrec = ws + L.mx_xrec;
+    a.xs = (float*)(ws + L.f8_xs);
+    a.hrec = ws + L.mx_hrec;
+    a.hs = (float*)(ws + L.f8_hs);
+    a.perm = (int32_t*)(ws + L.mx_perm);
+    a.inv = (int32_t*)(ws + L.mx_inv);
+    a.hist = (int32_t*)(ws + L.mx_hist);
+    a.tiles = (int32_t*)(ws + L.mx_tiles);
+    a.counts = (int32_t*)(ws + L.mx_counts);
+    a.tile_m = f8_tile_m(a.F, a.E, a.xbf);
+    a.max_tiles = (int)mx_max_tiles(m, T, a.tile_m);
+    tm_ext(m, SLOT_X_F16, s);
+    HX_HIP(launch_f8_prep(a, s));
+    tm_ext_done(m, SLOT_X_F16);
+    if (mx_chunks(a.F) > 1) {
+      tm_ext(m, SLOT_DISPATCH, s);
+      HX_HIP(launch_mx_dispatch(a, s));
+      tm_ext_done(m, SLOT_DISPATCH);
+    }
+  }
+  tm_ext(m, SLOT_GATE_UP, s);
+  HX_HIP(a.few_rows ? launch_f8_few_gate_up(a, s) : launch_f8_gate_up(a, s));
+  tm_ext_done(m, SLOT_GATE_UP);
+  tm_ext(m, SLOT_DOWN, s);
+  HX_HIP(a.few_rows ? launch_f8_few_down(a, s) : launch_f8_down(a, s));
+  tm_ext_done(m, SLOT_DOWN);
+  if (a.T > 1) {   // one token's down kernel combines
+    tm_ext(m, SLOT_COMBINE, s);
+    HX_HIP(launch_mx_combine(a, s));
+    tm_ext_done(m, SLOT_COMBINE);
+  }
+  if (m->tm.on && m->tm.calls < m->tm.max_calls && !capturing(s)) m->tm.calls++;
+  return HX_OK;
+}
+
 static int forward_impl(hx_moe* m, const void* x, int64_t T, void* y, void* ws, size_t ws_bytes,
                         const float* bias, hipStream_t s, const DecoderFuse* fz = nullptr) {
   WsLayout L;
   int rc = get_ws(m, T, ws, ws_bytes, L);
   if (rc) return rc;
-  if (is_mx(m)) {
+  if (is_mx(m) || is_f8(m)) {
     // the router and the per-token routing of every format, then hx_moe_experts' path
     if ((rc = check_mx_ws(ws))) return rc;
     Plan p;
@@ -758,7 +871,7 @@ static int forward_impl(hx_moe* m, const void* x, int64_t T, void* y, void* ws, 
     else launch_route_tokens(p.ra, s);
     tm_ext_done(m, SLOT_ROUTE_TOKENS);
     HX_HIP(hipGetLastError());
-    return run_mx(m, x, T, p.ra.d.topk_idx, p.ra.topk_w, p.ra.has_shared ? p.ra.sgw : nullptr, y, fz ? fz->x : nullptr,
+    return (is_mx(m) ? run_mx : run_f8)(m, x, T, p.ra.d.topk_idx, p.ra.topk_w, p.ra.has_shared ? p.ra.sgw : nullptr, y, fz ? fz->x : nullptr,
                   (uint8_t*)ws, L, s);
   }
   Plan p;
@@ -948,7 +1061,8 @@ extern "C" int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const 
                               const float* shared_w, void* y, void* workspace, size_t workspace_bytes, void* stream) {
   if (!m || n_tokens < 0 || (n_tokens > 0 && (!x || !y || !topk_idx || !topk_w)))
     return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
-  if (!is_mx(m)) return fail(HX_ERR_UNSUPPORTED, "hx_moe_experts: the block's experts are not HX_MXFP4");
+  if (!is_mx(m) && !is_f8(m))
+    return fail(HX_ERR_UNSUPPORTED, "hx_moe_experts: the block's experts are neither HX_MXFP4 nor HX_F8_E4M3");
   if (shared_w && m->cfg.shared_expert_intermediate_size == 0)
     return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_experts: shared_w for a block without a shared expert");
   if (n_tokens == 0) return HX_OK;
@@ -961,7 +1075,7 @@ extern "C" int hx_moe_experts(hx_moe* m, const void* x, int64_t n_tokens, const 
   WsLayout L;
   int rc = get_ws(m, n_tokens, workspace, workspace_bytes, L);
   if (rc || (rc = check_mx_ws(workspace))) return rc;
-  return run_mx(m, x, n_tokens, topk_idx, topk_w, shared_w, y, nullptr, (uint8_t*)workspace, L, s);
+  return (is_mx(m) ? run_mx : run_f8)(m, x, n_tokens, topk_idx, topk_w, shared_w, y, nullptr, (uint8_t*)workspace, L, s);
 }
 
 extern "C" int hx_moe_forward_noalloc(hx_moe* m, const void* x, int64_t n_tokens, void* y,

@@ -71,6 +71,7 @@ struct MxArgs {
   int32_t* tiles;                           // [max_tiles][4]: expert (E: shared), first row, rows
   int32_t* counts;                          // [1] tiles
   int tile_m, max_tiles;
+  bool few_rows;                            // obuf as the few-token kernels leave it
 };
 
 // whether a call of T tokens takes the few-token kernels

@@ -13,7 +13,7 @@
 // features, then one token's down, which combines, or down with a workgroup per expert and
 // 128 outputs, and the combine. More: the tokens' records and the expert counts, the
 // dispatch, grouped products over tiles of tile_m rows, and the combine.
-#include "hx_mx.h"
+#include "hx_mx_routing.h"
 
 #include <type_traits>
 
@@ -257,53 +257,6 @@ HX_DEV mx_v16f mx_zero16() {
 HX_DEV float mx_swiglu(float g, float u) { return silu_rcp(g) * u; }
 
 // ---------------------------------------------------------------- few tokens
-// The routing of a few tokens in LDS.
-struct MxFew {
-  int idx[MX_FEW_T * HX_MAX_TOPK];
-  uint32_t bits[32];   // the experts that some token chose
-};
-HX_DEV void mx_few_bits(const MxArgs& a, MxFew& sm) {
-  if (threadIdx.x < 32) sm.bits[threadIdx.x] = 0u;
-  lds_barrier();
-  for (int f = threadIdx.x; f < a.F; f += blockDim.x) {
-    const int e = a.idx[f];
-    sm.idx[f] = e;
-    if ((unsigned)e < (unsigned)a.E) atomicOr(&sm.bits[e >> 5], 1u << (e & 31));
-  }
-  lds_barrier();
-}
-// the number of chosen experts, and (in every lane) the s-th of them in ascending
-// order, -1 if there are fewer
-HX_DEV int mx_few_slot(const MxFew& sm, int s, int& n) {
-  const int l = lane_id();
-  const uint32_t w = l < 32 ? sm.bits[l] : 0u;
-  int c = __popc(w), x = c;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int y = __shfl_up(x, off, 64);
-    if (l >= off) x += y;
-  }
-  n = __shfl(x, 31, 64);
-  const unsigned long long hit = __ballot(l < 32 && x - c <= s && s < x);
-  if (!hit) return -1;
-  const int L = __ffsll(hit) - 1;
-  const uint32_t word = (uint32_t)__shfl((int)w, L, 64);
-  const int r = s - __shfl(x - c, L, 64);
-  const unsigned long long b =
-      __ballot(l < 32 && ((word >> l) & 1u) && __popc(word & ((1u << l) - 1u)) == r);
-  return 32 * L + __ffsll(b) - 1;
-}
-
-// the row of h and of the outputs of token t with expert e (E: the shared one): at the
-// token's first entry with it, -1 if there is none
-HX_DEV int mx_few_row(const MxArgs& a, const MxFew& sm, int e, int t) {
-  int row = e == a.E ? a.F + t : -1;
-  if (e != a.E)
-    for (int j = a.k - 1; j >= 0; j--)
-      if (sm.idx[t * a.k + j] == e) row = t * a.k + j;
-  return row;
-}
-
 // steps of K a wave takes where W waves share them: 1, 2 or whole words of scales
 __host__ __device__ inline int mx_wave_steps(int S, int W) {
   const int c = (S + W - 1) / W;
@@ -324,7 +277,7 @@ template <int P, int KW, bool ONE>
 __global__ __launch_bounds__(512, ONE || P == 5 ? 2 : 4) void k_mx_few_gate_up(MxArgs a) {
   constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, FW = 8 / KW;
   extern __shared__ __align__(16) uint8_t sm[];
-  __shared__ MxFew few;
+  __shared__ MxFewT<MX_FEW_T> few;
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = ONE ? 1 : a.T;
   const int slot = blockIdx.y, fb = blockIdx.x * FW + wave / KW, kq = wave % KW;
   const int S = mx_steps(a.H), S4 = (S + 3) / 4, HB = mx_blocks(a.H);
@@ -497,17 +450,6 @@ bool mx_few(int T, int k, int H, bool xbf) { return T <= MX_FEW_T && mx_few_lds(
 // most chosen experts of a call (one token: its entries)
 static int mx_few_slots(int T, int k, int E) { return T == 1 ? k : min(T * k, E); }
 
-HX_DEV void mx_store(const MxArgs& a, int64_t at, float y) {
-  if (a.xbf) {
-    uint16_t* p = (uint16_t*)(a.resid ? a.resid : a.y) + at;
-    const uint16_t b = f32_to_bf16(y);
-    *p = a.resid ? f32_to_bf16(bf16_to_f32(*p) + bf16_to_f32(b)) : b;
-  } else {
-    float* p = (float*)(a.resid ? a.resid : a.y) + at;
-    *p = a.resid ? *p + y : y;
-  }
-}
-
 // 8 steps of K of an expert's 32 outputs nb for up to 8 tokens: d += the weights of
 // steps s .. of mat (inter columns) x the planes of the lanes' rows (row < 0: zeros)
 template <int P>
@@ -641,91 +583,6 @@ hipError_t launch_mx_few_down(const MxArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- dispatch
-// Positions of a chunk's entries by expert, and (chunk 0) the tiles, from the experts'
-// counts: thread i has the counts of experts EPT i .. and how many of each come in
-// earlier chunks. The entries get their places by LDS counters; their order among an
-// expert's rows is free: a row's results do not depend on its place in a tile, and the
-// combine sums a token's entries in their order.
-struct MxPlace {
-  int base[HX_MAX_EXPERTS], off[HX_MAX_EXPERTS], cnt[HX_MAX_EXPERTS], first[HX_MAX_EXPERTS];
-  int sh[2][17];
-};
-template <int NT>
-HX_DEV void mx_place(const MxArgs& a, MxPlace& sm, int c, const int (&count)[HX_MAX_EXPERTS / NT],
-                     const int (&pre)[HX_MAX_EXPERTS / NT]) {
-  constexpr int EPT = HX_MAX_EXPERTS / NT, NW = NT / 64;
-  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, e0 = EPT * tid;
-  int n0 = 0, n1 = 0;   // rows, tiles
-#pragma unroll
-  for (int i = 0; i < EPT; i++) {
-    n0 += count[i];
-    n1 += (count[i] + a.tile_m - 1) / a.tile_m;
-  }
-  int x0 = n0, x1 = n1;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y0 = __shfl_up(x0, off, 64), y1 = __shfl_up(x1, off, 64);
-    if (lane >= off) {
-      x0 += y0;
-      x1 += y1;
-    }
-  }
-  if (lane == 63) {
-    sm.sh[0][wave] = x0;
-    sm.sh[1][wave] = x1;
-  }
-  __syncthreads();
-  if (tid < 2) {
-    int run = 0;
-    for (int w = 0; w < NW; w++) {
-      const int v = sm.sh[tid][w];
-      sm.sh[tid][w] = run;
-      run += v;
-    }
-    sm.sh[tid][16] = run;
-  }
-  __syncthreads();
-  int off = sm.sh[0][wave] + x0 - n0, first = sm.sh[1][wave] + x1 - n1;
-  const int total = sm.sh[1][16];
-#pragma unroll
-  for (int i = 0; i < EPT; i++) {
-    sm.base[e0 + i] = off + pre[i];
-    sm.off[e0 + i] = off;
-    sm.cnt[e0 + i] = count[i];
-    sm.first[e0 + i] = first;
-    off += count[i];
-    first += (count[i] + a.tile_m - 1) / a.tile_m;
-  }
-  __syncthreads();
-  const int per = mx_chunk(a.F), f0 = c * per, f1 = min(a.F, f0 + per);
-  for (int f = f0 + tid; f < f1; f += NT) {
-    const int x = a.idx[f];
-    int pos = -1;
-    if ((unsigned)x < (unsigned)a.E) {
-      pos = atomicAdd(&sm.base[x], 1);
-      a.perm[pos] = f;
-    }
-    a.inv[f] = pos;
-  }
-  if (c != 0) return;
-  for (int i = tid; i < total; i += NT) {
-    int lo = 0, hi = a.E - 1;   // the largest expert with first <= i
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (sm.first[mid] <= i) lo = mid;
-      else hi = mid - 1;
-    }
-    const int m0 = (i - sm.first[lo]) * a.tile_m;
-    ((int4*)a.tiles)[i] = make_int4(lo, sm.off[lo] + m0, min(a.tile_m, sm.cnt[lo] - m0), 0);
-  }
-  const int nst = a.Is > 0 ? (a.T + a.tile_m - 1) / a.tile_m : 0;
-  for (int i = tid; i < nst; i += NT) {
-    const int m0 = i * a.tile_m;
-    ((int4*)a.tiles)[total + i] = make_int4(a.E, a.F + m0, min(a.tile_m, a.T - m0), 0);
-  }
-  if (tid == 0) a.counts[0] = total + nst;
-}
-
 // Workgroups 0 .. chunks - 1: the chunk's entries by expert, and where there is one
 // chunk alone (a launch less: about 4 us) their places too; the others: the tokens' records,
 // a thread a block of 32. Bound by launch and latency up to some hundred tokens (4.5 us),
@@ -733,31 +590,13 @@ HX_DEV void mx_place(const MxArgs& a, MxPlace& sm, int c, const int (&count)[HX_
 // record a lane).
 template <int P>
 __global__ __launch_bounds__(256) void k_mx_prep(MxArgs a) {
-  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS, EPT = HX_MAX_EXPERTS / 256;
+  constexpr int RB = MxRec<P>::BYTES, RV = MxRec<P>::VECS;
   static_assert(sizeof(MxPlace) <= 256 * RB, "one of the two is used");
   __shared__ __align__(16) uint8_t rows[256 * RB];
   MxPlace& sm = *(MxPlace*)rows;
   const int nch = mx_chunks(a.F), tid = threadIdx.x;
   if ((int)blockIdx.x < nch) {
-    for (int e = tid; e < HX_MAX_EXPERTS; e += 256) sm.cnt[e] = 0;
-    __syncthreads();
-    const int per = mx_chunk(a.F), f0 = blockIdx.x * per, f1 = min(a.F, f0 + per);
-    for (int f = f0 + tid; f < f1; f += 256) {
-      const int e = a.idx[f];
-      if ((unsigned)e < (unsigned)a.E) atomicAdd(&sm.cnt[e], 1);
-    }
-    __syncthreads();
-    if (nch > 1) {
-      for (int e = tid; e < a.E; e += 256) a.hist[(int64_t)blockIdx.x * a.E + e] = sm.cnt[e];
-      return;
-    }
-    int count[EPT], pre[EPT];
-#pragma unroll
-    for (int i = 0; i < EPT; i++) {
-      count[i] = sm.cnt[EPT * tid + i];
-      pre[i] = 0;
-    }
-    mx_place<256>(a, sm, 0, count, pre);
+    mx_chunk_entries(a, sm, nch);
     return;
   }
   // a wave's 64 records leave through LDS, by whole KiB
@@ -912,18 +751,6 @@ struct MxRing {
     }
   }
 };
-
-// workgroup -> (feature group, tile) of N tiles; tile -1: none. XCD x (workgroup id
-// mod 8) takes the x-th eighth of the list in order, so that the tiles of an expert,
-// which are neighbours in the list, and the NX workgroups of a tile run side by side
-// on one XCD and meet each other's weights and rows in its L2. (Tiles dealt to the XCDs
-// in turn: every XCD fetched every expert.)
-HX_DEV void mx_tile(int NX, int N, int& nt, int& tile) {
-  const int L = blockIdx.x, per = (N + 7) / 8, i = L / (8 * NX);
-  nt = (L >> 3) % NX;
-  tile = (L & 7) * per + i;
-  if (i >= per || tile >= N) tile = -1;
-}
 
 // a turn of the ring from step s of S: acc += its weights x the rows at rec; LAST: no
 // steps of a turn after it are fetched
@@ -1309,7 +1136,7 @@ hipError_t launch_mx_combine(const MxArgs& a, hipStream_t s) {
   const int64_t waves = (int64_t)a.T * ((a.H + 511) / 512);
   const dim3 g((unsigned)((waves + 3) / 4));
   const int64_t rows = ((int64_t)a.F + (a.Is > 0 ? a.T : 0)) * a.H * (a.xbf ? 2 : 4);   // bytes
-  const bool few = mx_few(a.T, a.k, a.H, a.xbf), nt = rows > MX_CACHE;
+  const bool few = a.few_rows, nt = rows > MX_CACHE;
 #define COMBINE(BF, FEW, NT) hx_launch(k_mx_combine<BF, FEW, NT>, g, dim3(256), 0, s, a)
   if (a.xbf) {
     if (few) COMBINE(true, true, false);

@@ -6,7 +6,7 @@ Names follow the reference so callers and tests read like neuron's own:
     Qwen3_5MoeBlock      crates/neuron/src/harness/arch/qwen3_5/moe.rs:39-199
       .load(cfg, weights)      moe.rs:55 (validation moe.rs:56-69)
       .forward(xs)             moe.rs:164-199, input (b, l, hidden), same shape/dtype out
-      .experts(xs, idx, w)     the same with a routing of the caller's (MXFP4 experts)
+      .experts(xs, idx, w)     the same with a routing of the caller's (MXFP4 and E4M3 experts)
       .route(xs)               route_scatter moe.rs:124-162 + the dispatch sort of
                                tp_qwen3_5.rs:1189
     quantize                   isq.rs:39-55 (on the device)
@@ -28,13 +28,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libhxmoe.so")
 
 # storage formats (GGML type ids) and status codes, as in include/hx_moe.h
-F32, F16, Q8_0, Q4_K, Q6_K, BF16, MXFP4 = 0, 1, 8, 12, 14, 30, 39
+F32, F16, Q8_0, Q4_K, Q6_K, BF16, MXFP4, F8_E4M3 = 0, 1, 8, 12, 14, 30, 39, 256
 HX_HOST, HX_DEVICE = 0, 1
 STATUS = {0: "HX_OK", 1: "HX_ERR_INVALID_ARGUMENT", 2: "HX_ERR_UNSUPPORTED", 3: "HX_ERR_DEVICE",
           4: "HX_ERR_WORKSPACE_TOO_SMALL", 5: "HX_ERR_OUT_OF_MEMORY"}
 
 # every entry point include/hx_moe.h declares
-EXPORTS = ("hx_moe_create", "hx_moe_destroy", "hx_moe_workspace_size", "hx_moe_forward", "hx_moe_forward_noalloc",
+EXPORTS = ("hx_moe_create", "hx_moe_create_f8", "hx_quantize_f8", "hx_linear_create", "hx_linear_destroy",
+           "hx_linear_workspace_size", "hx_linear_forward", "hx_moe_destroy", "hx_moe_workspace_size", "hx_moe_forward", "hx_moe_forward_noalloc",
            "hx_moe_forward_host", "hx_moe_experts",
            "hx_moe_balance_workspace_size", "hx_moe_expert_counts", "hx_moe_balance_loss",
            "hx_moe_route", "hx_moe_router_logits", "hx_moe_decoder_mlp", "hx_quantize", "hx_dequantize",
@@ -66,6 +67,11 @@ class HxWeights(C.Structure):
                 ("shared_expert_gate_dtype", C.c_int32), ("shared_expert_gate", C.c_void_p)]
 
 
+class HxF8Scales(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("experts_gate", "experts_up", "experts_down", "shared_gate", "shared_up",
+                                          "shared_down")]
+
+
 _lib: Optional[C.CDLL] = None
 
 
@@ -79,6 +85,12 @@ def lib() -> C.CDLL:
         vp, i64, i32 = C.c_void_p, C.c_int64, C.c_int
         sig = {
             "hx_moe_create": (i32, [C.POINTER(HxConfig), C.POINTER(HxWeights), i32, C.POINTER(vp)]),
+            "hx_moe_create_f8": (i32, [C.POINTER(HxConfig), C.POINTER(HxWeights), C.POINTER(HxF8Scales), i32, C.POINTER(vp)]),
+            "hx_quantize_f8": (i32, [vp, i32, i64, i64, i32, vp, vp, vp]),
+            "hx_linear_create": (i32, [i64, i64, vp, vp, i32, i32, C.POINTER(vp)]),
+            "hx_linear_destroy": (i32, [vp]),
+            "hx_linear_workspace_size": (i32, [vp, i64, C.POINTER(C.c_size_t)]),
+            "hx_linear_forward": (i32, [vp, vp, i32, i64, vp, i32, vp, C.c_size_t, vp]),
             "hx_moe_destroy": (i32, [vp]),
             "hx_moe_workspace_size": (i32, [vp, i64, C.POINTER(C.c_size_t)]),
             "hx_moe_forward": (i32, [vp, vp, i64, vp, vp, C.c_size_t, vp, vp]),
@@ -229,14 +241,35 @@ def _act_dtype(torch_dtype) -> int:
     raise TypeError(f"activations must be float32 or bfloat16, got {torch_dtype}")
 
 
+def _f8_shape(cfg: TextConfig, key: str) -> tuple:
+    """shape of a block's projection"""
+    inter = cfg.shared_expert_intermediate_size if key[0] == "s" else cfg.moe_intermediate_size
+    shape = (cfg.hidden_size, inter) if key.endswith("down") else (inter, cfg.hidden_size)
+    return shape if key[0] == "s" else (cfg.num_experts,) + shape
+
+
+def _check_f8(what: str, codes, scales, shape=None) -> None:
+    """E4M3 codes and their scales by 128 x 128"""
+    import torch
+    if codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or codes.dim() < 2 or not codes.is_contiguous():
+        raise ValueError(f"{what}: codes must be a contiguous float8_e4m3fn or uint8 tensor [.., rows, cols]")
+    if shape is not None and tuple(codes.shape) != shape:
+        raise ValueError(f"{what}: codes of shape {tuple(codes.shape)}, not {shape}")
+    want = tuple(codes.shape[:-2]) + ((codes.shape[-2] + 127) // 128, (codes.shape[-1] + 127) // 128)
+    if (scales.dtype != torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous()
+            or scales.device != codes.device):
+        raise ValueError(f"{what}: scales must be a contiguous float32 tensor {want} on {codes.device}")
+
+
 class Qwen3_5MoeBlock:
     """One sparse-MoE block resident on a GPU.
 
     weights: dict name -> (dtype, torch tensor) with names router, gate, up, down,
     sgate, sup, sdown, seg (mlp.gate, experts.*.{gate,up,down}_proj,
     shared_expert.{gate,up,down}_proj, shared_expert_gate). Float tensors are
-    float32 / bfloat16; quantised ones are uint8 GGUF rows. All on the same
-    device (cuda) or all on the CPU.
+    float32 / bfloat16; quantised ones are uint8 GGUF rows. E4M3 projections are
+    (F8_E4M3, codes, scales): float8_e4m3fn or uint8 codes [.., rows, cols], float32 scales
+    [.., ceil(rows / 128), ceil(cols / 128)]. All on the same device (cuda) or all on the CPU.
     """
 
     def __init__(self, handle: int, cfg: TextConfig, act_dtype: int, device: int):
@@ -249,23 +282,33 @@ class Qwen3_5MoeBlock:
     def load(cls, cfg: TextConfig, weights: dict, act_dtype: int = BF16, device: int = 0) -> "Qwen3_5MoeBlock":
         c = HxConfig(cfg.hidden_size, cfg.num_experts, cfg.num_experts_per_tok, cfg.moe_intermediate_size,
                      cfg.shared_expert_intermediate_size, int(bool(cfg.norm_topk_prob)), act_dtype)
-        w = HxWeights()
-        tensors = [t for _, t in weights.values()]
+        w, scales = HxWeights(), HxF8Scales()
+        tensors = [t for entry in weights.values() for t in entry[1:]]
         on_dev = any(getattr(t, "is_cuda", False) for t in tensors)
         w.location = HX_DEVICE if on_dev else HX_HOST
         for key, field_ in (("router", "router"), ("gate", "experts_gate"), ("up", "experts_up"),
                             ("down", "experts_down"), ("sgate", "shared_gate"), ("sup", "shared_up"),
                             ("sdown", "shared_down"), ("seg", "shared_expert_gate")):
             if key in weights:
-                dt, t = weights[key]
+                dt, t, *rest = weights[key]
                 if not t.is_contiguous():
                     raise ValueError(f"weight {key} must be contiguous")
+                if (dt == F8_E4M3) != bool(rest):
+                    raise ValueError(f"weight {key}: scales come with F8_E4M3 codes, and only with them")
+                if rest:
+                    _check_f8(f"weight {key}", t, rest[0], _f8_shape(cfg, key))
+                    if t.is_cuda != on_dev:
+                        raise ValueError(f"weight {key} is not where the others are")
+                    setattr(scales, field_, _ptr(rest[0]))
                 dname = {"experts_gate": "gate_dtype", "experts_up": "up_dtype", "experts_down": "down_dtype",
                          "router": "router_dtype"}.get(field_, field_ + "_dtype")
                 setattr(w, dname, dt)
                 setattr(w, field_, _ptr(t))
         out = C.c_void_p()
-        check(lib().hx_moe_create(C.byref(c), C.byref(w), device, C.byref(out)), "hx_moe_create")
+        if any(len(entry) > 2 for entry in weights.values()):
+            check(lib().hx_moe_create_f8(C.byref(c), C.byref(w), C.byref(scales), device, C.byref(out)), "hx_moe_create_f8")
+        else:
+            check(lib().hx_moe_create(C.byref(c), C.byref(w), device, C.byref(out)), "hx_moe_create")
         return cls(out.value, cfg, act_dtype, device)
 
     def close(self) -> None:
@@ -325,7 +368,7 @@ class Qwen3_5MoeBlock:
 
     def experts(self, xs, topk_idx, topk_w, shared_w=None, workspace=None, stream=None, out=None):
         """The experts' part of forward() with the caller's routing, on a block of
-        MXFP4 experts: xs (b, l, hidden) or (T, hidden), topk_idx int32 and topk_w
+        MXFP4 or E4M3 experts: xs (b, l, hidden) or (T, hidden), topk_idx int32 and topk_w
         float32 with last dim k (indices outside 0 .. E - 1 are no expert), shared_w
         float32 of one value a token, or None for a call without the shared expert
         -> same shape as xs. `out` as in forward(). A call on another stream than the
@@ -492,6 +535,114 @@ def quantize_activations(weight_dtype: int, x, stream=None):
     check(lib().hx_quantize_activations(weight_dtype, _ptr(x), act, rows, cols, _ptr(codes), _ptr(d), _stream(stream)),
           "hx_quantize_activations")
     return codes, d
+
+
+# ---------------------------------------------------------------------------- E4M3
+def quantize_f8(x, block_rows: int = 1, stream=None):
+    """E4M3 codes and float32 scales of x, a float32 or bfloat16 cuda tensor [.., rows, cols], by
+    blocks of 128 columns of block_rows rows: 1 (activations, [.., cols]) or 128 (weights; each
+    matrix of a stack by itself), shorter at the edges -> (codes float8_e4m3fn like x, scales
+    [.., rows or ceil(rows / 128), ceil(cols / 128)]). A scale is max(max|x| / 448, 2^-126); a
+    code is the E4M3 value nearest to x / scale, ties to even; a block that holds a NaN or an
+    infinity gets the scale NaN."""
+    import torch
+    if not x.is_cuda or x.dim() == 0 or x.shape[-1] == 0:
+        raise TypeError("quantize_f8 needs a cuda tensor with columns")
+    if block_rows != 1 and (block_rows != 128 or x.dim() < 2):
+        raise ValueError("quantize_f8: blocks of 1 row, or of 128 of a matrix")
+    dt = _act_dtype(x.dtype)
+    x = _contiguous(x, stream)
+    cols = x.shape[-1]
+    nb = (cols + 127) // 128
+    rows = x.numel() // cols if block_rows == 1 else x.shape[-2]
+    codes = _empty(x, stream, x.shape, torch.float8_e4m3fn)
+    scales = _empty(x, stream, x.shape[:-1] + (nb,) if block_rows == 1 else x.shape[:-2] + ((rows + 127) // 128, nb),
+                    torch.float32)
+    _used_on(stream, x)
+    if not x.numel():
+        return codes, scales
+    count = x.numel() // (rows * cols)
+    if block_rows == 128 and rows % 128 == 0:   # whole blocks: the stack is one matrix
+        rows, count = rows * count, 1
+    with torch.cuda.device(x.device):
+        for i in range(count):
+            check(lib().hx_quantize_f8(_ptr(x) + i * rows * cols * x.element_size(), dt, rows, cols, block_rows,
+                                       _ptr(codes) + i * rows * cols, _ptr(scales) + i * ((rows + 127) // 128) * nb * 4,
+                                       _stream(stream, x.device)), "hx_quantize_f8")
+    return codes, scales
+
+
+class F8Linear:
+    """A linear layer on E4M3 weights with a float32 scale for each block of 128 x 128, without
+    bias: y = q(x) W^T, q the quantisation of x's rows by blocks of 128 (quantize_f8)."""
+
+    def __init__(self, handle: int, out_features: int, in_features: int, device: int):
+        self._h = C.c_void_p(handle)
+        self.out_features, self.in_features, self.device = out_features, in_features, device
+
+    @classmethod
+    def load(cls, codes, scales, device: Optional[int] = None) -> "F8Linear":
+        """codes float8_e4m3fn or uint8 [out, in], scales float32 [ceil(out / 128), ceil(in / 128)], on the
+        CPU or a GPU; the layer lies on `device` (their GPU, or 0)."""
+        import torch
+        _check_f8("weight", codes, scales)
+        if codes.dim() != 2:
+            raise ValueError("weight: codes must be [out, in]")
+        if codes.is_cuda:
+            if device is not None and device != codes.get_device():
+                raise ValueError(f"the weight is on {codes.device}, not on device {device}")
+            device = codes.get_device()
+            torch.cuda.current_stream(device).synchronize()   # the copy runs on the default stream
+        device = device or 0
+        out = C.c_void_p()
+        check(lib().hx_linear_create(codes.shape[0], codes.shape[1], _ptr(codes), _ptr(scales),
+                                     HX_DEVICE if codes.is_cuda else HX_HOST, device, C.byref(out)), "hx_linear_create")
+        return cls(out.value, codes.shape[0], codes.shape[1], device)
+
+    def close(self) -> None:
+        if self._h:
+            lib().hx_linear_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def workspace_size(self, n_rows: int) -> int:
+        n = C.c_size_t()
+        check(lib().hx_linear_workspace_size(self._h, n_rows, C.byref(n)), "hx_linear_workspace_size")
+        return n.value
+
+    def forward(self, xs, out_dtype=None, workspace=None, stream=None, out=None):
+        """xs [.., in] float32 or bfloat16 on the layer's GPU -> [.., out] of xs's type or out_dtype.
+        `out`, if given, is a contiguous tensor of that shape and type to write. Without a
+        workspace of workspace_size() bytes the layer keeps its own; a captured call must
+        bring it."""
+        import torch
+        if not xs.is_cuda or xs.get_device() != self.device:
+            raise ValueError(f"xs must be on cuda:{self.device}")
+        if xs.dim() == 0 or xs.shape[-1] != self.in_features:
+            raise ValueError(f"xs: last dim of {tuple(xs.shape)} != {self.in_features}")
+        xdt = _act_dtype(xs.dtype)
+        x = _contiguous(xs, stream)
+        shape = x.shape[:-1] + (self.out_features,)
+        if out is None:
+            out = _empty(x, stream, shape, out_dtype or x.dtype)
+        elif (out.shape != shape or out.dtype != (out_dtype or out.dtype) or not out.is_contiguous()
+              or out.device != x.device):
+            raise ValueError(f"out must be a contiguous {tuple(shape)} tensor on {x.device}")
+        ydt = _act_dtype(out.dtype)
+        if workspace is not None and (workspace.device != x.device or not workspace.is_contiguous()):
+            raise ValueError(f"workspace must be a contiguous tensor on {x.device}")
+        _used_on(stream, x, workspace, out)
+        ws, ws_n = (None, 0) if workspace is None else (_ptr(workspace), workspace.nbytes)
+        check(lib().hx_linear_forward(self._h, _ptr(x), xdt, x.numel() // self.in_features, _ptr(out), ydt, ws, ws_n,
+                                      _stream(stream, self.device)), "hx_linear_forward")
+        return out
+
+    __call__ = forward
 
 
 # ---------------------------------------------------------------------------- balance

@@ -53,6 +53,10 @@ extern "C" {
 #define HX_Q6_K 14
 #define HX_BF16 30
 #define HX_MXFP4 39
+/* no GGML type: E4M3 codes (8-bit floats of 4 exponent and 3 mantissa bits, largest
+ * 448, NaN 0x7f and 0xff) [rows][cols] with f32 scales [ceil(rows / 128)][ceil(cols / 128)],
+ * a value being code * scale: expert projections (hx_moe_create_f8), linear layers */
+#define HX_F8_E4M3 256
 
 /* where the pointers in hx_moe_weights live */
 #define HX_HOST 0
@@ -91,6 +95,26 @@ typedef struct hx_moe hx_moe;
  * (isq.rs:62-68), uploads the weights to `device`. */
 int hx_moe_create(const hx_moe_config* cfg, const hx_moe_weights* w, int device, hx_moe** out);
 
+/* Scales of a block of HX_F8_E4M3 projections, f32, in the weights' location, copied as
+ * they are: gate and up [E, ceil(I / 128), ceil(H / 128)], down [E, ceil(H / 128), ceil(I / 128)],
+ * the shared expert's [ceil(Is / 128), ceil(H / 128)] and [ceil(H / 128), ceil(Is / 128)]. */
+typedef struct hx_moe_f8_scales {
+    const float* experts_gate;
+    const float* experts_up;
+    const float* experts_down;
+    const float* shared_gate;
+    const float* shared_up;
+    const float* shared_down;
+} hx_moe_f8_scales;
+
+/* hx_moe_create for experts (all projections, the shared expert's included) of
+ * HX_F8_E4M3; H, I and Is multiples of 32. Every call on a block takes such a handle.
+ * Its arithmetic is that of these checkpoints: the rows that meet a projection (the
+ * tokens, then h = silu(g) u) are quantised by hx_quantize_f8's rule with blocks of 1 x 128,
+ * products are of the codes, sums in f32 per block times both scales. */
+int hx_moe_create_f8(const hx_moe_config* cfg, const hx_moe_weights* w, const hx_moe_f8_scales* scales, int device,
+                     hx_moe** out);
+
 /* Drop: frees the handle's device memory. NULL is accepted. */
 int hx_moe_destroy(hx_moe* m);
 
@@ -101,7 +125,7 @@ int hx_moe_workspace_size(const hx_moe* m, int64_t n_tokens, size_t* bytes);
 /* Module::forward (moe.rs:164-199 / tp_qwen3_5.rs:1240-1275), device resident:
  * x and y are device pointers to [n_tokens, H] in act_dtype (the reference's
  * (b, l, H) input flattened, moe.rs:166-167). workspace may be NULL, in which
- * case the handle grows its own; on a block of HX_MXFP4 experts it must start on 16
+ * case the handle grows its own; on a block of HX_MXFP4 or HX_F8_E4M3 experts it must start on 16
  * bytes (HX_ERR_INVALID_ARGUMENT before anything is launched; hx_moe_decoder_mlp
  * alike). router_bias is an optional device [E] f32 added
  * to the router logits before the softmax (a benchmark hook with no reference
@@ -127,15 +151,16 @@ int hx_moe_forward_noalloc(hx_moe* m, const void* x, int64_t n_tokens, void* y, 
 
 /* No counterpart in the reference: the experts' part of hx_moe_forward for a caller
  * that has the routing (its own router, a routing shared by several calls, tokens
- * sent here by another device), on a block whose expert projections are HX_MXFP4
- * (others: HX_ERR_UNSUPPORTED):
+ * sent here by another device), on a block whose expert projections are HX_MXFP4 or
+ * HX_F8_E4M3 (others: HX_ERR_UNSUPPORTED):
  *   y[t] = sum_j topk_w[t, j] * expert[topk_idx[t, j]](x[t]) + shared_w[t] * shared_expert(x[t])
  * topk_idx int32 and topk_w f32 are device [n_tokens, k], k the block's
  * num_experts_per_tok. An index outside 0 .. E - 1 is no expert: the entry adds
  * nothing, its weight is not read into the sum, and a token of such entries alone
  * gets its shared expert's part, or zeros (padding). The same index twice in a token
  * counts twice. shared_w is device f32 [n_tokens], or NULL for a call without the
- * shared expert. Products are of the stored weights and the activations to 13 bits
+ * shared expert. HX_F8_E4M3: as hx_moe_create_f8 says. HX_MXFP4: products are of the stored
+ * weights and the activations to 13 bits
  * below each 32-wide block's largest (act HX_F32: 23) or to 2^-130 where that is more,
  * sums in f32; h = silu(g) u is taken to the same bits; above the few tokens of a decode step each expert's
  * output is rounded to act_dtype before the weighted sum (f32). A token that holds a
@@ -236,6 +261,36 @@ int64_t hx_row_bytes(int dtype, int64_t n);
  * d = 1 / iscale). cols must be a multiple of the block. */
 int hx_quantize_activations(int weight_dtype, const void* x, int x_dtype, int64_t rows, int64_t cols, int8_t* codes,
                             float* d, void* stream);
+
+/* E4M3 codes and scales of x [rows, cols] (HX_F32 or HX_BF16, on the device) by blocks of
+ * 128 columns of block_rows rows, 1 (activations) or 128 (weights: HX_F8_E4M3), shorter at
+ * the edges: codes [rows, cols] bytes, scales f32 [ceil(rows / block_rows), ceil(cols / 128)].
+ * A block's scale is max(max|x| / 448, 2^-126), rounded to f32; a code is the E4M3 value
+ * nearest to x / scale, the exact quotient, ties to the even code. A block that holds a NaN
+ * or an infinity gets the scale NaN and codes 0. On the current device. */
+int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t cols, int block_rows, void* codes, float* scales,
+                   void* stream);
+
+/* A linear layer on HX_F8_E4M3 weights (no bias), the arithmetic of hx_moe_create_f8's
+ * projections: y = q(x) W^T, q the rows' quantisation by blocks of 1 x 128, f32 sums, one
+ * rounding to y's type. The reference's quantised linear layers
+ * (crates/neuron/src/harness/tp/tp_linear.rs:47-140) have no such format.
+ * hx_linear_create copies codes [out, in] and scales [ceil(out / 128), ceil(in / 128)] from
+ * location (HX_HOST or HX_DEVICE) to device memory of its own and lays them out; sizes need not be
+ * whole blocks (out at most 2^20, in 2^17). hx_linear_forward: x [n_rows, in] and y
+ * [n_rows, out], HX_F32 or HX_BF16 each, not overlapping; n_rows 0 is a no-op. A row that
+ * holds a NaN or an infinity gets NaN, the others' results do not depend on it nor on how the
+ * rows are split into calls, but for the last bits of the sums. workspace: hx_linear_workspace_size
+ * bytes for n_rows rows or any fewer (0: none is used), 16-byte aligned; NULL: the handle grows its own,
+ * but a call under stream capture must bring it. Calls on one handle are serialised by the
+ * caller, or bring a workspace each. */
+typedef struct hx_linear hx_linear;
+int hx_linear_create(int64_t out_features, int64_t in_features, const void* codes, const float* scales, int location,
+                     int device, hx_linear** out);
+int hx_linear_destroy(hx_linear* l);
+int hx_linear_workspace_size(const hx_linear* l, int64_t n_rows, size_t* bytes);
+int hx_linear_forward(hx_linear* l, const void* x, int x_dtype, int64_t n_rows, void* y, int y_dtype, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* Per-kernel timing (a measurement hook with no reference counterpart): HIP
  * events recorded on the forward's stream around each kernel it launches.
