@@ -5,9 +5,9 @@
 
 Flags: -ffp-contract=off keeps every multiply-add explicit (the routing contract
 spells out its fmaf chains); packed fp32 instructions are disabled. The MFMA
-router (hx_route_mfma.hip) is compiled with MFMA results in VGPRs: it adds every
-MFMA's result to its running sums with VALU instructions, which would otherwise
-first copy each result out of the accumulation registers.
+router (hx_route_mfma.hip) and the E4M3 products (hx_f8.hip) are compiled with MFMA
+results in VGPRs: they add every MFMA's result to running sums with VALU instructions,
+which would otherwise first copy each result out of the accumulation registers.
 """
 from __future__ import annotations
 
@@ -35,7 +35,7 @@ CFLAGS = [
 ]
 
 
-EXTRA = {"hx_route_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("hx_route_mfma.hip", "hx_f8.hip")}
 
 
 def _compile(src: str) -> str:

@@ -33,7 +33,7 @@ struct BalArgs {
 };
 
 // tokens a workgroup of the counts takes, and their most
-constexpr int BAL_CHUNK = 1024, BAL_MAX_G1 = 64, BAL_MAX_G2 = 1024;
+constexpr int BAL_CHUNK = 1024, BAL_MAX_G1 = 64, BAL_MAX_G2 = 2048;
 static int bal_g1(int64_t T) { return (int)std::min<int64_t>((T + BAL_CHUNK - 1) / BAL_CHUNK, BAL_MAX_G1); }
 // the most of the row pass: a wave has two turns at least
 static int bal_g2(int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t>((T + 7) / 8, BAL_MAX_G2)); }
@@ -42,24 +42,29 @@ static int bal_g2(int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t
 HX_DEV void bal_count(const BalArgs& a, int64_t t0, int64_t t1, int* hist) {
   for (int64_t t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
     bool live = false;
-    for (int j = 0; j < a.k; j++) {
-      const int e = a.idx[t * a.k + j];
-      if ((unsigned)e >= (unsigned)a.E) continue;
-      live = true;
-      atomicAdd(&hist[e], 1);
+    for (int j0 = 0; j0 < a.k; j0 += 8) {   // eight loads on their way together
+      int e[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) e[j] = j0 + j < a.k ? a.idx[t * a.k + j0 + j] : -1;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        if ((unsigned)e[j] >= (unsigned)a.E) continue;
+        live = true;
+        atomicAdd(&hist[e[j]], 1);
+      }
     }
     if (live) atomicAdd(&hist[a.E], 1);
   }
 }
 
-__global__ __launch_bounds__(256) void k_bal_counts(BalArgs a) {
+__global__ __launch_bounds__(1024) void k_bal_counts(BalArgs a) {
   __shared__ int hist[HX_MAX_EXPERTS + 1];
-  for (int e = threadIdx.x; e <= a.E; e += 256) hist[e] = 0;
+  for (int e = threadIdx.x; e <= a.E; e += 1024) hist[e] = 0;
   __syncthreads();
   const int64_t per = (a.T + a.G1 - 1) / a.G1, t0 = blockIdx.x * per;
   bal_count(a, t0, min(a.T, t0 + per), hist);
   __syncthreads();
-  for (int e = threadIdx.x; e <= a.E; e += 256) a.hist[(int64_t)blockIdx.x * (a.E + 1) + e] = hist[e];
+  for (int e = threadIdx.x; e <= a.E; e += 1024) a.hist[(int64_t)blockIdx.x * (a.E + 1) + e] = hist[e];
 }
 
 // the chunks' counts of column e, eight loads on their way together
@@ -92,35 +97,28 @@ HX_DEV float bal_row_max(float v, int lpr) {
   return v;
 }
 
-// exp(x), x <= 0 or NaN: the product with log2 e in two parts, so that its rounding (3e-6 of
-// the result at -60) is not in the exponent
-HX_DEV float bal_exp(float x) {
-  x = x < -150.f ? -150.f : x;   // not a maximum: a NaN stays
-  const float hi = x * 1.44269502e+00f;
-  const float lo = __builtin_fmaf(x, 1.44269502e+00f, -hi) + x * 1.92596303e-08f;
-  const float e = __builtin_amdgcn_exp2f(hi);
-  return __builtin_fmaf(e, lo * 6.93147182e-01f, e);
-}
-
-// V elements at p
+// V elements at p: as they come, and their values
 template <bool BF, int V>
-HX_DEV void bal_load(const void* base, int64_t at, float (&f)[V]) {
-  if constexpr (BF && V == 8) {
-    const uint4 v = *(const uint4*)((const uint16_t*)base + at);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      f[2 * i] = __uint_as_float(u[i] << 16);
-      f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+struct BalRaw {
+  static constexpr int W = V == 1 ? 1 : 4;   // words
+  uint32_t u[W];
+  HX_DEV void load(const void* base, int64_t at) {
+    if constexpr (V == 1) {
+      u[0] = BF ? (uint32_t)((const uint16_t*)base)[at] << 16 : ((const uint32_t*)base)[at];
+    } else {
+      const uint4 v = *(const uint4*)((const uint8_t*)base + at * (BF ? 2 : 4));
+      u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
     }
-  } else if constexpr (!BF && V == 4) {
-    const float4 v = *(const float4*)((const float*)base + at);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-  } else {
-    static_assert(V == 1, "16 bytes or one element");
-    f[0] = ld_act(base, at, BF);
   }
-}
+  HX_DEV void none() {   // -inf: adds nothing, is no maximum
+#pragma unroll
+    for (int i = 0; i < W; i++) u[i] = BF && V > 1 ? 0xff80ff80u : 0xff800000u;
+  }
+  HX_DEV float value(int i) const {
+    if constexpr (BF && V > 1) return __uint_as_float(i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
+    else return __uint_as_float(u[i]);
+  }
+};
 template <bool BF, int V>
 HX_DEV void bal_store(void* base, int64_t at, const float (&f)[V]) {
   if constexpr (BF && V == 8) {
@@ -186,21 +184,32 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
   const float scale = live_n > 0 ? a.coef * E / live_n : 0.f;
   float s_sum = 0.f;
   const int64_t step = (int64_t)gridDim.x * NW * rpw;
-  for (int64_t t0 = ((int64_t)blockIdx.x * NW + wave) * rpw; t0 < a.T; t0 += step) {
+  // a row on its way while the one before is computed
+  BalRaw<BF, V> next[NJ];
+  bool next_mine;
+  auto fetch = [&](int64_t t) {
+    const bool row = t < a.T;
+#pragma unroll
+    for (int i = 0; i < NJ; i++) {
+      const int c = (i * lpr + sub) * V;
+      if (row && c < E) next[i].load(a.logits, t * E + c);
+      else next[i].none();
+    }
+    next_mine = false;
+    for (int j = sub; row && j < k; j += lpr) next_mine |= (unsigned)a.idx[t * k + j] < (unsigned)E;
+  };
+  int64_t t0 = ((int64_t)blockIdx.x * NW + wave) * rpw;
+  if (t0 < a.T) fetch(t0 + grp);
+  for (; t0 < a.T; t0 += step) {
     const int64_t t = t0 + grp;
     const bool row = t < a.T;
     float x[NJ][V];
 #pragma unroll
-    for (int i = 0; i < NJ; i++) {
-      const int c = (i * lpr + sub) * V;
-      if (row && c < E) bal_load<BF, V>(a.logits, t * E + c, x[i]);
-      else
+    for (int i = 0; i < NJ; i++)
 #pragma unroll
-        for (int v = 0; v < V; v++) x[i][v] = -__builtin_inff();
-    }
-    bool mine = false;
-    for (int j = sub; row && j < k; j += lpr) mine |= (unsigned)a.idx[t * k + j] < (unsigned)E;
-    const unsigned long long any = __ballot(mine);
+      for (int v = 0; v < V; v++) x[i][v] = next[i].value(v);
+    const unsigned long long any = __ballot(next_mine);
+    if (t0 + step < a.T) fetch(t0 + step + grp);
     const bool live = lpr == 64 ? any != 0 : ((any >> (grp * lpr)) & ((1ull << lpr) - 1)) != 0;
     float m = -__builtin_inff();
 #pragma unroll
@@ -209,12 +218,14 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
       for (int v = 0; v < V; v++) m = fmaxf(m, x[i][v]);
     m = bal_row_max(m, lpr);
     float z = 0.f, s = 0.f;
+    // exp2((x - m) log2 e): two roundings, together 2 |x - m| half steps of the result
 #pragma unroll
     for (int i = 0; i < NJ; i++)
 #pragma unroll
       for (int v = 0; v < V; v++) {
         const bool in = (i * lpr + sub) * V < E;
-        x[i][v] = in ? bal_exp(x[i][v] - m) : 0.f;
+        const float e = __builtin_amdgcn_exp2f((x[i][v] - m) * 1.44269502e+00f);
+        x[i][v] = in ? e : 0.f;   // a row of -inf alone has m = -inf: NaN behind its end too
         z += x[i][v];
         s = __builtin_fmaf(f[i][v], x[i][v], s);
       }
@@ -224,6 +235,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
     s *= r;
     // a row that is not live, whatever it holds, adds nothing
     if (live) s_sum += s;
+    const float ss = scale * s;
 #pragma unroll
     for (int i = 0; i < NJ; i++) {
       const int c = (i * lpr + sub) * V;
@@ -232,7 +244,8 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
       for (int v = 0; v < V; v++) {
         const float p = live ? x[i][v] * r : 0.f;
         sum[i][v] += p;
-        g[v] = live ? scale * p * (f[i][v] - s) : 0.f;
+        const float d = p * __builtin_fmaf(f[i][v], scale, -ss);
+        g[v] = live ? d : 0.f;
       }
       if (row && a.dlogits && c < E) bal_store<BF, V>(a.dlogits, t * E + c, g);
     }
@@ -263,23 +276,29 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
   }
 }
 
-// the workgroups' sums: a workgroup 64 columns (of the E + 1), 16 threads a column
+// the workgroups' sums: a workgroup 16 columns (of the E + 1), 64 threads a column
 __global__ __launch_bounds__(1024) void k_bal_last(BalArgs a) {
-  __shared__ double red[16][64];
+  __shared__ double red[64][16];
   __shared__ int live_sm;
-  const int c = threadIdx.x & 63, q = threadIdx.x >> 6, e = blockIdx.x * 64 + c;
+  const int c = threadIdx.x & 15, q = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
   if (threadIdx.x == 0) live_sm = 0;
   __syncthreads();
   if (threadIdx.x < a.G1) atomicAdd(&live_sm, a.hist[(int64_t)threadIdx.x * (a.E + 1) + a.E]);
   double v = 0.0;
   if (e <= a.E)
-    for (int g = q; g < a.G2; g += 16) v += a.part[(int64_t)g * (a.E + 1) + e];
+    for (int g0 = q; g0 < a.G2; g0 += 1024) {   // sixteen loads on their way together
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; i++) p[i] = g0 + 64 * i < a.G2 ? a.part[(int64_t)(g0 + 64 * i) * (a.E + 1) + e] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) v += p[i];
+    }
   red[q][c] = v;
   __syncthreads();
   if (q == 0 && e <= a.E) {
     const int n = live_sm;
     v = 0.0;
-    for (int w = 0; w < 16; w++) v += red[w][c];
+    for (int w = 0; w < 64; w++) v += red[w][c];
     if (e < a.E) a.probs[e] = n > 0 ? (float)(v / n) : 0.f;
     else a.loss[0] = n > 0 ? (float)(v * a.coef * a.E / n) : 0.f;
   }
@@ -304,7 +323,7 @@ static hipError_t launch_balance(BalArgs a, bool bf, hipStream_t s) {
   const int chunks = vec ? a.E / per : a.E;
   a.lpr = 64;
   while (a.lpr > 1 && a.lpr / 2 >= chunks) a.lpr /= 2;
-  if (!one) hx_launch(k_bal_counts, dim3(a.G1), dim3(256), 0, s, a);
+  if (!one) hx_launch(k_bal_counts, dim3(a.G1), dim3(1024), 0, s, a);
   const int nj = (chunks + 63) / 64;
   if (bf && vec) {
     if (nj <= 1) launch_rows<true, 8, 1>(a, one, s);
@@ -320,7 +339,7 @@ static hipError_t launch_balance(BalArgs a, bool bf, hipStream_t s) {
     if (nj <= 4) launch_rows<false, 1, 4>(a, one, s);
     else launch_rows<false, 1, 16>(a, one, s);
   }
-  if (!one) hx_launch(k_bal_last, dim3((a.E + 1 + 63) / 64), dim3(1024), 0, s, a);
+  if (!one) hx_launch(k_bal_last, dim3((a.E + 1 + 15) / 16), dim3(1024), 0, s, a);
   return hipGetLastError();
 }
 
@@ -372,7 +391,7 @@ extern "C" int hx_moe_expert_counts(const int32_t* topk_idx, int64_t n_tokens, i
   if ((rc = bal_args(a, topk_idx, n_tokens, k, num_experts, workspace, workspace_bytes))) return rc;
   a.counts = counts;
   hipStream_t s = (hipStream_t)stream;
-  if (n_tokens > 0) hx_launch(k_bal_counts, dim3(a.G1), dim3(256), 0, s, a);
+  if (n_tokens > 0) hx_launch(k_bal_counts, dim3(a.G1), dim3(1024), 0, s, a);
   hx_launch(k_bal_counts_sum, dim3((num_experts + 255) / 256), dim3(256), 0, s, a);
   HX_HIP(hipGetLastError());
   return HX_OK;

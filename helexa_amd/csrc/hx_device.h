@@ -30,6 +30,12 @@ HX_DEV void dma16(const void* g, uint32_t lds_base) {
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(g), "s"(lds_base) : "memory");
 }
+// the same, the lanes' bytes `off` from a base in scalar registers
+HX_DEV void dma16(const void* base, uint32_t off, uint32_t lds_base) {
+  uint32_t save;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(save) : "v"(off), "s"(base), "s"(lds_base) : "memory");
+}
 // a workgroup barrier that orders LDS accesses only: global loads still in
 // flight stay in flight across it (__syncthreads' fence waits for all of them)
 HX_DEV void lds_barrier() {
@@ -43,6 +49,13 @@ HX_DEV void dma4(const void* g, uint32_t lds_base) {
   uint32_t save;
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(g), "s"(lds_base) : "memory");
+}
+
+// the same, the lanes' bytes `off` from a base in scalar registers
+HX_DEV void dma4(const void* base, uint32_t off, uint32_t lds_base) {
+  uint32_t save;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(save) : "v"(off), "s"(base), "s"(lds_base) : "memory");
 }
 
 // v_and_or_b32 with its two constants in registers (a VOP3 instruction on this

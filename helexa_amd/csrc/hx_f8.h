@@ -33,8 +33,9 @@ __host__ __device__ inline int64_t f8_row(int64_t K) { return (int64_t)f8_blocks
 
 // tokens up to which a block takes the few-token kernels: an MFMA's 16 columns
 constexpr int F8_FEW_T = 16;
-// rows up to which a layer takes the few-row kernel, and up to which that one quantises
-constexpr int F8_FEW_ROWS = 64, F8_QUANT_ROWS = 16;
+// rows up to which a layer takes the few-row kernel, and up to which that one may quantise them
+// (f8_quant_inside)
+constexpr int F8_FEW_ROWS = 64, F8_QUANT_ROWS = 4;
 
 // experts: MxArgs with xrec and hrec the quantised rows of x and h, hblocks the blocks of
 // a row of h
@@ -62,10 +63,11 @@ hipError_t launch_f8_repack(const void* codes, const float* scales, int64_t coun
 hipError_t launch_f8_rows(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, bool padded,
                           hipStream_t s);
 hipError_t launch_f8_blocks(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, hipStream_t s);
+bool f8_quant_inside(int64_t M, int64_t K);
 hipError_t launch_f8_linear(const F8LinearArgs& a, hipStream_t s);
 
 bool f8_few(int T);
-int f8_tile_m(int64_t F, int E, bool xbf);
+int f8_tile_m(int64_t T, int64_t F, int E, int H, bool xbf);   // rows of a tile
 hipError_t launch_f8_few_gate_up(const F8Args& a, hipStream_t s);
 hipError_t launch_f8_few_down(const F8Args& a, hipStream_t s);
 hipError_t launch_f8_prep(const F8Args& a, hipStream_t s);

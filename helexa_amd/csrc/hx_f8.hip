@@ -82,6 +82,17 @@ HX_DEV void f8_codes(const float (&f)[N], float s, bool fine, uint32_t (&w)[N / 
     w[i] = fine ? f8_pack(div(f[4 * i]), div(f[4 * i + 1]), div(f[4 * i + 2]), div(f[4 * i + 3])) : 0u;
 }
 
+// The same by a product with 1 / s, within 1.5 steps of float32 of the quotient: for h, whose values
+// are off by more than that already, a border between codes is no sharper than they are (the exact
+// quotients took a third of the gate/up kernel's vector instructions)
+template <int N>
+HX_DEV void f8_codes_near(const float (&f)[N], float s, bool fine, uint32_t (&w)[N / 4]) {
+  const float r = 1.f / (fine ? s : 1.f);
+#pragma unroll
+  for (int i = 0; i < N / 4; i++)
+    w[i] = fine ? f8_pack(f[4 * i] * r, f[4 * i + 1] * r, f[4 * i + 2] * r, f[4 * i + 3] * r) : 0u;
+}
+
 // N elements from p, 16 bytes at a time (VEC: aligned) or n of them singly, zeros behind
 template <bool BF, bool VEC, int N>
 HX_DEV void f8_load(const void* base, int64_t at, int n, float (&f)[N]) {
@@ -338,32 +349,51 @@ HX_DEV uint32_t f8_max_of_4(uint32_t m) {
   return max((uint32_t)b[0], (uint32_t)b[1]);
 }
 
-// A lane's values of a block of its row (columns 64 h + 16 (l / 16) .. of it) and their
-// quantised form: the rows of a call of few are quantised by every wave that reads them
-struct F8Operand {
-  f8_v8i v;
+// A block of a row by 32 lanes, 4 values a lane, into LDS: its 128 codes and its scale. (By the lanes
+// that hold an operand each value is quantised by all 16 columns of a row alone: 7.4 us
+// where this takes 5.)
+template <bool BF, bool NEAR = false>
+HX_DEV void f8_block_to_lds(const void* x, int64_t row_at, int K, int b, bool vec, uint8_t* codes, float* scale) {
+  const int l = lane_id() & 31, c0 = 128 * b + 4 * l;
+  float f[4];
+  if (vec && c0 < K) {
+    if constexpr (BF) {
+      const uint2 v = *(const uint2*)((const uint16_t*)x + row_at + c0);
+      f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+      f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+    } else {
+      const float4 v = *(const float4*)((const float*)x + row_at + c0);
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = c0 + i < K ? ld_act(x, row_at + c0 + i, BF) : 0.f;
+  }
+  uint32_t m = f8_amax(f);
+  m = max(m, (uint32_t)dpp_mov<0xB1>((int)m));    // quad_perm 1,0,3,2
+  m = max(m, (uint32_t)dpp_mov<0x4E>((int)m));    // quad_perm 2,3,0,1
+  m = max(m, (uint32_t)dpp_mov<0x141>((int)m));   // row_half_mirror
+  m = max(m, (uint32_t)dpp_mov<0x140>((int)m));   // row_mirror
+  const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
   float s;
-  template <bool BF, bool VEC>
-  HX_DEV void load(const void* x, int64_t row_at, int64_t K, int b) {
-    float f[32];
-    const int c = 128 * b + 16 * (lane_id() >> 4);
-    float lo[16], hi[16];
-    f8_load<BF, VEC>(x, row_at + c, (int)min<int64_t>(K - c, 16), lo);
-    f8_load<BF, VEC>(x, row_at + c + 64, (int)min<int64_t>(K - c - 64, 16), hi);
-    const uint32_t m = f8_max_of_4(max(f8_amax(lo), f8_amax(hi)));
-    const bool fine = f8_scale(m, s);
-    uint32_t a[4], z[4];
-    f8_codes(lo, s, fine, a);
-    f8_codes(hi, s, fine, z);
-    v = f8_v8i{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)z[0], (int)z[1], (int)z[2], (int)z[3]};
-  }
-  // quantised rows
-  HX_DEV void load(const uint8_t* codes, const float* scales, int b) {
-    const uint8_t* p = codes + 128 * b + 16 * (lane_id() >> 4);
-    v = f8_op(*(const uint4*)p, *(const uint4*)(p + 64));
-    s = scales[b];
-  }
-};
+  const bool fine = f8_scale(max((uint32_t)r[0], (uint32_t)r[1]), s);
+  uint32_t w[1];
+  if constexpr (NEAR) f8_codes_near(f, s, fine, w);
+  else f8_codes(f, s, fine, w);
+  *(uint32_t*)(codes + 4 * l) = w[0];
+  if (l == 0) *scale = s;
+}
+// whether 4 values of a row come in one load
+template <bool BF>
+__host__ __device__ inline bool f8_vec4(const void* x, int64_t K) { return K % 4 == 0 && ((uintptr_t)x & (BF ? 7 : 15)) == 0; }
+// bytes between rows in LDS: 16 more than the codes, so that the rows' pieces start on other banks
+__host__ __device__ inline int f8_pitch(int K) { return f8_blocks(K) * 128 + 16; }
+
+// a lane's part of block b of a quantised row as an operand
+HX_DEV f8_v8i f8_operand(const uint8_t* row, int b) {
+  const uint8_t* p = row + 128 * b + 16 * (lane_id() >> 4);
+  return f8_op(*(const uint4*)p, *(const uint4*)(p + 64));
+}
 
 HX_DEV void f8_store(void* y, int64_t at, float v, bool bf) {
   if (bf) ((uint16_t*)y)[at] = f32_to_bf16(v);
@@ -372,28 +402,59 @@ HX_DEV void f8_store(void* y, int64_t at, float v, bool bf) {
 
 // ---------------------------------------------------------------- linear layer, few rows
 // Workgroup: 16 features; its 8 waves share K block by block and add up in LDS. CT columns
-// of 16 rows; QUANT: rows as the caller has them, quantised by each wave for its blocks.
-template <bool BF, bool VEC, int CT, bool QUANT, bool WIDE>
+// of 16 rows. QUANT: a few rows as the caller has them, quantised into LDS by every workgroup (a
+// launch less); the weights are on their way meanwhile. Bound by latency: 1 row, 4096 x 2048, 8.4 MB
+// in 5 us (a launch, two round trips to memory, the sum through LDS).
+template <bool BF, int CT, bool QUANT, bool WIDE>
 __global__ __launch_bounds__(512) void k_f8_few_rows(F8LinearArgs a) {
   constexpr int PITCH = 16 * CT + 1;
+  extern __shared__ __align__(16) uint8_t sm[];
   __shared__ float red[8 * 16 * PITCH];
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = blockIdx.x, KB = f8_blocks(a.K), M = (int)a.M, col = lane & 15;
   const uint8_t* w = a.w + (int64_t)n * KB * 2048 + lane * 16;
   const float* ws = (const float*)(a.w + f8_code_bytes(a.N, a.K)) + (int64_t)(n >> 3) * f8_scale_row(a.K);
+  uint4 ring[2][2];
+  float rs[2];
+  auto fetch = [&](int i, int b) {   // past the last: the last again
+    b = min(b, KB - 1);
+    ring[i][0] = *(const uint4*)(w + (int64_t)b * 2048);
+    ring[i][1] = *(const uint4*)(w + (int64_t)b * 2048 + 1024);
+    rs[i] = ws[b];
+  };
+  fetch(0, wave);
+  fetch(1, wave + 8);
+  const int pitch = QUANT ? f8_pitch(a.K) : 0;
+  float* const qs = (float*)(sm + M * pitch);   // [M][KB]
+  if constexpr (QUANT) {
+    const bool vec = f8_vec4<BF>(a.x, a.K);
+    for (int u = 2 * wave + (lane >> 5); u < M * KB; u += 16) {
+      const int r = u / KB, b = u % KB;
+      f8_block_to_lds<BF>(a.x, (int64_t)r * a.K, a.K, b, vec, sm + r * pitch + 128 * b, qs + u);
+    }
+    lds_barrier();
+  }
   f8_v4f acc[CT];
 #pragma unroll
   for (int c = 0; c < CT; c++) acc[c] = f8_zero4();
-  for (int b = wave; b < KB; b += 8) {
-    const F8Arg<WIDE> wv(f8_op(*(const uint4*)(w + (int64_t)b * 2048), *(const uint4*)(w + (int64_t)b * 2048 + 1024)));
-    const float sw = ws[b];
+  for (int b0 = wave; b0 < KB; b0 += 16) {
 #pragma unroll
-    for (int c = 0; c < CT; c++) {
-      const int r = min(16 * c + col, M - 1);
-      F8Operand x;
-      if constexpr (QUANT) x.load<BF, VEC>(a.x, (int64_t)r * a.K, a.K, b);
-      else x.load(a.xq + r * f8_row(a.K), a.xs + (int64_t)r * f8_scale_row(a.K), b);
-      f8_add(acc[c], f8_mfma(wv, F8Arg<WIDE>(x.v)), x.s * sw);
+    for (int i = 0; i < 2; i++) {
+      const int b = b0 + 8 * i;
+      if (b >= KB) break;
+      const F8Arg<WIDE> wv(f8_op(ring[i][0], ring[i][1]));
+      const float sw = rs[i];
+      f8_v8i x[CT];
+      float sx[CT];
+#pragma unroll
+      for (int c = 0; c < CT; c++) {
+        const int r = min(16 * c + col, M - 1);
+        x[c] = f8_operand(QUANT ? sm + r * pitch : a.xq + r * f8_row(a.K), b);
+        sx[c] = QUANT ? qs[r * KB + b] : a.xs[(int64_t)r * f8_scale_row(a.K) + b];
+      }
+      fetch(i, b + 16);
+#pragma unroll
+      for (int c = 0; c < CT; c++) f8_add(acc[c], f8_mfma(wv, F8Arg<WIDE>(x[c])), sx[c] * sw);
     }
   }
 #pragma unroll
@@ -502,70 +563,255 @@ HX_DEV void f8_products(const uint8_t* const (&w)[NM], const float* const (&ws)[
   }
 }
 
-// Linear layer over tiles of TM rows: workgroup: a tile and 256 features, 64 a wave
-template <int TM, bool WIDE>
-__global__ __launch_bounds__(256, 2) void k_f8_linear(F8LinearArgs a) {
-  constexpr int TT = TM / 16, NM = 4;
-  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM>::BYTES];
-  int nt, tile;
-  const int NT = f8_tiles(a.N);
-  mx_tile((NT + 15) / 16, (int)((a.M + TM - 1) / TM), nt, tile);
-  if (tile < 0) return;
-  const int64_t r0 = (int64_t)tile * TM;
-  const int rows = (int)min<int64_t>(TM, a.M - r0), KB = f8_blocks(a.K);
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = (4 * nt + wave) * NM;
-  F8Tile<TM> rw;
-  rw.init(wave, [&](int r) { return a.xq + (r0 + min(r, rows - 1)) * f8_row(a.K); });
-  const float* xs[TT];
+// Both operands through LDS: a workgroup of WF WR waves, a wave FT tiles of 16 features and TT of
+// 16 rows. A stage is one block of K: the features' tiles as they are stored, the rows (16-byte
+// piece j of row r at j ^ r % 8: the rows' pieces would all start on one bank), the rows' scales, the
+// features' scales; NS stages are in LDS, all but one of them on their way. They come in by direct
+// loads only: a load into a register would wait for the direct ones before it.
+template <int FT, int TT, int WF, int WR, int NS>
+struct F8Core {
+  static constexpr int NW = WF * WR, TF = 16 * FT * WF, TR = 16 * TT * WR;
+  static constexpr int ROWS = TF * 128, SX = ROWS + TR * 128, SW = SX + (TR * 4 + 255) / 256 * 256, STAGE = SW + 256;
+  static constexpr int APW = TF / 8 / NW, BPW = TR / 8 / NW, SPW = (TR / 64 + NW) / NW;   // loads of a wave
+  static constexpr int LOADS = APW + BPW + SPW, BYTES = NS * STAGE;
+  static_assert(TF % (8 * NW) == 0 && TR % (8 * NW) == 0 && TR % 64 == 0, "whole loads");
+  // where a wave's loads are: the features' tiles from base registers, rows and scales by the lanes'
+  // offsets from theirs
+  const uint8_t *a[APW], *rows, *xs, *ws;
+  uint32_t b[BPW], s[SPW];   // SPW: one wave's or several waves' loads are of the features' scales
+  int wave, wf, wr;
+  // tile(i): the stored tiles of the workgroup's i-th 16 features; row(r), scale(r): the offsets of the
+  // quantised row r from `rows` and of its scales from `xs`, within 32 bits; fscale(i): the i-th 16
+  // features' scales
+  template <typename A, typename B, typename S, typename W>
+  HX_DEV F8Core(const uint8_t* rows_, const float* xs_, A tile, B row, S scale, W fscale) : rows(rows_), xs((const uint8_t*)xs_) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wf = wave / WR;
+    wr = wave % WR;
+    const int lane = lane_id();
 #pragma unroll
-  for (int t = 0; t < TT; t++) xs[t] = a.xs + (r0 + min(16 * t + (lane & 15), rows - 1)) * f8_scale_row(a.K);
-  const uint8_t* w[NM];
+    for (int i = 0; i < APW; i++) {
+      const int q = i * NW + wave;
+      a[i] = tile(q >> 1) + (q & 1) * 1024;
+    }
 #pragma unroll
-  for (int m = 0; m < NM; m++) w[m] = a.w + (int64_t)min(n0 + m, NT - 1) * KB * 2048 + lane * 16;
-  const float* const ws[1] = {(const float*)(a.w + f8_code_bytes(a.N, a.K)) + (int64_t)(min(n0, NT - 1) >> 3) * f8_scale_row(a.K)};
-  f8_v4f acc[NM][TT];
-  f8_products<WIDE, TM, NM, 1>(w, ws, rw, xs, wave, buf, KB, acc);
-  const bool vec = a.N % 4 == 0 && ((uintptr_t)a.y & 15) == 0;
+    for (int i = 0; i < BPW; i++) {
+      const int r = (i * NW + wave) * 8 + (lane >> 3);
+      b[i] = row(r) + ((lane & 7) ^ (r & 7)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < SPW; i++) {   // the last waves' loads of rows that are not there go to the features' place
+      const int q = i * NW + wave;
+      s[i] = q < TR / 64 ? scale(64 * q + lane) : 0u;
+    }
+    ws = (const uint8_t*)fscale(min(lane, TF / 16 - 1));
+  }
+  HX_DEV void load(int k, uint32_t lds) const {
+#pragma unroll
+    for (int i = 0; i < APW; i++) dma16(a[i] + (int64_t)k * 2048, lane_id() * 16, lds + (i * NW + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < BPW; i++) dma16(rows + (int64_t)k * 128, b[i], lds + ROWS + (i * NW + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < SPW; i++) {
+      if (i * NW + wave < TR / 64) dma4(xs + (int64_t)k * 4, s[i], lds + SX + (i * NW + wave) * 256);
+      else dma4(ws + (int64_t)k * 4, lds + SW);
+    }
+  }
+  // acc[f][t] = the sums over KB blocks; tile f's scale is that of tile f % NQ of the wave. A tile's
+  // products are added to the sums while the next one's run, its codes come while the one before runs
+  // (work false: a wave without rows brings its loads only).
+  template <bool WIDE, int NQ>
+  HX_DEV void run(int KB, uint8_t* buf, bool work, f8_v4f (&acc)[FT][TT]) const {
+    static_assert(FT % 2 == 0 && FT % NQ == 0, "pairs of tiles, whole groups of scales");
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
+    const int lane = lane_id();
+    f8_v4f d[2][TT];
+    float last[TT];
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+#pragma unroll
+      for (int f = 0; f < FT; f++) acc[f][t] = f8_zero4();
+      d[1][t] = f8_zero4();
+      last[t] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < NS - 1; i++)
+      if (i < KB) load(i, lds + i * STAGE);
+    const uint8_t* const x0 = buf + ROWS + (wr * TT * 16 + (lane & 15)) * 128 + ((lane >> 4) ^ (lane & 7)) * 16;
+    const uint8_t* const x1 = buf + ROWS + (wr * TT * 16 + (lane & 15)) * 128 + ((4 + (lane >> 4)) ^ (lane & 7)) * 16;
+    const uint8_t* const w0 = buf + wf * FT * 2048 + lane * 16;
+    const uint8_t* const s0 = buf + SX + (wr * TT * 16 + (lane & 15)) * 4;
+    int at = 0;   // the stage of block k
+    for (int k = 0; k < KB; k++) {
+      // block k has come; after the barrier also the other waves', and the stage before it has been read
+      if (k + NS - 2 < KB) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * LOADS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      lds_barrier();
+      if (k + NS - 1 < KB) load(k + NS - 1, lds + (at == 0 ? NS - 1 : at - 1) * STAGE);
+      const int st = at * STAGE;
+      at = at == NS - 1 ? 0 : at + 1;
+      if (!work) continue;
+      auto tile = [&](int f) { return f8_op(*(const uint4*)(w0 + st + f * 2048), *(const uint4*)(w0 + st + f * 2048 + 1024)); };
+      f8_v8i w[2];
+      w[0] = tile(0);
+      F8Arg<WIDE> x[TT];
+#pragma unroll
+      for (int t = 0; t < TT; t++)
+        x[t] = F8Arg<WIDE>(f8_op(*(const uint4*)(x0 + st + t * 2048), *(const uint4*)(x1 + st + t * 2048)));
+      float s[NQ][TT];
+      const float* const fs = (const float*)(buf + SW + st) + wf * FT;
+#pragma unroll
+      for (int t = 0; t < TT; t++)
+#pragma unroll
+        for (int q = 0; q < NQ; q++) s[q][t] = *(const float*)(s0 + st + t * 64) * fs[q];
+#pragma unroll
+      for (int f = 0; f < FT; f++) {
+        if (f + 1 < FT) w[(f + 1) & 1] = tile(f + 1);
+        const F8Arg<WIDE> wv(w[f & 1]);
+#pragma unroll
+        for (int t = 0; t < TT; t++) {
+          d[f & 1][t] = f8_mfma(wv, x[t]);
+          f8_add(acc[f == 0 ? FT - 1 : f - 1][t], d[(f & 1) ^ 1][t], f == 0 ? last[t] : s[(f - 1) % NQ][t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int t = 0; t < TT; t++) last[t] = s[(FT - 1) % NQ][t];
+    }
+#pragma unroll
+    for (int t = 0; t < TT; t++) f8_add(acc[FT - 1][t], d[1][t], last[t]);
+  }
+};
+
+// A wave's results, BYTES a row in LDS, to dst(r): whole rows by neighbouring lanes
+template <int BYTES>
+struct F8Out {
+  static constexpr int PITCH = BYTES + 16, PIECES = BYTES / 16;   // 16 bytes more: fewer rows on the same banks
+  template <typename F>
+  HX_DEV static void store(const uint8_t* tile, int rows, int bytes, F dst) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    for (int i = lane_id(); i < rows * PIECES; i += 64) {
+      const int r = i / PIECES, b = i % PIECES * 16;
+      if (b < bytes) *(uint4*)(dst(r) + b) = *(const uint4*)(tile + r * PITCH + b);
+    }
+  }
+};
+HX_DEV uint32_t f8_bf16x2(float a, float b) { return f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16); }
+
+// workgroup -> (features, rows) of NF x NR tiles: each XCD (workgroup id mod 8) takes an eighth of a
+// list that goes through the features four tiles of rows at a time, so that the workgroups that
+// run together on an XCD meet each other's operands in its L2
+HX_DEV bool f8_place(int NF, int NR, int& nf, int& nr) {
+  const int64_t N = (int64_t)NF * NR, per = (N + 7) / 8, i = blockIdx.x >> 3, j = (blockIdx.x & 7) * per + i;
+  if (i >= per || j >= N) return false;
+  const int g = (int)(j / (4 * NF)), in = (int)(j % (4 * NF)), h = min(4, NR - 4 * g);
+  nf = in / h;
+  nr = 4 * g + in % h;
+  return true;
+}
+
+// Linear layer of many rows
+template <int FT, int TT, int WF, int WR, int NS, bool WIDE>
+__global__ __launch_bounds__(64 * WF * WR, 2) void k_f8_linear(F8LinearArgs a) {
+  typedef F8Core<FT, TT, WF, WR, NS> Core;
+  typedef F8Out<32 * FT> Out;
+  constexpr int OUT = WIDE ? 0 : WF * WR * 16 * TT * Out::PITCH;
+  __shared__ __align__(16) uint8_t buf[Core::BYTES > OUT ? Core::BYTES : OUT];
+  static_assert(128 % (16 * FT) == 0, "a wave's features have one scale");
+  const int NT = f8_tiles(a.N), KB = f8_blocks(a.K), lane = lane_id();
+  int nf, nr;
+  if (!f8_place((a.N + Core::TF - 1) / Core::TF, (int)((a.M + Core::TR - 1) / Core::TR), nf, nr)) return;
+  const int64_t r0 = (int64_t)nr * Core::TR;
+  const int rows = (int)min<int64_t>(Core::TR, a.M - r0), n0 = nf * (Core::TF / 16);
+  const float* const ws = (const float*)(a.w + f8_code_bytes(a.N, a.K));
+  const Core core(a.xq + r0 * f8_row(a.K), a.xs + r0 * f8_scale_row(a.K),
+                  [&](int i) { return a.w + (int64_t)min(n0 + i, NT - 1) * KB * 2048; },
+                  [&](int r) { return (uint32_t)(min(r, rows - 1) * f8_row(a.K)); },
+                  [&](int r) { return (uint32_t)(min(r, rows - 1) * f8_scale_row(a.K) * 4); },
+                  [&](int i) { return ws + (int64_t)(min(n0 + i, NT - 1) >> 3) * f8_scale_row(a.K); });
+  f8_v4f acc[FT][TT];
+  core.template run<WIDE, 1>(KB, buf, core.wr * TT * 16 < rows, acc);
+  const int f0 = 16 * (n0 + core.wf * FT), wr0 = core.wr * TT * 16, wrows = rows - wr0;   // the wave's
+  if (!WIDE && a.N % 8 == 0 && ((uintptr_t)a.y & 15) == 0) {
+    lds_barrier();   // the last stage has been read
+    uint8_t* const tl = buf + core.wave * (16 * TT * Out::PITCH);
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+#pragma unroll
+      for (int f = 0; f < FT; f++) {
+        const f8_v4f& v = acc[f][t];
+        *(uint2*)(tl + (16 * t + (lane & 15)) * Out::PITCH + 32 * f + 8 * (lane >> 4)) = make_uint2(f8_bf16x2(v[0], v[1]), f8_bf16x2(v[2], v[3]));
+      }
+    Out::store(tl, min(wrows, 16 * TT), 2 * (a.N - f0),
+               [&](int r) { return (uint8_t*)a.y + ((r0 + wr0 + r) * a.N + f0) * 2; });
+    return;
+  }
+  const bool vec = WIDE && a.N % 4 == 0 && ((uintptr_t)a.y & 15) == 0;
 #pragma unroll
   for (int t = 0; t < TT; t++) {
     const int r = 16 * t + (lane & 15);
-    if (r >= rows) continue;
+    if (r >= wrows) continue;
 #pragma unroll
-    for (int m = 0; m < NM; m++) {
-      const int f = 16 * (n0 + m) + 4 * (lane >> 4);
-      const int64_t at = (r0 + r) * a.N + f;
-      const f8_v4f& v = acc[m][t];
-      if (vec && f < a.N) {
-        if (!WIDE) *(uint2*)((uint16_t*)a.y + at) = make_uint2(f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
-                                                               f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
-        else *(float4*)((float*)a.y + at) = make_float4(v[0], v[1], v[2], v[3]);
+    for (int f = 0; f < FT; f++) {
+      const int c = f0 + 16 * f + 4 * (lane >> 4);
+      const int64_t at = (r0 + wr0 + r) * a.N + c;
+      const f8_v4f& v = acc[f][t];
+      if (vec) {
+        if (c < a.N) *(float4*)((float*)a.y + at) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          if (f + i < a.N) f8_store(a.y, at + i, v[i], !WIDE);
+          if (c + i < a.N) f8_store(a.y, at + i, v[i], !WIDE);
       }
     }
   }
 }
 
+template <int FT, int TT, int WF, int WR, int NS, bool WIDE>
+static void f8_linear_tiled(const F8LinearArgs& a, hipStream_t s) {
+  typedef F8Core<FT, TT, WF, WR, NS> Core;
+  const int64_t n = ((a.N + Core::TF - 1) / Core::TF) * ((a.M + Core::TR - 1) / Core::TR);
+  hx_launch(k_f8_linear<FT, TT, WF, WR, NS, WIDE>, dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * WF * WR), 0, s, a);
+}
+
+// Rows that the few-row kernel quantises itself: what that takes grows with them, a launch for it
+// costs about 3 us; and they have to fit in LDS.
+static size_t f8_few_lds(int64_t M, int64_t K) { return (size_t)M * (f8_pitch((int)K) + 4 * f8_blocks(K)); }
+bool f8_quant_inside(int64_t M, int64_t K) { return M <= F8_QUANT_ROWS && f8_few_lds(M, K) <= 40 * 1024; }
+
 template <bool WIDE>
 static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
   const dim3 few((unsigned)f8_tiles(a.N));
-  if (a.M <= F8_QUANT_ROWS) {
-    const bool vec = a.K % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
-    if (a.xbf && vec) hx_launch(k_f8_few_rows<true, true, 1, true, WIDE>, few, dim3(512), 0, s, a);
-    else if (a.xbf) hx_launch(k_f8_few_rows<true, false, 1, true, WIDE>, few, dim3(512), 0, s, a);
-    else if (vec) hx_launch(k_f8_few_rows<false, true, 1, true, WIDE>, few, dim3(512), 0, s, a);
-    else hx_launch(k_f8_few_rows<false, false, 1, true, WIDE>, few, dim3(512), 0, s, a);
+  if (f8_quant_inside(a.M, a.K)) {
+    const uint32_t lds = (uint32_t)f8_few_lds(a.M, a.K);
+    if (a.xbf) hx_launch(k_f8_few_rows<true, 1, true, WIDE>, few, dim3(512), lds, s, a);
+    else hx_launch(k_f8_few_rows<false, 1, true, WIDE>, few, dim3(512), lds, s, a);
     return hipGetLastError();
   }
   hipError_t e = launch_f8_rows(a.x, a.xbf, a.M, a.K, a.xq, a.xs, true, s);
   if (e != hipSuccess) return e;
-  if (a.M <= 32) hx_launch(k_f8_few_rows<true, true, 2, false, WIDE>, few, dim3(512), 0, s, a);
-  else if (a.M <= F8_FEW_ROWS) hx_launch(k_f8_few_rows<true, true, 4, false, WIDE>, few, dim3(512), 0, s, a);
+  if (a.M <= 16) hx_launch(k_f8_few_rows<true, 1, false, WIDE>, few, dim3(512), 0, s, a);
+  else if (a.M <= 32) hx_launch(k_f8_few_rows<true, 2, false, WIDE>, few, dim3(512), 0, s, a);
+  else if (a.M <= F8_FEW_ROWS) hx_launch(k_f8_few_rows<true, 4, false, WIDE>, few, dim3(512), 0, s, a);
   else {
-    const int64_t tiles = (a.M + 63) / 64, nx = (f8_tiles(a.N) + 15) / 16;
-    hx_launch(k_f8_linear<64, WIDE>, dim3((unsigned)(nx * ((tiles + 7) / 8 * 8))), dim3(256), 0, s, a);
+    // The larger a tile, the fewer loads and LDS reads a product takes, if the tiles fill the chip: one
+    // of 256 x 256 a CU, two of 128 x 128, which take a third of its time. us with tiles of 256, 128, 64
+    // (quantisation included): 512 rows x 4096 x 2048 48, 19.4, 15.5; 768 rows 37, 21.6, 20.5; 1024 37, 22.5,
+    // 25.0; 4096 44.9, 47.9, 64; 5000 (320 tiles of 256) 74, 59, 77; 8192 x 4096: 1024 rows 65, 45, 63; 1536
+    // 67, 70, 89; 2304 128, 102, 131; 8192 281, 319, -.
+    auto tiles = [&](int t) { return ((a.N + t - 1) / t) * ((a.M + t - 1) / t); };
+    if constexpr (WIDE) {   // operands of 16 bits: smaller tiles fit the registers
+      if (tiles(128) >= 128) f8_linear_tiled<4, 2, 2, 2, 2, WIDE>(a, s);
+      else f8_linear_tiled<2, 2, 2, 2, 3, WIDE>(a, s);
+    } else if (3 * ((tiles(256) + 255) / 256) <= (tiles(128) + 255) / 256) {
+      f8_linear_tiled<8, 4, 2, 4, 2, WIDE>(a, s);
+    } else if (tiles(128) >= 224) {
+      f8_linear_tiled<4, 4, 2, 2, 2, WIDE>(a, s);
+    } else {
+      f8_linear_tiled<2, 2, 2, 2, 3, WIDE>(a, s);
+    }
   }
   return hipGetLastError();
 }
@@ -574,10 +820,12 @@ hipError_t launch_f8_linear(const F8LinearArgs& a, hipStream_t s) { return a.ybf
 // ---------------------------------------------------------------- experts, few tokens
 // Gate/up of up to 16 tokens. Workgroup: a chosen expert (slot) and 8 / KW groups of 16
 // features; KW waves share a group's K and add up in LDS. h leaves in f32: its blocks of 128
-// are of several workgroups, the down kernels quantise it.
-template <bool BF, bool VEC, int KW, bool ONE>
+// are of several workgroups, the down kernels quantise it. ONE token: an expert a chosen entry, its
+// weights on their way before the token is quantised, by every workgroup; more tokens come quantised.
+template <bool BF, int KW, bool ONE>
 __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
   constexpr int FW = 8 / KW;
+  extern __shared__ __align__(16) uint8_t sm[];   // ONE: the token's codes, then its scales
   __shared__ MxFewT<ONE ? 1 : F8_FEW_T> few;
   __shared__ float red[8][2][16][17];
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = ONE ? 1 : a.T;
@@ -604,21 +852,44 @@ __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
   if (!ONE && blockIdx.x == 0 && tid < 33)   // for the down kernel
     a.few[slot * MX_FEW_TAB + tid] = tid == 32 ? e : tid < T ? mx_few_row(a, few, e, tid) : -1;
   if (16 * (int)blockIdx.x * FW >= inter) return;
+  const bool work = 16 * fb < inter;
+  const uint8_t* const mat[2] = {sh ? a.sgate.base : a.gate.mat(e), sh ? a.sup.base : a.up.mat(e)};
+  const int64_t at = (int64_t)(work ? fb : 0) * KB * 2048 + lane * 16;
+  const int64_t sat = f8_code_bytes(inter, a.H) + (int64_t)((work ? fb : 0) >> 3) * f8_scale_row(a.H) * 4;
+  uint4 ring[2][2][2];   // two blocks, gate and up
+  float rs[2][2];
+  auto fetch = [&](int i, int b) {
+    b = min(b, KB - 1);
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+      const uint8_t* p = mat[m] + at + (int64_t)b * 2048;
+      ring[i][m][0] = *(const uint4*)p;
+      ring[i][m][1] = *(const uint4*)(p + 1024);
+      rs[i][m] = ((const float*)(mat[m] + sat))[b];
+    }
+  };
+  fetch(0, kq);
+  fetch(1, kq + KW);
+  if (ONE) {
+    const bool vec = f8_vec4<BF>(a.x, a.H);
+    for (int b = 2 * wave + (lane >> 5); b < KB; b += 16)
+      f8_block_to_lds<BF>(a.x, 0, a.H, b, vec, sm + 128 * b, (float*)(sm + 128 * KB) + b);
+    lds_barrier();
+  }
   f8_v4f ag = f8_zero4(), au = f8_zero4();
-  if (16 * fb < inter) {
-    const uint8_t* gm = sh ? a.sgate.base : a.gate.mat(e);
-    const uint8_t* um = sh ? a.sup.base : a.up.mat(e);
-    const int64_t at = (int64_t)fb * KB * 2048 + lane * 16, sat = f8_code_bytes(inter, a.H) + (int64_t)(fb >> 3) * f8_scale_row(a.H) * 4;
-    const int64_t row = (int64_t)min(col, T - 1) * a.H;
-    for (int b = kq; b < KB; b += KW) {
-      const uint8_t *g = gm + at + (int64_t)b * 2048, *u = um + at + (int64_t)b * 2048;
-      const F8Arg<!BF> wg(f8_op(*(const uint4*)g, *(const uint4*)(g + 1024))), wu(f8_op(*(const uint4*)u, *(const uint4*)(u + 1024)));
-      const float sg = ((const float*)(gm + sat))[b], su = ((const float*)(um + sat))[b];
-      F8Operand x;
-      x.load<BF, VEC>(a.x, row, a.H, b);
-      const F8Arg<!BF> xv(x.v);
-      f8_add(ag, f8_mfma(wg, xv), x.s * sg);
-      f8_add(au, f8_mfma(wu, xv), x.s * su);
+  const uint8_t* const row = ONE ? sm : a.xrec + min(col, T - 1) * f8_row(a.H);
+  const float* const xs = ONE ? (const float*)(sm + 128 * KB) : a.xs + (int64_t)min(col, T - 1) * f8_scale_row(a.H);
+  for (int b0 = kq; b0 < KB; b0 += 2 * KW) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int b = b0 + i * KW;
+      if (b >= KB) break;
+      const F8Arg<!BF> wg(f8_op(ring[i][0][0], ring[i][0][1])), wu(f8_op(ring[i][1][0], ring[i][1][1]));
+      const F8Arg<!BF> x(f8_operand(row, b));
+      const float s = xs[b], sg = s * rs[i][0], su = s * rs[i][1];
+      fetch(i, b + 2 * KW);
+      f8_add(ag, f8_mfma(wg, x), sg);
+      f8_add(au, f8_mfma(wu, x), su);
     }
   }
 #pragma unroll
@@ -644,31 +915,50 @@ __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
 // most chosen experts of a call (one token: its entries), and the shared one
 static int f8_few_slots(const F8Args& a) { return (a.T == 1 ? a.k : std::min(a.T * a.k, a.E)) + (a.Is > 0 ? 1 : 0); }
 
-// Down and combine of one token. Workgroup: 16 outputs; its 16 waves take the units (entry,
-// block of K) in turn, weigh each product in f32, and add up in LDS.
+// Down and combine of one token. Workgroup: 16 outputs; its 16 waves take the entries in turn, 4 blocks
+// of K together, half a wave quantises a block of h, each product is weighed in f32, and the waves
+// add up in LDS.
 template <bool WIDE>
 __global__ __launch_bounds__(1024) void k_f8_one_down(F8Args a) {
   __shared__ float red[16][16];
-  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), nb = blockIdx.x;
-  const int k = a.k, KB = f8_blocks(a.I), KS = a.Is ? f8_blocks(a.Is) : 0;
+  __shared__ __align__(16) uint8_t hq[16][4 * 128];
+  __shared__ float hs[16][4];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), nb = blockIdx.x, k = a.k;
   f8_v4f acc = f8_zero4();
-  for (int u = wave; u < k * KB + KS; u += 16) {
-    const bool sh = u >= k * KB;
-    const int j = sh ? k : u / KB, b = sh ? u - k * KB : u % KB;
-    int e = a.E;
+  for (int j = wave; j < k + (a.Is > 0 ? 1 : 0); j += 16) {
+    const bool sh = j == k;
+    int e = 0;
     if (!sh) e = __builtin_amdgcn_readfirstlane(a.idx[j]);
-    if (!sh && (unsigned)e >= (unsigned)a.E) continue;
+    if ((unsigned)e >= (unsigned)a.E) continue;
     const float wt = sh ? a.shared_w[0] : a.w[j];
-    const int inter = sh ? a.Is : a.I, kb = sh ? KS : KB;
+    const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter);
     const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
-    const uint8_t* w = mat + ((int64_t)nb * kb + b) * 2048 + lane * 16;
-    const F8Arg<WIDE> wv(f8_op(*(const uint4*)w, *(const uint4*)(w + 1024)));
-    const float sw = ((const float*)(mat + f8_code_bytes(a.H, inter)))[(int64_t)(nb >> 3) * f8_scale_row(inter) + b];
-    F8Operand h;
-    h.load<false, true>(a.hf, (int64_t)(sh ? a.F : j) * a.hcols, inter, b);
-    f8_v4f d = f8_zero4();
-    f8_add(d, f8_mfma(wv, F8Arg<WIDE>(h.v)), h.s * sw);
-    f8_add(acc, d, wt);
+    const uint8_t* w = mat + (int64_t)nb * KB * 2048 + lane * 16;
+    const float* ws = (const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)(nb >> 3) * f8_scale_row(inter);
+    const int64_t row = (int64_t)(sh ? a.F : j) * a.hcols;
+    for (int b0 = 0; b0 < KB; b0 += 4) {
+      uint4 wq[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {   // past the last: the last again
+        const uint8_t* p = w + min(b0 + i, KB - 1) * 2048;
+        wq[i][0] = *(const uint4*)p;
+        wq[i][1] = *(const uint4*)(p + 1024);
+      }
+      const float4 sw = *(const float4*)(ws + b0);
+#pragma unroll 1
+      for (int i = lane >> 5; i < 4; i += 2)
+        if (b0 + i < KB) f8_block_to_lds<false, true>(a.hf, row, inter, b0 + i, true, hq[wave] + 128 * i, &hs[wave][i]);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (b0 + i >= KB) break;
+        const float s = hs[wave][i] * (i == 0 ? sw.x : i == 1 ? sw.y : i == 2 ? sw.z : sw.w);
+        f8_add(acc, f8_mfma(F8Arg<WIDE>(f8_op(wq[i][0], wq[i][1])), F8Arg<WIDE>(f8_operand(hq[wave], i))), s * wt);
+      }
+      __builtin_amdgcn_wave_barrier();   // read before the next blocks are written
+    }
   }
   if ((lane & 15) == 0) {
 #pragma unroll
@@ -684,33 +974,59 @@ __global__ __launch_bounds__(1024) void k_f8_one_down(F8Args a) {
 }
 
 // Outputs of the experts for 2 to 16 tokens, unweighted and in f32, in the row of the token's
-// first entry with the expert. Workgroup: a chosen expert (slot) and 128 outputs, 32 a wave.
+// first entry with the expert. Workgroup: a chosen expert (slot) and 128 outputs, 32 a wave; 4 blocks of
+// h at a time, quantised into LDS.
 template <bool WIDE>
 __global__ __launch_bounds__(256) void k_f8_few_down(F8Args a) {
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = 8 * blockIdx.x + 2 * wave;
+  constexpr int PITCH = 4 * 128 + 16;
+  __shared__ __align__(16) uint8_t hq[16 * PITCH];
+  __shared__ float hs[16][4];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t* tab = a.few + blockIdx.y * MX_FEW_TAB;   // k_f8_few_gate_up's
   const int e = tab[32], row = tab[lane & 15];
-  if (e < 0 || 16 * n0 >= a.H) return;
+  if (e < 0) return;
   const bool sh = e == a.E;
-  const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter);
+  const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter), NT = a.H / 16;
+  const int n0 = min(8 * (int)blockIdx.x + 2 * wave, NT - 2);   // past the last: computed, not stored
   const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
   const uint8_t* w = mat + (int64_t)n0 * KB * 2048 + lane * 16;
   const float* ws = (const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)(n0 >> 3) * f8_scale_row(inter);
   f8_v4f acc[2] = {f8_zero4(), f8_zero4()};
-  for (int b = 0; b < KB; b++) {
-    F8Arg<WIDE> wv[2];
+  const unsigned long long rows = __ballot(row >= 0) & 0xffffu;
+  for (int b0 = 0; b0 < KB; b0 += 4) {
+    uint4 wq[4][2][2];
+    float sw[4];
 #pragma unroll
-    for (int m = 0; m < 2; m++) {
-      const uint8_t* p = w + ((int64_t)m * KB + b) * 2048;
-      wv[m] = F8Arg<WIDE>(f8_op(*(const uint4*)p, *(const uint4*)(p + 1024)));
+    for (int i = 0; i < 4; i++) {
+      const int b = min(b0 + i, KB - 1);
+      sw[i] = ws[b];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        const uint8_t* p = w + ((int64_t)m * KB + b) * 2048;
+        wq[i][m][0] = *(const uint4*)p;
+        wq[i][m][1] = *(const uint4*)(p + 1024);
+      }
     }
-    F8Operand h;   // columns without a row read row 0 and are not stored
-    h.load<false, true>(a.hf, (int64_t)max(row, 0) * a.hcols, inter, b);
-    const F8Arg<WIDE> hv(h.v);
+    if (b0 > 0) lds_barrier();   // the blocks before have been read
+    int c = -1;
+    for (unsigned long long left = rows; left; left &= left - 1) {   // half a wave a block of a row
+      c = __ffsll(left) - 1;
+      const int i = (wave & 1) * 2 + (lane >> 5), r = __shfl(row, c, 64);
+      if ((__popcll(rows & ((1ull << c) - 1)) & 1) == (wave >> 1) && b0 + i < KB)
+        f8_block_to_lds<false, true>(a.hf, (int64_t)r * a.hcols, inter, b0 + i, true, hq + c * PITCH + 128 * i, &hs[c][i]);
+    }
+    lds_barrier();
+    const int mine = row >= 0 ? lane & 15 : c;   // a column without a row: any
 #pragma unroll
-    for (int m = 0; m < 2; m++) f8_add(acc[m], f8_mfma(wv[m], hv), h.s * ws[b]);
+    for (int i = 0; i < 4; i++) {
+      if (b0 + i >= KB) break;
+      const F8Arg<WIDE> h(f8_operand(hq + mine * PITCH, i));
+      const float s = hs[mine][i] * sw[i];
+#pragma unroll
+      for (int m = 0; m < 2; m++) f8_add(acc[m], f8_mfma(F8Arg<WIDE>(f8_op(wq[i][m][0], wq[i][m][1])), h), s);
+    }
   }
-  if (row < 0) return;
+  if (row < 0 || 8 * (int)blockIdx.x + 2 * wave >= NT) return;
 #pragma unroll
   for (int m = 0; m < 2; m++)
     *(float4*)((float*)a.obuf + (int64_t)row * a.H + 16 * (n0 + m) + 4 * (lane >> 4)) =
@@ -719,21 +1035,20 @@ __global__ __launch_bounds__(256) void k_f8_few_down(F8Args a) {
 
 bool f8_few(int T) { return T <= F8_FEW_T; }
 
-template <bool BF, bool VEC>
-static void f8_few_gate_up(const F8Args& a, hipStream_t s) {
+template <bool BF>
+static hipError_t f8_few_gate_up(const F8Args& a, hipStream_t s) {
   const int slots = f8_few_slots(a), groups = (std::max(a.I, a.Is) + 15) / 16;
-  if (a.T == 1) hx_launch(k_f8_few_gate_up<BF, VEC, 8, true>, dim3(groups, slots), dim3(512), 0, s, a);
-  else if (slots * groups >= 1200) hx_launch(k_f8_few_gate_up<BF, VEC, 2, false>, dim3((groups + 3) / 4, slots), dim3(512), 0, s, a);
-  else hx_launch(k_f8_few_gate_up<BF, VEC, 8, false>, dim3(groups, slots), dim3(512), 0, s, a);
+  if (a.T == 1) {
+    hx_launch(k_f8_few_gate_up<BF, 8, true>, dim3(groups, slots), dim3(512), (uint32_t)f8_blocks(a.H) * 132, s, a);
+    return hipGetLastError();
+  }
+  if (slots * groups >= 1200) hx_launch(k_f8_few_gate_up<BF, 2, false>, dim3((groups + 3) / 4, slots), dim3(512), 0, s, a);
+  else hx_launch(k_f8_few_gate_up<BF, 8, false>, dim3(groups, slots), dim3(512), 0, s, a);
+  return hipGetLastError();
 }
 
 hipError_t launch_f8_few_gate_up(const F8Args& a, hipStream_t s) {
-  const bool vec = a.H % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
-  if (a.xbf && vec) f8_few_gate_up<true, true>(a, s);
-  else if (a.xbf) f8_few_gate_up<true, false>(a, s);
-  else if (vec) f8_few_gate_up<false, true>(a, s);
-  else f8_few_gate_up<false, false>(a, s);
-  return hipGetLastError();
+  return a.xbf ? f8_few_gate_up<true>(a, s) : f8_few_gate_up<false>(a, s);
 }
 
 template <bool WIDE>
@@ -772,7 +1087,15 @@ hipError_t launch_f8_prep(const F8Args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-int f8_tile_m(int64_t F, int E, bool xbf) { return F <= 12 * (int64_t)E ? 16 : !xbf || F <= 28 * (int64_t)E ? 32 : 64; }
+// Rows of a tile: F entries over all E experts, so that padding and experts without rows count too
+// (the routing is on the device). us for 512 experts of 512 x 2048, 10 chosen, with tiles of 16, 32, 64, 128: 17
+// tokens 113, 114, 120, -; 64 tokens 241, 223, 222, -; 800 (16 rows an expert) 367, 317, 330, -; 1024 (20) 403, 335,
+// 333, -; 2048 (40) -, -, 382, 425; 3000 (59, skewed) -, -, 466, 459; 4096 (80) -, -, 577, 496. Tiles of 128 have
+// kernels of their own, which find a token's codes by 32 bits; f32 results' operands leave room for 32.
+int f8_tile_m(int64_t T, int64_t F, int E, int H, bool xbf) {
+  if (!xbf || F <= 18 * (int64_t)E) return 32;
+  return F <= 56 * (int64_t)E || T * f8_row(H) >= (int64_t)1 << 32 ? 64 : 128;
+}
 
 // h = q(silu(G x) * (U x)). Workgroup: a tile of TM rows and 128 features, a block of h's
 // columns: 32 a wave, gate and up of a feature in the same lane.
@@ -827,7 +1150,7 @@ __global__ __launch_bounds__(256, 2) void k_f8_gate_up(F8Args a) {
     float s;
     const bool fine = f8_scale(max(max(amax[0][r], amax[1][r]), max(amax[2][r], amax[3][r])), s);
     uint32_t c[2];
-    f8_codes(h[t], s, fine, c);
+    f8_codes_near(h[t], s, fine, c);
     if (r >= rows) continue;
     uint32_t* o = (uint32_t*)(a.hrec + ((int64_t)(p0 + r) * a.hblocks + nt) * 128 + 32 * wave + 4 * (lane >> 4));
     o[0] = c[0];
@@ -836,8 +1159,46 @@ __global__ __launch_bounds__(256, 2) void k_f8_gate_up(F8Args a) {
   }
 }
 
-// Outputs of the experts, unweighted: D h, in the activations' type. Workgroup: a tile of TM
-// rows and 256 outputs, 64 a wave.
+// A wave's outputs of 64 features from tile n0 for rows p0 .. of obuf: f16 with a scale, a power of
+// two that gives the largest finite magnitude of a row's 64 the exponent 2^14 (infinities and
+// NaN stay what they are)
+template <int NM, int TT>
+HX_DEV void f8_out_rows(const F8Args& a, const f8_v4f (&acc)[NM][TT], uint8_t* tl, int64_t p0, int rows, int n0) {
+  static_assert(NM == 4, "64 outputs have a scale");
+  typedef F8Out<32 * NM> Out;
+  const int lane = lane_id(), tiles = a.H / 16;
+#pragma unroll
+  for (int t = 0; t < TT; t++) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int m = 0; m < NM; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t u = __float_as_uint(acc[m][t][i]) & 0x7fffffffu;
+        top = max(top, n0 + m < tiles && u < 0x7f800000u ? u : 0u);
+      }
+    const int ex = max((int)(f8_max_of_4(top) >> 23), 15), r = 16 * t + (lane & 15);
+    const float up = __uint_as_float((uint32_t)(268 - ex) << 23);
+#pragma unroll
+    for (int m = 0; m < NM; m++) {
+      uint32_t h[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const _Float16 lo = (_Float16)(acc[m][t][2 * i] * up), hi = (_Float16)(acc[m][t][2 * i + 1] * up);
+        h[i] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+      }
+      *(uint2*)(tl + r * Out::PITCH + 32 * m + 8 * (lane >> 4)) = make_uint2(h[0], h[1]);
+    }
+    if (lane < 16 && r < rows && n0 < tiles)
+      a.oscale[(p0 + r) * ((a.H + 63) / 64) + (n0 >> 2)] = __uint_as_float((uint32_t)(ex - 14) << 23);
+  }
+  Out::store(tl, min(rows, 16 * TT), 2 * (a.H - 16 * n0), [&](int r) { return (uint8_t*)a.obuf + ((p0 + r) * a.H + 16 * n0) * 2; });
+}
+
+// Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 outputs, 64 a
+// wave. bf16 activations: 64 outputs of a row leave as f16 of a scale of their own, 2^-12 of a value at
+// most for half of the bytes that float32 takes here and in the combine (bf16, 2^-9, would be half
+// of the result's own error on top of it).
 template <int TM, bool WIDE>
 __global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
   constexpr int TT = TM / 16, NM = 4;
@@ -848,7 +1209,7 @@ __global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
   const int4 ti = ((const int4*)a.tiles)[tile];
   const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
   const bool sh = e == a.E;
-  const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter), NT = a.H / 16;
+  const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter), tiles = a.H / 16;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = (4 * nt + wave) * NM;
   F8Tile<TM> rw;
   rw.init(wave, [&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * 128; });
@@ -858,39 +1219,137 @@ __global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
   const uint8_t* mat = sh ? a.sdown.base : a.down.mat(e);
   const uint8_t* w[NM];
 #pragma unroll
-  for (int m = 0; m < NM; m++) w[m] = mat + (int64_t)min(n0 + m, NT - 1) * KB * 2048 + lane * 16;   // past the last: not stored
-  const float* const ws[1] = {(const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)(min(n0, NT - 1) >> 3) * f8_scale_row(inter)};
+  for (int m = 0; m < NM; m++) w[m] = mat + (int64_t)min(n0 + m, tiles - 1) * KB * 2048 + lane * 16;   // past the last: not stored
+  const float* const ws[1] = {(const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)(min(n0, tiles - 1) >> 3) * f8_scale_row(inter)};
   f8_v4f acc[NM][TT];
   f8_products<WIDE, TM, NM, 1>(w, ws, rw, xs, wave, buf, KB, acc);
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+      const int r = 16 * t + (lane & 15);
+      if (r >= rows) continue;
+#pragma unroll
+      for (int m = 0; m < NM; m++) {
+        if (n0 + m >= tiles) continue;
+        const f8_v4f& v = acc[m][t];
+        *(float4*)((float*)a.obuf + (int64_t)(p0 + r) * a.H + 16 * (n0 + m) + 4 * (lane >> 4)) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    }
+  } else {
+    static_assert(4 * TM * F8Out<32 * NM>::PITCH <= 2 * F8Tile<TM>::BYTES, "the rows' place holds the results");
+    lds_barrier();   // the rows have been read
+    f8_out_rows<NM, TT>(a, acc, buf + wave * (TM * F8Out<32 * NM>::PITCH), p0, rows, n0);
+  }
+}
+
+// The same two products where experts have many rows: both operands through LDS (F8Core), tiles of
+// 128 rows; the waves of a tile's second half bring loads only where it has 64 rows or fewer.
+__global__ __launch_bounds__(512, 2) void k_f8_gate_up_many(F8Args a) {
+  typedef F8Core<4, 4, 4, 2, 2> Core;
+  constexpr int TT = 4, TR = Core::TR, PITCH = 128 + 16;
+  static_assert(TR * PITCH <= Core::BYTES, "the stages' place holds the results");
+  __shared__ __align__(16) uint8_t buf[Core::BYTES];
+  __shared__ uint32_t amax[4][TR];
+  int nt, tile;
+  mx_tile(a.hblocks, a.counts[0], nt, tile);
+  if (tile < 0) return;
+  const int4 ti = ((const int4*)a.tiles)[tile];
+  const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I;
+  if (128 * nt >= inter) return;
+  const int lane = lane_id(), KB = f8_blocks(a.H);
+  auto token = [&](int r) {
+    const int p = p0 + min(r, rows - 1);
+    return sh ? p - a.F : a.perm[p] / a.k;
+  };
+  const uint8_t* const gm = sh ? a.sgate.base : a.gate.mat(e);
+  const uint8_t* const um = sh ? a.sup.base : a.up.mat(e);
+  const int64_t sat = f8_code_bytes(inter, a.H) + (int64_t)nt * f8_scale_row(a.H) * 4;
+  // a wave's tiles: gate, up, gate, up of its 32 features
+  const Core core(a.xrec, a.xs,
+                  [&](int i) { return (i & 1 ? um : gm) + (int64_t)min(8 * nt + (i >> 1), inter / 16 - 1) * KB * 2048; },
+                  [&](int r) { return (uint32_t)(token(r) * (uint32_t)f8_row(a.H)); },
+                  [&](int r) { return (uint32_t)(token(r) * (uint32_t)f8_scale_row(a.H) * 4); },
+                  [&](int i) { return (const float*)((i & 1 ? um : gm) + sat); });
+  f8_v4f acc[4][TT];
+  const int r0 = core.wr * 64;   // the wave's first row
+  const bool work = r0 < rows;
+  core.run<false, 2>(KB, buf, work, acc);
+  const bool in = 128 * nt + 32 * core.wf < inter;   // features behind the last are zeros
+  float h[TT][8];
 #pragma unroll
   for (int t = 0; t < TT; t++) {
-    const int r = 16 * t + (lane & 15);
-    if (r >= rows) continue;
 #pragma unroll
-    for (int m = 0; m < NM; m++) {
-      if (n0 + m >= NT) continue;
-      const int64_t at = (int64_t)(p0 + r) * a.H + 16 * (n0 + m) + 4 * (lane >> 4);
-      const f8_v4f& v = acc[m][t];
-      if (!WIDE) *(uint2*)((uint16_t*)a.obuf + at) = make_uint2(f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
-                                                                f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
-      else *(float4*)((float*)a.obuf + at) = make_float4(v[0], v[1], v[2], v[3]);
+    for (int i = 0; i < 8; i++) {
+      const int m = 2 * (i >> 2);
+      h[t][i] = in ? silu_rcp(acc[m][t][i & 3]) * acc[m + 1][t][i & 3] : 0.f;
+    }
+    const uint32_t m = f8_max_of_4(f8_amax(h[t]));
+    if (lane < 16) amax[core.wf][r0 + 16 * t + lane] = m;
+  }
+  lds_barrier();   // the last stage has been read, too
+  if (work) {
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+      const int r = r0 + 16 * t + (lane & 15);
+      float s;
+      const bool fine = f8_scale(max(max(amax[0][r], amax[1][r]), max(amax[2][r], amax[3][r])), s);
+      uint32_t c[2];
+      f8_codes_near(h[t], s, fine, c);
+      uint8_t* const o = buf + r * PITCH + 32 * core.wf + 4 * (lane >> 4);
+      *(uint32_t*)o = c[0];
+      *(uint32_t*)(o + 16) = c[1];
+      if (core.wf == 0 && lane < 16 && r < rows) a.hs[(int64_t)(p0 + r) * a.hscale + nt] = s;
     }
   }
+  lds_barrier();
+  for (int i = threadIdx.x; i < rows * 8; i += 512)
+    *(uint4*)(a.hrec + ((int64_t)(p0 + (i >> 3)) * a.hblocks + nt) * 128 + (i & 7) * 16) = *(const uint4*)(buf + (i >> 3) * PITCH + (i & 7) * 16);
+}
+
+__global__ __launch_bounds__(256, 2) void k_f8_down_many(F8Args a) {
+  typedef F8Core<4, 4, 2, 2, 2> Core;
+  __shared__ __align__(16) uint8_t buf[Core::BYTES];
+  int nt, tile;
+  mx_tile((a.H + 127) / 128, a.counts[0], nt, tile);
+  if (tile < 0) return;
+  const int4 ti = ((const int4*)a.tiles)[tile];
+  const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
+  const bool sh = e == a.E;
+  const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter), tiles = a.H / 16;
+  const uint8_t* const mat = sh ? a.sdown.base : a.down.mat(e);
+  const float* const ws = (const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)nt * f8_scale_row(inter);
+  const Core core(a.hrec + (int64_t)p0 * a.hblocks * 128, a.hs + (int64_t)p0 * a.hscale,
+                  [&](int i) { return mat + (int64_t)min(8 * nt + i, tiles - 1) * KB * 2048; },
+                  [&](int r) { return (uint32_t)(min(r, rows - 1) * a.hblocks * 128); },
+                  [&](int r) { return (uint32_t)(min(r, rows - 1) * a.hscale * 4); }, [&](int) { return ws; });
+  f8_v4f acc[4][4];
+  const int r0 = core.wr * 64;
+  core.run<false, 1>(KB, buf, r0 < rows, acc);
+  lds_barrier();   // the last stage has been read
+  f8_out_rows<4, 4>(a, acc, buf + core.wave * (64 * F8Out<128>::PITCH), p0 + r0, rows - r0, 8 * nt + 4 * core.wf);
 }
 
 #define F8_LAUNCH(KERNEL, NX)                                                                  \
   const dim3 g((unsigned)((int64_t)(NX) * ((a.max_tiles + 7) / 8 * 8)));                       \
-  if (a.xbf && a.tile_m == 16) hx_launch(KERNEL<16, false>, g, dim3(256), 0, s, a);            \
-  else if (a.xbf && a.tile_m == 32) hx_launch(KERNEL<32, false>, g, dim3(256), 0, s, a);       \
-  else if (a.xbf) hx_launch(KERNEL<64, false>, g, dim3(256), 0, s, a);                         \
-  else if (a.tile_m == 16) hx_launch(KERNEL<16, true>, g, dim3(256), 0, s, a);                 \
-  else hx_launch(KERNEL<32, true>, g, dim3(256), 0, s, a)
+  if (!a.xbf) hx_launch(KERNEL<32, true>, g, dim3(256), 0, s, a);                              \
+  else if (a.tile_m == 32) hx_launch(KERNEL<32, false>, g, dim3(256), 0, s, a);                \
+  else hx_launch(KERNEL<64, false>, g, dim3(256), 0, s, a)
 
 hipError_t launch_f8_gate_up(const F8Args& a, hipStream_t s) {
+  if (a.tile_m == 128) {
+    hx_launch(k_f8_gate_up_many, dim3((unsigned)((int64_t)a.hblocks * ((a.max_tiles + 7) / 8 * 8))), dim3(512), 0, s, a);
+    return hipGetLastError();
+  }
   F8_LAUNCH(k_f8_gate_up, a.hblocks);
   return hipGetLastError();
 }
 hipError_t launch_f8_down(const F8Args& a, hipStream_t s) {
+  if (a.tile_m == 128) {
+    hx_launch(k_f8_down_many, dim3((unsigned)((int64_t)((a.H + 127) / 128) * ((a.max_tiles + 7) / 8 * 8))), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
   F8_LAUNCH(k_f8_down, (a.H + 255) / 256);
   return hipGetLastError();
 }

@@ -95,7 +95,7 @@ extern "C" int hx_linear_create(int64_t out_features, int64_t in_features, const
 // what a call of M rows keeps: the quantised rows, where the kernel does not quantise by itself
 static size_t linear_codes(const hx_linear* l, int64_t M) { return ((size_t)(M * f8_row(l->K)) + 255) & ~(size_t)255; }
 static size_t linear_ws(const hx_linear* l, int64_t M) {
-  return M <= F8_QUANT_ROWS ? 0 : linear_codes(l, M) + sizeof(float) * (size_t)M * f8_scale_row(l->K);
+  return f8_quant_inside(M, l->K) ? 0 : linear_codes(l, M) + sizeof(float) * (size_t)M * f8_scale_row(l->K);
 }
 
 extern "C" int hx_linear_workspace_size(const hx_linear* l, int64_t n_rows, size_t* bytes) {

@@ -129,7 +129,7 @@ static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 struct WsLayout {
   size_t logits, topk_idx, topk_w, sgw, perm, inv, offsets, slots, tiles, counts, plan, dmap, hbuf, hbf, xh, xq, xq32, xcv,
       hrec, obuf, xn, ym, dpart, wpos, mx_xrec, mx_hrec, mx_few, mx_perm, mx_inv, mx_hist, mx_tiles, mx_counts, f8_xs,
-      f8_hs, f8_hf, total;
+      f8_hs, f8_hf, f8_os, total;
   int hstride, max_slots, max_tiles;
 };
 
@@ -219,20 +219,21 @@ static WsLayout ws_layout(const hx_moe* m, int64_t T) {
     const int inter = f8_inter(m);
     L.xn = take(act * T * H);
     L.ym = take(act * T * H);
+    L.mx_xrec = take((size_t)T * f8_row(H));
+    L.f8_xs = take(sizeof(float) * (size_t)T * f8_scale_row(H));
     if (T <= F8_FEW_T) {
       L.f8_hf = take(sizeof(float) * (size_t)(F + T) * inter);
       L.obuf = take(sizeof(float) * (size_t)(F + T) * H);
       L.mx_few = take(sizeof(int32_t) * MX_FEW_TAB * (size_t)L.max_slots);
     } else {
-      L.mx_xrec = take((size_t)T * f8_row(H));
-      L.f8_xs = take(sizeof(float) * (size_t)T * f8_scale_row(H));
       L.mx_hrec = take((size_t)(F + T) * f8_row(inter));
       L.f8_hs = take(sizeof(float) * (size_t)(F + T) * f8_scale_row(inter));
       L.obuf = take(act * (size_t)(F + T) * H);
+      L.f8_os = act == 2 ? take(sizeof(float) * (size_t)(F + T) * ((H + 63) / 64)) : 0;
       L.mx_perm = take(sizeof(int32_t) * F);
       L.mx_inv = take(sizeof(int32_t) * F);
       L.mx_hist = take(sizeof(int32_t) * (size_t)std::min<int64_t>((F + MX_CHUNK - 1) / MX_CHUNK, MX_MAX_CHUNKS) * E);
-      L.mx_tiles = take(sizeof(int32_t) * 4 * (size_t)mx_max_tiles(m, T, 16));
+      L.mx_tiles = take(sizeof(int32_t) * 4 * (size_t)mx_max_tiles(m, T, 32));
       L.mx_counts = take(sizeof(int32_t) * 4);
     }
     L.total = o;
@@ -810,20 +811,26 @@ static int run_f8(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
   a.hcols = f8_inter(m);
   a.obuf = ws + L.obuf;
   a.few_rows = f8_few(a.T);
+  a.xrec = ws + L.mx_xrec;
+  a.xs = (float*)(ws + L.f8_xs);
   if (a.few_rows) {
     a.few = (int32_t*)(ws + L.mx_few);
     a.hf = (float*)(ws + L.f8_hf);
+    if (T > 1) {   // one token's gate/up kernel quantises
+      tm_ext(m, SLOT_X_F16, s);
+      HX_HIP(launch_f8_rows(x, a.xbf, T, a.H, a.xrec, a.xs, true, s));
+      tm_ext_done(m, SLOT_X_F16);
+    }
   } else {
-    a.xrec = ws + L.mx_xrec;
-    a.xs = (float*)(ws + L.f8_xs);
     a.hrec = ws + L.mx_hrec;
     a.hs = (float*)(ws + L.f8_hs);
+    a.oscale = a.xbf ? (float*)(ws + L.f8_os) : nullptr;
     a.perm = (int32_t*)(ws + L.mx_perm);
     a.inv = (int32_t*)(ws + L.mx_inv);
     a.hist = (int32_t*)(ws + L.mx_hist);
     a.tiles = (int32_t*)(ws + L.mx_tiles);
     a.counts = (int32_t*)(ws + L.mx_counts);
-    a.tile_m = f8_tile_m(a.F, a.E, a.xbf);
+    a.tile_m = f8_tile_m(T, a.F, a.E, a.H, a.xbf);
     a.max_tiles = (int)mx_max_tiles(m, T, a.tile_m);
     tm_ext(m, SLOT_X_F16, s);
     HX_HIP(launch_f8_prep(a, s));

@@ -1018,12 +1018,13 @@ HX_DEV uint4 mx_row16(const void* p) {
 // (an entry without an expert reads row 0 and counts nothing). Bound by HBM, few
 // tokens by latency (4 us). FEW: rows in f32, a
 // token's entry at that of its first with the same expert; else rows in the
-// activations' type by inv; NT: more of them than MX_CACHE, read non-temporally (8192
+// activations' type by inv, SC: in f16 with a scale for each 64; NT: more of them than MX_CACHE, read non-temporally (8192
 // tokens' 369 MB: 65 us against 78; 2048 tokens' 92 MB: 19 against 17). f32 rows of 2048 tokens:
 // 34 us.
-template <bool BF, bool FEW, bool NT>
+template <bool BF, bool FEW, bool NT, bool SC>
 __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
   constexpr bool R16 = BF && !FEW;
+  static_assert(R16 || !SC, "rows of 16 bits");
   constexpr int B = 8;
   const int lane = lane_id(), segs = (a.H + 511) / 512, k = a.k;
   const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1052,13 +1053,14 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
   for (int j0 = 0; j0 <= k; j0 += B) {
     uint4 q[B], r[B];
     int pj[B];
-    float wj[B];
+    float wj[B], sc[B];
 #pragma unroll
     for (int j = 0; j < B; j++) {
       const int jj = j0 + j;
       pj[j] = jj < k ? __builtin_amdgcn_readlane(p, jj) : jj == k ? ps : -1;
       wj[j] = jj < k ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), jj)) : ws;
       const int64_t at = (int64_t)max(pj[j], 0) * a.H + (mine ? n0 : 0);
+      if constexpr (SC) sc[j] = a.oscale[(int64_t)max(pj[j], 0) * ((a.H + 63) / 64) + ((mine ? n0 : 0) >> 6)];
       if constexpr (R16) {
         q[j] = mx_row16<NT>((const uint16_t*)a.obuf + at);
       } else {
@@ -1073,7 +1075,10 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        if constexpr (R16) {
+        if constexpr (SC) {
+          v[2 * i] = f16_to_f32((uint16_t)u[i]);
+          v[2 * i + 1] = f16_to_f32((uint16_t)(u[i] >> 16));
+        } else if constexpr (R16) {
           v[2 * i] = __uint_as_float(u[i] << 16);
           v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         } else {
@@ -1084,8 +1089,9 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
         v[4] = __uint_as_float(r[j].x); v[5] = __uint_as_float(r[j].y);
         v[6] = __uint_as_float(r[j].z); v[7] = __uint_as_float(r[j].w);
       }
+      const float wt = SC ? wj[j] * sc[j] : wj[j];
 #pragma unroll
-      for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wj[j], v[i], acc[i]);
+      for (int i = 0; i < 8; i++) acc[i] = __builtin_fmaf(wt, v[i], acc[i]);
     }
   }
   if (!mine) return;
@@ -1137,8 +1143,11 @@ hipError_t launch_mx_combine(const MxArgs& a, hipStream_t s) {
   const dim3 g((unsigned)((waves + 3) / 4));
   const int64_t rows = ((int64_t)a.F + (a.Is > 0 ? a.T : 0)) * a.H * (a.xbf ? 2 : 4);   // bytes
   const bool few = a.few_rows, nt = rows > MX_CACHE;
-#define COMBINE(BF, FEW, NT) hx_launch(k_mx_combine<BF, FEW, NT>, g, dim3(256), 0, s, a)
-  if (a.xbf) {
+#define COMBINE(BF, FEW, NT) hx_launch(k_mx_combine<BF, FEW, NT, false>, g, dim3(256), 0, s, a)
+  if (a.oscale && !few) {
+    if (nt) hx_launch(k_mx_combine<true, false, true, true>, g, dim3(256), 0, s, a);
+    else hx_launch(k_mx_combine<true, false, false, true>, g, dim3(256), 0, s, a);
+  } else if (a.xbf) {
     if (few) COMBINE(true, true, false);
     else if (nt) COMBINE(true, false, true);
     else COMBINE(true, false, false);

@@ -42,11 +42,11 @@ def reference(x, idx, coef, counts=None):
 
 
 def bounds(x, r, T, out_eps):
-    """How far a kernel in 32 bits may be off: exp of d = x - max has a relative error of |d| + 4
-    half steps (the difference's rounding, the exponential's own), a sum over a row 32 more
-    (16 columns a lane, 6 steps over lanes; products' roundings), so that p has 2 D + 72 and
-    the means, over at most 64 + T / 4096 rows in a lane's sum and 16 in the tables',
-    2 D + 160 + T / 4096. The difference f - s keeps the errors of both terms. Probabilities
+    """How far a kernel in 32 bits may be off: exp of d = x - max has a relative error of 2.3 |d| + 4
+    half steps (the difference's rounding, the product's with log2 e and the constant's, the
+    exponential's own), a sum over a row 32 more (16 columns a lane, 6 steps over lanes; products'
+    roundings), so that p has 5 D + 72 and the means, over at most 64 + T / 4096 rows in a lane's
+    sum and 16 in the tables', 5 D + 160 + T / 4096. The difference f - s keeps the errors of both terms. Probabilities
     below 2^-126 may be zero. out_eps: half a step of the gradient's type."""
     live = r["live"]
     d = 0.0
@@ -55,7 +55,7 @@ def bounds(x, r, T, out_eps):
         xl = np.where(np.isneginf(xl), xl.max(axis=1, keepdims=True), xl)
         d = min(104.0, float((xl.max(axis=1, keepdims=True) - xl).max()))   # exp(-104) is below float32's smallest
     tiny = 2.0 ** -126
-    row, mean = (2 * d + 80) * U, (2 * d + 160 + T / 4096) * U
+    row, mean = (5 * d + 80) * U, (5 * d + 160 + T / 4096) * U
     grad = row * r["scale"] * r["p"] * (np.abs(r["f"]) + np.abs(r["s"])[:, None]) + out_eps * np.abs(r["dlogits"])
     return dict(loss=mean * abs(r["loss"]) + tiny, probs=mean * r["probs"] + tiny,
                 dlogits=(grad * (1 + 2.0 ** -6) + tiny * (1 + r["scale"] * (r["f"].max(initial=0) + 1))) * live[:, None])

@@ -269,3 +269,42 @@ def test_a_model_is_quantised_routed_run_and_balanced():
     layer = hx.F8Linear.load(*hx.quantize_f8(draw(192, H), block_rows=128))
     assert layer(y).shape == (T, 192)
     blk.close(), ref.close(), layer.close()
+
+
+@pytest.mark.parametrize("T,E,k,skew", [(90, 4, 3, 0), (250, 3, 3, 0), (333, 6, 4, 3), (129, 1, 1, 0), (700, 5, 2, 3)])
+def test_many_rows_an_expert(T, E, k, skew):
+    """tiles of 128 rows: their halves full, in part and empty, sizes that are no whole blocks, the same
+    token twice with an expert, padded tokens"""
+    for H, I, Is in ((256, 128, 128), (160, 96, 64), (544, 416, 0), (128, 32, 288)):
+        d = F.block(T + H, H, E, I, Is)
+        blk = F.load(d, H, E, k, I, Is, BF16)
+        print("case", T, E, k, H, I, Is, flush=True)
+        x = acts(T, T, H, BF16)
+        idx, w, sw = F.routing(T, T, E, k, padded=T // 7)
+        rng = np.random.default_rng(T)
+        if skew:
+            idx = np.where((rng.random(idx.shape) < 0.5) & (idx >= 0), 0, idx).astype(np.int32)
+        check(blk.experts(cuda(x, True), cuda(idx), cuda(w), shared_w=cuda(sw) if Is else None), x, idx, w, d, sw if Is else None, BF16)
+        x[1, 3] = np.nan
+        y = blk.experts(cuda(x, True), cuda(idx), cuda(w), shared_w=cuda(sw) if Is else None)
+        import torch
+        assert torch.isnan(y[1]).all() and torch.isfinite(y[2:]).all() and torch.isfinite(y[0]).all()
+        blk.close()
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 9000, 260), (1100, 4100, 130), (5000, 3300, 100), (257, 16640, 384)])
+def test_a_layers_large_tiles(M, N, K):
+    """rows and features that fill tiles of 256 and 128 in part"""
+    import helexa_amd as hx
+    import torch
+    codes, scales = F.make_weights(M, N, K)
+    x = F.bf16(np.random.default_rng(M).standard_normal((M, K)).astype(np.float32))
+    y = hx.F8Linear.load(cuda(codes), cuda(scales))(cuda(x, True))
+    rows = np.unique(np.concatenate([np.arange(3), np.arange(M - 3, M), np.random.default_rng(1).integers(0, M, 40)]))
+    ref, mag, fixed = F.linear(x[rows], codes, scales)
+    bound = (F.sum_steps(K) * F.U * mag + fixed) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(ref) + 2.0 ** -140
+    off = np.abs(y[torch.from_numpy(rows).cuda()].float().cpu().numpy().astype(np.float64) - ref)
+    assert (off <= bound).all()
+    # every element, against the same product in bf16 operands and float32 sums by another path of the layer
+    z = hx.F8Linear.load(cuda(codes), cuda(scales))(cuda(x, True), out_dtype=torch.float32)
+    assert (y.float() - z).norm() <= 2.0 ** -8 * z.norm() and ((y.float() - z).abs() <= 2.0 ** -7 * z.abs() + 2.0 ** -7 * z.std()).all()
