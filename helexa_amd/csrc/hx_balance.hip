@@ -33,10 +33,10 @@ struct BalArgs {
 };
 
 // tokens a workgroup of the counts takes, and their most
-constexpr int BAL_CHUNK = 1024, BAL_MAX_G1 = 64, BAL_MAX_G2 = 2048;
+constexpr int BAL_CHUNK = 1024, BAL_MAX_G1 = 64, BAL_MAX_G2 = 1024;
 static int bal_g1(int64_t T) { return (int)std::min<int64_t>((T + BAL_CHUNK - 1) / BAL_CHUNK, BAL_MAX_G1); }
 // the most of the row pass: a wave has two turns at least
-static int bal_g2(int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t>((T + 7) / 8, BAL_MAX_G2)); }
+static int bal_g2(int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t>((T + 15) / 16, BAL_MAX_G2)); }
 
 // hist[0 .. E - 1] += the entries by expert of tokens t0 .. t1 - 1, hist[E] += the live ones
 HX_DEV void bal_count(const BalArgs& a, int64_t t0, int64_t t1, int* hist) {
@@ -136,11 +136,12 @@ HX_DEV void bal_store(void* base, int64_t at, const float (&f)[V]) {
 }
 
 // The row pass: lpr lanes a row (64 / lpr rows a wave at a time), lane j of a row its
-// columns (i lpr + j) V .. + V - 1 for i < NJ. ONE: one workgroup does it all, counts and
-// last sums included.
-template <bool BF, int V, int NJ, bool ONE>
-__global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
-  constexpr int NW = ONE ? 16 : 4, NT = 64 * NW;
+// columns (i lpr + j) V .. + V - 1 for i < NJ. WHOLE: lpr is 64. ONE: one workgroup does it all, counts
+// and last sums included. Bound by HBM and the vector instructions together (about 16 an element):
+// 196608 rows of 512 in bf16, 411 MB, 3.9 TB/s.
+template <bool BF, int V, int NJ, bool WHOLE, bool ONE>
+__global__ __launch_bounds__(ONE ? 1024 : 512) void k_bal_rows(BalArgs a) {
+  constexpr int NW = ONE ? 16 : 8, NT = 64 * NW;
   extern __shared__ __align__(16) float sm[];
   float* const f_of = sm;                         // [E] f
   float* const sums = sm + a.E;                   // [NW][E + 1] the waves' sums
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
     f_of[e] = total > 0.0 ? (float)((double)k * c / total) : 0.f;
   }
   __syncthreads();
-  const int lpr = a.lpr, rpw = 64 / lpr, sub = lane & (lpr - 1), grp = lane / lpr;
+  const int lpr = WHOLE ? 64 : a.lpr, rpw = 64 / lpr, sub = lane & (lpr - 1), grp = lane / lpr;
   float f[NJ][V], sum[NJ][V];
 #pragma unroll
   for (int i = 0; i < NJ; i++)
@@ -195,8 +196,12 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
       if (row && c < E) next[i].load(a.logits, t * E + c);
       else next[i].none();
     }
-    next_mine = false;
-    for (int j = sub; row && j < k; j += lpr) next_mine |= (unsigned)a.idx[t * k + j] < (unsigned)E;
+    if (WHOLE) {   // at most 64 entries
+      next_mine = lane < k && (unsigned)a.idx[t * k + lane] < (unsigned)E;
+    } else {
+      next_mine = false;
+      for (int j = sub; row && j < k; j += lpr) next_mine |= (unsigned)a.idx[t * k + j] < (unsigned)E;
+    }
   };
   int64_t t0 = ((int64_t)blockIdx.x * NW + wave) * rpw;
   if (t0 < a.T) fetch(t0 + grp);
@@ -210,7 +215,15 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
       for (int v = 0; v < V; v++) x[i][v] = next[i].value(v);
     const unsigned long long any = __ballot(next_mine);
     if (t0 + step < a.T) fetch(t0 + step + grp);
-    const bool live = lpr == 64 ? any != 0 : ((any >> (grp * lpr)) & ((1ull << lpr) - 1)) != 0;
+    const bool live = WHOLE ? any != 0 : ((any >> (grp * lpr)) & ((1ull << lpr) - 1)) != 0;
+    // a row that is not live, whatever it holds, adds nothing and has no gradient
+    if (WHOLE && !live) {
+      const float none[V] = {};
+#pragma unroll
+      for (int i = 0; i < NJ; i++)
+        if (a.dlogits && (i * 64 + lane) * V < E) bal_store<BF, V>(a.dlogits, t * E + (i * 64 + lane) * V, none);
+      continue;
+    }
     float m = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < NJ; i++)
@@ -223,9 +236,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
     for (int i = 0; i < NJ; i++)
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const bool in = (i * lpr + sub) * V < E;
-        const float e = __builtin_amdgcn_exp2f((x[i][v] - m) * 1.44269502e+00f);
-        x[i][v] = in ? e : 0.f;   // a row of -inf alone has m = -inf: NaN behind its end too
+        x[i][v] = __builtin_amdgcn_exp2f((x[i][v] - m) * 1.44269502e+00f);
         z += x[i][v];
         s = __builtin_fmaf(f[i][v], x[i][v], s);
       }
@@ -233,8 +244,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
     s = bal_row_sum(s, lpr);
     const float r = 1.f / z;
     s *= r;
-    // a row that is not live, whatever it holds, adds nothing
-    if (live) s_sum += s;
+    if (WHOLE || live) s_sum += s;
     const float ss = scale * s;
 #pragma unroll
     for (int i = 0; i < NJ; i++) {
@@ -242,10 +252,10 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_bal_rows(BalArgs a) {
       float g[V];
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const float p = live ? x[i][v] * r : 0.f;
+        const float p = WHOLE || live ? x[i][v] * r : 0.f;
         sum[i][v] += p;
         const float d = p * __builtin_fmaf(f[i][v], scale, -ss);
-        g[v] = live ? d : 0.f;
+        g[v] = WHOLE || live ? d : 0.f;
       }
       if (row && a.dlogits && c < E) bal_store<BF, V>(a.dlogits, t * E + c, g);
     }
@@ -308,8 +318,15 @@ static uint32_t bal_lds(int E, int waves) { return (uint32_t)((E + (waves + 1) *
 
 template <bool BF, int V, int NJ>
 static void launch_rows(const BalArgs& a, bool one, hipStream_t s) {
-  if (one) hx_launch(k_bal_rows<BF, V, NJ, true>, dim3(1), dim3(1024), bal_lds(a.E, 16), s, a);
-  else hx_launch(k_bal_rows<BF, V, NJ, false>, dim3(a.G2), dim3(256), bal_lds(a.E, 4), s, a);
+  const dim3 g(one ? 1 : a.G2), b(one ? 1024 : 512);
+  const uint32_t lds = bal_lds(a.E, one ? 16 : 8);
+  if (a.lpr == 64) {
+    if (one) hx_launch(k_bal_rows<BF, V, NJ, true, true>, g, b, lds, s, a);
+    else hx_launch(k_bal_rows<BF, V, NJ, true, false>, g, b, lds, s, a);
+  } else if constexpr (NJ == 1) {   // rows of fewer lanes
+    if (one) hx_launch(k_bal_rows<BF, V, NJ, false, true>, g, b, lds, s, a);
+    else hx_launch(k_bal_rows<BF, V, NJ, false, false>, g, b, lds, s, a);
+  }
 }
 
 // Where one workgroup does it all: what two more launches cost (about 4 us each) is less
@@ -333,10 +350,12 @@ static hipError_t launch_balance(BalArgs a, bool bf, hipStream_t s) {
     else if (nj <= 2) launch_rows<false, 4, 2>(a, one, s);
     else launch_rows<false, 4, 4>(a, one, s);
   } else if (bf) {
-    if (nj <= 4) launch_rows<true, 1, 4>(a, one, s);
+    if (nj <= 1) launch_rows<true, 1, 1>(a, one, s);
+    else if (nj <= 4) launch_rows<true, 1, 4>(a, one, s);
     else launch_rows<true, 1, 16>(a, one, s);
   } else {
-    if (nj <= 4) launch_rows<false, 1, 4>(a, one, s);
+    if (nj <= 1) launch_rows<false, 1, 1>(a, one, s);
+    else if (nj <= 4) launch_rows<false, 1, 4>(a, one, s);
     else launch_rows<false, 1, 16>(a, one, s);
   }
   if (!one) hx_launch(k_bal_last, dim3((a.E + 1 + 15) / 16), dim3(1024), 0, s, a);

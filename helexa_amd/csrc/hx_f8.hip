@@ -475,16 +475,16 @@ __global__ __launch_bounds__(512) void k_f8_few_rows(F8LinearArgs a) {
 // A tile's rows in LDS, 4 blocks of K at a time: [4][TM][128 bytes], 16-byte piece j of row r
 // at j ^ r % 8 (the rows' pieces would all start on one bank). They come in by direct
 // loads, a chunk ahead.
-template <int TM>
+template <int TM, int NW>
 struct F8Tile {
-  static constexpr int CB = 4, BYTES = CB * TM * 128, LOADS = BYTES / 4096;   // KiB a wave and chunk
+  static constexpr int CB = 4, BYTES = CB * TM * 128, LOADS = BYTES / 1024 / NW;   // KiB a wave and chunk
   const uint8_t* src[LOADS];
   // rowptr(r): the quantised row r of the tile
   template <typename F>
   HX_DEV void init(int wave, F rowptr) {
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-      const int q = (i * 4 + wave) * 64 + lane_id(), row = q / 8 % TM;
+      const int q = (i * NW + wave) * 64 + lane_id(), row = q / 8 % TM;
       src[i] = rowptr(row) + q / (8 * TM) * 128 + ((q % 8) ^ (row & 7)) * 16;
     }
   }
@@ -492,17 +492,17 @@ struct F8Tile {
   HX_DEV void load(int wave, int b0, int nblk, uint32_t lds) const {
 #pragma unroll
     for (int i = 0; i < LOADS; i++)
-      if (b0 + (i * 4 + wave) * 8 / TM < nblk) dma16(src[i] + (int64_t)b0 * 128, lds + (i * 4 + wave) * 1024);
+      if (b0 + (i * NW + wave) * 8 / TM < nblk) dma16(src[i] + (int64_t)b0 * 128, lds + (i * NW + wave) * 1024);
   }
 };
 
 // acc[m][t] = the sums over KB blocks of K of a wave's NM tiles of 16 features (their codes
 // from w[m], a lane's place in it included; tiles m with m % 2 == q, or all, by the scales ws[q])
 // times the tile's rows; xs[t]: a lane's row's scales. Two blocks of weights are on their way.
-template <bool WIDE, int TM, int NM, int NQ>
-HX_DEV void f8_products(const uint8_t* const (&w)[NM], const float* const (&ws)[NQ], const F8Tile<TM>& rows,
+template <bool WIDE, int TM, int NW, int NM, int NQ>
+HX_DEV void f8_products(const uint8_t* const (&w)[NM], const float* const (&ws)[NQ], const F8Tile<TM, NW>& rows,
                         const float* const (&xs)[TM / 16], int wave, uint8_t* buf, int KB, f8_v4f (&acc)[NM][TM / 16]) {
-  constexpr int TT = TM / 16, CB = F8Tile<TM>::CB, BYTES = F8Tile<TM>::BYTES, R = 2;
+  constexpr int TT = TM / 16, CB = F8Tile<TM, NW>::CB, BYTES = F8Tile<TM, NW>::BYTES, R = 2;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
   const int lane = lane_id();
 #pragma unroll
@@ -1088,22 +1088,23 @@ hipError_t launch_f8_prep(const F8Args& a, hipStream_t s) {
 }
 
 // Rows of a tile: F entries over all E experts, so that padding and experts without rows count too
-// (the routing is on the device). us for 512 experts of 512 x 2048, 10 chosen, with tiles of 16, 32, 64, 128: 17
-// tokens 113, 114, 120, -; 64 tokens 241, 223, 222, -; 800 (16 rows an expert) 367, 317, 330, -; 1024 (20) 403, 335,
-// 333, -; 2048 (40) -, -, 382, 425; 3000 (59, skewed) -, -, 466, 459; 4096 (80) -, -, 577, 496. Tiles of 128 have
-// kernels of their own, which find a token's codes by 32 bits; f32 results' operands leave room for 32.
+// (the routing is on the device). us for 512 experts of 512 x 2048, 10 chosen, with tiles of 32, 64, 128: 64 tokens
+// 218, 224, 262; 512 (10 rows an expert) 314, 324, 378; 1024 (20) 357, 348, 394; 2048 (40) 447, 370, 422; 3000 (59,
+// skewed) 517, 432, 457; 4096 (80) 607, 533, 491; 8192 (160, skewed) 943, 791, 764. (16: 241 and 341 for the
+// first two.) Tiles of 128 have kernels of their own, which find a token's codes by 32 bits; f32
+// results' operands leave room for 32.
 int f8_tile_m(int64_t T, int64_t F, int E, int H, bool xbf) {
   if (!xbf || F <= 18 * (int64_t)E) return 32;
-  return F <= 56 * (int64_t)E || T * f8_row(H) >= (int64_t)1 << 32 ? 64 : 128;
+  return F <= 68 * (int64_t)E || T * f8_row(H) >= (int64_t)1 << 32 ? 64 : 128;
 }
 
 // h = q(silu(G x) * (U x)). Workgroup: a tile of TM rows and 128 features, a block of h's
 // columns: 32 a wave, gate and up of a feature in the same lane.
-template <int TM, bool WIDE>
-__global__ __launch_bounds__(256, 2) void k_f8_gate_up(F8Args a) {
-  constexpr int TT = TM / 16, NM = 4;
-  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM>::BYTES];
-  __shared__ uint32_t amax[4][TM];
+template <int TM, bool WIDE, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_gate_up(F8Args a) {
+  constexpr int TT = TM / 16, NF = 8 / NW, NM = 2 * NF;   // NF: a wave's tiles of features
+  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM, NW>::BYTES];
+  __shared__ uint32_t amax[NW][TM];
   int nt, tile;
   mx_tile(a.hblocks, a.counts[0], nt, tile);
   if (tile < 0) return;
@@ -1117,28 +1118,28 @@ __global__ __launch_bounds__(256, 2) void k_f8_gate_up(F8Args a) {
     const int p = p0 + min(r, rows - 1);
     return (int64_t)(sh ? p - a.F : a.perm[p] / a.k);
   };
-  F8Tile<TM> rw;
+  F8Tile<TM, NW> rw;
   rw.init(wave, [&](int r) { return a.xrec + token(r) * f8_row(a.H); });
   const float* xs[TT];
 #pragma unroll
   for (int t = 0; t < TT; t++) xs[t] = a.xs + token(16 * t + (lane & 15)) * f8_scale_row(a.H);
   const uint8_t* const mat[2] = {sh ? a.sgate.base : a.gate.mat(e), sh ? a.sup.base : a.up.mat(e)};
-  const uint8_t* w[NM];   // gate, up, gate, up
+  const uint8_t* w[NM];   // gate, up of each
 #pragma unroll
   for (int m = 0; m < NM; m++)
-    w[m] = mat[m & 1] + (int64_t)min(8 * nt + 2 * wave + (m >> 1), inter / 16 - 1) * KB * 2048 + lane * 16;
+    w[m] = mat[m & 1] + (int64_t)min(8 * nt + NF * wave + (m >> 1), inter / 16 - 1) * KB * 2048 + lane * 16;
   const int64_t sat = f8_code_bytes(inter, a.H) + (int64_t)nt * f8_scale_row(a.H) * 4;
   const float* const ws[2] = {(const float*)(mat[0] + sat), (const float*)(mat[1] + sat)};
   f8_v4f acc[NM][TT];
-  f8_products<WIDE, TM, NM, 2>(w, ws, rw, xs, wave, buf, KB, acc);
-  const bool in = 128 * nt + 32 * wave < inter;   // features behind the last are zeros
-  float h[TT][8];
+  f8_products<WIDE, TM, NW, NM, 2>(w, ws, rw, xs, wave, buf, KB, acc);
+  float h[TT][4 * NF];
 #pragma unroll
   for (int t = 0; t < TT; t++) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int m = 2 * (i >> 2);
-      h[t][i] = in ? silu_rcp(acc[m][t][i & 3]) * acc[m + 1][t][i & 3] : 0.f;
+    for (int f = 0; f < NF; f++) {
+      const bool in = 128 * nt + 16 * (NF * wave + f) < inter;   // features behind the last are zeros
+#pragma unroll
+      for (int i = 0; i < 4; i++) h[t][4 * f + i] = in ? silu_rcp(acc[2 * f][t][i]) * acc[2 * f + 1][t][i] : 0.f;
     }
     const uint32_t m = f8_max_of_4(f8_amax(h[t]));
     if (lane < 16) amax[wave][16 * t + lane] = m;
@@ -1147,24 +1148,27 @@ __global__ __launch_bounds__(256, 2) void k_f8_gate_up(F8Args a) {
 #pragma unroll
   for (int t = 0; t < TT; t++) {
     const int r = 16 * t + (lane & 15);
+    uint32_t m = 0;
+#pragma unroll
+    for (int v = 0; v < NW; v++) m = max(m, amax[v][r]);
     float s;
-    const bool fine = f8_scale(max(max(amax[0][r], amax[1][r]), max(amax[2][r], amax[3][r])), s);
-    uint32_t c[2];
+    const bool fine = f8_scale(m, s);
+    uint32_t c[NF];
     f8_codes_near(h[t], s, fine, c);
     if (r >= rows) continue;
-    uint32_t* o = (uint32_t*)(a.hrec + ((int64_t)(p0 + r) * a.hblocks + nt) * 128 + 32 * wave + 4 * (lane >> 4));
-    o[0] = c[0];
-    o[4] = c[1];
+    uint32_t* o = (uint32_t*)(a.hrec + ((int64_t)(p0 + r) * a.hblocks + nt) * 128 + 16 * NF * wave + 4 * (lane >> 4));
+#pragma unroll
+    for (int f = 0; f < NF; f++) o[4 * f] = c[f];
     if (wave == 0 && lane < 16) a.hs[(int64_t)(p0 + r) * a.hscale + nt] = s;
   }
 }
 
-// A wave's outputs of 64 features from tile n0 for rows p0 .. of obuf: f16 with a scale, a power of
-// two that gives the largest finite magnitude of a row's 64 the exponent 2^14 (infinities and
+// A wave's outputs of NM tiles from n0 for rows p0 .. of obuf: f16 with a scale for each 32, a power of
+// two that gives the largest finite magnitude of the row's outputs here the exponent 2^14 (infinities and
 // NaN stay what they are)
 template <int NM, int TT>
 HX_DEV void f8_out_rows(const F8Args& a, const f8_v4f (&acc)[NM][TT], uint8_t* tl, int64_t p0, int rows, int n0) {
-  static_assert(NM == 4, "64 outputs have a scale");
+  static_assert(NM % 2 == 0, "32 outputs have a scale");
   typedef F8Out<32 * NM> Out;
   const int lane = lane_id(), tiles = a.H / 16;
 #pragma unroll
@@ -1189,20 +1193,22 @@ HX_DEV void f8_out_rows(const F8Args& a, const f8_v4f (&acc)[NM][TT], uint8_t* t
       }
       *(uint2*)(tl + r * Out::PITCH + 32 * m + 8 * (lane >> 4)) = make_uint2(h[0], h[1]);
     }
-    if (lane < 16 && r < rows && n0 < tiles)
-      a.oscale[(p0 + r) * ((a.H + 63) / 64) + (n0 >> 2)] = __uint_as_float((uint32_t)(ex - 14) << 23);
+    if (lane < 16 && r < rows)
+#pragma unroll
+      for (int m = 0; m < NM; m += 2)
+        if (n0 + m < tiles) a.oscale[(p0 + r) * (a.H / 32) + ((n0 + m) >> 1)] = __uint_as_float((uint32_t)(ex - 14) << 23);
   }
   Out::store(tl, min(rows, 16 * TT), 2 * (a.H - 16 * n0), [&](int r) { return (uint8_t*)a.obuf + ((p0 + r) * a.H + 16 * n0) * 2; });
 }
 
-// Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 outputs, 64 a
-// wave. bf16 activations: 64 outputs of a row leave as f16 of a scale of their own, 2^-12 of a value at
+// Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256
+// outputs. bf16 activations: outputs leave as f16 with a scale for each 32, 2^-12 of a value at
 // most for half of the bytes that float32 takes here and in the combine (bf16, 2^-9, would be half
 // of the result's own error on top of it).
-template <int TM, bool WIDE>
-__global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
-  constexpr int TT = TM / 16, NM = 4;
-  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM>::BYTES];
+template <int TM, bool WIDE, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_down(F8Args a) {
+  constexpr int TT = TM / 16, NM = 16 / NW;
+  __shared__ __align__(16) uint8_t buf[2 * F8Tile<TM, NW>::BYTES];
   int nt, tile;
   mx_tile((a.H + 255) / 256, a.counts[0], nt, tile);
   if (tile < 0) return;
@@ -1210,8 +1216,8 @@ __global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
   const int e = __builtin_amdgcn_readfirstlane(ti.x), p0 = ti.y, rows = ti.z;
   const bool sh = e == a.E;
   const int inter = sh ? a.Is : a.I, KB = f8_blocks(inter), tiles = a.H / 16;
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = (4 * nt + wave) * NM;
-  F8Tile<TM> rw;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = 16 * nt + wave * NM;
+  F8Tile<TM, NW> rw;
   rw.init(wave, [&](int r) { return a.hrec + (int64_t)(p0 + min(r, rows - 1)) * a.hblocks * 128; });
   const float* xs[TT];
 #pragma unroll
@@ -1222,7 +1228,7 @@ __global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
   for (int m = 0; m < NM; m++) w[m] = mat + (int64_t)min(n0 + m, tiles - 1) * KB * 2048 + lane * 16;   // past the last: not stored
   const float* const ws[1] = {(const float*)(mat + f8_code_bytes(a.H, inter)) + (int64_t)(min(n0, tiles - 1) >> 3) * f8_scale_row(inter)};
   f8_v4f acc[NM][TT];
-  f8_products<WIDE, TM, NM, 1>(w, ws, rw, xs, wave, buf, KB, acc);
+  f8_products<WIDE, TM, NW, NM, 1>(w, ws, rw, xs, wave, buf, KB, acc);
   if constexpr (WIDE) {
 #pragma unroll
     for (int t = 0; t < TT; t++) {
@@ -1236,7 +1242,7 @@ __global__ __launch_bounds__(256, 2) void k_f8_down(F8Args a) {
       }
     }
   } else {
-    static_assert(4 * TM * F8Out<32 * NM>::PITCH <= 2 * F8Tile<TM>::BYTES, "the rows' place holds the results");
+    static_assert(NW * TM * F8Out<32 * NM>::PITCH <= 2 * F8Tile<TM, NW>::BYTES, "the rows' place holds the results");
     lds_barrier();   // the rows have been read
     f8_out_rows<NM, TT>(a, acc, buf + wave * (TM * F8Out<32 * NM>::PITCH), p0, rows, n0);
   }
@@ -1333,9 +1339,9 @@ __global__ __launch_bounds__(256, 2) void k_f8_down_many(F8Args a) {
 
 #define F8_LAUNCH(KERNEL, NX)                                                                  \
   const dim3 g((unsigned)((int64_t)(NX) * ((a.max_tiles + 7) / 8 * 8)));                       \
-  if (!a.xbf) hx_launch(KERNEL<32, true>, g, dim3(256), 0, s, a);                              \
-  else if (a.tile_m == 32) hx_launch(KERNEL<32, false>, g, dim3(256), 0, s, a);                \
-  else hx_launch(KERNEL<64, false>, g, dim3(256), 0, s, a)
+  if (!a.xbf) hx_launch(KERNEL<32, true, 4>, g, dim3(256), 0, s, a);                           \
+  else if (a.tile_m == 32) hx_launch(KERNEL<32, false, 4>, g, dim3(256), 0, s, a);             \
+  else hx_launch(KERNEL<64, false, 8>, g, dim3(512), 0, s, a)
 
 hipError_t launch_f8_gate_up(const F8Args& a, hipStream_t s) {
   if (a.tile_m == 128) {

@@ -229,7 +229,7 @@ static WsLayout ws_layout(const hx_moe* m, int64_t T) {
       L.mx_hrec = take((size_t)(F + T) * f8_row(inter));
       L.f8_hs = take(sizeof(float) * (size_t)(F + T) * f8_scale_row(inter));
       L.obuf = take(act * (size_t)(F + T) * H);
-      L.f8_os = act == 2 ? take(sizeof(float) * (size_t)(F + T) * ((H + 63) / 64)) : 0;
+      L.f8_os = act == 2 ? take(sizeof(float) * (size_t)(F + T) * (H / 32)) : 0;
       L.mx_perm = take(sizeof(int32_t) * F);
       L.mx_inv = take(sizeof(int32_t) * F);
       L.mx_hist = take(sizeof(int32_t) * (size_t)std::min<int64_t>((F + MX_CHUNK - 1) / MX_CHUNK, MX_MAX_CHUNKS) * E);

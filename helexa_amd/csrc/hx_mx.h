@@ -64,7 +64,7 @@ struct MxArgs {
   uint8_t* hrec;                            // [F + T][mx_blocks(max(I, Is))] records
   int hblocks;                              // records of a row of hrec
   void* obuf;                               // [F + T, H] expert outputs, act dtype (few tokens: f32)
-  float* oscale;                            // or null; [F + T][ceil(H / 64)]: obuf is f16 times these
+  float* oscale;                            // or null; [F + T][H / 32]: obuf is f16 times these
   int32_t* few;                             // [slots][MX_FEW_TAB], 2 to 8 tokens: rows of the columns, then the expert
   int32_t* perm;                            // [F] entries by expert
   int32_t* inv;                             // [F] their positions, -1: no expert

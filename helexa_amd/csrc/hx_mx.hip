@@ -1018,7 +1018,7 @@ HX_DEV uint4 mx_row16(const void* p) {
 // (an entry without an expert reads row 0 and counts nothing). Bound by HBM, few
 // tokens by latency (4 us). FEW: rows in f32, a
 // token's entry at that of its first with the same expert; else rows in the
-// activations' type by inv, SC: in f16 with a scale for each 64; NT: more of them than MX_CACHE, read non-temporally (8192
+// activations' type by inv, SC: in f16 with a scale for each 32; NT: more of them than MX_CACHE, read non-temporally (8192
 // tokens' 369 MB: 65 us against 78; 2048 tokens' 92 MB: 19 against 17). f32 rows of 2048 tokens:
 // 34 us.
 template <bool BF, bool FEW, bool NT, bool SC>
@@ -1060,7 +1060,7 @@ __global__ __launch_bounds__(256) void k_mx_combine(MxArgs a) {
       pj[j] = jj < k ? __builtin_amdgcn_readlane(p, jj) : jj == k ? ps : -1;
       wj[j] = jj < k ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), jj)) : ws;
       const int64_t at = (int64_t)max(pj[j], 0) * a.H + (mine ? n0 : 0);
-      if constexpr (SC) sc[j] = a.oscale[(int64_t)max(pj[j], 0) * ((a.H + 63) / 64) + ((mine ? n0 : 0) >> 6)];
+      if constexpr (SC) sc[j] = a.oscale[(int64_t)max(pj[j], 0) * (a.H / 32) + ((mine ? n0 : 0) >> 5)];
       if constexpr (R16) {
         q[j] = mx_row16<NT>((const uint16_t*)a.obuf + at);
       } else {

@@ -182,6 +182,22 @@ def _stream(stream=None, device=None) -> int:
     return int(s.cuda_stream)
 
 
+def _raw_stream(stream, index: int) -> int:
+    """the handle of `stream`, or of the current one of GPU `index`, without an object for it (1.5 us
+    of a call of 9)"""
+    import torch
+    return int(stream.cuda_stream) if stream is not None else torch._C._cuda_getCurrentRawStream(index)
+
+
+def _on_device(index: int, call, *args) -> int:
+    """call(*args) with GPU `index` as the current one (switching costs more than most calls)"""
+    import torch
+    if index == torch.cuda.current_device():
+        return call(*args)
+    with torch.cuda.device(index):
+        return call(*args)
+
+
 def _used_on(stream, *tensors) -> None:
     """tensors that a call on another stream than the current one reads or writes: their
     memory goes to nobody else before that stream is done with it"""
@@ -552,23 +568,23 @@ def quantize_f8(x, block_rows: int = 1, stream=None):
         raise ValueError("quantize_f8: blocks of 1 row, or of 128 of a matrix")
     dt = _act_dtype(x.dtype)
     x = _contiguous(x, stream)
-    cols = x.shape[-1]
+    shape, dev = x.shape, x.get_device()
+    cols, n = shape[-1], x.numel()
     nb = (cols + 127) // 128
-    rows = x.numel() // cols if block_rows == 1 else x.shape[-2]
-    codes = _empty(x, stream, x.shape, torch.float8_e4m3fn)
-    scales = _empty(x, stream, x.shape[:-1] + (nb,) if block_rows == 1 else x.shape[:-2] + ((rows + 127) // 128, nb),
-                    torch.float32)
+    rows = n // cols if block_rows == 1 else shape[-2]
+    codes = _empty(x, stream, shape, torch.float8_e4m3fn)
+    scales = _empty(x, stream, shape[:-1] + (nb,) if block_rows == 1 else shape[:-2] + ((rows + 127) // 128, nb), torch.float32)
     _used_on(stream, x)
-    if not x.numel():
+    if not n:
         return codes, scales
-    count = x.numel() // (rows * cols)
+    count = n // (rows * cols)
     if block_rows == 128 and rows % 128 == 0:   # whole blocks: the stack is one matrix
         rows, count = rows * count, 1
-    with torch.cuda.device(x.device):
-        for i in range(count):
-            check(lib().hx_quantize_f8(_ptr(x) + i * rows * cols * x.element_size(), dt, rows, cols, block_rows,
-                                       _ptr(codes) + i * rows * cols, _ptr(scales) + i * ((rows + 127) // 128) * nb * 4,
-                                       _stream(stream, x.device)), "hx_quantize_f8")
+    s, px, pc, ps = _raw_stream(stream, dev), x.data_ptr(), codes.data_ptr(), scales.data_ptr()
+    for i in range(count):
+        m = i * rows * cols
+        check(_on_device(dev, lib().hx_quantize_f8, px + m * x.element_size(), dt, rows, cols, block_rows, pc + m,
+                         ps + i * ((rows + 127) // 128) * nb * 4, s), "hx_quantize_f8")
     return codes, scales
 
 
@@ -637,9 +653,9 @@ class F8Linear:
         if workspace is not None and (workspace.device != x.device or not workspace.is_contiguous()):
             raise ValueError(f"workspace must be a contiguous tensor on {x.device}")
         _used_on(stream, x, workspace, out)
-        ws, ws_n = (None, 0) if workspace is None else (_ptr(workspace), workspace.nbytes)
-        check(lib().hx_linear_forward(self._h, _ptr(x), xdt, x.numel() // self.in_features, _ptr(out), ydt, ws, ws_n,
-                                      _stream(stream, self.device)), "hx_linear_forward")
+        ws, ws_n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+        check(lib().hx_linear_forward(self._h, x.data_ptr(), xdt, x.numel() // self.in_features, out.data_ptr(), ydt, ws, ws_n,
+                                      _raw_stream(stream, self.device)), "hx_linear_forward")
         return out
 
     __call__ = forward
@@ -680,9 +696,9 @@ def expert_counts(topk_idx, num_experts: int, workspace=None, stream=None):
     import torch
     idx, T, k, ws = _balance_call(topk_idx, num_experts, None, workspace, stream)
     out = _empty(idx, stream, num_experts, torch.int32)
-    with torch.cuda.device(idx.device):
-        check(lib().hx_moe_expert_counts(_ptr(idx), T, k, num_experts, _ptr(out), _ptr(ws), ws.nbytes,
-                                         _stream(stream, idx.device)), "hx_moe_expert_counts")
+    dev = idx.get_device()
+    check(_on_device(dev, lib().hx_moe_expert_counts, idx.data_ptr(), T, k, num_experts, out.data_ptr(), ws.data_ptr(),
+                     ws.nbytes, _raw_stream(stream, dev)), "hx_moe_expert_counts")
     return out
 
 
@@ -705,8 +721,8 @@ def balance_loss(logits, topk_idx, coef: float = 1.0, counts=None, grad: bool = 
     _used_on(stream, x)
     out = dict(loss=_empty(x, stream, (), torch.float32), counts=_empty(x, stream, E, torch.int32),
                probs=_empty(x, stream, E, torch.float32), dlogits=_empty(x, stream, x.shape, x.dtype) if grad else None)
-    with torch.cuda.device(x.device):
-        check(lib().hx_moe_balance_loss(_ptr(x), dt, T, E, _ptr(idx), k, _ptr(counts), float(coef), _ptr(out["loss"]),
-                                        _ptr(out["counts"]), _ptr(out["probs"]), _ptr(out["dlogits"]), _ptr(ws), ws.nbytes,
-                                        _stream(stream, x.device)), "hx_moe_balance_loss")
+    dev = x.get_device()
+    check(_on_device(dev, lib().hx_moe_balance_loss, x.data_ptr(), dt, T, E, idx.data_ptr(), k, _ptr(counts), float(coef),
+                     out["loss"].data_ptr(), out["counts"].data_ptr(), out["probs"].data_ptr(), _ptr(out["dlogits"]),
+                     ws.data_ptr(), ws.nbytes, _raw_stream(stream, dev)), "hx_moe_balance_loss")
     return out
