@@ -93,63 +93,34 @@ HX_DEV void f8_codes_near(const float (&f)[N], float s, bool fine, uint32_t (&w)
     w[i] = fine ? f8_pack(f[4 * i] * r, f[4 * i + 1] * r, f[4 * i + 2] * r, f[4 * i + 3] * r) : 0u;
 }
 
-// N elements from p, 16 bytes at a time (VEC: aligned) or n of them singly, zeros behind
-template <bool BF, bool VEC, int N>
+// loads and stores of whole words at any address (the hardware splits what crosses a line)
+typedef uint32_t f8_any4 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t f8_any1 __attribute__((aligned(1)));
+
+// N elements from p or, at a row's end, n of them, zeros behind
+template <bool BF, int N>
 HX_DEV void f8_load(const void* base, int64_t at, int n, float (&f)[N]) {
-  if constexpr (VEC) {
-    if (n <= 0) {
+  if (n >= N) {
+    constexpr int W = BF ? N / 2 : N;   // words
+    uint32_t u[W];
+    const uint8_t* p = (const uint8_t*)base + at * (BF ? 2 : 4);
+    if constexpr (W >= 4) {
 #pragma unroll
-      for (int i = 0; i < N; i++) f[i] = 0.f;
-      return;
-    }
-    if constexpr (BF) {
-#pragma unroll
-      for (int i = 0; i < N / 8; i++) {
-        const uint4 v = ((const uint4*)((const uint16_t*)base + at))[i];
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          f[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
-          f[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-        }
+      for (int i = 0; i < W / 4; i++) {
+        const f8_any4 v = ((const f8_any4*)p)[i];
+        u[4 * i] = v[0]; u[4 * i + 1] = v[1]; u[4 * i + 2] = v[2]; u[4 * i + 3] = v[3];
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < N / 4; i++) {
-        const float4 v = ((const float4*)((const float*)base + at))[i];
-        f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
-      }
+      for (int i = 0; i < W; i++) u[i] = ((const f8_any1*)p)[i];
     }
-  } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = i < n ? ld_act(base, at + i, BF) : 0.f;
-  }
-}
-
-// One block of a row by 8 lanes, 16 values a lane. The lanes' codes of columns c0 ..
-template <bool BF, bool VEC>
-HX_DEV void f8_row_block(const void* x, int64_t rows, int64_t cols, int64_t r, int b, uint4& codes, float& s) {
-  const int c0 = 128 * b + 16 * (lane_id() & 7);
-  float f[16];
-  f8_load<BF, VEC>(x, r * cols + c0, (int)min<int64_t>(cols - c0, 16), f);
-  uint32_t m = f8_amax(f);
-  m = max(m, (uint32_t)dpp_mov<0xB1>((int)m));    // quad_perm 1,0,3,2
-  m = max(m, (uint32_t)dpp_mov<0x4E>((int)m));    // quad_perm 2,3,0,1
-  m = max(m, (uint32_t)dpp_mov<0x141>((int)m));   // row_half_mirror
-  const bool fine = f8_scale(m, s);
-  uint32_t w[4];
-  f8_codes(f, s, fine, w);
-  codes = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// codes to a row's place, 16 bytes or n of them singly
-HX_DEV void f8_put(uint8_t* p, const uint4& c, bool vec, int n) {
-  if (vec) {
-    if (n > 0) *(uint4*)p = c;
+    for (int i = 0; i < N; i++)
+      f[i] = __uint_as_float(!BF ? u[BF ? 0 : i] : i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
     return;
   }
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  for (int i = 0; i < n && i < 16; i++) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+#pragma unroll
+  for (int i = 0; i < N; i++) f[i] = i < n ? ld_act(base, at + i, BF) : 0.f;
 }
 
 struct F8Rows {
@@ -159,44 +130,51 @@ struct F8Rows {
   int64_t ldc;       // bytes of a row of codes, cols or more
   float* scales;
   int lds;           // floats of a row of scales
-  bool vec_out;
 };
 
-// rows of x, a thread 16 of its values (x and the codes 16-byte aligned: VEC)
-template <bool BF, bool VEC>
+// Rows of x, a thread 16 of its values, 8 threads a block. Bound by HBM: 8192 rows of 4096 in bf16, 101
+// MB, in 21 us (4.8 TB/s); few rows by a launch, 3.3 us.
+template <bool BF>
 HX_DEV void f8_quant_rows(const F8Rows& q, int64_t id) {
   const int nb = f8_blocks(q.cols);
   const int64_t blk = id >> 3, r = blk / nb;
   const int b = (int)(blk % nb), c0 = 128 * b + 16 * (int)(id & 7);
   const bool has = r < q.rows;   // the lanes of a block agree
-  uint4 c;
+  float f[16];
+  f8_load<BF>(q.x, (has ? r : 0) * q.cols + c0, (int)min<int64_t>(q.cols - c0, 16), f);
+  uint32_t m = f8_amax(f);
+  m = max(m, (uint32_t)dpp_mov<0xB1>((int)m));    // quad_perm 1,0,3,2
+  m = max(m, (uint32_t)dpp_mov<0x4E>((int)m));    // quad_perm 2,3,0,1
+  m = max(m, (uint32_t)dpp_mov<0x141>((int)m));   // row_half_mirror
   float s;
-  f8_row_block<BF, VEC>(q.x, q.rows, q.cols, has ? r : 0, b, c, s);
+  const bool fine = f8_scale(m, s);
+  uint32_t w[4];
+  f8_codes(f, s, fine, w);
   if (!has) return;
-  f8_put(q.codes + r * q.ldc + c0, c, q.vec_out, (int)min<int64_t>(q.ldc - c0, 16));
+  uint8_t* const p = q.codes + r * q.ldc + c0;
+  const int n = (int)min<int64_t>(q.ldc - c0, 16);
+  if (n == 16) *(f8_any4*)p = f8_any4{w[0], w[1], w[2], w[3]};
+  else
+    for (int i = 0; i < n; i++) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
   if ((id & 7) == 0) q.scales[r * q.lds + b] = s;
 }
-template <bool BF, bool VEC>
+template <bool BF>
 __global__ __launch_bounds__(256) void k_f8_rows(F8Rows q) {
-  f8_quant_rows<BF, VEC>(q, (int64_t)blockIdx.x * 256 + threadIdx.x);
+  f8_quant_rows<BF>(q, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
 hipError_t launch_f8_rows(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, bool padded,
                           hipStream_t s) {
-  F8Rows q{x, rows, cols, (uint8_t*)codes, padded ? f8_row(cols) : cols, scales, padded ? f8_scale_row(cols) : f8_blocks(cols), false};
-  q.vec_out = (q.ldc & 15) == 0 && ((uintptr_t)codes & 15) == 0;
-  const bool vec = cols % 16 == 0 && ((uintptr_t)x & 15) == 0;
+  const F8Rows q{x, rows, cols, (uint8_t*)codes, padded ? f8_row(cols) : cols, scales, padded ? f8_scale_row(cols) : f8_blocks(cols)};
   const dim3 g((unsigned)((rows * f8_blocks(cols) * 8 + 255) / 256));
-  if (xbf && vec) hx_launch(k_f8_rows<true, true>, g, dim3(256), 0, s, q);
-  else if (xbf) hx_launch(k_f8_rows<true, false>, g, dim3(256), 0, s, q);
-  else if (vec) hx_launch(k_f8_rows<false, true>, g, dim3(256), 0, s, q);
-  else hx_launch(k_f8_rows<false, false>, g, dim3(256), 0, s, q);
+  if (xbf) hx_launch(k_f8_rows<true>, g, dim3(256), 0, s, q);
+  else hx_launch(k_f8_rows<false>, g, dim3(256), 0, s, q);
   return hipGetLastError();
 }
 
-// blocks of 128 x 128: a workgroup a block, 64 values a thread in registers, 4 columns of
-// 16 rows, 8 rows apart
-template <bool BF, bool VEC>
+// Blocks of 128 x 128: a workgroup a block, 64 values a thread in registers, 4 columns of
+// 16 rows, 8 rows apart. Bound by HBM: 262144 rows of 2048 in float32, 2.7 GB, in 442 us (6.1 TB/s).
+template <bool BF>
 __global__ __launch_bounds__(256) void k_f8_blocks(F8Rows q) {
   __shared__ uint32_t part[4];
   const int nb = f8_blocks(q.cols), tid = threadIdx.x;
@@ -209,15 +187,7 @@ __global__ __launch_bounds__(256) void k_f8_blocks(F8Rows q) {
 #pragma unroll
   for (int i = 0; i < 16; i++) {
     const int64_t r = r0 + 8 * i;
-    const int has = r < q.rows ? n : 0;
-    if constexpr (VEC && BF) {
-      uint2 v = make_uint2(0u, 0u);
-      if (has > 0) v = *(const uint2*)((const uint16_t*)q.x + r * q.cols + c0);
-      f[i][0] = __uint_as_float(v.x << 16); f[i][1] = __uint_as_float(v.x & 0xffff0000u);
-      f[i][2] = __uint_as_float(v.y << 16); f[i][3] = __uint_as_float(v.y & 0xffff0000u);
-    } else {
-      f8_load<BF, VEC>(q.x, r * q.cols + c0, has, f[i]);
-    }
+    f8_load<BF>(q.x, r * q.cols + c0, r < q.rows ? n : 0, f[i]);
   }
 #pragma unroll
   for (int i = 0; i < 16; i++) m = max(m, f8_amax(f[i]));
@@ -234,23 +204,18 @@ __global__ __launch_bounds__(256) void k_f8_blocks(F8Rows q) {
     f8_codes(f[i], s, fine, w);
     if (r >= q.rows) continue;
     uint8_t* p = q.codes + r * q.cols + c0;
-    if (VEC && q.vec_out) {
-      if (n > 0) *(uint32_t*)p = w[0];
-    } else {
+    if (n == 4) *(f8_any1*)p = w[0];
+    else
       for (int j = 0; j < n; j++) p[j] = (uint8_t)(w[0] >> (8 * j));
-    }
   }
   if (tid == 0) q.scales[rb * nb + b] = s;
 }
 
 hipError_t launch_f8_blocks(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, hipStream_t s) {
-  F8Rows q{x, rows, cols, (uint8_t*)codes, cols, scales, f8_blocks(cols), ((uintptr_t)codes & 3) == 0};
-  const bool vec = cols % 4 == 0 && ((uintptr_t)x & (xbf ? 7 : 15)) == 0;
+  const F8Rows q{x, rows, cols, (uint8_t*)codes, cols, scales, f8_blocks(cols)};
   const dim3 g((unsigned)((int64_t)f8_blocks(rows) * f8_blocks(cols)));
-  if (xbf && vec) hx_launch(k_f8_blocks<true, true>, g, dim3(256), 0, s, q);
-  else if (xbf) hx_launch(k_f8_blocks<true, false>, g, dim3(256), 0, s, q);
-  else if (vec) hx_launch(k_f8_blocks<false, true>, g, dim3(256), 0, s, q);
-  else hx_launch(k_f8_blocks<false, false>, g, dim3(256), 0, s, q);
+  if (xbf) hx_launch(k_f8_blocks<true>, g, dim3(256), 0, s, q);
+  else hx_launch(k_f8_blocks<false>, g, dim3(256), 0, s, q);
   return hipGetLastError();
 }
 
@@ -353,22 +318,10 @@ HX_DEV uint32_t f8_max_of_4(uint32_t m) {
 // that hold an operand each value is quantised by all 16 columns of a row alone: 7.4 us
 // where this takes 5.)
 template <bool BF, bool NEAR = false>
-HX_DEV void f8_block_to_lds(const void* x, int64_t row_at, int K, int b, bool vec, uint8_t* codes, float* scale) {
+HX_DEV void f8_block_to_lds(const void* x, int64_t row_at, int K, int b, uint8_t* codes, float* scale) {
   const int l = lane_id() & 31, c0 = 128 * b + 4 * l;
   float f[4];
-  if (vec && c0 < K) {
-    if constexpr (BF) {
-      const uint2 v = *(const uint2*)((const uint16_t*)x + row_at + c0);
-      f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
-      f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
-    } else {
-      const float4 v = *(const float4*)((const float*)x + row_at + c0);
-      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = c0 + i < K ? ld_act(x, row_at + c0 + i, BF) : 0.f;
-  }
+  f8_load<BF>(x, row_at + c0, K - c0, f);
   uint32_t m = f8_amax(f);
   m = max(m, (uint32_t)dpp_mov<0xB1>((int)m));    // quad_perm 1,0,3,2
   m = max(m, (uint32_t)dpp_mov<0x4E>((int)m));    // quad_perm 2,3,0,1
@@ -383,9 +336,6 @@ HX_DEV void f8_block_to_lds(const void* x, int64_t row_at, int K, int b, bool ve
   *(uint32_t*)(codes + 4 * l) = w[0];
   if (l == 0) *scale = s;
 }
-// whether 4 values of a row come in one load
-template <bool BF>
-__host__ __device__ inline bool f8_vec4(const void* x, int64_t K) { return K % 4 == 0 && ((uintptr_t)x & (BF ? 7 : 15)) == 0; }
 // bytes between rows in LDS: 16 more than the codes, so that the rows' pieces start on other banks
 __host__ __device__ inline int f8_pitch(int K) { return f8_blocks(K) * 128 + 16; }
 
@@ -427,10 +377,9 @@ __global__ __launch_bounds__(512) void k_f8_few_rows(F8LinearArgs a) {
   const int pitch = QUANT ? f8_pitch(a.K) : 0;
   float* const qs = (float*)(sm + M * pitch);   // [M][KB]
   if constexpr (QUANT) {
-    const bool vec = f8_vec4<BF>(a.x, a.K);
     for (int u = 2 * wave + (lane >> 5); u < M * KB; u += 16) {
       const int r = u / KB, b = u % KB;
-      f8_block_to_lds<BF>(a.x, (int64_t)r * a.K, a.K, b, vec, sm + r * pitch + 128 * b, qs + u);
+      f8_block_to_lds<BF>(a.x, (int64_t)r * a.K, a.K, b, sm + r * pitch + 128 * b, qs + u);
     }
     lds_barrier();
   }
@@ -871,9 +820,8 @@ __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
   fetch(0, kq);
   fetch(1, kq + KW);
   if (ONE) {
-    const bool vec = f8_vec4<BF>(a.x, a.H);
     for (int b = 2 * wave + (lane >> 5); b < KB; b += 16)
-      f8_block_to_lds<BF>(a.x, 0, a.H, b, vec, sm + 128 * b, (float*)(sm + 128 * KB) + b);
+      f8_block_to_lds<BF>(a.x, 0, a.H, b, sm + 128 * b, (float*)(sm + 128 * KB) + b);
     lds_barrier();
   }
   f8_v4f ag = f8_zero4(), au = f8_zero4();
@@ -947,7 +895,7 @@ __global__ __launch_bounds__(1024) void k_f8_one_down(F8Args a) {
       const float4 sw = *(const float4*)(ws + b0);
 #pragma unroll 1
       for (int i = lane >> 5; i < 4; i += 2)
-        if (b0 + i < KB) f8_block_to_lds<false, true>(a.hf, row, inter, b0 + i, true, hq[wave] + 128 * i, &hs[wave][i]);
+        if (b0 + i < KB) f8_block_to_lds<false, true>(a.hf, row, inter, b0 + i, hq[wave] + 128 * i, &hs[wave][i]);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
@@ -1013,7 +961,7 @@ __global__ __launch_bounds__(256) void k_f8_few_down(F8Args a) {
       c = __ffsll(left) - 1;
       const int i = (wave & 1) * 2 + (lane >> 5), r = __shfl(row, c, 64);
       if ((__popcll(rows & ((1ull << c) - 1)) & 1) == (wave >> 1) && b0 + i < KB)
-        f8_block_to_lds<false, true>(a.hf, (int64_t)r * a.hcols, inter, b0 + i, true, hq + c * PITCH + 128 * i, &hs[c][i]);
+        f8_block_to_lds<false, true>(a.hf, (int64_t)r * a.hcols, inter, b0 + i, hq + c * PITCH + 128 * i, &hs[c][i]);
     }
     lds_barrier();
     const int mine = row >= 0 ? lane & 15 : c;   // a column without a row: any
@@ -1065,7 +1013,7 @@ hipError_t launch_f8_few_down(const F8Args& a, hipStream_t s) {
 // ---------------------------------------------------------------- experts, grouped
 // Workgroups 0 .. chunks - 1: the chunk's entries by expert (mx_chunk_entries); the others: the
 // tokens' rows, a thread 16 values.
-template <bool BF, bool VEC>
+template <bool BF>
 __global__ __launch_bounds__(256) void k_f8_prep(F8Args a) {
   __shared__ MxPlace sm;
   const int nch = mx_chunks(a.F);
@@ -1073,17 +1021,14 @@ __global__ __launch_bounds__(256) void k_f8_prep(F8Args a) {
     mx_chunk_entries(a, sm, nch);
     return;
   }
-  const F8Rows q{a.x, a.T, a.H, a.xrec, f8_row(a.H), a.xs, f8_scale_row(a.H), true};
-  f8_quant_rows<BF, VEC>(q, (int64_t)(blockIdx.x - nch) * 256 + threadIdx.x);
+  const F8Rows q{a.x, a.T, a.H, a.xrec, f8_row(a.H), a.xs, f8_scale_row(a.H)};
+  f8_quant_rows<BF>(q, (int64_t)(blockIdx.x - nch) * 256 + threadIdx.x);
 }
 
 hipError_t launch_f8_prep(const F8Args& a, hipStream_t s) {
-  const bool vec = a.H % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
   const dim3 g((unsigned)(((int64_t)a.T * f8_blocks(a.H) * 8 + 255) / 256 + mx_chunks(a.F)));
-  if (a.xbf && vec) hx_launch(k_f8_prep<true, true>, g, dim3(256), 0, s, a);
-  else if (a.xbf) hx_launch(k_f8_prep<true, false>, g, dim3(256), 0, s, a);
-  else if (vec) hx_launch(k_f8_prep<false, true>, g, dim3(256), 0, s, a);
-  else hx_launch(k_f8_prep<false, false>, g, dim3(256), 0, s, a);
+  if (a.xbf) hx_launch(k_f8_prep<true>, g, dim3(256), 0, s, a);
+  else hx_launch(k_f8_prep<false>, g, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -322,6 +322,9 @@ class Qwen3_5MoeBlock:
                 setattr(w, field_, _ptr(t))
         out = C.c_void_p()
         if any(len(entry) > 2 for entry in weights.values()):
+            if on_dev:   # the library copies on the default stream
+                import torch
+                torch.cuda.current_stream(device).synchronize()
             check(lib().hx_moe_create_f8(C.byref(c), C.byref(w), C.byref(scales), device, C.byref(out)), "hx_moe_create_f8")
         else:
             check(lib().hx_moe_create(C.byref(c), C.byref(w), device, C.byref(out)), "hx_moe_create")
