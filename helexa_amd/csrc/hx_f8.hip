@@ -516,25 +516,28 @@ HX_DEV void f8_products(const uint8_t* const (&w)[NM], const float* const (&ws)[
 // 16 rows. A stage is one block of K: the features' tiles as they are stored, the rows (16-byte
 // piece j of row r at j ^ r % 8: the rows' pieces would all start on one bank), the rows' scales, the
 // features' scales; NS stages are in LDS, all but one of them on their way. They come in by direct
-// loads only: a load into a register would wait for the direct ones before it.
-template <int FT, int TT, int WF, int WR, int NS>
+// loads only: a load into a register would wait for the direct ones before it. KS groups of waves
+// take the blocks of K in turn, each with stages of its own, and the first gets all sums.
+template <int FT, int TT, int WF, int WR, int NS, int KS = 1>
 struct F8Core {
   static constexpr int NW = WF * WR, TF = 16 * FT * WF, TR = 16 * TT * WR;
   static constexpr int ROWS = TF * 128, SX = ROWS + TR * 128, SW = SX + (TR * 4 + 255) / 256 * 256, STAGE = SW + 256;
   static constexpr int APW = TF / 8 / NW, BPW = TR / 8 / NW, SPW = (TR / 64 + NW) / NW;   // loads of a wave
-  static constexpr int LOADS = APW + BPW + SPW, BYTES = NS * STAGE;
+  static constexpr int LOADS = APW + BPW + SPW, GROUP = NS * STAGE, BYTES = KS * GROUP;
   static_assert(TF % (8 * NW) == 0 && TR % (8 * NW) == 0 && TR % 64 == 0, "whole loads");
   // where a wave's loads are: the features' tiles from base registers, rows and scales by the lanes'
   // offsets from theirs
   const uint8_t *a[APW], *rows, *xs, *ws;
   uint32_t b[BPW], s[SPW];   // SPW: one wave's or several waves' loads are of the features' scales
-  int wave, wf, wr;
+  int wave, group, wf, wr;   // wave: of the group
   // tile(i): the stored tiles of the workgroup's i-th 16 features; row(r), scale(r): the offsets of the
   // quantised row r from `rows` and of its scales from `xs`, within 32 bits; fscale(i): the i-th 16
   // features' scales
   template <typename A, typename B, typename S, typename W>
   HX_DEV F8Core(const uint8_t* rows_, const float* xs_, A tile, B row, S scale, W fscale) : rows(rows_), xs((const uint8_t*)xs_) {
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wave = all % NW;
+    group = all / NW;
     wf = wave / WR;
     wr = wave % WR;
     const int lane = lane_id();
@@ -572,8 +575,10 @@ struct F8Core {
   template <bool WIDE, int NQ>
   HX_DEV void run(int KB, uint8_t* buf, bool work, f8_v4f (&acc)[FT][TT]) const {
     static_assert(FT % 2 == 0 && FT % NQ == 0, "pairs of tiles, whole groups of scales");
+    uint8_t* const all = buf;
+    buf += group * GROUP;
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)buf;
-    const int lane = lane_id();
+    const int lane = lane_id(), KG = (KB + KS - 1) / KS;   // blocks of a group; the last may not be there
     f8_v4f d[2][TT];
     float last[TT];
 #pragma unroll
@@ -585,21 +590,21 @@ struct F8Core {
     }
 #pragma unroll
     for (int i = 0; i < NS - 1; i++)
-      if (i < KB) load(i, lds + i * STAGE);
+      if (i * KS + group < KB) load(i * KS + group, lds + i * STAGE);
     const uint8_t* const x0 = buf + ROWS + (wr * TT * 16 + (lane & 15)) * 128 + ((lane >> 4) ^ (lane & 7)) * 16;
     const uint8_t* const x1 = buf + ROWS + (wr * TT * 16 + (lane & 15)) * 128 + ((4 + (lane >> 4)) ^ (lane & 7)) * 16;
     const uint8_t* const w0 = buf + wf * FT * 2048 + lane * 16;
     const uint8_t* const s0 = buf + SX + (wr * TT * 16 + (lane & 15)) * 4;
     int at = 0;   // the stage of block k
-    for (int k = 0; k < KB; k++) {
+    for (int k = 0; k < KG; k++) {
       // block k has come; after the barrier also the other waves', and the stage before it has been read
-      if (k + NS - 2 < KB) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * LOADS) : "memory");
+      if ((k + NS - 2) * KS + group < KB) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * LOADS) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       lds_barrier();
-      if (k + NS - 1 < KB) load(k + NS - 1, lds + (at == 0 ? NS - 1 : at - 1) * STAGE);
+      if ((k + NS - 1) * KS + group < KB) load((k + NS - 1) * KS + group, lds + (at == 0 ? NS - 1 : at - 1) * STAGE);
       const int st = at * STAGE;
       at = at == NS - 1 ? 0 : at + 1;
-      if (!work) continue;
+      if (!work || (KS > 1 && k * KS + group >= KB)) continue;
       auto tile = [&](int f) { return f8_op(*(const uint4*)(w0 + st + f * 2048), *(const uint4*)(w0 + st + f * 2048 + 1024)); };
       f8_v8i w[2];
       w[0] = tile(0);
@@ -629,6 +634,27 @@ struct F8Core {
     }
 #pragma unroll
     for (int t = 0; t < TT; t++) f8_add(acc[FT - 1][t], d[1][t], last[t]);
+    if constexpr (KS > 1) {
+      static_assert(KS == 2 && NW * FT * TT * 1024 <= BYTES, "the stages' place holds the second group's sums");
+      lds_barrier();   // the last stages have been read
+      float4* const p = (float4*)all + (size_t)wave * FT * TT * 64 + lane;
+      if (group == 1) {
+#pragma unroll
+        for (int i = 0; i < FT * TT; i++) {
+          const f8_v4f& v = acc[i / TT][i % TT];
+          p[i * 64] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      lds_barrier();
+      if (group == 0) {
+#pragma unroll
+        for (int i = 0; i < FT * TT; i++) {
+          const float4 o = p[i * 64];
+          f8_v4f& v = acc[i / TT][i % TT];
+          v[0] += o.x; v[1] += o.y; v[2] += o.z; v[3] += o.w;
+        }
+      }
+    }
   }
 };
 
@@ -661,10 +687,14 @@ HX_DEV bool f8_place(int NF, int NR, int& nf, int& nr) {
   return true;
 }
 
-// Linear layer of many rows
-template <int FT, int TT, int WF, int WR, int NS, bool WIDE>
-__global__ __launch_bounds__(64 * WF * WR, 2) void k_f8_linear(F8LinearArgs a) {
-  typedef F8Core<FT, TT, WF, WR, NS> Core;
+// Linear layer of many rows. Tiles of 256: 8192 rows, 8192 x 4096, 550 GFLOP in 265 to 295 us (1.9 to 2.1
+// PFLOP/s by the box; a library product of the same codes with one scale for all takes 223): the
+// matrix cores work half of the time, the scales' multiply-adds take half as many cycles as
+// the products, and two waves a SIMD, a stage's barrier and its LDS reads leave gaps. Tiles of 64: bound by
+// the chain of stages, 0.6 us each, and the launch before: 512 rows, 4096 x 2048, 12 us.
+template <int FT, int TT, int WF, int WR, int NS, int KS, bool WIDE>
+__global__ __launch_bounds__(64 * WF * WR * KS, 2) void k_f8_linear(F8LinearArgs a) {
+  typedef F8Core<FT, TT, WF, WR, NS, KS> Core;
   typedef F8Out<32 * FT> Out;
   constexpr int OUT = WIDE ? 0 : WF * WR * 16 * TT * Out::PITCH;
   __shared__ __align__(16) uint8_t buf[Core::BYTES > OUT ? Core::BYTES : OUT];
@@ -684,7 +714,8 @@ __global__ __launch_bounds__(64 * WF * WR, 2) void k_f8_linear(F8LinearArgs a) {
   core.template run<WIDE, 1>(KB, buf, core.wr * TT * 16 < rows, acc);
   const int f0 = 16 * (n0 + core.wf * FT), wr0 = core.wr * TT * 16, wrows = rows - wr0;   // the wave's
   if (!WIDE && a.N % 8 == 0 && ((uintptr_t)a.y & 15) == 0) {
-    lds_barrier();   // the last stage has been read
+    lds_barrier();   // the last stage has been read (or the second group's sums)
+    if (core.group > 0) return;
     uint8_t* const tl = buf + core.wave * (16 * TT * Out::PITCH);
 #pragma unroll
     for (int t = 0; t < TT; t++)
@@ -697,6 +728,7 @@ __global__ __launch_bounds__(64 * WF * WR, 2) void k_f8_linear(F8LinearArgs a) {
                [&](int r) { return (uint8_t*)a.y + ((r0 + wr0 + r) * a.N + f0) * 2; });
     return;
   }
+  if (core.group > 0) return;
   const bool vec = WIDE && a.N % 4 == 0 && ((uintptr_t)a.y & 15) == 0;
 #pragma unroll
   for (int t = 0; t < TT; t++) {
@@ -718,11 +750,11 @@ __global__ __launch_bounds__(64 * WF * WR, 2) void k_f8_linear(F8LinearArgs a) {
   }
 }
 
-template <int FT, int TT, int WF, int WR, int NS, bool WIDE>
+template <int FT, int TT, int WF, int WR, int NS, int KS, bool WIDE>
 static void f8_linear_tiled(const F8LinearArgs& a, hipStream_t s) {
-  typedef F8Core<FT, TT, WF, WR, NS> Core;
+  typedef F8Core<FT, TT, WF, WR, NS, KS> Core;
   const int64_t n = ((a.N + Core::TF - 1) / Core::TF) * ((a.M + Core::TR - 1) / Core::TR);
-  hx_launch(k_f8_linear<FT, TT, WF, WR, NS, WIDE>, dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * WF * WR), 0, s, a);
+  hx_launch(k_f8_linear<FT, TT, WF, WR, NS, KS, WIDE>, dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * WF * WR * KS), 0, s, a);
 }
 
 // Rows that the few-row kernel quantises itself: what that takes grows with them, a launch for it
@@ -752,14 +784,16 @@ static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
     // 67, 70, 89; 2304 128, 102, 131; 8192 281, 319, -.
     auto tiles = [&](int t) { return ((a.N + t - 1) / t) * ((a.M + t - 1) / t); };
     if constexpr (WIDE) {   // operands of 16 bits: smaller tiles fit the registers
-      if (tiles(128) >= 128) f8_linear_tiled<4, 2, 2, 2, 2, WIDE>(a, s);
-      else f8_linear_tiled<2, 2, 2, 2, 3, WIDE>(a, s);
+      if (tiles(128) >= 128) f8_linear_tiled<4, 2, 2, 2, 2, 1, WIDE>(a, s);
+      else f8_linear_tiled<2, 2, 2, 2, 3, 1, WIDE>(a, s);
     } else if (3 * ((tiles(256) + 255) / 256) <= (tiles(128) + 255) / 256) {
-      f8_linear_tiled<8, 4, 2, 4, 2, WIDE>(a, s);
+      f8_linear_tiled<8, 4, 2, 4, 2, 1, WIDE>(a, s);
     } else if (tiles(128) >= 224) {
-      f8_linear_tiled<4, 4, 2, 2, 2, WIDE>(a, s);
-    } else {
-      f8_linear_tiled<2, 2, 2, 2, 3, WIDE>(a, s);
+      f8_linear_tiled<4, 4, 2, 2, 2, 1, WIDE>(a, s);
+    } else if (tiles(64) > 256) {
+      f8_linear_tiled<2, 2, 2, 2, 3, 1, WIDE>(a, s);
+    } else {   // a workgroup a CU: twice the waves share K. 128 rows x 4096 x 2048 11.6 -> 10.5; 512 (2 a CU) 15.5 -> 18.3
+      f8_linear_tiled<2, 2, 2, 2, 3, 2, WIDE>(a, s);
     }
   }
   return hipGetLastError();
