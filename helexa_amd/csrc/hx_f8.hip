@@ -760,7 +760,7 @@ static void f8_linear_tiled(const F8LinearArgs& a, hipStream_t s) {
 // Rows that the few-row kernel quantises itself: what that takes grows with them, a launch for it
 // costs about 3 us; and they have to fit in LDS.
 static size_t f8_few_lds(int64_t M, int64_t K) { return (size_t)M * (f8_pitch((int)K) + 4 * f8_blocks(K)); }
-bool f8_quant_inside(int64_t M, int64_t K) { return M <= F8_QUANT_ROWS && f8_few_lds(M, K) <= 40 * 1024; }
+bool f8_quant_inside(int64_t M, int64_t K) { return M <= F8_QUANT_ROWS && f8_few_lds(M, K) <= 32 * 1024; }
 
 template <bool WIDE>
 static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
@@ -803,12 +803,13 @@ hipError_t launch_f8_linear(const F8LinearArgs& a, hipStream_t s) { return a.ybf
 // ---------------------------------------------------------------- experts, few tokens
 // Gate/up of up to 16 tokens. Workgroup: a chosen expert (slot) and 8 / KW groups of 16
 // features; KW waves share a group's K and add up in LDS. h leaves in f32: its blocks of 128
-// are of several workgroups, the down kernels quantise it. ONE token: an expert a chosen entry, its
-// weights on their way before the token is quantised, by every workgroup; more tokens come quantised.
-template <bool BF, int KW, bool ONE>
+// are of several workgroups, the down kernels quantise it. ONE token: an expert a chosen entry. QUANT: the
+// tokens are quantised into LDS by every workgroup, their expert's weights on their way meanwhile;
+// more tokens come quantised. Bound by latency and the weight stream: one token's 23 MB in 7.5 us.
+template <bool BF, int KW, bool ONE, bool QUANT>
 __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
   constexpr int FW = 8 / KW;
-  extern __shared__ __align__(16) uint8_t sm[];   // ONE: the token's codes, then its scales
+  extern __shared__ __align__(16) uint8_t sm[];   // QUANT: the tokens' codes, then their scales
   __shared__ MxFewT<ONE ? 1 : F8_FEW_T> few;
   __shared__ float red[8][2][16][17];
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), T = ONE ? 1 : a.T;
@@ -853,14 +854,19 @@ __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
   };
   fetch(0, kq);
   fetch(1, kq + KW);
-  if (ONE) {
-    for (int b = 2 * wave + (lane >> 5); b < KB; b += 16)
-      f8_block_to_lds<BF>(a.x, 0, a.H, b, sm + 128 * b, (float*)(sm + 128 * KB) + b);
+  const int pitch = f8_pitch(a.H);
+  float* const qs = (float*)(sm + T * pitch);   // [T][KB]
+  if (QUANT) {
+    for (int u = 2 * wave + (lane >> 5); u < T * KB; u += 16) {
+      const int t = ONE ? 0 : u / KB, b = ONE ? u : u % KB;
+      f8_block_to_lds<BF>(a.x, (int64_t)t * a.H, a.H, b, sm + t * pitch + 128 * b, qs + u);
+    }
     lds_barrier();
   }
   f8_v4f ag = f8_zero4(), au = f8_zero4();
-  const uint8_t* const row = ONE ? sm : a.xrec + min(col, T - 1) * f8_row(a.H);
-  const float* const xs = ONE ? (const float*)(sm + 128 * KB) : a.xs + (int64_t)min(col, T - 1) * f8_scale_row(a.H);
+  const int tok = min(col, T - 1);
+  const uint8_t* const row = QUANT ? sm + tok * pitch : a.xrec + tok * f8_row(a.H);
+  const float* const xs = QUANT ? qs + tok * KB : a.xs + (int64_t)tok * f8_scale_row(a.H);
   for (int b0 = kq; b0 < KB; b0 += 2 * KW) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -1020,12 +1026,18 @@ bool f8_few(int T) { return T <= F8_FEW_T; }
 template <bool BF>
 static hipError_t f8_few_gate_up(const F8Args& a, hipStream_t s) {
   const int slots = f8_few_slots(a), groups = (std::max(a.I, a.Is) + 15) / 16;
-  if (a.T == 1) {
-    hx_launch(k_f8_few_gate_up<BF, 8, true>, dim3(groups, slots), dim3(512), (uint32_t)f8_blocks(a.H) * 132, s, a);
-    return hipGetLastError();
-  }
-  if (slots * groups >= 1200) hx_launch(k_f8_few_gate_up<BF, 2, false>, dim3((groups + 3) / 4, slots), dim3(512), 0, s, a);
-  else hx_launch(k_f8_few_gate_up<BF, 8, false>, dim3(groups, slots), dim3(512), 0, s, a);
+  const bool in = f8_quant_inside(a.T, a.H);
+  const uint32_t lds = in ? (uint32_t)f8_few_lds(a.T, a.H) : 0;
+  // K shared by 8 waves where there are few of them, by 2 where a wave's start costs more than it saves
+  const bool few = slots * groups < 1200;
+  const dim3 g(few ? groups : (groups + 3) / 4, slots);
+#define FGU(KW, ONE, QUANT) hx_launch(k_f8_few_gate_up<BF, KW, ONE, QUANT>, g, dim3(512), lds, s, a)
+  if (a.T == 1) hx_launch(k_f8_few_gate_up<BF, 8, true, true>, dim3(groups, slots), dim3(512), lds, s, a);
+  else if (in && few) FGU(8, false, true);
+  else if (in) FGU(2, false, true);
+  else if (few) FGU(8, false, false);
+  else FGU(2, false, false);
+#undef FGU
   return hipGetLastError();
 }
 

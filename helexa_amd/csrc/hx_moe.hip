@@ -816,7 +816,7 @@ static int run_f8(hx_moe* m, const void* x, int64_t T, const int32_t* idx, const
   if (a.few_rows) {
     a.few = (int32_t*)(ws + L.mx_few);
     a.hf = (float*)(ws + L.f8_hf);
-    if (T > 1) {   // one token's gate/up kernel quantises
+    if (!f8_quant_inside(T, a.H)) {   // the gate/up kernel quantises the fewest itself
       tm_ext(m, SLOT_X_F16, s);
       HX_HIP(launch_f8_rows(x, a.xbf, T, a.H, a.xrec, a.xs, true, s));
       tm_ext_done(m, SLOT_X_F16);

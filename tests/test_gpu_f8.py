@@ -266,3 +266,14 @@ def test_refusals():
                      (lambda: hx.quantize_f8(x, 64), ValueError), (lambda: hx.quantize_f8(x[0], 128), ValueError)):
         with pytest.raises(err):
             bad()
+
+
+@pytest.mark.parametrize("N,K", [(70, 16400), (33, 60000), (17, 131072)])
+def test_long_rows(N, K):
+    """rows whose codes do not fit in LDS with few of them, and the longest a layer takes"""
+    import helexa_amd as hx
+    codes, scales = F.make_weights(K, N, K)
+    layer = hx.F8Linear.load(cuda(codes), cuda(scales))
+    for M in (1, 3, 5, 20, 70):
+        x = rows_of(M, M, K)
+        check_linear(layer(cuda(x)), x, codes, scales)
