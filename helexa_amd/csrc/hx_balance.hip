@@ -425,6 +425,9 @@ extern "C" int hx_moe_balance_loss(const void* logits, int logits_dtype, int64_t
   if (!loss || !probs || (n_tokens > 0 && (!logits || !topk_idx))) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
   if (logits_dtype != HX_F32 && logits_dtype != HX_BF16)
     return fail(HX_ERR_UNSUPPORTED, "hx_moe_balance_loss: logits dtype %d", logits_dtype);
+  // one workgroup writes the routing's own counts while the others read the given ones
+  if (given_counts && counts && given_counts < counts + num_experts && counts < given_counts + num_experts)
+    return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_balance_loss: counts and given_counts overlap");
   BalArgs a{};
   if ((rc = bal_args(a, topk_idx, n_tokens, k, num_experts, workspace, workspace_bytes))) return rc;
   a.logits = logits; a.given = given_counts; a.coef = coef;

@@ -64,3 +64,10 @@ def test_the_references_gradient_is_that_of_its_loss():
         v[10:] = 0.0
         hi, lo = (B.reference(x + h * v, idx, 0.3)["loss"] for h in (1e-5, -1e-5))
         assert abs((hi - lo) / 2e-5 - (r["dlogits"] * v).sum()) < 1e-9
+
+
+@pytest.mark.parametrize("given,own,code", [(P, P, 1), (P, P + 60, 1), (P + 60, P, 1)])
+def test_the_counts_that_are_read_are_not_those_written(given, own, code):
+    call = lambda: hx.lib().hx_moe_balance_loss(P, hx.F32, 8, 16, P, 4, given, 1.0, P, own, P, None, P, 1 << 20, None)
+    rc, text = alone(call)
+    assert rc == code and "overlap" in text
