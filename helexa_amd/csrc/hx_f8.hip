@@ -163,12 +163,22 @@ __global__ __launch_bounds__(256) void k_f8_rows(F8Rows q) {
   f8_quant_rows<BF>(q, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
+// a launch has less than 2^32 threads
+constexpr int64_t F8_LAUNCH_THREADS = (int64_t)1 << 31;
+
 hipError_t launch_f8_rows(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, bool padded,
                           hipStream_t s) {
-  const F8Rows q{x, rows, cols, (uint8_t*)codes, padded ? f8_row(cols) : cols, scales, padded ? f8_scale_row(cols) : f8_blocks(cols)};
-  const dim3 g((unsigned)((rows * f8_blocks(cols) * 8 + 255) / 256));
-  if (xbf) hx_launch(k_f8_rows<true>, g, dim3(256), 0, s, q);
-  else hx_launch(k_f8_rows<false>, g, dim3(256), 0, s, q);
+  F8Rows q{x, rows, cols, (uint8_t*)codes, padded ? f8_row(cols) : cols, scales, padded ? f8_scale_row(cols) : f8_blocks(cols)};
+  const int64_t most = F8_LAUNCH_THREADS / (8 * (int64_t)f8_blocks(cols));   // rows of a launch
+  for (int64_t left = rows; left > 0; left -= most) {
+    q.rows = std::min(left, most);
+    const dim3 g((unsigned)((q.rows * f8_blocks(cols) * 8 + 255) / 256));
+    if (xbf) hx_launch(k_f8_rows<true>, g, dim3(256), 0, s, q);
+    else hx_launch(k_f8_rows<false>, g, dim3(256), 0, s, q);
+    q.x = (const uint8_t*)q.x + most * cols * (xbf ? 2 : 4);
+    q.codes += most * q.ldc;
+    q.scales += most * q.lds;
+  }
   return hipGetLastError();
 }
 
@@ -212,20 +222,27 @@ __global__ __launch_bounds__(256) void k_f8_blocks(F8Rows q) {
 }
 
 hipError_t launch_f8_blocks(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, hipStream_t s) {
-  const F8Rows q{x, rows, cols, (uint8_t*)codes, cols, scales, f8_blocks(cols)};
-  const dim3 g((unsigned)((int64_t)f8_blocks(rows) * f8_blocks(cols)));
-  if (xbf) hx_launch(k_f8_blocks<true>, g, dim3(256), 0, s, q);
-  else hx_launch(k_f8_blocks<false>, g, dim3(256), 0, s, q);
+  F8Rows q{x, rows, cols, (uint8_t*)codes, cols, scales, f8_blocks(cols)};
+  const int64_t most = std::max<int64_t>(F8_LAUNCH_THREADS / 256 / f8_blocks(cols), 1) * 128;
+  for (int64_t left = rows; left > 0; left -= most) {
+    q.rows = std::min(left, most);
+    const dim3 g((unsigned)((int64_t)f8_blocks(q.rows) * f8_blocks(cols)));
+    if (xbf) hx_launch(k_f8_blocks<true>, g, dim3(256), 0, s, q);
+    else hx_launch(k_f8_blocks<false>, g, dim3(256), 0, s, q);
+    q.x = (const uint8_t*)q.x + most * cols * (xbf ? 2 : 4);
+    q.codes += most * cols;
+    q.scales += most / 128 * q.lds;
+  }
   return hipGetLastError();
 }
 
 // ---------------------------------------------------------------- stored weights
 // a thread per 16 bytes of a tile, padding included, then the scales
 __global__ __launch_bounds__(256) void k_repack_f8(const uint8_t* codes, const float* scales, int64_t count, int64_t rows,
-                                                   int64_t K, uint8_t* dst, int64_t dst_stride) {
+                                                   int64_t K, uint8_t* dst, int64_t dst_stride, int64_t first) {
   const int KB = f8_blocks(K), SR = f8_scale_row(K), RB = f8_blocks(rows);
   const int64_t pieces = (int64_t)f8_tiles(rows) * KB * 128, per = pieces + (int64_t)RB * SR;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= per * count) return;
   const int64_t m = id / per, q = id % per;
   uint8_t* mat = dst + m * dst_stride;
@@ -255,8 +272,9 @@ __global__ __launch_bounds__(256) void k_repack_f8(const uint8_t* codes, const f
 hipError_t launch_f8_repack(const void* codes, const float* scales, int64_t count, int64_t rows, int64_t K, void* dst,
                             int64_t dst_stride, hipStream_t s) {
   const int64_t per = (int64_t)f8_tiles(rows) * f8_blocks(K) * 128 + (int64_t)f8_blocks(rows) * f8_scale_row(K);
-  hipLaunchKernelGGL(k_repack_f8, dim3((unsigned)((per * count + 255) / 256)), dim3(256), 0, s, (const uint8_t*)codes, scales,
-                     count, rows, K, (uint8_t*)dst, dst_stride);
+  for (int64_t first = 0; first < per * count; first += F8_LAUNCH_THREADS)
+    hipLaunchKernelGGL(k_repack_f8, dim3((unsigned)((std::min(per * count - first, F8_LAUNCH_THREADS) + 255) / 256)), dim3(256),
+                       0, s, (const uint8_t*)codes, scales, count, rows, K, (uint8_t*)dst, dst_stride, first);
   return hipGetLastError();
 }
 
@@ -1032,7 +1050,7 @@ static hipError_t f8_few_gate_up(const F8Args& a, hipStream_t s) {
   const bool few = slots * groups < 1200;
   const dim3 g(few ? groups : (groups + 3) / 4, slots);
 #define FGU(KW, ONE, QUANT) hx_launch(k_f8_few_gate_up<BF, KW, ONE, QUANT>, g, dim3(512), lds, s, a)
-  if (a.T == 1) hx_launch(k_f8_few_gate_up<BF, 8, true, true>, dim3(groups, slots), dim3(512), lds, s, a);
+  if (a.T == 1) hx_launch(k_f8_few_gate_up<BF, 8, true, true>, dim3(groups, slots), dim3(512), lds, s, a);   // H is at most 16384
   else if (in && few) FGU(8, false, true);
   else if (in) FGU(2, false, true);
   else if (few) FGU(8, false, false);

@@ -24,8 +24,9 @@ extern "C" int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t 
   if (block_rows != 1 && block_rows != 128)
     return fail(HX_ERR_UNSUPPORTED, "hx_quantize_f8: blocks of 1 or 128 rows, not %d", block_rows);
   if ((uintptr_t)x & (x_dtype == HX_F32 ? 3 : 1)) return fail(HX_ERR_INVALID_ARGUMENT, "x does not start on an element");
-  // a launch has less than 2^31 workgroups
-  if (cols > (int64_t)1 << 32 || rows > (int64_t)1 << 32 || rows * f8_blocks(cols) / (block_rows == 1 ? 32 : 128) >= ((int64_t)1 << 31) - 1)
+  if ((uintptr_t)scales & 3) return fail(HX_ERR_INVALID_ARGUMENT, "the scales do not start on an element");
+  // a row's columns are indexed by 32 bits, bytes by 64
+  if (cols > ((int64_t)1 << 31) - 128 || rows > (int64_t)1 << 38)
     return fail(HX_ERR_UNSUPPORTED, "hx_quantize_f8: %lld rows of %lld are too many", (long long)rows, (long long)cols);
   if (rows == 0) return HX_OK;
   if (block_rows == 1) HX_HIP(launch_f8_rows(x, x_dtype == HX_BF16, rows, cols, codes, scales, false, (hipStream_t)stream));

@@ -206,7 +206,7 @@ int hx_moe_router_logits(hx_moe* m, const void* x, int64_t n_tokens, const float
  * (the counts are no function of the logits). c is the routing's own counts, or
  * given_counts (device int32 [E]; null: own) where the load of several calls or
  * devices is balanced together. Outputs: loss f32 [1], probs f32 [E] (P), counts
- * int32 [E] (the routing's own; may be null), dlogits (logits' type; may be null, may
+ * int32 [E] (the routing's own; may be null, not given_counts' place), dlogits (logits' type; may be null, may
  * be logits). No live token, or no entry in c: loss 0, gradient 0. A live row that
  * holds a NaN, +inf or nothing but -inf makes loss, probs and its own gradient NaN.
  * Sums run in a fixed order: the same bits for the same inputs. Both calls run on the
@@ -267,7 +267,7 @@ int hx_quantize_activations(int weight_dtype, const void* x, int x_dtype, int64_
  * the edges: codes [rows, cols] bytes, scales f32 [ceil(rows / block_rows), ceil(cols / 128)].
  * A block's scale is max(max|x| / 448, 2^-126), rounded to f32; a code is the E4M3 value
  * nearest to x / scale, the exact quotient, ties to the even code. A block that holds a NaN
- * or an infinity gets the scale NaN and codes 0. On the current device. */
+ * or an infinity gets the scale NaN and codes 0. cols at most 2^31 - 128. On the current device. */
 int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t cols, int block_rows, void* codes, float* scales,
                    void* stream);
 

@@ -92,3 +92,11 @@ def test_a_block_refuses_wrong_scales_and_mixtures():
     assert create(gate=hx.F32, up=hx.F32, down=hx.F32)[0] == 1
     assert create(down=hx.MXFP4)[0] == 2 and create(down=hx.BF16)[0] == 2 and create(up=hx.F32)[0] == 2
     assert create(hidden_size=264)[0] == 2 and create(moe_intermediate_size=40)[0] == 2
+
+
+@built
+@pytest.mark.parametrize("args,code", [
+    ((P, 0, 1, 1 << 31, 1, P, P), 2), ((P, 0, 1, 1 << 31, 128, P, P), 2), ((P, 0, 1, (1 << 31) - 127, 1, P, P), 2),
+    ((P, 0, 4, 128, 1, P, P + 2), 1), ((P, 0, 0, (1 << 31) - 128, 1, P, P), 0)])
+def test_the_quantisers_longest_row(args, code):
+    assert alone(lambda: hx.lib().hx_quantize_f8(*args, None))[0] == code

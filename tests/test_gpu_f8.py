@@ -277,3 +277,24 @@ def test_long_rows(N, K):
     for M in (1, 3, 5, 20, 70):
         x = rows_of(M, M, K)
         check_linear(layer(cuda(x)), x, codes, scales)
+
+
+@pytest.mark.parametrize("rows,block_rows", [((1 << 29) + 5, 1), ((1 << 30) + 200, 128)])
+def test_more_rows_than_a_launch_takes(rows, block_rows):
+    """one column: a launch has less than 2^32 threads. A block's largest has the code of +-448, the
+    others are smaller: the codes of 1, 1/2 and 1/4 of it"""
+    import torch
+    import helexa_amd as hx
+    pattern = torch.tensor([4.0, -2.0, 1.0, -4.0, 2.0, 1.0, -1.0], device="cuda", dtype=torch.bfloat16)
+    x = pattern.repeat(rows // 7 + 1)[:rows].reshape(rows, 1)
+    codes, scales = hx.quantize_f8(x, block_rows)
+    want = 4.0 if block_rows == 128 else x.reshape(-1).abs()
+    s = torch.as_tensor(want, device="cuda", dtype=torch.float32) / torch.tensor(448.0, device="cuda")
+    assert scales.shape == ((rows + block_rows - 1) // block_rows, 1) and bool((scales.reshape(-1) == s).all())
+    names = {448.0: 0x7e, 224.0: 0x76, 112.0: 0x6e}
+    if block_rows == 128:
+        byte = [names[abs(v) * 112] | (0x80 if v < 0 else 0) for v in pattern.tolist()]
+    else:
+        byte = [0x7e | (0x80 if v < 0 else 0) for v in pattern.tolist()]
+    byte = torch.tensor(byte, device="cuda", dtype=torch.uint8).repeat(rows // 7 + 1)[:rows]
+    assert bool((codes.view(torch.uint8).reshape(-1) == byte).all())

@@ -308,3 +308,18 @@ def test_a_layers_large_tiles(M, N, K):
     # every element, against the same product in bf16 operands and float32 sums by another path of the layer
     z = hx.F8Linear.load(cuda(codes), cuda(scales))(cuda(x, True), out_dtype=torch.float32)
     assert (y.float() - z).norm() <= 2.0 ** -8 * z.norm() and ((y.float() - z).abs() <= 2.0 ** -7 * z.abs() + 2.0 ** -7 * z.std()).all()
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+def test_the_widest_tokens(act):
+    """the codes of one fit where the few-token kernel quantises them, those of two do not"""
+    H, E, k, I, Is = 16384, 3, 2, 64, 32
+    d = F.block(5, H, E, I, Is)
+    blk = F.load(d, H, E, k, I, Is, act)
+    for T in (1, 2, 5, 20):
+        print("case", act, T, flush=True)
+        x = acts(T, T, H, act)
+        idx, w, sw = F.routing(T, T, E, k, 0)
+        y = blk.experts(cuda(x, act == BF16), cuda(idx), cuda(w), shared_w=cuda(sw))
+        check(y, x, idx, w, d, sw, act)
+    blk.close()
