@@ -138,7 +138,7 @@ HX_DEV void bal_store(void* base, int64_t at, const float (&f)[V]) {
 // The row pass: lpr lanes a row (64 / lpr rows a wave at a time), lane j of a row its
 // columns (i lpr + j) V .. + V - 1 for i < NJ. WHOLE: lpr is 64. ONE: one workgroup does it all, counts
 // and last sums included. Bound by HBM and the vector instructions together (about 16 an element):
-// 196608 rows of 512 in bf16, 411 MB, 3.9 TB/s.
+// 196608 rows of 512 in bf16, 411 MB, in 92 us (4.5 TB/s); 8192 in float32 11 us, half of it the counts' sum and the start.
 template <bool BF, int V, int NJ, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 512) void k_bal_rows(BalArgs a) {
   constexpr int NW = ONE ? 16 : 8, NT = 64 * NW;
@@ -329,12 +329,16 @@ static void launch_rows(const BalArgs& a, bool one, hipStream_t s) {
   }
 }
 
-// Where one workgroup does it all: what two more launches cost (about 4 us each) is less
-// than what one CU takes longer.
-static bool bal_one(int64_t T, int E) { return T * E <= 32768 && T <= 1024 && bal_lds(E, 16) <= 60 * 1024; }
+// Where one workgroup does it all: few tokens, entries (they are counted by atomics on one LDS) and logits,
+// so that what one CU takes longer is less than what two more launches cost. us with one and with
+// three, f32: 33 tokens x 512 experts, top 10, 8.0 and 10.9; 64 x 512 10.1 and 11.2; 80 x 512 11.4 and 11.1; 64 x 848 14.2
+// and 13.0; 80 x 128, top 8, 9.1 and 10.5; 128 x 128 11.9 and 10.5; 128 x 16, top 4, 6.3 and 10.2.
+static bool bal_one(const BalArgs& a) {
+  return a.T <= 128 && a.T * a.k <= 768 && a.T * a.E <= 32768 && bal_lds(a.E, 16) <= 60 * 1024;
+}
 
 static hipError_t launch_balance(BalArgs a, bool bf, hipStream_t s) {
-  const bool one = bal_one(a.T, a.E);
+  const bool one = bal_one(a);
   const int per = bf ? 8 : 4;
   const bool vec = a.E % per == 0 && (((uintptr_t)a.logits | (uintptr_t)a.dlogits) & 15) == 0;
   const int chunks = vec ? a.E / per : a.E;

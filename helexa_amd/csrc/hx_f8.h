@@ -33,9 +33,9 @@ __host__ __device__ inline int64_t f8_row(int64_t K) { return (int64_t)f8_blocks
 
 // tokens up to which a block takes the few-token kernels: an MFMA's 16 columns
 constexpr int F8_FEW_T = 16;
-// rows up to which a layer takes the few-row kernel, and up to which that one and the few-token
-// gate/up may quantise them themselves (f8_quant_inside)
-constexpr int F8_FEW_ROWS = 64, F8_QUANT_ROWS = 4;
+// rows up to which a layer takes the few-row kernel, and blocks of rows up to which that one and the
+// few-token gate/up quantise them themselves (f8_quant_inside)
+constexpr int F8_FEW_ROWS = 48, F8_QUANT_BLOCKS = 80;
 
 // experts: MxArgs with xrec and hrec the quantised rows of x and h, hblocks the blocks of
 // a row of h

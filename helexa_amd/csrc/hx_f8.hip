@@ -132,8 +132,8 @@ struct F8Rows {
   int lds;           // floats of a row of scales
 };
 
-// Rows of x, a thread 16 of its values, 8 threads a block. Bound by HBM: 8192 rows of 4096 in bf16, 101
-// MB, in 21 us (4.8 TB/s); few rows by a launch, 3.3 us.
+// Rows of x, a thread 16 of its values, 8 threads a block. Bound by HBM: 8192 rows of 4096 in bf16, 102
+// MB, in 22 to 24 us (4.2 to 4.6 TB/s); few rows by a launch, 3.5 us.
 template <bool BF>
 HX_DEV void f8_quant_rows(const F8Rows& q, int64_t id) {
   const int nb = f8_blocks(q.cols);
@@ -183,7 +183,8 @@ hipError_t launch_f8_rows(const void* x, bool xbf, int64_t rows, int64_t cols, v
 }
 
 // Blocks of 128 x 128: a workgroup a block, 64 values a thread in registers, 4 columns of
-// 16 rows, 8 rows apart. Bound by HBM: 262144 rows of 2048 in float32, 2.7 GB, in 442 us (6.1 TB/s).
+// 16 rows, 8 rows apart. Bound by HBM: 262144 rows of 2048 in float32, 2.7 GB, in 440 to 470 us by the card (5.7
+// to 6.1 TB/s).
 template <bool BF>
 __global__ __launch_bounds__(256) void k_f8_blocks(F8Rows q) {
   __shared__ uint32_t part[4];
@@ -333,8 +334,8 @@ HX_DEV uint32_t f8_max_of_4(uint32_t m) {
 }
 
 // A block of a row by 32 lanes, 4 values a lane, into LDS: its 128 codes and its scale. (By the lanes
-// that hold an operand each value is quantised by all 16 columns of a row alone: 7.4 us
-// where this takes 5.)
+// that hold an operand each value is quantised by all 16 columns of a row alone: a layer of 4096 x
+// 2048 took 7.4 us for a row so, and 5 by this.)
 template <bool BF, bool NEAR = false>
 HX_DEV void f8_block_to_lds(const void* x, int64_t row_at, int K, int b, uint8_t* codes, float* scale) {
   const int l = lane_id() & 31, c0 = 128 * b + 4 * l;
@@ -372,7 +373,7 @@ HX_DEV void f8_store(void* y, int64_t at, float v, bool bf) {
 // Workgroup: 16 features; its 8 waves share K block by block and add up in LDS. CT columns
 // of 16 rows. QUANT: a few rows as the caller has them, quantised into LDS by every workgroup (a
 // launch less); the weights are on their way meanwhile. Bound by latency: 1 row, 4096 x 2048, 8.4 MB
-// in 5 us (a launch, two round trips to memory, the sum through LDS).
+// in 3.7 us (a launch, two round trips to memory, the sum through LDS).
 template <bool BF, int CT, bool QUANT, bool WIDE>
 __global__ __launch_bounds__(512) void k_f8_few_rows(F8LinearArgs a) {
   constexpr int PITCH = 16 * CT + 1;
@@ -775,16 +776,18 @@ static void f8_linear_tiled(const F8LinearArgs& a, hipStream_t s) {
   hx_launch(k_f8_linear<FT, TT, WF, WR, NS, KS, WIDE>, dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * WF * WR * KS), 0, s, a);
 }
 
-// Rows that the few-row kernel quantises itself: what that takes grows with them, a launch for it
-// costs about 3 us; and they have to fit in LDS.
-static size_t f8_few_lds(int64_t M, int64_t K) { return (size_t)M * (f8_pitch((int)K) + 4 * f8_blocks(K)); }
-bool f8_quant_inside(int64_t M, int64_t K) { return M <= F8_QUANT_ROWS && f8_few_lds(M, K) <= 32 * 1024; }
+// Rows that the few-row kernel quantises itself: every workgroup takes about 0.5 us for 16 blocks, a launch for
+// it 2 us. us with one and with the other: layers of 4096 x 2048, 2 rows 4.2 and 5.7, 4 rows 5.2 and 6.0, 5 rows
+// (80 blocks) 5.7 and 6.1, 6 rows 6.3 and 6.1; 2048 x 4096, 2 rows 6.1 and 6.9, 3 rows 7.2 and 6.9. A tile
+// of rows at most.
+bool f8_quant_inside(int64_t M, int64_t K) { return M <= 16 && M * f8_blocks(K) <= F8_QUANT_BLOCKS; }
+static uint32_t f8_few_lds(int64_t M, int64_t K) { return (uint32_t)(M * (f8_pitch((int)K) + 4 * f8_blocks(K))); }
 
 template <bool WIDE>
 static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
   const dim3 few((unsigned)f8_tiles(a.N));
   if (f8_quant_inside(a.M, a.K)) {
-    const uint32_t lds = (uint32_t)f8_few_lds(a.M, a.K);
+    const uint32_t lds = f8_few_lds(a.M, a.K);
     if (a.xbf) hx_launch(k_f8_few_rows<true, 1, true, WIDE>, few, dim3(512), lds, s, a);
     else hx_launch(k_f8_few_rows<false, 1, true, WIDE>, few, dim3(512), lds, s, a);
     return hipGetLastError();
@@ -793,7 +796,8 @@ static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
   if (e != hipSuccess) return e;
   if (a.M <= 16) hx_launch(k_f8_few_rows<true, 1, false, WIDE>, few, dim3(512), 0, s, a);
   else if (a.M <= 32) hx_launch(k_f8_few_rows<true, 2, false, WIDE>, few, dim3(512), 0, s, a);
-  else if (a.M <= F8_FEW_ROWS) hx_launch(k_f8_few_rows<true, 4, false, WIDE>, few, dim3(512), 0, s, a);
+  else if (a.M <= F8_FEW_ROWS)   // 33, 40, 48 rows x 4096 x 2048 8.8, 9.3, 9.9 us, by tiles 10.0 to 10.1; x 2048 x 4096 12.1, 13.4, 14.4 and 13.9
+    hx_launch(k_f8_few_rows<true, 3, false, WIDE>, few, dim3(512), 0, s, a);
   else {
     // The larger a tile, the fewer loads and LDS reads a product takes, if the tiles fill the chip: one
     // of 256 x 256 a CU, two of 128 x 128, which take a third of its time. us with tiles of 256, 128, 64
@@ -823,7 +827,8 @@ hipError_t launch_f8_linear(const F8LinearArgs& a, hipStream_t s) { return a.ybf
 // features; KW waves share a group's K and add up in LDS. h leaves in f32: its blocks of 128
 // are of several workgroups, the down kernels quantise it. ONE token: an expert a chosen entry. QUANT: the
 // tokens are quantised into LDS by every workgroup, their expert's weights on their way meanwhile;
-// more tokens come quantised. Bound by latency and the weight stream: one token's 23 MB in 7.5 us.
+// more tokens come quantised. Bound by latency and the weight stream: one token's 23 MB (11 experts of
+// 512 x 2048) in 7.4 to 8.1 us, 3 TB/s with a launch and the tokens' round trip in it.
 template <bool BF, int KW, bool ONE, bool QUANT>
 __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
   constexpr int FW = 8 / KW;
@@ -923,7 +928,8 @@ static int f8_few_slots(const F8Args& a) { return (a.T == 1 ? a.k : std::min(a.T
 
 // Down and combine of one token. Workgroup: 16 outputs; its 16 waves take the entries in turn, 4 blocks
 // of K together, half a wave quantises a block of h, each product is weighed in f32, and the waves
-// add up in LDS.
+// add up in LDS. Bound by latency: 11.5 MB (11 experts, 2048 outputs) in 4.2 to 4.8 us, on 128 workgroups: the entry, its
+// weights and h, the sum.
 template <bool WIDE>
 __global__ __launch_bounds__(1024) void k_f8_one_down(F8Args a) {
   __shared__ float red[16][16];
@@ -981,7 +987,8 @@ __global__ __launch_bounds__(1024) void k_f8_one_down(F8Args a) {
 
 // Outputs of the experts for 2 to 16 tokens, unweighted and in f32, in the row of the token's
 // first entry with the expert. Workgroup: a chosen expert (slot) and 128 outputs, 32 a wave; 4 blocks of
-// h at a time, quantised into LDS.
+// h at a time, quantised into LDS (its workgroups share no block's codes: 16 of 2048 outputs quantise an h of
+// 512 each, less than a launch for it). Bound by the weight stream and its start: a workgroup has 64 KB.
 template <bool WIDE>
 __global__ __launch_bounds__(256) void k_f8_few_down(F8Args a) {
   constexpr int PITCH = 4 * 128 + 16;
@@ -1045,16 +1052,19 @@ template <bool BF>
 static hipError_t f8_few_gate_up(const F8Args& a, hipStream_t s) {
   const int slots = f8_few_slots(a), groups = (std::max(a.I, a.Is) + 15) / 16;
   const bool in = f8_quant_inside(a.T, a.H);
-  const uint32_t lds = in ? (uint32_t)f8_few_lds(a.T, a.H) : 0;
-  // K shared by 8 waves where there are few of them, by 2 where a wave's start costs more than it saves
-  const bool few = slots * groups < 1200;
-  const dim3 g(few ? groups : (groups + 3) / 4, slots);
+  const uint32_t lds = in ? f8_few_lds(a.T, a.H) : 0;
+  // K shared by 8 waves where there are few groups, else by 4: a workgroup's start is shared by more work. us with 8
+  // and 4 (2), experts of 512 x 2048: 672 groups 24.9 and 23.5 (23.8), 1312 41.8 and 36.5 (38.2), 5152
+  // 103.7 and 97.6 (100.7); of 256 x 2048: 384 groups 19.9 and 18.8 (19.2); of 128 x 2048: 200 groups 17.1 (2: 18.4).
+  const bool few = a.T == 1 || slots * groups < 350;
+  const dim3 g(few ? groups : (groups + 1) / 2, slots);
 #define FGU(KW, ONE, QUANT) hx_launch(k_f8_few_gate_up<BF, KW, ONE, QUANT>, g, dim3(512), lds, s, a)
-  if (a.T == 1) hx_launch(k_f8_few_gate_up<BF, 8, true, true>, dim3(groups, slots), dim3(512), lds, s, a);   // H is at most 16384
+  if (a.T == 1 && in) FGU(8, true, true);
+  else if (a.T == 1) FGU(8, true, false);
   else if (in && few) FGU(8, false, true);
-  else if (in) FGU(2, false, true);
+  else if (in) FGU(4, false, true);
   else if (few) FGU(8, false, false);
-  else FGU(2, false, false);
+  else FGU(4, false, false);
 #undef FGU
   return hipGetLastError();
 }
@@ -1076,7 +1086,8 @@ hipError_t launch_f8_few_down(const F8Args& a, hipStream_t s) {
 
 // ---------------------------------------------------------------- experts, grouped
 // Workgroups 0 .. chunks - 1: the chunk's entries by expert (mx_chunk_entries); the others: the
-// tokens' rows, a thread 16 values.
+// tokens' rows, a thread 16 values. Bound by the launch (64 tokens of 2048: 6 us), then by HBM: 8192 tokens,
+// 50 MB, 13 to 15 us, the entries by expert meanwhile.
 template <bool BF>
 __global__ __launch_bounds__(256) void k_f8_prep(F8Args a) {
   __shared__ MxPlace sm;
@@ -1108,7 +1119,9 @@ int f8_tile_m(int64_t T, int64_t F, int E, int H, bool xbf) {
 }
 
 // h = q(silu(G x) * (U x)). Workgroup: a tile of TM rows and 128 features, a block of h's
-// columns: 32 a wave, gate and up of a feature in the same lane.
+// columns: 32 (16 of 8) a wave, gate and up of a feature in the same lane. Bound by the weights' way
+// from HBM into the CU: 512 experts of 512 x 2048, 1.07 GB, 64 tokens 0.69 of them in 118 to 127 us (5.5 to
+// 5.9 TB/s); 512 tokens 200 us (5.4 TB/s), the load units 97 % of the time at work, the matrix cores 8.
 template <int TM, bool WIDE, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_gate_up(F8Args a) {
   constexpr int TT = TM / 16, NF = 8 / NW, NM = 2 * NF;   // NF: a wave's tiles of features
@@ -1211,7 +1224,7 @@ HX_DEV void f8_out_rows(const F8Args& a, const f8_v4f (&acc)[NM][TT], uint8_t* t
 }
 
 // Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256
-// outputs. bf16 activations: outputs leave as f16 with a scale for each 32, 2^-12 of a value at
+// outputs. Bound as gate/up: 512 tokens, 0.54 GB, in 107 us (5 TB/s); 64 tokens 61 to 65 us. bf16 activations: outputs leave as f16 with a scale for each 32, 2^-12 of a value at
 // most for half of the bytes that float32 takes here and in the combine (bf16, 2^-9, would be half
 // of the result's own error on top of it).
 template <int TM, bool WIDE, int NW>
@@ -1258,7 +1271,10 @@ __global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_down(F8Args a) {
 }
 
 // The same two products where experts have many rows: both operands through LDS (F8Core), tiles of
-// 128 rows; the waves of a tile's second half bring loads only where it has 64 rows or fewer.
+// 128 rows; the waves of a tile's second half bring loads only where it has 64 rows or fewer. Bound by the
+// loads' latency at two waves a SIMD, with a barrier a stage: 8192 tokens, ten experts each, gate/up 378 GFLOP in 355 to 430 us by
+// the routing (1 PFLOP/s; the load units 73 % at work, the matrix cores 28 %), down 189 GFLOP in 270 to 310 us (86 %, 18 %:
+// K is four stages, each output leaves with 2 bytes and the rows' 0.39 GB are written).
 __global__ __launch_bounds__(512, 2) void k_f8_gate_up_many(F8Args a) {
   typedef F8Core<4, 4, 4, 2, 2> Core;
   constexpr int TT = 4, TR = Core::TR, PITCH = 128 + 16;
