@@ -18,7 +18,8 @@
 // (weighted rows) and combine. MXFP4 experts take the router and the per-token routing
 // (hx_moe_experts: the caller's), then hx_mx.hip's kernels: gate/up, down and combine of
 // up to 8 tokens (one token's down combines), else records, dispatch, gate/up, down,
-// combine.
+// combine. E4M3 experts alike, by hx_f8.hip's: up to 16 tokens gate/up (which quantises a few
+// tokens itself), down and combine, else rows and places, dispatch, gate/up, down, combine.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>

@@ -111,7 +111,10 @@ typedef struct hx_moe_f8_scales {
  * HX_F8_E4M3; H, I and Is multiples of 32. Every call on a block takes such a handle.
  * Its arithmetic is that of these checkpoints: the rows that meet a projection (the
  * tokens, then h = silu(g) u) are quantised by hx_quantize_f8's rule with blocks of 1 x 128,
- * products are of the codes, sums in f32 per block times both scales. */
+ * products are of the codes, sums in f32 per block times both scales. A block of a row that holds a NaN
+ * or an infinity makes its row's outputs NaN. For HX_BF16 activations a block's products are added
+ * by the matrix cores in fixed point (about 1e-5 of their norm), and above 16 tokens the experts'
+ * outputs are held with 11 bits until the weighted f32 sum; for HX_F32 neither. */
 int hx_moe_create_f8(const hx_moe_config* cfg, const hx_moe_weights* w, const hx_moe_f8_scales* scales, int device,
                      hx_moe** out);
 
