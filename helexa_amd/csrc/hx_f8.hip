@@ -1119,8 +1119,8 @@ int f8_tile_m(int64_t T, int64_t F, int E, int H, bool xbf) {
 }
 
 // h = q(silu(G x) * (U x)). Workgroup: a tile of TM rows and 128 features, a block of h's
-// columns: 32 (16 of 8) a wave, gate and up of a feature in the same lane. Bound by the weights' way
-// from HBM into the CU: 512 experts of 512 x 2048, 1.07 GB, 64 tokens 0.69 of them in 118 to 127 us (5.5 to
+// columns: 32 a wave (16 where there are 8), gate and up of a feature in the same lane. Bound by the weights' way
+// from HBM into the CU: 512 experts of 512 x 2048, 1.07 GB; 64 tokens, 0.69 GB of it, 118 to 127 us (5.5 to
 // 5.9 TB/s); 512 tokens 200 us (5.4 TB/s), the load units 97 % of the time at work, the matrix cores 8.
 template <int TM, bool WIDE, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_gate_up(F8Args a) {
@@ -1223,10 +1223,10 @@ HX_DEV void f8_out_rows(const F8Args& a, const f8_v4f (&acc)[NM][TT], uint8_t* t
   Out::store(tl, min(rows, 16 * TT), 2 * (a.H - 16 * n0), [&](int r) { return (uint8_t*)a.obuf + ((p0 + r) * a.H + 16 * n0) * 2; });
 }
 
-// Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256
-// outputs. Bound as gate/up: 512 tokens, 0.54 GB, in 107 us (5 TB/s); 64 tokens 61 to 65 us. bf16 activations: outputs leave as f16 with a scale for each 32, 2^-12 of a value at
-// most for half of the bytes that float32 takes here and in the combine (bf16, 2^-9, would be half
-// of the result's own error on top of it).
+// Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 outputs. Bound as
+// gate/up: 512 tokens, 0.54 GB, in 107 us (5 TB/s); 64 tokens 61 to 65 us. bf16 activations: outputs leave
+// as f16 with a scale for each 32, 2^-12 of a value at most for half of the bytes that float32 takes
+// here and in the combine (bf16, 2^-9, would be half of the result's own error on top of it).
 template <int TM, bool WIDE, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_down(F8Args a) {
   constexpr int TT = TM / 16, NM = 16 / NW;
