@@ -13,9 +13,11 @@
 //
 // The instruction adds the products that a lane holds in fixed point, 13 bits below the
 // exponent of the largest (measured: 2^14 + 2^1 is kept, of 2^14 + 2^0 the second is lost; what
-// the four lanes of a row hold is added in float32). A sum is off by about 1e-5 of its norm so,
-// far below a bf16 result's own rounding. Float32 results (WIDE) take the codes as bf16,
-// which is exact, and v_mfma_f32_16x16x32_bf16, four for a block at half the rate: 3e-7.
+// the four lanes of a row hold is added in float32). A sum is off by 1.4e-5 of its norm so for normal
+// inputs, by 3e-5 where one column in 100 is 16 times the others (measured); a bf16 result's own
+// rounding is 1.7e-3. Float32 results (WIDE) take the codes as bf16, which is exact, and
+// v_mfma_f32_16x16x32_bf16, four for a block at half the rate: 1e-8 a block. Gate/up's sums are
+// taken so for bf16 too where it costs little (launch_f8_gate_up): h's codes hang on them.
 #include <algorithm>
 
 #include "hx_f8.h"
@@ -286,6 +288,17 @@ HX_DEV f8_v4f f8_zero4() { return f8_v4f{0.f, 0.f, 0.f, 0.f}; }
 HX_DEV f8_v8i f8_op(const uint4& a, const uint4& b) {
   return f8_v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
+// part c of 4 of an operand's codes as bf16, which is exact
+HX_DEV f8_v8bf f8_part(const f8_v8i& v, int c) {
+  f8_v8bf r;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const f8_v2bf lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)v[2 * c + j], 1.f, false);
+    const f8_v2bf hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)v[2 * c + j], 1.f, true);
+    r[4 * j] = lo[0]; r[4 * j + 1] = lo[1]; r[4 * j + 2] = hi[0]; r[4 * j + 3] = hi[1];
+  }
+  return r;
+}
 // an operand as the products take it
 template <bool WIDE>
 struct F8Arg;
@@ -301,13 +314,7 @@ struct F8Arg<true> {
   HX_DEV F8Arg() {}
   HX_DEV explicit F8Arg(const f8_v8i& c) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const f8_v2bf lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)c[2 * i + j], 1.f, false);
-        const f8_v2bf hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)c[2 * i + j], 1.f, true);
-        v[i][4 * j] = lo[0]; v[i][4 * j + 1] = lo[1]; v[i][4 * j + 2] = hi[0]; v[i][4 * j + 3] = hi[1];
-      }
+    for (int i = 0; i < 4; i++) v[i] = f8_part(c, i);
   }
 };
 // a block of K: scales of 0 select the instruction's form without any
@@ -319,6 +326,18 @@ HX_DEV f8_v4f f8_mfma(const F8Arg<true>& w, const F8Arg<true>& x) {
 #pragma unroll
   for (int i = 0; i < 4; i++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], d, 0, 0, 0);
   return d;
+}
+// two tiles of features with the same rows, exact, a part of the operands at a time (as bf16 all at
+// once they took 20 registers more and a CU a workgroup less: 4 tokens' experts 38.3 us for 35.7)
+HX_DEV void f8_exact_two(const f8_v8i& w0, const f8_v8i& w1, const f8_v8i& x, f8_v4f& d0, f8_v4f& d1) {
+  d0 = d1 = f8_zero4();
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const f8_v8bf xc = f8_part(x, c);
+    d0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_part(w0, c), xc, d0, 0, 0, 0);
+    d1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_part(w1, c), xc, d1, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 HX_DEV void f8_add(f8_v4f& acc, const f8_v4f& d, float s) {
 #pragma unroll
@@ -895,12 +914,12 @@ __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
     for (int i = 0; i < 2; i++) {
       const int b = b0 + i * KW;
       if (b >= KB) break;
-      const F8Arg<!BF> wg(f8_op(ring[i][0][0], ring[i][0][1])), wu(f8_op(ring[i][1][0], ring[i][1][1]));
-      const F8Arg<!BF> x(f8_operand(row, b));
-      const float s = xs[b], sg = s * rs[i][0], su = s * rs[i][1];
+      const float s = xs[b];
+      f8_v4f g, u;
+      f8_exact_two(f8_op(ring[i][0][0], ring[i][0][1]), f8_op(ring[i][1][0], ring[i][1][1]), f8_operand(row, b), g, u);
+      f8_add(ag, g, s * rs[i][0]);
+      f8_add(au, u, s * rs[i][1]);
       fetch(i, b + 2 * KW);
-      f8_add(ag, f8_mfma(wg, x), sg);
-      f8_add(au, f8_mfma(wu, x), su);
     }
   }
 #pragma unroll
@@ -1054,9 +1073,10 @@ static hipError_t f8_few_gate_up(const F8Args& a, hipStream_t s) {
   const bool in = f8_quant_inside(a.T, a.H);
   const uint32_t lds = in ? f8_few_lds(a.T, a.H) : 0;
   // K shared by 8 waves where there are few groups, else by 4: a workgroup's start is shared by more work. us with 8
-  // and 4 (2), experts of 512 x 2048: 672 groups 24.9 and 23.5 (23.8), 1312 41.8 and 36.5 (38.2), 5152
-  // 103.7 and 97.6 (100.7); of 256 x 2048: 384 groups 19.9 and 18.8 (19.2); of 128 x 2048: 200 groups 17.1 (2: 18.4).
-  const bool few = a.T == 1 || slots * groups < 350;
+  // and 4, experts of 512 x 2048: 672 groups 26.5 and 26.0, 1312 41.0 and 35.9, 5152 105.3 and 98.9; of 256 x 2048: 320
+  // groups 18.6 and 17.3; of 128 x 2048: 168 groups 15.1 and 15.7, 248 16.4 and 17.1, 328 19.6 and 18.8; of 1024 x
+  // 4096, whose K is long: 512 groups 29.0 and 29.0, 1024 41.3 and 42.1.
+  const bool few = a.T == 1 || slots * groups < 300;
   const dim3 g(few ? groups : (groups + 1) / 2, slots);
 #define FGU(KW, ONE, QUANT) hx_launch(k_f8_few_gate_up<BF, KW, ONE, QUANT>, g, dim3(512), lds, s, a)
   if (a.T == 1 && in) FGU(8, true, true);
@@ -1362,26 +1382,28 @@ __global__ __launch_bounds__(256, 2) void k_f8_down_many(F8Args a) {
   f8_out_rows<4, 4>(a, acc, buf + core.wave * (64 * F8Out<128>::PITCH), p0 + r0, rows - r0, 8 * nt + 4 * core.wf);
 }
 
-#define F8_LAUNCH(KERNEL, NX)                                                                  \
-  const dim3 g((unsigned)((int64_t)(NX) * ((a.max_tiles + 7) / 8 * 8)));                       \
-  if (!a.xbf) hx_launch(KERNEL<32, true, 4>, g, dim3(256), 0, s, a);                           \
-  else if (a.tile_m == 32) hx_launch(KERNEL<32, false, 4>, g, dim3(256), 0, s, a);             \
-  else hx_launch(KERNEL<64, false, 8>, g, dim3(512), 0, s, a)
+// workgroups for the tiles of a call, nx for each
+static dim3 f8_grid(const F8Args& a, int nx) { return dim3((unsigned)((int64_t)nx * ((a.max_tiles + 7) / 8 * 8))); }
 
+// Gate/up's products are exact for few tokens and with tiles of 32 rows, whichever the activations' type: what the
+// fp8 instruction drops moves some of h's codes to a neighbour, and so the outputs by another 1.0e-3 to 2.5e-3 of their
+// norm, as much as bf16's own rounding (1.7e-3). us of a call by the fp8 instruction and exact: 1 token 13.0 and 13.4, 4
+// 35.2 and 35.7, 16 97.9 and 98.8, 64 219.1 and 217.7, 512 311.2 and 310.4, 900 325.1 and 322.7. With larger tiles it stays with the
+// fp8 instruction, which is off by 1.3e-3 there: exact sums cost 12 to 15 % (1024 tokens 332 and 383, 2048 365 and
+// 410, 8192 762 and 866).
 hipError_t launch_f8_gate_up(const F8Args& a, hipStream_t s) {
-  if (a.tile_m == 128) {
-    hx_launch(k_f8_gate_up_many, dim3((unsigned)((int64_t)a.hblocks * ((a.max_tiles + 7) / 8 * 8))), dim3(512), 0, s, a);
-    return hipGetLastError();
-  }
-  F8_LAUNCH(k_f8_gate_up, a.hblocks);
+  const dim3 g = f8_grid(a, a.hblocks);
+  if (a.tile_m == 32) hx_launch(k_f8_gate_up<32, true, 4>, g, dim3(256), 0, s, a);
+  else if (a.tile_m == 64) hx_launch(k_f8_gate_up<64, false, 8>, g, dim3(512), 0, s, a);
+  else hx_launch(k_f8_gate_up_many, g, dim3(512), 0, s, a);
   return hipGetLastError();
 }
 hipError_t launch_f8_down(const F8Args& a, hipStream_t s) {
-  if (a.tile_m == 128) {
-    hx_launch(k_f8_down_many, dim3((unsigned)((int64_t)((a.H + 127) / 128) * ((a.max_tiles + 7) / 8 * 8))), dim3(256), 0, s, a);
-    return hipGetLastError();
-  }
-  F8_LAUNCH(k_f8_down, (a.H + 255) / 256);
+  const dim3 g = f8_grid(a, (a.H + 255) / 256);
+  if (!a.xbf) hx_launch(k_f8_down<32, true, 4>, g, dim3(256), 0, s, a);
+  else if (a.tile_m == 32) hx_launch(k_f8_down<32, false, 4>, g, dim3(256), 0, s, a);
+  else if (a.tile_m == 64) hx_launch(k_f8_down<64, false, 8>, g, dim3(512), 0, s, a);
+  else hx_launch(k_f8_down_many, f8_grid(a, (a.H + 127) / 128), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

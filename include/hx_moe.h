@@ -112,9 +112,12 @@ typedef struct hx_moe_f8_scales {
  * Its arithmetic is that of these checkpoints: the rows that meet a projection (the
  * tokens, then h = silu(g) u) are quantised by hx_quantize_f8's rule with blocks of 1 x 128,
  * products are of the codes, sums in f32 per block times both scales. A block of a row that holds a NaN
- * or an infinity makes its row's outputs NaN. For HX_BF16 activations a block's products are added
- * by the matrix cores in fixed point (about 1e-5 of their norm), and above 16 tokens the experts'
- * outputs are held with 11 bits until the weighted f32 sum; for HX_F32 neither. */
+ * or an infinity makes its row's outputs NaN. For HX_F32 activations products are exact and every sum is
+ * in f32. For HX_BF16 down's products are added by the matrix cores in fixed point, 13 bits below the
+ * largest of each 32 (off by 1.4e-5 to 3e-5 of a sum's norm; the result's own rounding is 1.7e-3), and above
+ * 16 tokens the experts' outputs are held with 11 bits until the weighted f32 sum. Above 16 tokens and
+ * 18 chosen entries for each of the E experts gate's and up's products are added so too: some codes of h then
+ * become their neighbours, which adds about 1.3e-3 of the outputs' norm. */
 int hx_moe_create_f8(const hx_moe_config* cfg, const hx_moe_weights* w, const hx_moe_f8_scales* scales, int device,
                      hx_moe** out);
 
