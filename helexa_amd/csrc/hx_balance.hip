@@ -344,7 +344,7 @@ static hipError_t launch_balance(BalArgs a, bool bf, hipStream_t s) {
   const int chunks = vec ? a.E / per : a.E;
   a.lpr = 64;
   while (a.lpr > 1 && a.lpr / 2 >= chunks) a.lpr /= 2;
-  if (!one) hx_launch(k_bal_counts, dim3(a.G1), dim3(1024), 0, s, a);
+  if (!one && a.T > 0) hx_launch(k_bal_counts, dim3(a.G1), dim3(1024), 0, s, a);   // no tokens: no chunks
   const int nj = (chunks + 63) / 64;
   if (bf && vec) {
     if (nj <= 1) launch_rows<true, 8, 1>(a, one, s);
