@@ -1,6 +1,7 @@
 // What the files of the C ABI share: statuses with a message, the current device.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 #include "hx_moe.h"
 
@@ -20,6 +21,11 @@ inline bool capturing(hipStream_t s) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   (void)hipStreamIsCapturing(s, &st);
   return st != hipStreamCaptureStatusNone;
+}
+
+// whether the n bytes at a and the m bytes at b have one in common
+inline bool overlap(const void* a, size_t n, const void* b, size_t m) {
+  return (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
 }
 
 // a handle's device as the current one, and the caller's again

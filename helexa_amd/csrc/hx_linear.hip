@@ -114,6 +114,9 @@ extern "C" int hx_linear_forward(hx_linear* l, const void* x, int x_dtype, int64
   if (n_rows > HX_MAX_TOKENS) return fail(HX_ERR_UNSUPPORTED, "too many rows in one call");
   if (((uintptr_t)x & (x_dtype == HX_F32 ? 3 : 1)) || ((uintptr_t)y & (y_dtype == HX_F32 ? 3 : 1)))
     return fail(HX_ERR_INVALID_ARGUMENT, "x or y does not start on an element");
+  // few rows: every workgroup quantises all of x, while others write their features of y
+  if (overlap(x, (size_t)(n_rows * l->K) * (x_dtype == HX_F32 ? 4 : 2), y, (size_t)(n_rows * l->N) * (y_dtype == HX_F32 ? 4 : 2)))
+    return fail(HX_ERR_INVALID_ARGUMENT, "hx_linear_forward: x and y overlap");
   DeviceScope dev(l->device);
   HX_HIP(dev.err);
   hipStream_t s = (hipStream_t)stream;

@@ -636,8 +636,8 @@ class F8Linear:
 
     def forward(self, xs, out_dtype=None, workspace=None, stream=None, out=None):
         """xs [.., in] float32 or bfloat16 on the layer's GPU -> [.., out] of xs's type or out_dtype.
-        `out`, if given, is a contiguous tensor of that shape and type to write. Without a
-        workspace of workspace_size() bytes the layer keeps its own; a captured call must
+        `out`, if given, is a contiguous tensor of that shape and type to write, which shares no
+        memory with xs. Without a workspace of workspace_size() bytes the layer keeps its own; a captured call must
         bring it."""
         import torch
         if not xs.is_cuda or xs.get_device() != self.device:

@@ -284,7 +284,7 @@ int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t cols, int b
  * hx_linear_create copies codes [out, in] and scales [ceil(out / 128), ceil(in / 128)] from
  * location (HX_HOST or HX_DEVICE) to device memory of its own and lays them out; sizes need not be
  * whole blocks (out at most 2^20, in 2^17). hx_linear_forward: x [n_rows, in] and y
- * [n_rows, out], HX_F32 or HX_BF16 each, not overlapping; n_rows 0 is a no-op. A row that
+ * [n_rows, out], HX_F32 or HX_BF16 each, without a byte in common (HX_ERR_INVALID_ARGUMENT); n_rows 0 is a no-op. A row that
  * holds a NaN or an infinity gets NaN, the others' results do not depend on it nor on how the
  * rows are split into calls, but for the last bits of the sums. workspace: hx_linear_workspace_size
  * bytes for n_rows rows or any fewer (0: none is used), 16-byte aligned; NULL: the handle grows its own,

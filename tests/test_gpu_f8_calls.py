@@ -1,0 +1,44 @@
+"""E4M3 layers and their quantiser: calls whose memory overlaps, types and sizes at the edges of what they take."""
+import numpy as np
+import pytest
+
+import f8 as F
+
+pytestmark = pytest.mark.gpu
+
+
+def cuda(a, bf=False):
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t.to(torch.bfloat16) if bf else t
+
+
+@pytest.mark.parametrize("bf", [False, True])
+@pytest.mark.parametrize("M", [1, 4, 16, 17, 60, 300])
+def test_a_result_in_its_inputs_place_is_refused(M, bf):
+    """a square layer: in place, and with a row or an element in common on either side; neighbours are fine"""
+    import helexa_amd as hx
+    import torch
+    n = 256
+    layer = hx.F8Linear.load(*(cuda(a) for a in F.make_weights(M, n, n)))
+    x = cuda(np.random.default_rng(M).standard_normal((M, n)).astype(np.float32), bf)
+    want = layer(x)
+    place = torch.zeros(3 * M * n + 16, dtype=x.dtype, device="cuda")
+    mid = place[M * n:2 * M * n].view(M, n)
+    mid.copy_(x)
+    at = lambda i: place[i:i + M * n].view(M, n)
+    for i in (M * n, M * n - 8, M * n + 8, 1, 2 * M * n - 1):
+        with pytest.raises(hx.HxError, match="overlap"):
+            layer(mid, out=at(i))
+    assert torch.equal(mid, x)
+    for i in (0, 2 * M * n):
+        layer(mid, out=at(i))
+        assert torch.equal(at(i), want) and torch.equal(mid, x)
+    wide = torch.zeros(M * n + 2 * M * n, dtype=torch.float32, device="cuda")   # y's bytes are as many as its type says
+    if not bf:
+        wide[:M * n].view(M, n).copy_(x)
+        y = wide.view(torch.bfloat16)
+        with pytest.raises(hx.HxError, match="overlap"):
+            layer(wide[:M * n].view(M, n), out=y[2 * M * n - 1:3 * M * n - 1].view(M, n))
+        layer(wide[:M * n].view(M, n), out=y[2 * M * n:3 * M * n].view(M, n))
+    layer.close()
