@@ -432,6 +432,10 @@ extern "C" int hx_moe_balance_loss(const void* logits, int logits_dtype, int64_t
   // one workgroup writes the routing's own counts while the others read the given ones
   if (given_counts && counts && given_counts < counts + num_experts && counts < given_counts + num_experts)
     return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_balance_loss: counts and given_counts overlap");
+  // a row's gradient goes where the row was, or where no row is
+  const size_t row_bytes = (size_t)n_tokens * num_experts * (logits_dtype == HX_F32 ? 4 : 2);
+  if (dlogits && dlogits != logits && overlap(logits, row_bytes, dlogits, row_bytes))
+    return fail(HX_ERR_INVALID_ARGUMENT, "hx_moe_balance_loss: logits and dlogits overlap in part");
   BalArgs a{};
   if ((rc = bal_args(a, topk_idx, n_tokens, k, num_experts, workspace, workspace_bytes))) return rc;
   a.logits = logits; a.given = given_counts; a.coef = coef;

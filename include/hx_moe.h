@@ -213,7 +213,7 @@ int hx_moe_router_logits(hx_moe* m, const void* x, int64_t n_tokens, const float
  * given_counts (device int32 [E]; null: own) where the load of several calls or
  * devices is balanced together. Outputs: loss f32 [1], probs f32 [E] (P), counts
  * int32 [E] (the routing's own; may be null, not given_counts' place), dlogits (logits' type; may be null, may
- * be logits). No live token, or no entry in c: loss 0, gradient 0. A live row that
+ * be logits, else no byte of them). No live token, or no entry in c: loss 0, gradient 0. A live row that
  * holds a NaN, +inf or nothing but -inf makes loss, probs and its own gradient NaN.
  * Sums run in a fixed order: the same bits for the same inputs. Both calls run on the
  * current device, allocate nothing and need workspace of

@@ -1,0 +1,26 @@
+"""Calls of the E4M3 quantiser and the balance loss that are refused, or done, before they touch a device."""
+import os
+from concurrent.futures import ThreadPoolExecutor
+
+import pytest
+
+from helexa_amd import moe as hx
+
+pytestmark = pytest.mark.skipif(not os.path.exists(hx.LIB_PATH), reason="libhxmoe.so not built")
+P = 1 << 20   # a pointer that a refused call never follows
+
+
+def alone(f):
+    """f() and the error text in a thread of its own: the last error is the thread's"""
+    with ThreadPoolExecutor(1) as ex:
+        return ex.submit(lambda: (f(), hx.last_error())).result()
+
+
+@pytest.mark.parametrize("dt,size", [(hx.F32, 4), (hx.BF16, 2)])
+def test_a_gradient_over_other_rows_of_the_logits(dt, size):
+    """8 tokens x 16 experts: off by an element to all but one, on either side"""
+    n = 8 * 16 * size
+    for at in (size, -size, 16 * size, n - size, size - n):
+        rc, text = alone(lambda: hx.lib().hx_moe_balance_loss(P, dt, 8, 16, 1 << 24, 4, None, 1.0, 1 << 25, None, 1 << 26, P + at, 1 << 27,
+                                                              1 << 20, None))
+        assert rc == 1 and "overlap" in text
