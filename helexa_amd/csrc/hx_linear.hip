@@ -1,4 +1,5 @@
 // C ABI of the E4M3 quantiser and the linear layer on such weights.
+#include <algorithm>
 #include <new>
 
 #include "hx_abi.h"
@@ -26,9 +27,14 @@ extern "C" int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t 
   if ((uintptr_t)x & (x_dtype == HX_F32 ? 3 : 1)) return fail(HX_ERR_INVALID_ARGUMENT, "x does not start on an element");
   if ((uintptr_t)scales & 3) return fail(HX_ERR_INVALID_ARGUMENT, "the scales do not start on an element");
   // a row's columns are indexed by 32 bits, bytes by 64
-  if (cols > ((int64_t)1 << 31) - 128 || rows > (int64_t)1 << 38)
+  if (cols > ((int64_t)1 << 31) - 128 || rows > std::min((int64_t)1 << 38, ((int64_t)1 << 48) / cols))
     return fail(HX_ERR_UNSUPPORTED, "hx_quantize_f8: %lld rows of %lld are too many", (long long)rows, (long long)cols);
   if (rows == 0) return HX_OK;
+  // a block is read by several threads, its codes and scale leave while others are read
+  const size_t n = (size_t)rows * cols, xb = n * (x_dtype == HX_F32 ? 4 : 2),
+               sb = sizeof(float) * (size_t)((rows + block_rows - 1) / block_rows) * f8_blocks(cols);
+  if (overlap(x, xb, codes, n) || overlap(x, xb, scales, sb) || overlap(codes, n, scales, sb))
+    return fail(HX_ERR_INVALID_ARGUMENT, "hx_quantize_f8: x, codes and scales overlap");
   if (block_rows == 1) HX_HIP(launch_f8_rows(x, x_dtype == HX_BF16, rows, cols, codes, scales, false, (hipStream_t)stream));
   else HX_HIP(launch_f8_blocks(x, x_dtype == HX_BF16, rows, cols, codes, scales, (hipStream_t)stream));
   return HX_OK;

@@ -273,7 +273,8 @@ int hx_quantize_activations(int weight_dtype, const void* x, int x_dtype, int64_
  * the edges: codes [rows, cols] bytes, scales f32 [ceil(rows / block_rows), ceil(cols / 128)].
  * A block's scale is max(max|x| / 448, 2^-126), rounded to f32; a code is the E4M3 value
  * nearest to x / scale, the exact quotient, ties to the even code. A block that holds a NaN
- * or an infinity gets the scale NaN and codes 0. cols at most 2^31 - 128. On the current device. */
+ * or an infinity gets the scale NaN and codes 0. cols at most 2^31 - 128; x, codes and scales have no byte
+ * in common (HX_ERR_INVALID_ARGUMENT). On the current device. */
 int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t cols, int block_rows, void* codes, float* scales,
                    void* stream);
 

@@ -24,3 +24,16 @@ def test_a_gradient_over_other_rows_of_the_logits(dt, size):
         rc, text = alone(lambda: hx.lib().hx_moe_balance_loss(P, dt, 8, 16, 1 << 24, 4, None, 1.0, 1 << 25, None, 1 << 26, P + at, 1 << 27,
                                                               1 << 20, None))
         assert rc == 1 and "overlap" in text
+
+
+@pytest.mark.parametrize("dt,size", [(hx.F32, 4), (hx.BF16, 2)])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_the_quantiser_in_its_inputs_place(block_rows, dt, size):
+    """300 rows of 260: codes in x's place, at its last byte, its first; scales in x, in the codes"""
+    n, s = 300 * 260, 4 * 3 * (300 if block_rows == 1 else 3)
+    far = 1 << 28
+    for codes, scales in ((P, far), (P + n * size - 1, far), (P - n + 1, far), (far, P), (far, P + n * size - 4), (far, P - s + 4),
+                          (far, far), (far, far + n - 4), (far, far - s + 4)):
+        rc, text = alone(lambda: hx.lib().hx_quantize_f8(P, dt, 300, 260, block_rows, codes, scales, None))
+        assert rc == 1 and "overlap" in text, (codes, scales)
+    assert alone(lambda: hx.lib().hx_quantize_f8(P, dt, 1 << 38, 1 << 12, block_rows, far, far, None))[0] == 2
