@@ -20,7 +20,7 @@ static constexpr int64_t MAX_IN = 1 << 17, MAX_OUT = 1 << 20;
 
 extern "C" int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t cols, int block_rows, void* codes,
                               float* scales, void* stream) {
-  if (!x || !codes || !scales || rows < 0 || cols <= 0) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
+  if (rows < 0 || cols <= 0 || (rows > 0 && (!x || !codes || !scales))) return fail(HX_ERR_INVALID_ARGUMENT, "bad argument");
   if (x_dtype != HX_F32 && x_dtype != HX_BF16) return fail(HX_ERR_UNSUPPORTED, "hx_quantize_f8: x dtype %d", x_dtype);
   if (block_rows != 1 && block_rows != 128)
     return fail(HX_ERR_UNSUPPORTED, "hx_quantize_f8: blocks of 1 or 128 rows, not %d", block_rows);

@@ -37,3 +37,11 @@ def test_the_quantiser_in_its_inputs_place(block_rows, dt, size):
         rc, text = alone(lambda: hx.lib().hx_quantize_f8(P, dt, 300, 260, block_rows, codes, scales, None))
         assert rc == 1 and "overlap" in text, (codes, scales)
     assert alone(lambda: hx.lib().hx_quantize_f8(P, dt, 1 << 38, 1 << 12, block_rows, far, far, None))[0] == 2
+
+
+def test_no_rows_need_no_memory():
+    """an empty tensor has no address"""
+    for block_rows in (1, 128):
+        assert alone(lambda: hx.lib().hx_quantize_f8(None, hx.F32, 0, 128, block_rows, None, None, None))[0] == 0
+        assert alone(lambda: hx.lib().hx_quantize_f8(None, hx.F16, 0, 128, block_rows, None, None, None))[0] == 2
+        assert alone(lambda: hx.lib().hx_quantize_f8(None, hx.F32, 1, 128, block_rows, None, None, None))[0] == 1
