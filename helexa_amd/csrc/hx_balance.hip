@@ -35,7 +35,7 @@ struct BalArgs {
 // tokens a workgroup of the counts takes, and their most
 constexpr int BAL_CHUNK = 1024, BAL_MAX_G1 = 64, BAL_MAX_G2 = 1024;
 static int bal_g1(int64_t T) { return (int)std::min<int64_t>((T + BAL_CHUNK - 1) / BAL_CHUNK, BAL_MAX_G1); }
-// the most of the row pass: a wave has two turns at least
+// the most of the row pass: a wave that takes a row at a time has two turns at least (launch_balance: rows of fewer lanes)
 static int bal_g2(int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t>((T + 15) / 16, BAL_MAX_G2)); }
 
 // hist[0 .. E - 1] += the entries by expert of tokens t0 .. t1 - 1, hist[E] += the live ones
@@ -344,6 +344,11 @@ static hipError_t launch_balance(BalArgs a, bool bf, hipStream_t s) {
   const int chunks = vec ? a.E / per : a.E;
   a.lpr = 64;
   while (a.lpr > 1 && a.lpr / 2 >= chunks) a.lpr /= 2;
+  // a wave takes 64 / lpr rows at a time: a workgroup without rows would sum the counts and leave zeros for the last
+  // kernel to add. us for 16 experts in bf16, with as many workgroups as for whole waves and with these: 8192
+  // tokens 15.7 and 13.5, 32768 22.2 and 15.6, 131072 26.1 and 22.0; two turns a wave here too: 14.7, 16.4, 21.0.
+  const int rows = 8 * (64 / a.lpr);   // of a workgroup's waves
+  a.G2 = (int)std::min<int64_t>(a.G2, std::max<int64_t>(1, (a.T + rows - 1) / rows));
   if (!one && a.T > 0) hx_launch(k_bal_counts, dim3(a.G1), dim3(1024), 0, s, a);   // no tokens: no chunks
   const int nj = (chunks + 63) / 64;
   if (bf && vec) {
