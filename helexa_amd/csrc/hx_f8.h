@@ -64,6 +64,9 @@ hipError_t launch_f8_rows(const void* x, bool xbf, int64_t rows, int64_t cols, v
                           hipStream_t s);
 hipError_t launch_f8_blocks(const void* x, bool xbf, int64_t rows, int64_t cols, void* codes, float* scales, hipStream_t s);
 bool f8_quant_inside(int64_t M, int64_t K);
+// features (and rows, if not exact) of a tile of a layer of more than F8_FEW_ROWS rows: 256, 128, 64, or 0: 64 with K
+// shared by two groups of waves
+int f8_linear_tile(int64_t M, int64_t N, bool exact);
 hipError_t launch_f8_linear(const F8LinearArgs& a, hipStream_t s);
 
 bool f8_few(int T);

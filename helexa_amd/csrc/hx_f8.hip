@@ -802,6 +802,21 @@ static void f8_linear_tiled(const F8LinearArgs& a, hipStream_t s) {
 bool f8_quant_inside(int64_t M, int64_t K) { return M <= 16 && M * f8_blocks(K) <= F8_QUANT_BLOCKS; }
 static uint32_t f8_few_lds(int64_t M, int64_t K) { return (uint32_t)(M * (f8_pitch((int)K) + 4 * f8_blocks(K))); }
 
+// The larger a tile, the fewer loads and LDS reads a product takes, if the tiles fill the chip: one
+// of 256 x 256 a CU, two of 128 x 128, which take a third of its time. us with tiles of 256, 128, 64
+// (quantisation included): 512 rows x 4096 x 2048 48, 19.4, 15.5; 768 rows 37, 21.6, 20.5; 1024 37, 22.5,
+// 25.0; 4096 44.9, 47.9, 64; 5000 (320 tiles of 256) 74, 59, 77; 8192 x 4096: 1024 rows 65, 45, 63; 1536
+// 67, 70, 89; 2304 128, 102, 131; 8192 281, 319, -. A workgroup of 64 a CU: twice the waves share K. 128 rows x
+// 4096 x 2048 11.6 -> 10.5; 512 (2 a CU) 15.5 -> 18.3. Exact products have operands of 16 bits, which leave
+// registers for 128 features x 64 rows.
+int f8_linear_tile(int64_t M, int64_t N, bool exact) {
+  auto tiles = [&](int t) { return ((N + t - 1) / t) * ((M + t - 1) / t); };
+  if (exact) return tiles(128) >= 128 ? 128 : 64;
+  if (3 * ((tiles(256) + 255) / 256) <= (tiles(128) + 255) / 256) return 256;
+  if (tiles(128) >= 224) return 128;
+  return tiles(64) > 256 ? 64 : 0;
+}
+
 template <bool WIDE>
 static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
   const dim3 few((unsigned)f8_tiles(a.N));
@@ -818,23 +833,11 @@ static hipError_t f8_linear(const F8LinearArgs& a, hipStream_t s) {
   else if (a.M <= F8_FEW_ROWS)   // 33, 40, 48 rows x 4096 x 2048 8.8, 9.3, 9.9 us, by tiles 10.0 to 10.1; x 2048 x 4096 12.1, 13.4, 14.4 and 13.9
     hx_launch(k_f8_few_rows<true, 3, false, WIDE>, few, dim3(512), 0, s, a);
   else {
-    // The larger a tile, the fewer loads and LDS reads a product takes, if the tiles fill the chip: one
-    // of 256 x 256 a CU, two of 128 x 128, which take a third of its time. us with tiles of 256, 128, 64
-    // (quantisation included): 512 rows x 4096 x 2048 48, 19.4, 15.5; 768 rows 37, 21.6, 20.5; 1024 37, 22.5,
-    // 25.0; 4096 44.9, 47.9, 64; 5000 (320 tiles of 256) 74, 59, 77; 8192 x 4096: 1024 rows 65, 45, 63; 1536
-    // 67, 70, 89; 2304 128, 102, 131; 8192 281, 319, -.
-    auto tiles = [&](int t) { return ((a.N + t - 1) / t) * ((a.M + t - 1) / t); };
-    if constexpr (WIDE) {   // operands of 16 bits: smaller tiles fit the registers
-      if (tiles(128) >= 128) f8_linear_tiled<4, 2, 2, 2, 2, 1, WIDE>(a, s);
-      else f8_linear_tiled<2, 2, 2, 2, 3, 1, WIDE>(a, s);
-    } else if (3 * ((tiles(256) + 255) / 256) <= (tiles(128) + 255) / 256) {
-      f8_linear_tiled<8, 4, 2, 4, 2, 1, WIDE>(a, s);
-    } else if (tiles(128) >= 224) {
-      f8_linear_tiled<4, 4, 2, 2, 2, 1, WIDE>(a, s);
-    } else if (tiles(64) > 256) {
-      f8_linear_tiled<2, 2, 2, 2, 3, 1, WIDE>(a, s);
-    } else {   // a workgroup a CU: twice the waves share K. 128 rows x 4096 x 2048 11.6 -> 10.5; 512 (2 a CU) 15.5 -> 18.3
-      f8_linear_tiled<2, 2, 2, 2, 3, 2, WIDE>(a, s);
+    switch (f8_linear_tile(a.M, a.N, WIDE)) {
+      case 256: if constexpr (!WIDE) f8_linear_tiled<8, 4, 2, 4, 2, 1, WIDE>(a, s); break;
+      case 128: f8_linear_tiled<4, WIDE ? 2 : 4, 2, 2, 2, 1, WIDE>(a, s); break;
+      case 64: f8_linear_tiled<2, 2, 2, 2, 3, 1, WIDE>(a, s); break;
+      default: if constexpr (!WIDE) f8_linear_tiled<2, 2, 2, 2, 3, 2, WIDE>(a, s); break;
     }
   }
   return hipGetLastError();
