@@ -111,10 +111,11 @@ typedef struct hx_moe_f8_scales {
  * HX_F8_E4M3; H, I and Is multiples of 32. Every call on a block takes such a handle.
  * Its arithmetic is that of these checkpoints: the rows that meet a projection (the
  * tokens, then h = silu(g) u) are quantised by hx_quantize_f8's rule with blocks of 1 x 128,
- * products are of the codes, sums in f32 per block times both scales. A block of a row that holds a NaN
+ * products are of the codes, sums in f32 per block times both scales, whose product is an f32 of its own: below
+ * 2^-126 it has fewer bits (a block is off by 2^-125 at most), past 2^128 it is an infinity. A block of a row that holds a NaN
  * or an infinity makes its row's outputs NaN. For HX_F32 activations products are exact and every sum is
  * in f32. For HX_BF16 down's products are added by the matrix cores in fixed point, 13 bits below the
- * largest of each 32 (off by 1.4e-5 to 3e-5 of a sum's norm; the result's own rounding is 1.7e-3), and above
+ * largest of each 32 (off by 1.4e-5 to 5.5e-5 of a sum's norm; the result's own rounding is 1.7e-3), and above
  * 16 tokens the experts' outputs are held with 11 bits until the weighted f32 sum. Above 16 tokens and
  * 18 chosen entries for each of the E experts gate's and up's products are added so too: some codes of h then
  * become their neighbours, which adds about 1.3e-3 of the outputs' norm. */
@@ -280,7 +281,7 @@ int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t cols, int b
 
 /* A linear layer on HX_F8_E4M3 weights (no bias), the arithmetic of hx_moe_create_f8's
  * projections: y = q(x) W^T, q the rows' quantisation by blocks of 1 x 128, f32 sums, one
- * rounding to y's type. The reference's quantised linear layers
+ * rounding to y's type, whichever x's is: products are exact for HX_F32, added in fixed point for HX_BF16. The reference's quantised linear layers
  * (crates/neuron/src/harness/tp/tp_linear.rs:47-140) have no such format.
  * hx_linear_create copies codes [out, in] and scales [ceil(out / 128), ceil(in / 128)] from
  * location (HX_HOST or HX_DEVICE) to device memory of its own and lays them out; sizes need not be

@@ -42,3 +42,23 @@ def test_a_result_in_its_inputs_place_is_refused(M, bf):
             layer(wide[:M * n].view(M, n), out=y[2 * M * n - 1:3 * M * n - 1].view(M, n))
         layer(wide[:M * n].view(M, n), out=y[2 * M * n:3 * M * n].view(M, n))
     layer.close()
+
+
+@pytest.mark.parametrize("M", [1, 5, 17, 48, 100, 700])
+def test_scales_whose_product_is_subnormal(M):
+    """a product of scales keeps what float32 has there: a block is off by 2^-150 times its codes' products,
+    128 of 448^2 at most, on top of what it is off elsewhere"""
+    import helexa_amd as hx
+    import torch
+    N, K = 300, 520
+    codes, scales = F.make_weights(M, N, K)
+    x = np.random.default_rng(M).standard_normal((M, K)).astype(np.float32)
+    rows = np.arange(M) % 3
+    x *= np.exp2(np.choose(rows, [-100, -114, -125])).astype(np.float32)[:, None]
+    small = (scales * np.float32(2.0 ** -12)).astype(np.float32)
+    assert 0 < F.quantise(x, 1)[1].min() * float(small.max()) < 2.0 ** -126
+    ref, mag, fixed = F.linear(x, codes, small)
+    y = hx.F8Linear.load(cuda(codes), cuda(small))(cuda(x), out_dtype=torch.float32).cpu().numpy().astype(np.float64)
+    off, bound = np.abs(y - ref), F.sum_steps(K) * F.U * mag + F.blocks(K) * 2.0 ** -125
+    print(f"[err] worst {np.max(off / bound):.3f} of the bound", flush=True)
+    assert (off <= bound).all() and np.abs(ref).max() > 2.0 ** -110
