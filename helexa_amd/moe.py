@@ -302,6 +302,10 @@ class Qwen3_5MoeBlock:
         tensors = [t for entry in weights.values() for t in entry[1:]]
         on_dev = any(getattr(t, "is_cuda", False) for t in tensors)
         w.location = HX_DEVICE if on_dev else HX_HOST
+        f8 = any(len(entry) > 2 for entry in weights.values())
+        if f8 and any(t.is_cuda != on_dev or (on_dev and t.get_device() != device) for t in tensors):
+            # the library reads every pointer as of one place
+            raise ValueError(f"the weights must all be on the CPU or all on cuda:{device}")
         for key, field_ in (("router", "router"), ("gate", "experts_gate"), ("up", "experts_up"),
                             ("down", "experts_down"), ("sgate", "shared_gate"), ("sup", "shared_up"),
                             ("sdown", "shared_down"), ("seg", "shared_expert_gate")):
@@ -313,15 +317,13 @@ class Qwen3_5MoeBlock:
                     raise ValueError(f"weight {key}: scales come with F8_E4M3 codes, and only with them")
                 if rest:
                     _check_f8(f"weight {key}", t, rest[0], _f8_shape(cfg, key))
-                    if t.is_cuda != on_dev:
-                        raise ValueError(f"weight {key} is not where the others are")
                     setattr(scales, field_, _ptr(rest[0]))
                 dname = {"experts_gate": "gate_dtype", "experts_up": "up_dtype", "experts_down": "down_dtype",
                          "router": "router_dtype"}.get(field_, field_ + "_dtype")
                 setattr(w, dname, dt)
                 setattr(w, field_, _ptr(t))
         out = C.c_void_p()
-        if any(len(entry) > 2 for entry in weights.values()):
+        if f8:
             if on_dev:   # the library copies on the default stream
                 import torch
                 torch.cuda.current_stream(device).synchronize()

@@ -62,3 +62,21 @@ def test_scales_whose_product_is_subnormal(M):
     off, bound = np.abs(y - ref), F.sum_steps(K) * F.U * mag + F.blocks(K) * 2.0 ** -125
     print(f"[err] worst {np.max(off / bound):.3f} of the bound", flush=True)
     assert (off <= bound).all() and np.abs(ref).max() > 2.0 ** -110
+
+
+@pytest.mark.parametrize("key", ["router", "seg", "gate", "sdown"])
+def test_weights_of_two_places_are_refused(key):
+    """one tensor on the CPU among those on the GPU: a host address is none that a kernel may read"""
+    import helexa_amd as hx
+    import torch
+    H, E, k, I, Is = 96, 4, 2, 64, 32
+    cfg = hx.TextConfig(hidden_size=H, num_experts=E, num_experts_per_tok=k, moe_intermediate_size=I, shared_expert_intermediate_size=Is)
+    w = {n: (hx.F8_E4M3, cuda(c), cuda(s)) for n, (c, s) in F.block(1, H, E, I, Is).items()}
+    w["router"], w["seg"] = (hx.F32, torch.zeros((E, H), device="cuda")), (hx.F32, torch.zeros((1, H), device="cuda"))
+    mixed = {**w, key: (w[key][0],) + tuple(t.cpu() for t in w[key][1:])}
+    with pytest.raises(ValueError, match="all on"):
+        hx.Qwen3_5MoeBlock.load(cfg, mixed, act_dtype=hx.F32)
+    with pytest.raises(ValueError, match="all on"):
+        hx.Qwen3_5MoeBlock.load(cfg, w, act_dtype=hx.F32, device=1)
+    for good in (w, {n: (e[0],) + tuple(t.cpu() for t in e[1:]) for n, e in w.items()}):
+        hx.Qwen3_5MoeBlock.load(cfg, good, act_dtype=hx.F32).close()
