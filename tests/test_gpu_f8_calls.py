@@ -80,3 +80,64 @@ def test_weights_of_two_places_are_refused(key):
         hx.Qwen3_5MoeBlock.load(cfg, w, act_dtype=hx.F32, device=1)
     for good in (w, {n: (e[0],) + tuple(t.cpu() for t in e[1:]) for n, e in w.items()}):
         hx.Qwen3_5MoeBlock.load(cfg, good, act_dtype=hx.F32).close()
+
+
+@pytest.mark.parametrize("M", [4, 16, 30, 400])
+def test_two_calls_at_once(M):
+    """a layer and a block from two streams, a workspace each; then the same as two graphs replayed together"""
+    import helexa_amd as hx
+    import torch
+    n, E, k, I = 256, 8, 2, 128
+    layer = hx.F8Linear.load(*(cuda(a) for a in F.make_weights(M, n, n)))
+    blk = F.load(F.block(M, n, E, I, 0), n, E, k, I, 0, hx.BF16)
+    idx, w, _ = F.routing(M, M, E, k)
+    idx, w = cuda(idx), cuda(w)
+    xs = [cuda(np.random.default_rng(i).standard_normal((M, n)).astype(np.float32), True) for i in range(2)]
+    want = [(layer(x), blk.experts(x, idx, w)) for x in xs]
+    ws = [[torch.empty(max(s, 16), dtype=torch.uint8, device="cuda") for s in (layer.workspace_size(M), blk.workspace_size(M))] for _ in xs]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in xs], [], []
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, layer(xs[i], workspace=ws[i][0]), blk.experts(xs[i], idx, w, workspace=ws[i][1])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for i, a, b in got)
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append((layer(xs[i], workspace=ws[i][0]), blk.experts(xs[i], idx, w, workspace=ws[i][1])))
+        graphs.append(g)
+    for _ in range(5):
+        for a, b in outs:
+            a.zero_(), b.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) and torch.equal(b, d) for (a, b), (c, d) in zip(outs, want))
+    blk.close(), layer.close()
+
+
+def test_a_captured_call_without_the_memory_that_it_needs():
+    """refused while it is captured, the graph's other work stays; few rows need none"""
+    import helexa_amd as hx
+    import torch
+    layer = hx.F8Linear.load(*(cuda(a) for a in F.make_weights(1, 128, 256)))
+    x = cuda(np.random.default_rng(1).standard_normal((40, 256)).astype(np.float32))
+    want = layer(x[:16])
+    assert layer.workspace_size(16) == 0 and layer.workspace_size(40) > 0
+    out = torch.zeros((16, 128), device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(hx.HxError, match="captured"):
+            layer(x)
+        layer(x[:16], out=out)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
