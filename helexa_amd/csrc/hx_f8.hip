@@ -726,10 +726,11 @@ HX_DEV bool f8_place(int NF, int NR, int& nf, int& nr) {
 }
 
 // Linear layer of many rows. Tiles of 256: 8192 rows, 8192 x 4096, 550 GFLOP in 265 to 295 us (1.9 to 2.1
-// PFLOP/s by the box; a library product of the same codes with one scale for all takes 223): the
+// PFLOP/s by the card; a library product of the same codes with one scale for all takes 223): the
 // matrix cores work half of the time, the scales' multiply-adds take half as many cycles as
 // the products, and two waves a SIMD, a stage's barrier and its LDS reads leave gaps. Tiles of 64: bound by
-// the chain of stages, 0.6 us each, and the launch before: 512 rows, 4096 x 2048, 12 us.
+// the chain of stages, 0.6 us each, and the launch before: 512 rows, 4096 x 2048, 12 us. Results in bf16 of features that are
+// no multiple of 8 leave element by element, 2 bytes each: 8192 rows, 8196 x 4096, 408 us for 282, 512 rows 46 for 32.
 template <int FT, int TT, int WF, int WR, int NS, int KS, bool WIDE>
 __global__ __launch_bounds__(64 * WF * WR * KS, 2) void k_f8_linear(F8LinearArgs a) {
   typedef F8Core<FT, TT, WF, WR, NS, KS> Core;
@@ -850,7 +851,8 @@ hipError_t launch_f8_linear(const F8LinearArgs& a, hipStream_t s) { return a.ybf
 // are of several workgroups, the down kernels quantise it. ONE token: an expert a chosen entry. QUANT: the
 // tokens are quantised into LDS by every workgroup, their expert's weights on their way meanwhile;
 // more tokens come quantised. Bound by latency and the weight stream: one token's 23 MB (11 experts of
-// 512 x 2048) in 7.4 to 8.1 us, 3 TB/s with a launch and the tokens' round trip in it.
+// 512 x 2048) in 7.9 to 8.2 us, 2.9 TB/s with a launch and the tokens' round trip in it; 4 tokens' 82 MB in 22 us, the load
+// units 77 % of the time at work. The products are exact (launch_f8_gate_up).
 template <bool BF, int KW, bool ONE, bool QUANT>
 __global__ __launch_bounds__(512) void k_f8_few_gate_up(F8Args a) {
   constexpr int FW = 8 / KW;
@@ -1132,9 +1134,12 @@ hipError_t launch_f8_prep(const F8Args& a, hipStream_t s) {
 
 // Rows of a tile: F entries over all E experts, so that padding and experts without rows count too
 // (the routing is on the device). us for 512 experts of 512 x 2048, 10 chosen, with tiles of 32, 64, 128: 64 tokens
-// 218, 224, 262; 512 (10 rows an expert) 314, 324, 378; 1024 (20) 357, 348, 394; 2048 (40) 447, 370, 422; 3000 (59,
-// skewed) 517, 432, 457; 4096 (80) 607, 533, 491; 8192 (160, skewed) 943, 791, 764. (16: 241 and 341 for the
-// first two.) Tiles of 128 have kernels of their own, which find a token's codes by 32 bits; f32
+// 219, 225, 265; 512 (10 rows an expert) 310, 322, 380; 900 (18) 322, 332, 393; 1024 (20) 329, 333, 394; 2048 (40) 416, 365, 424;
+// 3000 (59) 472, 412, 449; 4096 (80) 579, 519, 487; 8192 (160, skewed) 946, 765, 765. (16, by the fp8 instruction: 241 and
+// 341 for 64 and 512 tokens.) 128 of 768 x 2048, 8 chosen: 18 rows an expert 129, 131, 150; 24 142, 134, 154; 60 180, 164, 172; 80 216,
+// 197, 182. 64 of 1408 x 4096, 6 chosen: 18 212, 217, 246; 24 238, 221, 250; 60 323, 272, 278; 80 359, 337, 294. Small experts, 256 of
+// 256 x 1024, 8 chosen, would take smaller ones a little longer: 24 rows 61, 69, 80; 40 74, 74, 85; 80 104, 101, 102. Few wide ones,
+// 16 of 2048 x 2048, 2 chosen, larger ones sooner: 40 63, 52, 53; 60 74, 64, 56; 80 76, 68, 59. Tiles of 128 have kernels of their own, which find a token's codes by 32 bits; f32
 // results' operands leave room for 32.
 int f8_tile_m(int64_t T, int64_t F, int E, int H, bool xbf) {
   if (!xbf || F <= 18 * (int64_t)E) return 32;
@@ -1143,8 +1148,8 @@ int f8_tile_m(int64_t T, int64_t F, int E, int H, bool xbf) {
 
 // h = q(silu(G x) * (U x)). Workgroup: a tile of TM rows and 128 features, a block of h's
 // columns: 32 a wave (16 where there are 8), gate and up of a feature in the same lane. Bound by the weights' way
-// from HBM into the CU: 512 experts of 512 x 2048, 1.07 GB; 64 tokens, 0.69 GB of it, 118 to 127 us (5.5 to
-// 5.9 TB/s); 512 tokens 200 us (5.4 TB/s), the load units 97 % of the time at work, the matrix cores 8.
+// from HBM into the CU: 512 experts of 512 x 2048, 1.07 GB; 64 tokens, 0.69 GB of it, 116 to 126 us (5.5 to
+// 5.9 TB/s); 512 tokens 197 us (5.5 TB/s), the load units 96 % of the time at work, the matrix cores 17.
 template <int TM, bool WIDE, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_gate_up(F8Args a) {
   constexpr int TT = TM / 16, NF = 8 / NW, NM = 2 * NF;   // NF: a wave's tiles of features
@@ -1248,8 +1253,9 @@ HX_DEV void f8_out_rows(const F8Args& a, const f8_v4f (&acc)[NM][TT], uint8_t* t
 
 // Outputs of the experts, unweighted: D h. Workgroup: a tile of TM rows and 256 outputs. Bound as
 // gate/up: 512 tokens, 0.54 GB, in 107 us (5 TB/s); 64 tokens 61 to 65 us. bf16 activations: outputs leave
-// as f16 with a scale for each 32, 2^-12 of a value at most for half of the bytes that float32 takes
-// here and in the combine (bf16, 2^-9, would be half of the result's own error on top of it).
+// as f16 with a scale for each 32, off by 2^-11 of a value at most (or, where that is more, 2^-39 of the power of two
+// below the largest that it shares the scale with) for half of the bytes that float32 takes here and in the
+// combine (bf16, 2^-8, would be the result's own error once more).
 template <int TM, bool WIDE, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_down(F8Args a) {
   constexpr int TT = TM / 16, NM = 16 / NW;
@@ -1295,8 +1301,8 @@ __global__ __launch_bounds__(64 * NW, NW / 2) void k_f8_down(F8Args a) {
 
 // The same two products where experts have many rows: both operands through LDS (F8Core), tiles of
 // 128 rows; the waves of a tile's second half bring loads only where it has 64 rows or fewer. Bound by the
-// loads' latency at two waves a SIMD, with a barrier a stage: 8192 tokens, ten experts each, gate/up 378 GFLOP in 355 to 430 us by
-// the routing (1 PFLOP/s; the load units 73 % at work, the matrix cores 28 %), down 189 GFLOP in 270 to 310 us (86 %, 18 %:
+// loads' latency at two waves a SIMD, with a barrier a stage: 8192 tokens, ten experts each, gate/up 378 GFLOP in 353 us, 441 where
+// the routing is skewed (1 PFLOP/s; the load units 73 % at work, the matrix cores 28 %), down 189 GFLOP in 267 and 317 us (87 %, 17 %:
 // K is four stages, each output leaves with 2 bytes and the rows' 0.39 GB are written).
 __global__ __launch_bounds__(512, 2) void k_f8_gate_up_many(F8Args a) {
   typedef F8Core<4, 4, 4, 2, 2> Core;
