@@ -24,16 +24,19 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 // global_load_lds_dwordx4: lane l's 16 bytes at g land at LDS byte lds_base +
 // 16 l, no registers involved; issued from inline assembly with M0 saved and
 // restored around it (the compiler does not know which LDS bytes it writes, so
-// the waits for it are placed by hand)
+// the waits for it are placed by hand). The hardware wants a wait state between a
+// write of M0 and a load that goes by it, and five between a VALU instruction that
+// writes a scalar register and a load that has its address there; in inline assembly
+// nobody else puts them in.
 HX_DEV void dma16(const void* g, uint32_t lds_base) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(g), "s"(lds_base) : "memory");
 }
 // the same, the lanes' bytes `off` from a base in scalar registers
 HX_DEV void dma16(const void* base, uint32_t off, uint32_t lds_base) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(off), "s"(base), "s"(lds_base) : "memory");
 }
 // a workgroup barrier that orders LDS accesses only: global loads still in
@@ -47,14 +50,14 @@ HX_DEV void lds_barrier() {
 // global_load_lds_dword: lane l's 4 bytes at g land at LDS byte lds_base + 4 l
 HX_DEV void dma4(const void* g, uint32_t lds_base) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(g), "s"(lds_base) : "memory");
 }
 
 // the same, the lanes' bytes `off` from a base in scalar registers
 HX_DEV void dma4(const void* base, uint32_t off, uint32_t lds_base) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(off), "s"(base), "s"(lds_base) : "memory");
 }
 
