@@ -96,7 +96,7 @@ typedef struct hx_moe hx_moe;
 int hx_moe_create(const hx_moe_config* cfg, const hx_moe_weights* w, int device, hx_moe** out);
 
 /* Scales of a block of HX_F8_E4M3 projections, f32, in the weights' location, copied as
- * they are: gate and up [E, ceil(I / 128), ceil(H / 128)], down [E, ceil(H / 128), ceil(I / 128)],
+ * they are, and complete when the call is made: gate and up [E, ceil(I / 128), ceil(H / 128)], down [E, ceil(H / 128), ceil(I / 128)],
  * the shared expert's [ceil(Is / 128), ceil(H / 128)] and [ceil(H / 128), ceil(Is / 128)]. */
 typedef struct hx_moe_f8_scales {
     const float* experts_gate;
@@ -116,9 +116,9 @@ typedef struct hx_moe_f8_scales {
  * or an infinity makes its row's outputs NaN. For HX_F32 activations products are exact and every sum is
  * in f32. For HX_BF16 down's products are added by the matrix cores in fixed point, 13 bits below the
  * largest of each 32 (off by 1.4e-5 to 5.5e-5 of a sum's norm; the result's own rounding is 1.7e-3), and above
- * 16 tokens the experts' outputs are held with 11 bits until the weighted f32 sum. Above 16 tokens and
- * 18 chosen entries for each of the E experts gate's and up's products are added so too: some codes of h then
- * become their neighbours, which adds about 1.3e-3 of the outputs' norm. */
+ * 16 tokens the experts' outputs are held with 11 bits until the weighted f32 sum. Gate's and up's products
+ * are exact in calls of up to 16 tokens or with n_tokens num_experts_per_tok <= 18 num_experts; in larger ones they are
+ * added in fixed point too: some codes of h then become their neighbours, about 1.3e-3 of the outputs' norm. */
 int hx_moe_create_f8(const hx_moe_config* cfg, const hx_moe_weights* w, const hx_moe_f8_scales* scales, int device,
                      hx_moe** out);
 
@@ -283,7 +283,7 @@ int hx_quantize_f8(const void* x, int x_dtype, int64_t rows, int64_t cols, int b
  * projections: y = q(x) W^T, q the rows' quantisation by blocks of 1 x 128, f32 sums, one
  * rounding to y's type, whichever x's is: products are exact for HX_F32, added in fixed point for HX_BF16. The reference's quantised linear layers
  * (crates/neuron/src/harness/tp/tp_linear.rs:47-140) have no such format.
- * hx_linear_create copies codes [out, in] and scales [ceil(out / 128), ceil(in / 128)] from
+ * hx_linear_create copies codes [out, in] and scales [ceil(out / 128), ceil(in / 128)], complete when it is called, from
  * location (HX_HOST or HX_DEVICE) to device memory of its own and lays them out; sizes need not be
  * whole blocks (out at most 2^20, in 2^17). hx_linear_forward: x [n_rows, in] and y
  * [n_rows, out], HX_F32 or HX_BF16 each, without a byte in common (HX_ERR_INVALID_ARGUMENT); n_rows 0 is a no-op. A row that
